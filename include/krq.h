@@ -18,6 +18,19 @@
  *               lane l (0..63) owns the 16 contiguous bytes of row (l % 16), columns
  *               64*t + 16*(l / 16) .. +16. One 64-lane 128-bit load reads one whole tile (1 KiB,
  *               contiguous). Needs N % 16 == 0 and K % 64 == 0. krq_unpack_fp8 inverts it.
+ *   mx        - OCP microscaling (MX v1.0): blocks of 32 consecutive k of a row, each with one E8M0 scale
+ *               byte c standing for 2^(c - 127) (255: NaN), elements e2m1 (4 bits) or e4m3. Quantising a
+ *               block of largest magnitude a: c = max(0, floor(log2 a) + 127 - emax) with emax 2 (e2m1) or 8
+ *               (e4m3), elements the values / 2^(c - 127) rounded to nearest even and clamped to 6 or 448;
+ *               a block with a NaN or an infinity gets c = 255 and elements 0.
+ *   mx tiled  - the operand layout of the MX products, for weights and activation rows alike. 16 rows x 128
+ *               k per tile, tiles [ceil(rows / 16)][ceil(K / 128)], lane l = 16 g + r of a tile owning of
+ *               row r: e2m1 (1 KiB a tile) the 16 bytes of k = 32 g .. 32 g + 31, element 2 i in the low
+ *               half of byte i; e4m3 (2 KiB) the 16 bytes of k = 16 g .. + 15 in the first KiB and of
+ *               64 + 16 g .. + 15 in the second. Scales: [ceil(rows / 16)][ceil(K / 512)][64 lanes], 4
+ *               bytes a lane, byte t of lane 16 g + r that of row r, k = 512 s + 128 t + 32 g .. + 31.
+ *               Rows past the last and k past K hold zeros. krq_mx_tiled_bytes / krq_mx_scale_bytes
+ *               give the sizes.
  *   partials  - split-K output: fp32 [split, M, N]; the consumer sums slices 0..split-1 in that
  *               order and rounds once to bf16 (reference engine/kernels/ops.py:29-39).
  */
@@ -402,6 +415,66 @@ int64_t krq_gemm_fp8_ws_bytes(int x_kind, int64_t M, int64_t N, int64_t K);
  * matrix pass its [N, 2K] byte view (K -> 2K). */
 int krq_pack_fp8(const void* w8_rowmajor, int64_t N, int64_t K, void* w8_tiled, void* stream);
 int krq_unpack_fp8(const void* w8_tiled, int64_t N, int64_t K, void* w8_rowmajor, void* stream);
+
+/* element types of MX blocks, and the activation kinds of krq_gemv_mxfp4 */
+#define KRQ_MX_E2M1 0
+#define KRQ_MX_E4M3 1
+#define KRQ_MX_X_BF16 0     /* bf16 rows, quantised in the kernel; at most KRQ_MX_BF16_ROWS of them */
+#define KRQ_MX_X_TILED 1    /* rows from krq_quant_mx_rows, with their scales */
+#define KRQ_MX_BF16_ROWS 8
+
+/* Bytes of the mx tiled elements and of their scales for M rows of K (-1: bad arguments). */
+int64_t krq_mx_tiled_bytes(int64_t M, int64_t K, int elem);
+int64_t krq_mx_scale_bytes(int64_t M, int64_t K);
+
+/*
+ * MXFP4 weight quantizer (the 4-bit counterpart of krq_quant_fp8_rows; no reference counterpart):
+ * w bf16 [N, K], rows ldw elements apart, to e2m1 blocks: w4 [N, K / 2] (element 2 i in the low half of
+ * byte i) and scale [N, K / 32] row-major, and the same in the mx tiled layout. K % 32 == 0; w and its
+ * rows start on 16 bytes.
+ */
+int krq_quant_mxfp4(const void* w_bf16, int64_t N, int64_t K, int64_t ldw, void* w4, void* scale, void* tiled,
+                    void* tiled_scale, void* stream);
+/* The mx tiled copy of row-major codes and scales (a checkpoint's; w4 on 16 bytes). */
+int krq_pack_mxfp4(const void* w4, const void* scale, int64_t N, int64_t K, void* tiled, void* tiled_scale, void* stream);
+/* Activation rows x bf16 [M, K] (rows ldx elements apart, on 16 bytes) to MX blocks of elem, mx tiled. */
+int krq_quant_mx_rows(const void* x_bf16, int64_t M, int64_t K, int64_t ldx, int elem, void* tiled, void* tiled_scale,
+                      void* stream);
+/* mx tiled blocks to the bf16 values they stand for (exact; below 2^-126 as bf16 holds them): out [M, K]. */
+int krq_dequant_mx(const void* tiled, const void* tiled_scale, int elem, int64_t M, int64_t K, void* out, void* stream);
+/*
+ * Rows of a packed table: out[i] = bf16(w[ids[i]] * mult), out bf16 [T, K], w4 / scale row-major [N, ..] as
+ * krq_quant_mxfp4 writes them, ids int64 (ids_64 != 0) or int32. An index outside [0, N) gives a row of NaN.
+ */
+int krq_embed_mxfp4(const void* ids, int ids_64, int64_t T, const void* w4, const void* scale, int64_t N, int64_t K, float mult,
+                    void* out, void* stream);
+
+/*
+ * MXFP4 skinny GEMM / GEMV, M <= 32 (krq_gemv_fp8 on MX blocks; no reference counterpart):
+ *   y[m,n] = sum_k x[m,k] w[n,k] over the blocks' values, fp32 accumulation
+ * x_kind KRQ_MX_X_BF16: x bf16 [M, K] (M <= KRQ_MX_BF16_ROWS, rows ldx elements apart, on 16 bytes), rounded to
+ * blocks of elem in the kernel; KRQ_MX_X_TILED: x and x_scale from krq_quant_mx_rows (ldx unused).
+ * w_tiled / w_scale: mx tiled e2m1 [N, K]. mode KRQ_OUT_BF16 -> bf16 [M, N] (split 1); KRQ_OUT_PARTIAL -> fp32
+ * [split, M, N], split s the sum over the groups of 512 k [s G / split, (s + 1) G / split), G = ceil(K / 512),
+ * split <= min(G, 64); KRQ_OUT_SWIGLU (w = [gate; up], N = 2 I, I % 16 == 0) -> bf16 [M, I] =
+ * bf16(silu(g) * u) from the fp32 g and u. K % 32 == 0, any N.
+ */
+int krq_gemv_mxfp4(const void* x, const void* x_scale, int x_kind, int elem, int64_t ldx, const void* w_tiled,
+                   const void* w_scale, int64_t M, int64_t N, int64_t K, int split, int mode, void* out, void* stream);
+/*
+ * MXFP4 GEMM for prefill (any M): out bf16 [M, N] = the product of krq_gemv_mxfp4 on rows from
+ * krq_quant_mx_rows. K % 32 == 0, any N.
+ */
+int krq_gemm_mxfp4(const void* x_tiled, const void* x_scale, int elem, const void* w_tiled, const void* w_scale, int64_t M,
+                   int64_t N, int64_t K, void* out, void* stream);
+/*
+ * krq_lmhead_argmax on an MXFP4 head: logits bf16 [M, V] of krq_gemv_mxfp4 (NULL to skip) and their argmax,
+ * first index of the maximum. x as krq_gemv_mxfp4's; ws: krq_lmhead_ws_bytes(M, V) bytes (overwritten; calls
+ * that overlap must not share it). V % 16 == 0.
+ */
+int krq_lmhead_argmax_mxfp4(const void* h, const void* h_scale, int x_kind, int elem, int64_t ldh, const void* w_tiled,
+                            const void* w_scale, int64_t M, int64_t V, int64_t K, void* logits, void* ws, int64_t ws_bytes,
+                            int64_t* idx_out, void* stream);
 
 const char* krq_version(void);
 const char* krq_last_error(void);

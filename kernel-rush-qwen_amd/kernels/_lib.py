@@ -19,6 +19,8 @@ W_ROWMAJOR, W_TILED = 0, 1
 LM_BF16, LM_FP8, LM_FP8_TILED_H = 0, 1, 2
 ALGO_AUTO, ALGO_MFMA, ALGO_VALU = 0, 1, 2
 X_FP8, X_BF16_DYN, X_BF16_STATIC, X_FP8_TILED = 0, 1, 2, 3
+MX_E2M1, MX_E4M3 = 0, 1
+MX_X_BF16, MX_X_TILED, MX_BF16_ROWS = 0, 1, 8
 LMHEAD_SCRATCH_BYTES = 4194304  # KRQ_LMHEAD_SCRATCH_BYTES
 
 _vp, _i64, _i32, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
@@ -71,6 +73,17 @@ EXPORTS = {
     "krq_gemm_fp8_ws_bytes": (_i64, [_i32, _i64, _i64, _i64]),
     "krq_pack_fp8": (_i32, [_vp, _i64, _i64, _vp, _vp]),
     "krq_unpack_fp8": (_i32, [_vp, _i64, _i64, _vp, _vp]),
+    "krq_mx_tiled_bytes": (_i64, [_i64, _i64, _i32]),
+    "krq_mx_scale_bytes": (_i64, [_i64, _i64]),
+    "krq_quant_mxfp4": (_i32, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "krq_pack_mxfp4": (_i32, [_vp, _vp, _i64, _i64, _vp, _vp, _vp]),
+    "krq_quant_mx_rows": (_i32, [_vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp]),
+    "krq_dequant_mx": (_i32, [_vp, _vp, _i32, _i64, _i64, _vp, _vp]),
+    "krq_embed_mxfp4": (_i32, [_vp, _i32, _i64, _vp, _vp, _i64, _i64, _f32, _vp, _vp]),
+    "krq_gemv_mxfp4": (_i32, [_vp, _vp, _i32, _i32, _i64, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp, _vp]),
+    "krq_gemm_mxfp4": (_i32, [_vp, _vp, _i32, _vp, _vp, _i64, _i64, _i64, _vp, _vp]),
+    "krq_lmhead_argmax_mxfp4": (_i32, [_vp, _vp, _i32, _i32, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp,
+                                       _vp]),
     "krq_version": (ctypes.c_char_p, []),
     "krq_last_error": (ctypes.c_char_p, []),
 }

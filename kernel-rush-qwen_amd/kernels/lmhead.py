@@ -12,6 +12,7 @@ FP8 heads take the activation scaling of the weight's form:
       engine.py:504-505): exactly linear_fp8(h, lm8) followed by torch.argmax (engine.py:989,
       :1022) - one ActScale over all of h (at M == 1 the same as per token, so inside the GEMV),
       or the given ActScale / SharedScale `a`.
+MXFP4 heads take h in e4m3 blocks (mxfp4.quant_rows), rounded inside the GEMV up to eight rows.
 """
 
 import torch
@@ -19,6 +20,7 @@ import torch
 from . import _lib as L
 from . import fp8 as _fp8
 from . import gemv as _gemv
+from . import mxfp4 as _mxfp4
 
 
 # The persistent head reads tiled rows from LDS (k_lmhead_fp8_persist); fewer rows cost less row-major,
@@ -58,9 +60,30 @@ def _fp8_operands(h, w, a, h_layout):
     return h8, hs.reshape(-1), 1, L.LM_FP8
 
 
+def _mxfp4_head(h, q, return_logits):
+    V, K = q.shape
+    h = _mxfp4._bf16_rows(h, "rows [M, K]")
+    M = h.shape[0]
+    if h.shape[1] != K or M < 1:
+        raise ValueError(f"h {tuple(h.shape)} and w [{V}, {K}] do not match")
+    _mxfp4._same_device(h, q.tiled)
+    idx = torch.empty((M,), device=h.device, dtype=torch.int64)
+    logits = torch.empty((M, V), device=h.device, dtype=torch.bfloat16) if return_logits else None
+    ws = torch.empty((int(L.lib().krq_lmhead_ws_bytes(M, V)),), device=h.device, dtype=torch.uint8)
+    if M <= L.MX_BF16_ROWS:
+        xin, xs, kind, ld = h, None, L.MX_X_BF16, _mxfp4._ld(h)
+    else:
+        rows = _mxfp4.quant_rows(h)
+        xin, xs, kind, ld = rows.tiled, rows.tiled_scale, L.MX_X_TILED, 0
+    _mxfp4._call(h, "krq_lmhead_argmax_mxfp4", L.ptr(xin), L.ptr(xs), kind, L.MX_E4M3, ld, L.ptr(q.tiled), L.ptr(q.tiled_scale),
+                 M, V, K, L.ptr(logits), L.ptr(ws), ws.numel(), L.ptr(idx))
+    return (idx, logits) if return_logits else idx
+
+
 def lm_head_argmax(h, w, return_logits=False, h_layout="auto", a=None):
-    """h [M, K] bf16 (M <= 32); w the tied embedding, bf16 [V, K], or an FP8Weight from
-    fp8.quantize (per channel) or fp8.quantize_weight (per tensor). Returns int64 [M] token ids,
+    """h [M, K] bf16 (M <= 32); w the tied embedding, bf16 [V, K], an FP8Weight from
+    fp8.quantize (per channel) or fp8.quantize_weight (per tensor), or an MXFP4Weight from mxfp4.quantize
+    (h in e4m3 blocks). Returns int64 [M] token ids,
     or (ids, bf16 logits [M, V]) with return_logits=True. h_layout ("auto", "tiled" or
     "rowmajor"): how a per-channel FP8 head's per-token rows are laid out at M > 1 (the same
     operands either way); "auto" takes tiled rows from fp8.TILED_MIN_ROWS, and from TILED_MIN_ROWS
@@ -70,6 +93,10 @@ def lm_head_argmax(h, w, return_logits=False, h_layout="auto", a=None):
     M, K = h.shape
     if M > 32:
         raise ValueError(f"lm_head_argmax: M={M} > 32")
+    if isinstance(w, _mxfp4.MXFP4Weight):
+        if a is not None:
+            raise ValueError("an MXFP4 head scales h by blocks: it takes no ActScale / SharedScale")
+        return _mxfp4_head(h, w, return_logits)
     if isinstance(w, tuple):
         w8, ws = w[0], w[1]
         tiled = getattr(w, "tiled", None)

@@ -26,6 +26,9 @@ coherent loads. act is bit-identical to the pair's; the partials equal the pair'
 rounding (the down blocks sum two weight waves). A wait that gives up makes that block's
 partials NaN and failed() reports it; zero_ctl() then clears the control words.
 
+MXFP4 weights (mxfp4.quantize) take the two launches, their activations in e4m3 blocks; act is
+bf16(silu(g) * u) from the fp32 g and u, and split is at most ceil(I / 512).
+
 For BF16 weights, one_launch=True or chained=True (any M) runs the chained launch of the BF16
 GEMVs, k_mlp_chain_bf16 (krq_mlp_chain_bf16): each stage keeps its standalone launch's plan, so
 act and the partials are the two-launch pair's, bit for bit; waits, failed() and zero_ctl() as
@@ -37,6 +40,7 @@ import torch
 from . import _lib as L
 from . import fp8 as _fp8
 from . import gemv as _gemv
+from . import mxfp4 as _mxfp4
 
 
 class PersistentMLP:
@@ -93,6 +97,18 @@ class PersistentMLP:
         self.act = act
         return out
 
+    def _mxfp4(self, h, w_gu, w_down):
+        H, I, S = self.H, self.I, self.split
+        if tuple(_mxfp4._weight(w_gu)) != (2 * I, H) or tuple(_mxfp4._weight(w_down)) != (H, I):
+            raise ValueError(f"PersistentMLP: weights {w_gu.shape} / {w_down.shape} do not match H={H}, I={I}")
+        if self.chained or self.one_launch:
+            raise ValueError("PersistentMLP: MXFP4 weights run as two launches")
+        h2 = _fp8._rows(h)
+        if h2.shape[0] != self.M:
+            raise ValueError(f"PersistentMLP built for M={self.M}, called with M={h2.shape[0]}")
+        self.act = _mxfp4.gemv_swiglu_mxfp4(h2, w_gu)
+        return _mxfp4._decode(self.act, w_down, S, L.OUT_PARTIAL, "e4m3")
+
     def __call__(self, h, w_gu, w_down, max_polls=None):
         """max_polls (one-launch form): bound on the phase-1 wait's polls (default: about a
         second's worth); a small value forces the timeout path, for tests."""
@@ -100,6 +116,8 @@ class PersistentMLP:
             if w_gu.dtype != torch.bfloat16 or w_down.dtype != torch.bfloat16:
                 raise ValueError("PersistentMLP: weights are FP8Weight tuples or bf16 tensors")
             return self._bf16(h, w_gu, w_down, max_polls)
+        if isinstance(w_gu, _mxfp4.MXFP4Weight) or isinstance(w_down, _mxfp4.MXFP4Weight):
+            return self._mxfp4(h, w_gu, w_down)
         if not (isinstance(w_gu, tuple) and isinstance(w_down, tuple)):
             raise ValueError("PersistentMLP: weights are FP8Weight tuples or bf16 tensors")
         H, I, S = self.H, self.I, self.split
