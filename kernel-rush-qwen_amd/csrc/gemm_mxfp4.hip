@@ -1,52 +1,395 @@
-// MXFP4 GEMM for prefill: out = bf16(x . w^T), x e4m3 or e2m1 blocks and w e2m1 blocks, both in the operand
-// tiles of mx_common.h, fp32 accumulation.
+// MXFP4 GEMM for prefill: out = bf16(x . w^T), x in e4m3 or e2m1 blocks, w in e2m1 blocks, both in the operand
+// tiles of mx_common.h, fp32 accumulation on v_mfma_scale_f32_32x32x64_f8f6f4.
 //
-// A workgroup owns 128 x 128 outputs, its four waves 64 x 64 each: per 128 k four activation and four weight
-// tiles straight from memory and sixteen v_mfma_scale_f32_16x16x128_f8f6f4.
+// Persistent workgroups of W waves own BM x BN outputs, each wave BM / 2 x 2 BN / W of them, in 32 x 32 pieces. The
+// stream of stages (a stage: 128 k, one tile of every row block) runs on from one output tile into the next:
+// direct loads bring a stage into one of NB LDS buffers, NB stages ahead of its use. A tile is stored in
+// lane order, so each load copies one whole KiB, and each 16-byte LDS read takes runs of 256 bytes: no padding, no
+// swizzle, no bank conflict, and no address arithmetic per lane. The scale bytes come a group of four stages at
+// a time into a ring of their own, from which every product reads its byte.
+//
+// Fragment of 32 rows, half h of the stage (64 k): lane l holds row l % 32, that is row r = l % 16 of row block
+// (l / 16) % 2, with c = l / 32
+//   e2m1: k = 64 h + 32 c + 0..31, the 16 bytes of tile lane 16 (2 h + c) + r;
+//   e4m3: k = 64 h + 16 c + 0..15 and 32 more, the bytes of tile lanes 16 c + r and 16 (c + 2) + r of KiB h;
+// its scale byte is that of block 2 h + c. Weights are the instruction's first operand, so a lane ends with four
+// adjacent columns of one row: element e of lane l is column 8 (e / 4) + 4 c + e % 4 of row l % 32.
+#include <algorithm>
+#include <type_traits>
+
 #include "mx_common.h"
 
 using namespace krq;
 
 namespace {
 
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+// 32-bit LDS address of a pointer into a __shared__ array, wave-uniform
+KRQ_DEV uint32_t lds_at(const uint8_t* p) {
+  return __builtin_amdgcn_readfirstlane(
+      static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t*)p)));
+}
+
+// Direct loads and their waits are assembly, so that the compiler, which does not know the ring's buffers apart, waits for
+// none of them by itself, and (the two that branch) so that a stage of the stream stays one basic block, within which
+// products, LDS reads and loads can be interleaved.
+KRQ_DEV uint64_t uniform(const uint8_t* p) {
+  const uint64_t b = reinterpret_cast<uint64_t>(p);
+  return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(b))) |
+         static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(b >> 32)))) << 32;
+}
+
+// 16 bytes per lane from base + off (base wave-uniform) to LDS at l + 16 lane (s_nop: M0 is read right after its scalar write)
+KRQ_DEV void load_lds(const uint8_t* base, uint32_t off, uint32_t l) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(l)), "v"(off),
+               "s"(uniform(base))
+               : "memory", "m0");
+}
+
+// the same, if on != 0 (wave-uniform)
+KRQ_DEV void load_lds_if(int on, const uint8_t* base, uint32_t off, uint32_t l) {
+  asm volatile(
+      "s_cmp_eq_u32 %3, 0\n\ts_cbranch_scc1 .Lkrq_no_load%=\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, "
+      "%2\n.Lkrq_no_load%=:" ::"s"(__builtin_amdgcn_readfirstlane(l)),
+      "v"(off), "s"(uniform(base)), "s"(__builtin_amdgcn_readfirstlane(on))
+      : "memory", "m0", "scc");
+}
+
+template <int N>
+KRQ_DEV void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N < 63 ? N : 63) : "memory");
+}
+
+// at most N operations in flight, or at most N + S where more != 0 (wave-uniform)
+template <int N, int S>
+KRQ_DEV void wait_loads_or(int more) {
+  asm volatile(
+      "s_cmp_eq_u32 %2, 0\n\ts_cbranch_scc0 .Lkrq_more%=\n\ts_waitcnt vmcnt(%0)\n.Lkrq_more%=:\n\ts_waitcnt vmcnt(%1)" ::"n"(N < 63 ? N : 63),
+      "n"(N + S < 63 ? N + S : 63), "s"(__builtin_amdgcn_readfirstlane(more))
+      : "memory", "scc");
+}
+
+// workgroup barrier for LDS accesses (the direct loads are waited for explicitly)
+KRQ_DEV void barrier_lds() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// after product U, its share of the NR LDS reads
+template <int U, int NP, int NR>
+KRQ_DEV void interleave() {
+  if constexpr (U < NP) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    constexpr int c = (U + 1) * NR / NP - U * NR / NP;
+    if constexpr (c > 0) __builtin_amdgcn_sched_group_barrier(0x100, c, 0);
+    interleave<U + 1, NP, NR>();
+  }
+}
+
+struct GemmArgs {
+  const uint8_t *x, *xs, *w, *ws;
+  int M, N, KT, groups, mbs, nbs;  // mbs, nbs: row blocks of x and w
+  int tiles_m, tiles, splits;
+  int wide;                        // out's rows start on 16 bytes: N % 8 == 0
+  float* part;                     // fp32 [splits][M][N] (PART)
+  uint16_t* out;
+};
+
+// PART: a work unit is (tile, split) and writes its fp32 sums to plane `split` of part; else bf16 to out.
+template <int ELEM, int BM, int BN, int W, int OCC, int NB, bool PART>
+__global__ __launch_bounds__(64 * W, OCC * W / 4) void k_gemm_mx(const GemmArgs a) {
+  constexpr int AB = ELEM == KRQ_MX_E2M1 ? 1 : 2;          // KiB per activation tile
+  constexpr int kA = BM / 16 * AB * 1024, kB = BN / 16 * 1024, kStage = kA + kB;
+  constexpr int QA = kA / 1024 / W, QB = kB / 1024 / W, kLoads = QA + QB;  // loads per wave per stage
+  constexpr int kScale = (BM + BN) / 16 * 256;             // scale bytes of a group
+  constexpr int kSl = (kScale / 1024 + W - 1) / W;             // loads per wave per group (some twice)
+  constexpr int FI = BM / 64, FJ = BN / (16 * W);          // 32-row fragments of a wave
+  constexpr int NP = FI * FJ, NR = FI * AB + FJ + FI + FJ; // products and LDS reads per half stage
+  constexpr int kStores = PART ? NP * 4 : NP * 2;
+  static_assert(NB >= 2 && NB <= 4 && BM % 64 == 0 && BN % (16 * W) == 0 && QA * W * 1024 == kA && QB * W * 1024 == kB, "tile shape");
+  // NB scale slots: a slot is filled again once NB - 1 more groups (of one stage at least each) have begun
+  __shared__ __align__(1024) uint8_t ring[NB * (kStage + kScale)];
+  uint8_t* const sring = ring + NB * kStage;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int c = lane >> 5, hi = (lane >> 4) & 1, r = lane & 15;
+  const int wmb = (wave & 1) * (BM / 32), wnb = (wave >> 1) * (2 * FJ);  // this wave's first row blocks
+  const int G = gridDim.x, bid = blockIdx.x, units = a.tiles * a.splits;
+
+  // the workgroup's k-th unit: units in order, M-fastest; in a whole round of G units the workgroups of one XCD
+  // (b, b + 8, ...) take a contiguous run
+  auto unit_of = [&](int k) {
+    const int base = k * G;
+    if (base + bid >= units) return -1;
+    if ((G & 7) == 0 && units - base >= G) return base + (bid & 7) * (G >> 3) + (bid >> 3);
+    return base + bid;
+  };
+
+  // ---- the stream's loading end: stage ls of ls1 of unit lk, into buffer lb ----
+  int lk = 0, ls = 0, ls1 = 0, lstep = 1, lb = 0, lslot = NB - 1, lnew = 1;  // lnew: the first stage of a unit
+  const uint8_t *xb = a.x, *wb = a.w, *xsb = a.xs, *wsb = a.ws;  // the unit's tiles, at stage ls; its scales
+  uint32_t off[kLoads], soff[kSl];
+  auto load_unit = [&](int u) {
+    const int p = u % a.tiles, sp = u / a.tiles;
+    const int mb0 = p % a.tiles_m * (BM / 16), nb0 = p / a.tiles_m * (BN / 16);
+    ls = static_cast<int>((int64_t)a.KT * sp / a.splits);
+    ls1 = static_cast<int>((int64_t)a.KT * (sp + 1) / a.splits);
+    lnew = 1;
+    xb = a.x + ((int64_t)mb0 * a.KT + ls) * (1024 * AB);
+    wb = a.w + ((int64_t)nb0 * a.KT + ls) * 1024;
+    xsb = a.xs + (int64_t)mb0 * a.groups * 256;
+    wsb = a.ws + (int64_t)nb0 * a.groups * 256;
+    int ln = lane;  // (opaque: computed here per unit, not kept live across units)
+    asm volatile("" : "+v"(ln));
+#pragma unroll
+    for (int q = 0; q < QA; ++q) {
+      const int i = wave + W * q, rb = min(mb0 + i / AB, a.mbs - 1) - mb0;
+      off[q] = static_cast<uint32_t>(rb * a.KT * (1024 * AB) + (i % AB) * 1024 + 16 * ln);
+    }
+#pragma unroll
+    for (int q = 0; q < QB; ++q)
+      off[QA + q] = static_cast<uint32_t>((min(nb0 + wave + W * q, a.nbs - 1) - nb0) * a.KT * 1024 + 16 * ln);
+#pragma unroll
+    for (int q = 0; q < kSl; ++q) {  // four row blocks' scales per load
+      const int rb = (wave + W * q) % (kScale / 1024) * 4 + (ln >> 4);
+      const int at = rb < BM / 16 ? min(mb0 + rb, a.mbs - 1) - mb0 : min(nb0 + rb - BM / 16, a.nbs - 1) - nb0;
+      soff[q] = static_cast<uint32_t>(at * a.groups * 256 + 16 * (ln & 15));
+    }
+  };
+  const uint32_t l0 = lds_at(ring), sl0 = lds_at(sring);
+  // the scales of the stage at the loading end, where it begins a group
+  auto load_scales = [&]() {
+    const int on = lstep & (lnew | ((ls & 3) == 0 ? 1 : 0));
+    lslot += on;
+    lslot = lslot == NB ? 0 : lslot;
+#pragma unroll
+    for (int q = 0; q < kSl; ++q) {
+      const int li = (wave + W * q) % (kScale / 1024);
+      load_lds_if(on, (li < BM / 64 ? xsb : wsb) + (int64_t)(ls >> 2) * 256, soff[q], sl0 + lslot * kScale + li * 1024);
+    }
+    lnew = 0;
+  };
+  auto load_tile = [&](int q) {
+    load_lds(q < QA ? xb : wb, off[q], l0 + lb * kStage + (q < QA ? 0 : kA) + 1024 * (wave + W * (q < QA ? q : q - QA)));
+  };
+  auto advance = [&]() {  // past the loaded stage
+    lb = lb + 1 == NB ? 0 : lb + 1;
+    ls += lstep;
+    xb += lstep * (1024 * AB);
+    wb += lstep * 1024;
+  };
+  // Behind the stream's last stage its loads repeat (lstep 0), into buffers that nobody reads any more, so that every stage
+  // issues as many.
+  auto next_unit = [&]() {
+    const int u = unit_of(++lk);
+    if (u >= 0) {
+      load_unit(u);
+    } else {
+      lstep = 0;
+      --ls;
+      ls1 = 0x7fffffff;
+      xb -= 1024 * AB;
+      wb -= 1024;
+    }
+  };
+  if (unit_of(0) < 0) return;
+  load_unit(unit_of(0));
+  for (int b = 0; b < NB; ++b) {
+    load_scales();
+#pragma unroll
+    for (int q = 0; q < kLoads; ++q) load_tile(q);
+    advance();
+  }
+
+  // ---- the consuming end ----
+  const int lo = hi * 1024 + c * 256 + r * 16;  // e2m1 tile: this lane's 16 bytes of half 0
+  const int loa = hi * (1024 * AB) + c * 256 + r * 16;
+  const int los = (hi * 64 + 16 * c + r) * 4;
+  uint4 fa[2][FI][AB], fb[2][FJ];
+  uint32_t sa[2][FI], sb[2][FJ];
+  // read n of the fragments of half h, stage byte t, buffer b, slot sl, into register set h
+  auto read = [&](int n, int h, int b, int sl, int t) {
+    const uint8_t* pa = ring + b * kStage + wmb * (1024 * AB) + loa;
+    const uint8_t* pb = ring + b * kStage + kA + wnb * 1024 + lo;
+    const uint8_t* ps = sring + sl * kScale + los + t + 128 * h;  // (block 2 h + c)
+    if (n < FI * AB) {
+      const int f = n / AB, e = n % AB;
+      fa[h][f][e] = *reinterpret_cast<const uint4*>(pa + f * (2048 * AB) + (AB == 2 ? 1024 * h + 512 * e : 512 * h));
+    } else if (n < FI * AB + FJ) {
+      const int f = n - FI * AB;
+      fb[h][f] = *reinterpret_cast<const uint4*>(pb + f * 2048 + 512 * h);
+    } else if (n < FI * AB + FJ + FI) {
+      const int f = n - FI * AB - FJ;
+      sa[h][f] = ps[(wmb + 2 * f) * 256];
+    } else {
+      const int f = n - FI * AB - FJ - FI;
+      sb[h][f] = ps[(BM / 16 + wnb + 2 * f) * 256];
+    }
+  };
+  v16f acc[FI][FJ];
+  auto zero = [&]() {
+#pragma unroll
+    for (int i = 0; i < FI; ++i)
+#pragma unroll
+      for (int j = 0; j < FJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+  };
+  // half h of a stage: its products, each followed by its share of the reads of the next half (half 1 - h of buffer b, ...;
+  // behind the stream's last stage they read what nobody uses) and, h = 1, of the loads of the stage at the loading end
+  auto half = [&](auto h_c, int b, int sl, int t) __attribute__((always_inline)) {
+    constexpr int h = decltype(h_c)::value;
+#pragma unroll
+    for (int u = 0; u < NP; ++u) {
+      const int i = u / FJ, j = u % FJ;
+      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+          pack_v8i(fb[h][j], zero4()), AB == 2 ? pack_v8i(fa[h][i][0], fa[h][i][AB - 1]) : pack_v8i(fa[h][i][0], zero4()),
+          acc[i][j], 4, ELEM == KRQ_MX_E2M1 ? 4 : 0, 0, static_cast<int>(sb[h][j]), 0, static_cast<int>(sa[h][i]));
+      if (h == 1) {
+#pragma unroll
+        for (int q = u * kLoads / NP; q < (u + 1) * kLoads / NP; ++q) load_tile(q);
+      }
+#pragma unroll
+      for (int n = u * NR / NP; n < (u + 1) * NR / NP; ++n) read(n, 1 - h, b, sl, t);
+    }
+    interleave<0, NP, NR>();
+  };
+  using yes = std::true_type;
+  using no = std::false_type;
+  using h0 = std::integral_constant<int, 0>;
+  using h1 = std::integral_constant<int, 1>;
+
+  // A lane's four adjacent columns of a row are 8 bytes in bf16; lanes l and l + 32 exchange halves of two such pieces
+  // (v_permlane32_swap), so that each stores 16 bytes. FULL: every row and column lies in the output.
+  auto store = [&](auto full_c, int m0, int n0, int sp) {
+    constexpr bool FULL = decltype(full_c)::value;
+    int le = lane;  // (opaque: addresses are computed here, not hoisted out of the stream and kept)
+    asm volatile("" : "+v"(le));
+    const int ce = le >> 5, mrow = m0 + 16 * wmb + (le & 31);
+#pragma unroll
+    for (int i = 0; i < FI; ++i) {
+      const int m = mrow + 32 * i;
+#pragma unroll
+      for (int j = 0; j < FJ; ++j) {
+        const int n = n0 + 16 * wnb + 32 * j;
+        if constexpr (PART) {
+          float* p = a.part + ((int64_t)sp * a.M + m) * a.N + n + 4 * ce;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            if (FULL || (a.wide && m < a.M && n + 8 * g + 4 * ce < a.N)) {
+              *reinterpret_cast<float4*>(p + 8 * g) =
+                  make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
+            } else if (!a.wide && m < a.M) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (n + 8 * g + 4 * ce + e < a.N) p[8 * g + e] = acc[i][j][4 * g + e];
+            }
+          }
+        } else if (FULL || a.wide) {
+#pragma unroll
+          for (int g = 0; g < 4; g += 2) {
+            uint32_t v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              v[e] = pack_bf16x2(acc[i][j][4 * g + 2 * e], acc[i][j][4 * g + 2 * e + 1]);
+            // (v[0], v[1]: columns 4 c .. of piece g; v[2], v[3]: of piece g + 1)
+            const auto s0 = __builtin_amdgcn_permlane32_swap(v[0], v[2], false, false);
+            const auto s1 = __builtin_amdgcn_permlane32_swap(v[1], v[3], false, false);
+            const int col = n + 8 * (g + ce);
+            if (FULL || (m < a.M && col < a.N))
+              *reinterpret_cast<uint4*>(a.out + (int64_t)m * a.N + col) = make_uint4(s0[0], s1[0], s0[1], s1[1]);
+          }
+        } else if (m < a.M) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int col = n + 8 * (e >> 2) + 4 * ce + (e & 3);
+            if (col < a.N) a.out[(int64_t)m * a.N + col] = f32_to_bf16(acc[i][j][e]);
+          }
+        }
+      }
+    }
+  };
+
+  // in flight: NB stages. Stage 0's loads are the oldest
+  wait_loads<(NB - 1) * kLoads>();
+  barrier_lds();
+#pragma unroll
+  for (int n = 0; n < NR; ++n) read(n, 0, 0, 0, static_cast<int>((int64_t)a.KT * (unit_of(0) / a.tiles) / a.splits) & 3);
+  int buf = 0, slot = 0;
+  int stores = 0;  // the last tile's kStores stores per lane are younger than the next stage's loads
+  auto first = [&](int unit) { return static_cast<int>((int64_t)a.KT * (unit / a.tiles) / a.splits); };
+  for (int k = 0, u = unit_of(0), un; u >= 0; ++k, u = un) {
+    un = unit_of(k + 1);
+    int s = first(u);
+    const int s1 = static_cast<int>((int64_t)a.KT * (u / a.tiles + 1) / a.splits), sfirst = un < 0 ? 0 : first(un);
+    zero();
+    // stage s; the loading end is NB stages ahead
+    auto stage = [&](bool last) __attribute__((always_inline)) {
+      half(h0{}, buf, slot, s & 3);
+      // the next stage has landed, and once every wave is here none reads this one's buffer any more: refill it
+      wait_loads_or<(NB - 2) * kLoads, kStores>(stores);
+      stores = 0;
+      barrier_lds();
+      ++s;
+      const int sn = last ? sfirst : s;  // the next stage: of this unit, or the next one's first
+      const int on = last || (sn & 3) == 0 ? 1 : 0;
+      buf = buf + 1 == NB ? 0 : buf + 1;
+      slot = slot + on == NB ? 0 : slot + on;
+      load_scales();
+      half(h1{}, buf, slot, sn & 3);
+      advance();
+    };
+#pragma clang loop unroll(disable)
+    while (s < s1 - NB) stage(false);
+    next_unit();  // the loading end goes on into the next unit
+#pragma clang loop unroll(disable)
+    while (s < s1) stage(s + 1 == s1);
+    const int p = u % a.tiles;
+    const int m0 = p % a.tiles_m * BM, n0 = p / a.tiles_m * BN;
+    if (m0 + BM <= a.M && n0 + BN <= a.N && a.wide) {
+      store(yes{}, m0, n0, u / a.tiles);
+      stores = 1;
+    } else {
+      store(no{}, m0, n0, u / a.tiles);
+    }
+  }
+  wait_loads<0>();  // no load into LDS outlives the workgroup
+}
+
+// K of fewer stages than the stream holds: 128 x 128 outputs per workgroup, four waves of 64 x 64, operands straight
+// from memory, v_mfma_scale_f32_16x16x128_f8f6f4 (element e of lane l: row 4 (l / 16) + e of x, column l % 16).
+constexpr int kMinStages = 4;
 template <int ELEM>
-__global__ __launch_bounds__(256) void k_gemm_mx(const uint8_t* __restrict__ x, const uint8_t* __restrict__ xs,
-                                                 const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws, int M, int N,
-                                                 int KT, int groups, int tiles_m, uint16_t* __restrict__ out) {
+__global__ __launch_bounds__(256) void k_gemm_mx_short(const GemmArgs a, int tiles_m) {
   constexpr int AB = ELEM == KRQ_MX_E2M1 ? 1 : 2;
-  constexpr int fa = ELEM == KRQ_MX_E2M1 ? 4 : 0;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int m0 = static_cast<int>(blockIdx.x % tiles_m) * 8 + 4 * (wave & 1);  // in row blocks of 16
   const int n0 = static_cast<int>(blockIdx.x / tiles_m) * 8 + 4 * (wave >> 1);
-  const int mbs = (M + 15) >> 4, nbs = (N + 15) >> 4;
   v4f acc[4][4];
+  uint32_t sa[4], sb[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 4; ++i) {  // (one group of scales: KT < 4)
+    sa[i] = *reinterpret_cast<const uint32_t*>(a.xs + ((int64_t)min(m0 + i, a.mbs - 1) * 64 + lane) * 4);
+    sb[i] = *reinterpret_cast<const uint32_t*>(a.ws + ((int64_t)min(n0 + i, a.nbs - 1) * 64 + lane) * 4);
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < groups; ++s) {
-    uint32_t sa[4], sb[4];
+  }
+  for (int t = 0; t < a.KT; ++t) {
+    v8i x[4], w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      sa[i] = *reinterpret_cast<const uint32_t*>(xs + (((int64_t)min(m0 + i, mbs - 1) * groups + s) * 64 + lane) * 4);
-      sb[i] = *reinterpret_cast<const uint32_t*>(ws + (((int64_t)min(n0 + i, nbs - 1) * groups + s) * 64 + lane) * 4);
+      const uint8_t* p = a.x + (((int64_t)min(m0 + i, a.mbs - 1) * a.KT + t) * (64 * AB) + lane) * 16;
+      x[i] = pack_v8i(ld16(p), AB == 2 ? ld16(p + 1024) : zero4());
+      w[i] = pack_v8i(ld16(a.w + (((int64_t)min(n0 + i, a.nbs - 1) * a.KT + t) * 64 + lane) * 16), zero4());
     }
-    for (int t = 0; t < min(4, KT - 4 * s); ++t) {
-      v8i a[4], b[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint8_t* p = x + (((int64_t)min(m0 + i, mbs - 1) * KT + 4 * s + t) * (64 * AB) + lane) * 16;
-        a[i] = pack_v8i(ld16(p), AB == 2 ? ld16(p + 1024) : zero4());
-        b[i] = pack_v8i(ld16(w + (((int64_t)min(n0 + i, nbs - 1) * KT + 4 * s + t) * 64 + lane) * 16), zero4());
-      }
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[i], b[j], acc[i][j], fa, 4, 0,
-                                                                       static_cast<int>(sa[i] >> (8 * t)), 0,
-                                                                       static_cast<int>(sb[j] >> (8 * t)));
-    }
+      for (int j = 0; j < 4; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x[i], w[j], acc[i][j], ELEM == KRQ_MX_E2M1 ? 4 : 0, 4, 0,
+                                                                     static_cast<int>(sa[i] >> (8 * t)), 0,
+                                                                     static_cast<int>(sb[j] >> (8 * t)));
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -55,29 +398,139 @@ __global__ __launch_bounds__(256) void k_gemm_mx(const uint8_t* __restrict__ x, 
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int64_t m = 16 * (m0 + i) + 4 * (lane >> 4) + e, n = 16 * (n0 + j) + (lane & 15);
-        if (m < M && n < N) out[m * N + n] = f32_to_bf16(acc[i][j][e]);
+        if (m < a.M && n < a.N) a.out[m * a.N + n] = f32_to_bf16(acc[i][j][e]);
       }
+}
+
+// out[m][n] = bf16(sum over s of part[s][m][n], s in order), V columns per thread
+template <int V>
+__global__ __launch_bounds__(256) void k_gemm_mx_reduce(const float* __restrict__ part, int splits, int64_t plane,
+                                                        uint16_t* __restrict__ out) {
+  const int64_t e = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * V;
+  if (e >= plane) return;
+  if constexpr (V == 4) {
+    float4 v = *reinterpret_cast<const float4*>(part + e);
+    for (int s = 1; s < splits; ++s) {
+      const float4 o = *reinterpret_cast<const float4*>(part + s * plane + e);
+      v.x += o.x;
+      v.y += o.y;
+      v.z += o.z;
+      v.w += o.w;
+    }
+    *reinterpret_cast<uint2*>(out + e) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+  } else {
+    float v = part[e];
+    for (int s = 1; s < splits; ++s) v += part[s * plane + e];
+    out[e] = f32_to_bf16(v);
+  }
+}
+
+struct GemmPlan {
+  int bm, splits;
+};
+
+// The output tile and the parts of K.
+GemmPlan plan_of(int64_t M, int64_t N, int64_t KT, int cus) {
+  auto tiles = [&](int64_t b) { return (M + b - 1) / b * ((N + b - 1) / b); };
+  if (tiles(256) >= cus / 2) return {256, 1};
+  if (tiles(128) >= cus / 2) return {128, 1};
+  int splits = 1;
+  while (splits < 8 && tiles(64) * splits * 2 <= 2 * cus && KT / (2 * splits) >= 8) splits *= 2;
+  return {64, splits};
+}
+
+int cu_count(int* cus) {
+  int dev = 0;
+  return hipGetDevice(&dev) == hipSuccess &&
+                 hipDeviceGetAttribute(cus, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && *cus > 0
+             ? KRQ_OK
+             : KRQ_EHIP;
+}
+
+template <int ELEM, int BM, int W, int OCC, int NB, bool PART>
+void launch(const GemmArgs& g, int cus, hipStream_t s) {
+  GemmArgs a = g;
+  a.tiles_m = (a.M + BM - 1) / BM;
+  a.tiles = a.tiles_m * ((a.N + BM - 1) / BM);
+  const int64_t units = (int64_t)a.tiles * a.splits, slots = (int64_t)cus * OCC;
+  hipLaunchKernelGGL((k_gemm_mx<ELEM, BM, BM, W, OCC, NB, PART>), dim3(static_cast<unsigned>(std::min(units, slots))), dim3(64 * W),
+                     0, s, a);
+}
+
+template <int ELEM>
+void launch_plan(const GemmArgs& a, const GemmPlan& p, int cus, hipStream_t s) {
+  constexpr int D = ELEM == KRQ_MX_E2M1 ? 1 : 0;  // e2m1 stages are shorter: one buffer more
+  if (a.KT < kMinStages) {
+    const int tm = (a.M + 127) / 128;
+    hipLaunchKernelGGL((k_gemm_mx_short<ELEM>), dim3(static_cast<unsigned>(tm * ((a.N + 127) / 128))), dim3(256), 0, s, a, tm);
+  } else if (p.bm == 256) launch<ELEM, 256, 8, 1, 2 + D, false>(a, cus, s);
+  else if (p.bm == 128) launch<ELEM, 128, 4, 2, 2 + D, false>(a, cus, s);
+  else if (p.splits == 1) launch<ELEM, 64, 4, 2, 4, false>(a, cus, s);
+  else launch<ELEM, 64, 4, 2, 4, true>(a, cus, s);
 }
 
 }  // namespace
 
-extern "C" int krq_gemm_mxfp4(const void* x_tiled, const void* x_scale, int elem, const void* w_tiled, const void* w_scale,
-                              int64_t M, int64_t N, int64_t K, void* out, void* stream) {
-  KRQ_REQUIRE(x_tiled && x_scale && w_tiled && w_scale && out, "gemm_mxfp4: null pointer");
+extern "C" int64_t krq_gemm_mxfp4_ws_bytes(int x_kind, int elem, int64_t M, int64_t N, int64_t K) {
+  if (M < 1 || N < 1 || K < 1 || K % kMxBlock != 0 || (elem != KRQ_MX_E2M1 && elem != KRQ_MX_E4M3)) return -1;
+  int cus = 0;
+  if (cu_count(&cus) != KRQ_OK) return -1;
+  const GemmPlan p = plan_of(M, N, mx_tiles(K), cus);
+  return (x_kind == KRQ_MX_X_BF16 ? mx_rows_bytes(elem, M, K) : 0) + (p.splits > 1 ? p.splits * M * N * 4 : 0);
+}
+
+extern "C" int krq_gemm_mxfp4(const void* x, const void* x_scale, int x_kind, int elem, int64_t ldx, const void* w_tiled,
+                              const void* w_scale, int64_t M, int64_t N, int64_t K, void* ws, int64_t ws_bytes, void* out,
+                              void* stream) {
+  KRQ_REQUIRE(x && w_tiled && w_scale && out, "gemm_mxfp4: null pointer");
   KRQ_REQUIRE(elem == KRQ_MX_E2M1 || elem == KRQ_MX_E4M3, "gemm_mxfp4: bad element type %d", elem);
-  KRQ_REQUIRE(aligned16(x_tiled) && aligned16(w_tiled), "gemm_mxfp4: x and w must start on 16 bytes");
-  KRQ_REQUIRE(M >= 1 && M <= 0x3fffffff && N >= 1 && N <= 0x3fffffff && K >= kMxBlock && K % kMxBlock == 0 && K <= 0x3fffffff,
-              "gemm_mxfp4: shape M=%lld N=%lld K=%lld (K a multiple of 32)", (long long)M, (long long)N, (long long)K);
-  const int64_t tiles_m = (M + 127) / 128, blocks = tiles_m * ((N + 127) / 128);
-  KRQ_REQUIRE(blocks <= 0xffffff, "gemm_mxfp4: M=%lld N=%lld are too large", (long long)M, (long long)N);
-  const dim3 grid(static_cast<unsigned>(blocks));
-  if (elem == KRQ_MX_E2M1)
-    hipLaunchKernelGGL((k_gemm_mx<KRQ_MX_E2M1>), grid, dim3(256), 0, (hipStream_t)stream, (const uint8_t*)x_tiled,
-                       (const uint8_t*)x_scale, (const uint8_t*)w_tiled, (const uint8_t*)w_scale, (int)M, (int)N,
-                       (int)mx_tiles(K), (int)mx_groups(K), (int)tiles_m, (uint16_t*)out);
-  else
-    hipLaunchKernelGGL((k_gemm_mx<KRQ_MX_E4M3>), grid, dim3(256), 0, (hipStream_t)stream, (const uint8_t*)x_tiled,
-                       (const uint8_t*)x_scale, (const uint8_t*)w_tiled, (const uint8_t*)w_scale, (int)M, (int)N,
-                       (int)mx_tiles(K), (int)mx_groups(K), (int)tiles_m, (uint16_t*)out);
+  KRQ_REQUIRE(x_kind == KRQ_MX_X_BF16 || x_kind == KRQ_MX_X_TILED, "gemm_mxfp4: bad x_kind %d", x_kind);
+  KRQ_REQUIRE(x_kind == KRQ_MX_X_BF16 || x_scale, "gemm_mxfp4: tiled rows need their scales");
+  KRQ_REQUIRE(aligned16(x) && aligned16(w_tiled) && aligned16(ws), "gemm_mxfp4: x, w and ws must start on 16 bytes");
+  KRQ_REQUIRE(M >= 1 && M <= 0x3fffffff && N >= 1 && N <= 0x3fffffff && K >= kMxBlock && K % kMxBlock == 0 && K <= (1 << 22),
+              "gemm_mxfp4: shape M=%lld N=%lld K=%lld (K a multiple of 32, at most 2^22)", (long long)M, (long long)N, (long long)K);
+  KRQ_REQUIRE(((M + 63) / 64) * ((N + 63) / 64) <= 0x0fffffff, "gemm_mxfp4: M=%lld N=%lld are too large", (long long)M, (long long)N);
+  int cus = 0;
+  if (cu_count(&cus) != KRQ_OK) {
+    krq_set_error("gemm_mxfp4: device query failed");
+    return KRQ_EHIP;
+  }
+  GemmPlan p = plan_of(M, N, mx_tiles(K), cus);
+  const int64_t rows = (x_kind == KRQ_MX_X_BF16 ? mx_rows_bytes(elem, M, K) : 0);
+  KRQ_REQUIRE(rows == 0 || (ws && ws_bytes >= rows), "gemm_mxfp4: bf16 rows need a workspace of %lld bytes", (long long)rows);
+  if (p.splits > 1 && (!ws || ws_bytes < rows + p.splits * M * N * 4)) p.splits = 1;
+  GemmArgs a;
+  if (rows) {
+    a.x = (const uint8_t*)ws;
+    a.xs = (const uint8_t*)ws + mx_rows_scale_at(elem, M, K);
+    if (const int rc = krq_quant_mx_rows(x, M, K, ldx, elem, ws, (uint8_t*)ws + mx_rows_scale_at(elem, M, K), stream)) return rc;
+  } else {
+    a.x = (const uint8_t*)x;
+    a.xs = (const uint8_t*)x_scale;
+  }
+  a.w = (const uint8_t*)w_tiled;
+  a.ws = (const uint8_t*)w_scale;
+  a.M = static_cast<int>(M);
+  a.N = static_cast<int>(N);
+  a.KT = static_cast<int>(mx_tiles(K));
+  a.groups = static_cast<int>(mx_groups(K));
+  a.mbs = static_cast<int>((M + 15) / 16);
+  a.nbs = static_cast<int>((N + 15) / 16);
+  a.splits = p.splits;
+  a.wide = N % 8 == 0 && aligned16(out);
+  a.part = (float*)((uint8_t*)ws + rows);
+  a.out = (uint16_t*)out;
+  hipStream_t s = (hipStream_t)stream;
+  if (elem == KRQ_MX_E2M1) launch_plan<KRQ_MX_E2M1>(a, p, cus, s);
+  else launch_plan<KRQ_MX_E4M3>(a, p, cus, s);
+  if (p.splits > 1) {
+    const int64_t plane = M * N;
+    if (plane % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0)
+      hipLaunchKernelGGL(k_gemm_mx_reduce<4>, dim3(static_cast<unsigned>((plane / 4 + 255) / 256)), dim3(256), 0, s, a.part, p.splits,
+                         plane, a.out);
+    else
+      hipLaunchKernelGGL(k_gemm_mx_reduce<1>, dim3(static_cast<unsigned>((plane + 255) / 256)), dim3(256), 0, s, a.part, p.splits,
+                         plane, a.out);
+  }
   return krq_check_launch("gemm_mxfp4");
 }

@@ -247,24 +247,32 @@ void launch_rows(const MxArgs& a, bool bf16, int blocks, int splits, int nw, hip
 namespace krq {
 
 // The checks and the launch of every product on MXFP4 weights of at most 32 rows (kOutArgmax: the head's).
-int gemv_mx_run(const char* what, const void* x, const void* x_scale, int x_kind, int elem, int64_t ldx, const void* w, const void* w_scale, int64_t M,
-                int64_t N, int64_t K, int split, int mode, void* out, Best* cand, void* stream) {
+int gemv_mx_run(const char* what, const void* x, const void* x_scale, int x_kind, int elem, int64_t ldx, const void* w,
+                const void* w_scale, int64_t M, int64_t N, int64_t K, int split, int mode, void* ws, int64_t ws_bytes, void* out,
+                Best* cand, void* stream) {
   KRQ_REQUIRE(x && w && w_scale && (out || mode == kOutArgmax), "%s: null pointer", what);
   KRQ_REQUIRE(elem == KRQ_MX_E2M1 || elem == KRQ_MX_E4M3, "%s: bad element type %d", what, elem);
   KRQ_REQUIRE(x_kind == KRQ_MX_X_BF16 || x_kind == KRQ_MX_X_TILED, "%s: bad x_kind %d", what, x_kind);
   KRQ_REQUIRE(M >= 1 && M <= 32, "%s: M=%lld outside 1..32", what, (long long)M);
   KRQ_REQUIRE(N >= 1 && N <= 0x7fffffff - 64 && K >= kMxBlock && K % kMxBlock == 0 && K <= 0x3fffffff, "%s: shape N=%lld K=%lld (K a multiple of 32)", what,
               (long long)N, (long long)K);
-  const bool bf16 = x_kind == KRQ_MX_X_BF16;
-  KRQ_REQUIRE(bf16 || x_scale, "%s: tiled rows need their scales", what);
-  KRQ_REQUIRE(!bf16 || (M <= KRQ_MX_BF16_ROWS && ldx >= K && ldx % 8 == 0),
-              "%s: at most %d bf16 rows, each on 16 bytes (M=%lld, ldx=%lld)", what, KRQ_MX_BF16_ROWS, (long long)M, (long long)ldx);
-  KRQ_REQUIRE(aligned16(x) && aligned16(w), "%s: x and w must start on 16 bytes", what);
+  const bool bf16 = x_kind == KRQ_MX_X_BF16 && M <= KRQ_MX_BF16_ROWS;  // rounded in the kernel
+  const int64_t rows = x_kind == KRQ_MX_X_BF16 && !bf16 ? mx_rows_bytes(elem, M, K) : 0;
+  KRQ_REQUIRE(x_kind == KRQ_MX_X_BF16 || x_scale, "%s: tiled rows need their scales", what);
+  KRQ_REQUIRE(x_kind != KRQ_MX_X_BF16 || (ldx >= K && ldx % 8 == 0), "%s: rows of x must start on 16 bytes (ldx=%lld)", what, (long long)ldx);
+  KRQ_REQUIRE(aligned16(x) && aligned16(w) && aligned16(ws), "%s: x, w and ws must start on 16 bytes", what);
+  KRQ_REQUIRE(rows == 0 || (ws && ws_bytes >= rows), "%s: bf16 rows need a workspace of %lld bytes", what, (long long)rows);
   const int groups = static_cast<int>(mx_groups(K));
   KRQ_REQUIRE(split >= 1 && split <= groups && split <= kMxSplitMax, "%s: split=%d of %d groups of 512", what, split, groups);
   KRQ_REQUIRE(split == 1 || mode == KRQ_OUT_PARTIAL, "%s: split=%d needs the partials output", what, split);
   const bool swiglu = mode == KRQ_OUT_SWIGLU;
   KRQ_REQUIRE(!swiglu || N % 32 == 0, "%s: SwiGLU needs N=%lld = 2 I with I %% 16 == 0", what, (long long)N);
+  if (rows) {
+    uint8_t* sc = (uint8_t*)ws + mx_rows_scale_at(elem, M, K);
+    if (const int rc = krq_quant_mx_rows(x, M, K, ldx, elem, ws, sc, stream)) return rc;
+    x = ws;
+    x_scale = sc;
+  }
   MxArgs a;
   a.x = (const uint8_t*)x;
   a.xs = (const uint8_t*)x_scale;
@@ -299,8 +307,15 @@ int gemv_mx_run(const char* what, const void* x, const void* x_scale, int x_kind
 
 }  // namespace krq
 
+extern "C" int64_t krq_gemv_mxfp4_ws_bytes(int x_kind, int elem, int64_t M, int64_t K) {
+  if (M < 1 || M > 32 || K < 1 || (elem != KRQ_MX_E2M1 && elem != KRQ_MX_E4M3)) return -1;
+  return x_kind == KRQ_MX_X_BF16 && M > KRQ_MX_BF16_ROWS ? mx_rows_bytes(elem, M, K) : 0;
+}
+
 extern "C" int krq_gemv_mxfp4(const void* x, const void* x_scale, int x_kind, int elem, int64_t ldx, const void* w_tiled,
-                              const void* w_scale, int64_t M, int64_t N, int64_t K, int split, int mode, void* out, void* stream) {
+                              const void* w_scale, int64_t M, int64_t N, int64_t K, int split, int mode, void* ws, int64_t ws_bytes,
+                              void* out, void* stream) {
   KRQ_REQUIRE(mode == KRQ_OUT_BF16 || mode == KRQ_OUT_PARTIAL || mode == KRQ_OUT_SWIGLU, "gemv_mxfp4: bad mode %d", mode);
-  return gemv_mx_run("gemv_mxfp4", x, x_scale, x_kind, elem, ldx, w_tiled, w_scale, M, N, K, split, mode, out, nullptr, stream);
+  return gemv_mx_run("gemv_mxfp4", x, x_scale, x_kind, elem, ldx, w_tiled, w_scale, M, N, K, split, mode, ws, ws_bytes, out, nullptr,
+                     stream);
 }

@@ -82,9 +82,14 @@ KRQ_DEV uint2 mx_quant8_e4m3(uint4 v, uint32_t c) {
   return make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
 }
 
+// Rows rounded into a workspace: elements, then scales, each on 256 bytes.
+inline int64_t mx_rows_scale_at(int elem, int64_t M, int64_t K) { return (krq_mx_tiled_bytes(M, K, elem) + 255) & ~(int64_t)255; }
+inline int64_t mx_rows_bytes(int elem, int64_t M, int64_t K) { return mx_rows_scale_at(elem, M, K) + krq_mx_scale_bytes(M, K); }
+
 // The checks and the launch of every product on MXFP4 weights of at most 32 rows (gemv_mxfp4.hip; kOutArgmax:
 // the lm head's, its candidates to cand).
 int gemv_mx_run(const char* what, const void* x, const void* x_scale, int x_kind, int elem, int64_t ldx, const void* w,
-                const void* w_scale, int64_t M, int64_t N, int64_t K, int split, int mode, void* out, Best* cand, void* stream);
+                const void* w_scale, int64_t M, int64_t N, int64_t K, int split, int mode, void* ws, int64_t ws_bytes, void* out,
+                Best* cand, void* stream);
 
 }  // namespace krq

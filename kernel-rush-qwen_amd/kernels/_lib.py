@@ -80,8 +80,12 @@ EXPORTS = {
     "krq_quant_mx_rows": (_i32, [_vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp]),
     "krq_dequant_mx": (_i32, [_vp, _vp, _i32, _i64, _i64, _vp, _vp]),
     "krq_embed_mxfp4": (_i32, [_vp, _i32, _i64, _vp, _vp, _i64, _i64, _f32, _vp, _vp]),
-    "krq_gemv_mxfp4": (_i32, [_vp, _vp, _i32, _i32, _i64, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp, _vp]),
-    "krq_gemm_mxfp4": (_i32, [_vp, _vp, _i32, _vp, _vp, _i64, _i64, _i64, _vp, _vp]),
+    "krq_gemv_mxfp4": (_i32, [_vp, _vp, _i32, _i32, _i64, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp, _i64, _vp,
+                              _vp]),
+    "krq_gemv_mxfp4_ws_bytes": (_i64, [_i32, _i32, _i64, _i64]),
+    "krq_gemm_mxfp4": (_i32, [_vp, _vp, _i32, _i32, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "krq_gemm_mxfp4_ws_bytes": (_i64, [_i32, _i32, _i64, _i64, _i64]),
+    "krq_lmhead_mxfp4_ws_bytes": (_i64, [_i32, _i32, _i64, _i64, _i64]),
     "krq_lmhead_argmax_mxfp4": (_i32, [_vp, _vp, _i32, _i32, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp,
                                        _vp]),
     "krq_version": (ctypes.c_char_p, []),

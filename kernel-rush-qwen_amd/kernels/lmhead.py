@@ -61,22 +61,15 @@ def _fp8_operands(h, w, a, h_layout):
 
 
 def _mxfp4_head(h, q, return_logits):
+    t, p, scale, kind, e, ld, M = _mxfp4._operand(h, q, "e4m3")
     V, K = q.shape
-    h = _mxfp4._bf16_rows(h, "rows [M, K]")
-    M = h.shape[0]
-    if h.shape[1] != K or M < 1:
-        raise ValueError(f"h {tuple(h.shape)} and w [{V}, {K}] do not match")
-    _mxfp4._same_device(h, q.tiled)
-    idx = torch.empty((M,), device=h.device, dtype=torch.int64)
-    logits = torch.empty((M, V), device=h.device, dtype=torch.bfloat16) if return_logits else None
-    ws = torch.empty((int(L.lib().krq_lmhead_ws_bytes(M, V)),), device=h.device, dtype=torch.uint8)
-    if M <= L.MX_BF16_ROWS:
-        xin, xs, kind, ld = h, None, L.MX_X_BF16, _mxfp4._ld(h)
-    else:
-        rows = _mxfp4.quant_rows(h)
-        xin, xs, kind, ld = rows.tiled, rows.tiled_scale, L.MX_X_TILED, 0
-    _mxfp4._call(h, "krq_lmhead_argmax_mxfp4", L.ptr(xin), L.ptr(xs), kind, L.MX_E4M3, ld, L.ptr(q.tiled), L.ptr(q.tiled_scale),
-                 M, V, K, L.ptr(logits), L.ptr(ws), ws.numel(), L.ptr(idx))
+    if M < 1:
+        raise ValueError("lm_head_argmax: no rows")
+    idx = t.new_empty((M,), dtype=torch.int64)
+    logits = t.new_empty((M, V), dtype=torch.bfloat16) if return_logits else None
+    ws = t.new_empty((L.lib().krq_lmhead_mxfp4_ws_bytes(kind, e, M, V, K),), dtype=torch.uint8)
+    _mxfp4._call(t, "krq_lmhead_argmax_mxfp4", p, scale, kind, e, ld, q.tiled.data_ptr(), q.tiled_scale.data_ptr(), M, V, K,
+                 L.ptr(logits), ws.data_ptr(), ws.numel(), idx.data_ptr())
     return (idx, logits) if return_logits else idx
 
 

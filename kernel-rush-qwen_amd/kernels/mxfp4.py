@@ -13,6 +13,8 @@ The kernels read operands in the tiled layout of include/krq.h ("mx tiled"). K i
 are any.
 """
 
+import contextlib
+
 import torch
 
 from . import _lib as L
@@ -20,6 +22,7 @@ from . import _lib as L
 ELEMS = {"e2m1": L.MX_E2M1, "e4m3": L.MX_E4M3}
 DECODE_MAX_ROWS = 32  # rows of the skinny kernels
 BLOCK = 32
+_HERE = contextlib.nullcontext()
 
 
 class MXFP4Weight(tuple):
@@ -35,10 +38,21 @@ class MXFP4Weight(tuple):
 
 
 class MXRows:
-    """Activation rows [M, K] in MX blocks of `elem`, tiled (quant_rows)."""
+    """Activation rows [M, K] in MX blocks of `elem`, tiled (quant_rows): `data` uint8, the elements, then
+    from byte scale_at the scales."""
 
-    def __init__(self, tiled, tiled_scale, shape, elem):
-        self.tiled, self.tiled_scale, self.shape, self.elem = tiled, tiled_scale, shape, elem
+    __slots__ = ("data", "scale_at", "shape", "elem")
+
+    def __init__(self, data, scale_at, shape, elem):
+        self.data, self.scale_at, self.shape, self.elem = data, scale_at, shape, elem
+
+    @property
+    def tiled(self):
+        return self.data[:L.lib().krq_mx_tiled_bytes(*self.shape, ELEMS[self.elem])]
+
+    @property
+    def tiled_scale(self):
+        return self.data[self.scale_at:]
 
 
 def _elem(elem):
@@ -47,18 +61,14 @@ def _elem(elem):
     return ELEMS[elem]
 
 
-def _on(t):
-    """t's device is made current for the launch where it is not (its stream belongs to it)."""
-    return torch.cuda.device(t.device)
-
-
 def _call(t, name, *args):
-    L_args = args + (L.stream(t),)
-    if t.get_device() == torch.cuda.current_device():
-        L.call(name, *L_args)
+    """L.call on t's device and torch's current stream of it."""
+    dev = t.get_device()
+    if dev == torch._C._cuda_getDevice():
+        L.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
     else:
-        with _on(t):
-            L.call(name, *L_args)
+        with torch.cuda.device(dev):
+            L.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
 
 
 def _same_device(first, *tensors):
@@ -69,20 +79,23 @@ def _same_device(first, *tensors):
 
 
 def _bf16_rows(x, what):
-    """x [M, K] bf16 as the kernels read it: contiguous rows that start on 16 bytes."""
-    L.require_device(x)
-    if x.dim() != 2 or x.dtype != torch.bfloat16:
+    """(x, row stride): x [M, K] bf16 as the kernels read it, rows of consecutive values that start on 16 bytes."""
+    if not x.is_cuda:
+        L.require_device(x)
+    if x.dtype != torch.bfloat16 or x.dim() != 2:
         raise ValueError(f"expected bf16 {what}, got {x.dtype} {tuple(x.shape)}")
     M, K = x.shape
     if K == 0 or K % BLOCK:
         raise ValueError(f"{what}: K={K} must be a positive multiple of {BLOCK}")
-    if x.stride(1) != 1 or (M > 1 and (x.stride(0) < K or x.stride(0) % 8)):
-        x = x.contiguous()
-    return x if x.data_ptr() % 16 == 0 else x.clone()
-
-
-def _ld(x):
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+    if x.is_contiguous():
+        ld = K
+    else:
+        ld, unit = x.stride()
+        if M == 1 and unit == 1:
+            ld = K
+        elif unit != 1 or ld < K or ld % 8:
+            x, ld = x.contiguous(), K
+    return (x if x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format), ld if x.data_ptr() % 16 == 0 else K)
 
 
 def _tiles(M, K, elem, device):
@@ -94,14 +107,14 @@ def _tiles(M, K, elem, device):
 @torch.no_grad()
 def quantize(w):
     """w [N, K] bf16 -> MXFP4Weight, w ~= e2m1 values times their blocks' scales. K % 32 == 0."""
-    w = _bf16_rows(w, "weight [N, K]")
+    w, ld = _bf16_rows(w, "weight [N, K]")
     N, K = w.shape
     if N == 0:
         raise ValueError("weight [N, K]: N must be positive")
     w4 = torch.empty((N, K // 2), device=w.device, dtype=torch.uint8)
     scale = torch.empty((N, K // BLOCK), device=w.device, dtype=torch.uint8)
     tiled, tscale = _tiles(N, K, L.MX_E2M1, w.device)
-    _call(w, "krq_quant_mxfp4", L.ptr(w), N, K, _ld(w), L.ptr(w4), L.ptr(scale), L.ptr(tiled), L.ptr(tscale))
+    _call(w, "krq_quant_mxfp4", L.ptr(w), N, K, ld, L.ptr(w4), L.ptr(scale), L.ptr(tiled), L.ptr(tscale))
     return MXFP4Weight(w4, scale, tiled, tscale)
 
 
@@ -132,61 +145,73 @@ def _weight(q):
 def dequantize(q):
     """The bf16 values an MXFP4Weight or MXRows stands for, [N, K] or [M, K] (its tiled copy's)."""
     if isinstance(q, MXRows):
-        (M, K), elem = q.shape, ELEMS[q.elem]
+        (M, K), elem, t = q.shape, ELEMS[q.elem], q.data
+        data = t.data_ptr()
+        scale = data + q.scale_at
     else:
-        (M, K), elem = _weight(q), L.MX_E2M1
-    out = torch.empty((M, K), device=q.tiled.device, dtype=torch.bfloat16)
+        (M, K), elem, t = _weight(q), L.MX_E2M1, q.tiled
+        data, scale = t.data_ptr(), q.tiled_scale.data_ptr()
+    out = t.new_empty((M, K), dtype=torch.bfloat16)
     if M:
-        _call(out, "krq_dequant_mx", L.ptr(q.tiled), L.ptr(q.tiled_scale), elem, M, K, L.ptr(out))
+        _call(out, "krq_dequant_mx", data, scale, elem, M, K, out.data_ptr())
     return out
 
 
 def quant_rows(x, elem="e4m3"):
     """x [M, K] bf16 -> MXRows: the rows rounded to MX blocks, in the layout the products read. Several
     products on the same rows can share them."""
-    x = _bf16_rows(x, "rows [M, K]")
+    x, ld = _bf16_rows(x, "rows [M, K]")
     M, K = x.shape
     e = _elem(elem)
     if M == 0:
-        none = torch.empty((0,), device=x.device, dtype=torch.uint8)
-        return MXRows(none, none, (0, K), elem)
-    tiled, tscale = _tiles(M, K, e, x.device)
-    _call(x, "krq_quant_mx_rows", L.ptr(x), M, K, _ld(x), e, L.ptr(tiled), L.ptr(tscale))
-    return MXRows(tiled, tscale, (M, K), elem)
+        return MXRows(x.new_empty((0,), dtype=torch.uint8), 0, (0, K), elem)
+    lib = L.lib()
+    at = lib.krq_mx_tiled_bytes(M, K, e)  # (whole KiB)
+    data = x.new_empty((at + lib.krq_mx_scale_bytes(M, K),), dtype=torch.uint8)
+    p = data.data_ptr()
+    _call(x, "krq_quant_mx_rows", x.data_ptr(), M, K, ld, e, p, p + at)
+    return MXRows(data, at, (M, K), elem)
+
+
+def _operand(x, q, elem):
+    """(the tensor that keeps x's memory, its address, its scales', x_kind, elem, row stride, M) of bf16 rows or MXRows."""
+    N, K = _weight(q)
+    if x.shape[-1] != K:
+        raise ValueError(f"x {tuple(x.shape)} and w [{N}, {K}] do not match")
+    if isinstance(x, MXRows):
+        t, (M, _), ld, kind, elem = x.data, x.shape, 0, L.MX_X_TILED, x.elem
+        scale = t.data_ptr() + x.scale_at
+    else:
+        t, ld = _bf16_rows(x, "rows [M, K]")
+        M, scale, kind = t.shape[0], None, L.MX_X_BF16
+    if t.get_device() != q.tiled.get_device():
+        _same_device(t, q.tiled)
+    return t, t.data_ptr(), scale, kind, _elem(elem), ld, M
 
 
 def _decode(x, q, split, mode, elem):
-    N, K = _weight(q)
-    if isinstance(x, MXRows):
-        rows = x
-    else:
-        x = _bf16_rows(x, "rows [M, K]")
-        rows = None
-    M, kx = x.shape
-    if kx != K:
-        raise ValueError(f"x [{M}, {kx}] and w [{N}, {K}] do not match")
+    t, p, scale, kind, e, ld, M = _operand(x, q, elem)
+    N, K = q.shape
     if M > DECODE_MAX_ROWS:
         raise ValueError(f"M={M} > {DECODE_MAX_ROWS} rows: use gemm_mxfp4 or linear_mxfp4")
-    if mode == L.OUT_SWIGLU and N % 32:
-        raise ValueError(f"SwiGLU needs w = [gate; up] of 2 I rows with I a multiple of 16, got N={N}")
-    e = _elem(elem)
-    dev = q.tiled.device
     if mode == L.OUT_PARTIAL:
-        out = torch.empty((split, M, N), device=dev, dtype=torch.float32)
+        if split < 1:
+            raise ValueError(f"split={split}")
+        out = t.new_empty((split, M, N), dtype=torch.float32)
+    elif mode == L.OUT_SWIGLU:
+        if N % 32:
+            raise ValueError(f"SwiGLU needs w = [gate; up] of 2 I rows with I a multiple of 16, got N={N}")
+        out = t.new_empty((M, N // 2), dtype=torch.bfloat16)
     else:
-        out = torch.empty((M, N // 2 if mode == L.OUT_SWIGLU else N), device=dev, dtype=torch.bfloat16)
+        out = t.new_empty((M, N), dtype=torch.bfloat16)
     if M == 0:
         return out
-    if rows is None and M > L.MX_BF16_ROWS:
-        rows = quant_rows(x, elem)
-    if rows is None:
-        _same_device(x, q.tiled)
-        _call(x, "krq_gemv_mxfp4", L.ptr(x), None, L.MX_X_BF16, e, _ld(x), L.ptr(q.tiled), L.ptr(q.tiled_scale), M, N, K,
-              split, mode, L.ptr(out))
-    else:
-        _same_device(rows.tiled, q.tiled)
-        _call(out, "krq_gemv_mxfp4", L.ptr(rows.tiled), L.ptr(rows.tiled_scale), L.MX_X_TILED, ELEMS[rows.elem], 0,
-              L.ptr(q.tiled), L.ptr(q.tiled_scale), M, N, K, split, mode, L.ptr(out))
+    ws, nbytes = None, 0
+    if kind == L.MX_X_BF16 and M > L.MX_BF16_ROWS:
+        nbytes = L.lib().krq_gemv_mxfp4_ws_bytes(kind, e, M, K)
+        ws = t.new_empty((nbytes,), dtype=torch.uint8)
+    _call(out, "krq_gemv_mxfp4", p, scale, kind, e, ld, q.tiled.data_ptr(), q.tiled_scale.data_ptr(), M, N, K, split, mode,
+          L.ptr(ws), nbytes, out.data_ptr())
     return out
 
 
@@ -206,24 +231,26 @@ def gemv_swiglu_mxfp4(x, q, elem="e4m3"):
 
 
 def gemm_mxfp4(x, q, elem="e4m3"):
-    """MXFP4 prefill product: x [M, K] bf16 (rounded to blocks of elem by quant_rows) or MXRows, any M;
-    q an MXFP4Weight [N, K]. Returns bf16 [M, N]."""
-    N, K = _weight(q)
-    if x.shape[1] != K:
-        raise ValueError(f"x {tuple(x.shape)} and w [{N}, {K}] do not match")
-    rows = x if isinstance(x, MXRows) else quant_rows(x, elem)
-    M = rows.shape[0]
-    _same_device(rows.tiled, q.tiled)
-    out = torch.empty((M, N), device=q.tiled.device, dtype=torch.bfloat16)
-    if M:
-        _call(out, "krq_gemm_mxfp4", L.ptr(rows.tiled), L.ptr(rows.tiled_scale), ELEMS[rows.elem], L.ptr(q.tiled),
-              L.ptr(q.tiled_scale), M, N, K, L.ptr(out))
+    """MXFP4 prefill product: x [M, K] bf16 (rounded to blocks of elem by a launch before the product's) or
+    MXRows, any M; q an MXFP4Weight [N, K]. Returns bf16 [M, N]."""
+    t, p, scale, kind, e, ld, M = _operand(x, q, elem)
+    N, K = q.shape
+    out = t.new_empty((M, N), dtype=torch.bfloat16)
+    if M == 0:
+        return out
+    with torch.cuda.device(t.get_device()) if t.get_device() != torch._C._cuda_getDevice() else _HERE:
+        nbytes = L.lib().krq_gemm_mxfp4_ws_bytes(kind, e, M, N, K)
+    if nbytes < 0:
+        raise RuntimeError("krq_gemm_mxfp4_ws_bytes: device query failed")
+    ws = t.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
+    _call(out, "krq_gemm_mxfp4", p, scale, kind, e, ld, q.tiled.data_ptr(), q.tiled_scale.data_ptr(), M, N, K, L.ptr(ws), nbytes,
+          out.data_ptr())
     return out
 
 
 def linear_mxfp4(x, q, elem="e4m3"):
     """bf16 [M, N] ~= x @ W^T on q = quantize(W): gemv_mxfp4 up to 32 rows, gemm_mxfp4 from 33."""
-    return gemv_mxfp4(x, q, 1, elem) if x.shape[0] <= DECODE_MAX_ROWS else gemm_mxfp4(x, q, elem)
+    return _decode(x, q, 1, L.OUT_BF16, elem) if x.shape[0] <= DECODE_MAX_ROWS else gemm_mxfp4(x, q, elem)
 
 
 def embedding(ids, q, scale=1.0):
@@ -233,10 +260,12 @@ def embedding(ids, q, scale=1.0):
     N, K = _weight(q)
     if ids.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"ids must be int64 or int32, got {ids.dtype}")
-    _same_device(ids, q[0])
+    w4, scale_codes = q
+    _same_device(ids, w4)
     ids = ids.contiguous()
-    out = torch.empty((*ids.shape, K), device=ids.device, dtype=torch.bfloat16)
-    if ids.numel():
-        _call(ids, "krq_embed_mxfp4", L.ptr(ids), int(ids.dtype == torch.int64), ids.numel(), L.ptr(q[0]), L.ptr(q[1]), N, K,
-              float(scale), L.ptr(out))
+    out = w4.new_empty((*ids.shape, K), dtype=torch.bfloat16)
+    n = ids.numel()
+    if n:
+        _call(out, "krq_embed_mxfp4", ids.data_ptr(), int(ids.dtype == torch.int64), n, w4.data_ptr(), scale_codes.data_ptr(), N, K,
+              scale, out.data_ptr())
     return out

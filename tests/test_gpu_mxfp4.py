@@ -242,8 +242,8 @@ def test_outputs_end_where_they_should(dev):
     for name, extra in (("krq_gemv_mxfp4", True), ("krq_gemm_mxfp4", False)):
         out = torch.full((M + 16, N), 7.0, device=dev, dtype=torch.bfloat16)
         tail = (1, L.OUT_BF16) if extra else ()
-        head = (L.ptr(rows.tiled), L.ptr(rows.tiled_scale)) + ((L.MX_X_TILED, L.MX_E4M3, 0) if extra else (L.MX_E4M3,))
-        L.call(name, *head, L.ptr(q.tiled), L.ptr(q.tiled_scale), M, N, K, *tail, L.ptr(out), L.stream(x))
+        L.call(name, L.ptr(rows.tiled), L.ptr(rows.tiled_scale), L.MX_X_TILED, L.MX_E4M3, 0, L.ptr(q.tiled), L.ptr(q.tiled_scale),
+               M, N, K, *tail, None, 0, L.ptr(out), L.stream(x))
         check(out[:M], ref, E, name)
         assert out[M:].eq(7).all()
 

@@ -120,8 +120,8 @@ def test_c_entry_points_refuse_before_any_launch():
     refuse("krq_embed_mxfp4", b"indices", p, 1, 0, p, p, 16, 64, 1.0, p, z)
     refuse("krq_embed_mxfp4", b"indices", p, 1, 1 << 40, p, p, 16, 64, 1.0, p, z)
     refuse("krq_embed_mxfp4", b"multiple of 32", p, 1, 4, p, p, 16, 40, 1.0, p, z)
-    gemv = lambda needle, x=p, xs=p, kind=1, elem=1, ld=0, w=p, M=4, N=64, K=1024, split=1, mode=0, out=p: refuse(
-        "krq_gemv_mxfp4", needle, x, xs, kind, elem, ld, w, p, M, N, K, split, mode, out, z)
+    gemv = lambda needle, x=p, xs=p, kind=1, elem=1, ld=0, w=p, M=4, N=64, K=1024, split=1, mode=0, ws=z, nb=0, out=p: refuse(
+        "krq_gemv_mxfp4", needle, x, xs, kind, elem, ld, w, p, M, N, K, split, mode, ws, nb, out, z)
     gemv(b"null", x=z)
     gemv(b"null", out=z)
     gemv(b"element type", elem=3)
@@ -132,7 +132,10 @@ def test_c_entry_points_refuse_before_any_launch():
     gemv(b"N=0", N=0)
     gemv(b"their scales", xs=z)
     gemv(b"bf16 rows", kind=0, M=9, ld=1024)
-    gemv(b"bf16 rows", kind=0, ld=1000)
+    gemv(b"bf16 rows", kind=0, M=9, ld=1024, ws=p, nb=100)
+    gemv(b"16 bytes", kind=0, ld=1000)
+    gemv(b"16 bytes", kind=0, ld=1028)
+    gemv(b"16 bytes", ws=odd)
     gemv(b"16 bytes", x=odd)
     gemv(b"16 bytes", w=odd)
     gemv(b"split=3 of 2", split=3, mode=1)
@@ -140,20 +143,30 @@ def test_c_entry_points_refuse_before_any_launch():
     gemv(b"partials", split=2)
     gemv(b"I % 16", mode=2, N=48)
     gemv(b"bad mode", mode=3)
-    gemm = lambda needle, x=p, elem=1, w=p, M=40, N=64, K=1024, out=p: refuse("krq_gemm_mxfp4", needle, x, p, elem, w, p, M, N, K, out, z)
+    gemm = lambda needle, x=p, xs=p, kind=1, elem=1, ld=1024, w=p, M=40, N=64, K=1024, ws=z, nb=0, out=p: refuse(
+        "krq_gemm_mxfp4", needle, x, xs, kind, elem, ld, w, p, M, N, K, ws, nb, out, z)
     gemm(b"null", out=z)
     gemm(b"element type", elem=2)
+    gemm(b"x_kind", kind=-1)
+    gemm(b"their scales", xs=z)
     gemm(b"16 bytes", x=odd)
+    gemm(b"16 bytes", ws=odd)
     gemm(b"multiple of 32", K=16)
+    gemm(b"at most 2^22", K=(1 << 22) + 32)
     gemm(b"M=0", M=0)
     gemm(b"too large", M=0x3fffffff, N=0x3fffffff)
-    head = lambda needle, V=1024, M=1, ws=p, nb=1 << 20, idx=p: refuse("krq_lmhead_argmax_mxfp4", needle, p, z, 0, 1, 64, p, p, M, V, 64, z, ws, nb,
-                                                                    idx, z)
+    head = lambda needle, V=1024, M=1, ws=p, nb=1 << 20, idx=p: refuse(
+        "krq_lmhead_argmax_mxfp4", needle, p, z, 0, 1, 64, p, p, M, V, 64, z, ws, nb, idx, z)
     head(b"null", ws=z)
     head(b"null", idx=z)
     head(b"multiple of 16", V=1000)
     head(b"workspace", nb=8)
     head(b"workspace", M=33)
+    lib = L.lib()
+    assert lib.krq_gemv_mxfp4_ws_bytes(0, 1, 8, 64) == lib.krq_gemv_mxfp4_ws_bytes(1, 1, 32, 64) == 0
+    assert lib.krq_gemv_mxfp4_ws_bytes(0, 1, 9, 64) == 2048 + 256 and lib.krq_gemv_mxfp4_ws_bytes(0, 0, 32, 64) == 2 * 1024 + 512
+    assert lib.krq_gemv_mxfp4_ws_bytes(0, 1, 33, 64) == lib.krq_gemm_mxfp4_ws_bytes(0, 3, 40, 64, 64) == -1
+    assert lib.krq_lmhead_mxfp4_ws_bytes(0, 1, 1, 1024, 64) == 512 and lib.krq_lmhead_mxfp4_ws_bytes(0, 1, 0, 1024, 64) == -1
 
 
 def _q(N=64, K=64, device="cpu"):
