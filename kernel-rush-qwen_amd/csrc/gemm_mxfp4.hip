@@ -40,6 +40,9 @@ KRQ_DEV uint64_t uniform(const uint8_t* p) {
          static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(b >> 32)))) << 32;
 }
 
+// a wave-uniform value that a division or a conversion left in vector registers, as a scalar
+KRQ_DEV int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // 16 bytes per lane from base + off (base wave-uniform) to LDS at l + 16 lane (s_nop: M0 is read right after its scalar write)
 KRQ_DEV void load_lds(const uint8_t* base, uint32_t off, uint32_t l) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(l)), "v"(off),
@@ -77,12 +80,18 @@ KRQ_DEV void barrier_lds() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// after product U, its share of the NR LDS reads
+// LDS reads issued up to product U of NP, of NR in all: spread over the first half of the products, so that the rest of
+// them cover the last reads' latency
+template <int NP, int NR>
+constexpr int reads_to(int u) {
+  constexpr int over = NP > 1 ? NP / 2 : 1;
+  return u >= over ? NR : u * NR / over;
+}
 template <int U, int NP, int NR>
 KRQ_DEV void interleave() {
   if constexpr (U < NP) {
+    constexpr int c = reads_to<NP, NR>(U + 1) - reads_to<NP, NR>(U);
     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-    constexpr int c = (U + 1) * NR / NP - U * NR / NP;
     if constexpr (c > 0) __builtin_amdgcn_sched_group_barrier(0x100, c, 0);
     interleave<U + 1, NP, NR>();
   }
@@ -102,15 +111,17 @@ template <int ELEM, int BM, int BN, int W, int OCC, int NB, bool PART>
 __global__ __launch_bounds__(64 * W, OCC * W / 4) void k_gemm_mx(const GemmArgs a) {
   constexpr int AB = ELEM == KRQ_MX_E2M1 ? 1 : 2;          // KiB per activation tile
   constexpr int kA = BM / 16 * AB * 1024, kB = BN / 16 * 1024, kStage = kA + kB;
-  constexpr int QA = kA / 1024 / W, QB = kB / 1024 / W, kLoads = QA + QB;  // loads per wave per stage
+  constexpr int QA = (kA / 1024 + W - 1) / W, QB = (kB / 1024 + W - 1) / W, kLoads = QA + QB;  // loads per wave per stage
   constexpr int kScale = (BM + BN) / 16 * 256;             // scale bytes of a group
   constexpr int kSl = (kScale / 1024 + W - 1) / W;             // loads per wave per group (some twice)
   constexpr int FI = BM / 64, FJ = BN / (16 * W);          // 32-row fragments of a wave
   constexpr int NP = FI * FJ, NR = FI * AB + FJ + FI + FJ; // products and LDS reads per half stage
   constexpr int kStores = PART ? NP * 4 : NP * 2;
-  static_assert(NB >= 2 && NB <= 4 && BM % 64 == 0 && BN % (16 * W) == 0 && QA * W * 1024 == kA && QB * W * 1024 == kB, "tile shape");
-  // NB scale slots: a slot is filled again once NB - 1 more groups (of one stage at least each) have begun
-  __shared__ __align__(1024) uint8_t ring[NB * (kStage + kScale)];
+  static_assert(NB >= 2 && NB <= 4 && BM % 64 == 0 && BN % (16 * W) == 0, "tile shape");
+  // Scales are loaded for the stage kLag before the tiles' (three buffers and more: they still come a whole stage early),
+  // so that a slot can be filled again when all of the next kSlots groups (of one stage at least each) lie ahead of it.
+  constexpr int kLag = NB > 2 ? 1 : 0, kSlots = NB - kLag;
+  __shared__ __align__(1024) uint8_t ring[NB * kStage + kSlots * kScale];
   uint8_t* const sring = ring + NB * kStage;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int c = lane >> 5, hi = (lane >> 4) & 1, r = lane & 15;
@@ -126,30 +137,48 @@ __global__ __launch_bounds__(64 * W, OCC * W / 4) void k_gemm_mx(const GemmArgs 
     return base + bid;
   };
 
+  // tile row, tile column (in tiles), first stage and end of unit u
+  struct Unit {
+    int tm, tn, s0, s1;
+  };
+  auto unit = [&](int u) {
+    const int sp = scalar(u / a.tiles), p = u - sp * a.tiles, tn = scalar(p / a.tiles_m);
+    return Unit{p - tn * a.tiles_m, tn, PART ? scalar(static_cast<int>((int64_t)a.KT * sp / a.splits)) : 0,
+                PART ? scalar(static_cast<int>((int64_t)a.KT * (sp + 1) / a.splits)) : a.KT};
+  };
+
   // ---- the stream's loading end: stage ls of ls1 of unit lk, into buffer lb ----
-  int lk = 0, ls = 0, ls1 = 0, lstep = 1, lb = 0, lslot = NB - 1, lnew = 1;  // lnew: the first stage of a unit
+  int lk = 0, ls = 0, ls1 = 0, lstep = 1, lb = 0;
+  int cs = 0, cstep = 1, cslot = kSlots - 1, cnew = 1;  // the scales' stage; cnew: the first of a unit
   const uint8_t *xb = a.x, *wb = a.w, *xsb = a.xs, *wsb = a.ws;  // the unit's tiles, at stage ls; its scales
   uint32_t off[kLoads], soff[kSl];
   auto load_unit = [&](int u) {
-    const int p = u % a.tiles, sp = u / a.tiles;
-    const int mb0 = p % a.tiles_m * (BM / 16), nb0 = p / a.tiles_m * (BN / 16);
-    ls = static_cast<int>((int64_t)a.KT * sp / a.splits);
-    ls1 = static_cast<int>((int64_t)a.KT * (sp + 1) / a.splits);
-    lnew = 1;
+    const Unit un = unit(u);
+    const int mb0 = un.tm * (BM / 16), nb0 = un.tn * (BN / 16);
+    ls = un.s0;
+    ls1 = un.s1;
     xb = a.x + ((int64_t)mb0 * a.KT + ls) * (1024 * AB);
     wb = a.w + ((int64_t)nb0 * a.KT + ls) * 1024;
-    xsb = a.xs + (int64_t)mb0 * a.groups * 256;
-    wsb = a.ws + (int64_t)nb0 * a.groups * 256;
     int ln = lane;  // (opaque: computed here per unit, not kept live across units)
     asm volatile("" : "+v"(ln));
 #pragma unroll
     for (int q = 0; q < QA; ++q) {
-      const int i = wave + W * q, rb = min(mb0 + i / AB, a.mbs - 1) - mb0;
+      const int i = (wave + W * q) % (kA / 1024), rb = min(mb0 + i / AB, a.mbs - 1) - mb0;
       off[q] = static_cast<uint32_t>(rb * a.KT * (1024 * AB) + (i % AB) * 1024 + 16 * ln);
     }
 #pragma unroll
     for (int q = 0; q < QB; ++q)
-      off[QA + q] = static_cast<uint32_t>((min(nb0 + wave + W * q, a.nbs - 1) - nb0) * a.KT * 1024 + 16 * ln);
+      off[QA + q] = static_cast<uint32_t>((min(nb0 + (wave + W * q) % (kB / 1024), a.nbs - 1) - nb0) * a.KT * 1024 + 16 * ln);
+  };
+  auto scale_unit = [&](int u) {
+    const Unit un = unit(u);
+    const int mb0 = un.tm * (BM / 16), nb0 = un.tn * (BN / 16);
+    cs = un.s0;
+    cnew = 1;
+    xsb = a.xs + (int64_t)mb0 * a.groups * 256;
+    wsb = a.ws + (int64_t)nb0 * a.groups * 256;
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
 #pragma unroll
     for (int q = 0; q < kSl; ++q) {  // four row blocks' scales per load
       const int rb = (wave + W * q) % (kScale / 1024) * 4 + (ln >> 4);
@@ -158,20 +187,21 @@ __global__ __launch_bounds__(64 * W, OCC * W / 4) void k_gemm_mx(const GemmArgs 
     }
   };
   const uint32_t l0 = lds_at(ring), sl0 = lds_at(sring);
-  // the scales of the stage at the loading end, where it begins a group
+  // the scales of the scales' stage, where it begins a group
   auto load_scales = [&]() {
-    const int on = lstep & (lnew | ((ls & 3) == 0 ? 1 : 0));
-    lslot += on;
-    lslot = lslot == NB ? 0 : lslot;
+    const int on = cstep & (cnew | ((cs & 3) == 0 ? 1 : 0));
+    cslot += on;
+    cslot = cslot == kSlots ? 0 : cslot;
 #pragma unroll
     for (int q = 0; q < kSl; ++q) {
       const int li = (wave + W * q) % (kScale / 1024);
-      load_lds_if(on, (li < BM / 64 ? xsb : wsb) + (int64_t)(ls >> 2) * 256, soff[q], sl0 + lslot * kScale + li * 1024);
+      load_lds_if(on, (li < BM / 64 ? xsb : wsb) + (int64_t)(cs >> 2) * 256, soff[q], sl0 + cslot * kScale + li * 1024);
     }
-    lnew = 0;
+    cnew = 0;
+    cs += cstep;
   };
   auto load_tile = [&](int q) {
-    load_lds(q < QA ? xb : wb, off[q], l0 + lb * kStage + (q < QA ? 0 : kA) + 1024 * (wave + W * (q < QA ? q : q - QA)));
+    load_lds(q < QA ? xb : wb, off[q], l0 + lb * kStage + (q < QA ? (wave + W * q) % (kA / 1024) * 1024 : kA + (wave + W * (q - QA)) % (kB / 1024) * 1024));
   };
   auto advance = [&]() {  // past the loaded stage
     lb = lb + 1 == NB ? 0 : lb + 1;
@@ -193,10 +223,16 @@ __global__ __launch_bounds__(64 * W, OCC * W / 4) void k_gemm_mx(const GemmArgs 
       wb -= 1024;
     }
   };
+  auto next_scale_unit = [&]() {  // (after next_unit)
+    const int u = unit_of(lk);
+    if (u >= 0) scale_unit(u);
+    else cstep = 0;
+  };
   if (unit_of(0) < 0) return;
   load_unit(unit_of(0));
+  scale_unit(unit_of(0));
   for (int b = 0; b < NB; ++b) {
-    load_scales();
+    if (b < NB - kLag) load_scales();
 #pragma unroll
     for (int q = 0; q < kLoads; ++q) load_tile(q);
     advance();
@@ -247,11 +283,12 @@ __global__ __launch_bounds__(64 * W, OCC * W / 4) void k_gemm_mx(const GemmArgs 
           pack_v8i(fb[h][j], zero4()), AB == 2 ? pack_v8i(fa[h][i][0], fa[h][i][AB - 1]) : pack_v8i(fa[h][i][0], zero4()),
           acc[i][j], 4, ELEM == KRQ_MX_E2M1 ? 4 : 0, 0, static_cast<int>(sb[h][j]), 0, static_cast<int>(sa[h][i]));
       if (h == 1) {
+        if (u == 0) load_scales();
 #pragma unroll
         for (int q = u * kLoads / NP; q < (u + 1) * kLoads / NP; ++q) load_tile(q);
       }
 #pragma unroll
-      for (int n = u * NR / NP; n < (u + 1) * NR / NP; ++n) read(n, 1 - h, b, sl, t);
+      for (int n = reads_to<NP, NR>(u); n < reads_to<NP, NR>(u + 1); ++n) read(n, 1 - h, b, sl, t);
     }
     interleave<0, NP, NR>();
   };
@@ -315,28 +352,27 @@ __global__ __launch_bounds__(64 * W, OCC * W / 4) void k_gemm_mx(const GemmArgs 
   wait_loads<(NB - 1) * kLoads>();
   barrier_lds();
 #pragma unroll
-  for (int n = 0; n < NR; ++n) read(n, 0, 0, 0, static_cast<int>((int64_t)a.KT * (unit_of(0) / a.tiles) / a.splits) & 3);
+  for (int n = 0; n < NR; ++n) read(n, 0, 0, 0, unit(unit_of(0)).s0 & 3);
   int buf = 0, slot = 0;
   int stores = 0;  // the last tile's kStores stores per lane are younger than the next stage's loads
-  auto first = [&](int unit) { return static_cast<int>((int64_t)a.KT * (unit / a.tiles) / a.splits); };
   for (int k = 0, u = unit_of(0), un; u >= 0; ++k, u = un) {
     un = unit_of(k + 1);
-    int s = first(u);
-    const int s1 = static_cast<int>((int64_t)a.KT * (u / a.tiles + 1) / a.splits), sfirst = un < 0 ? 0 : first(un);
+    const Unit cur = unit(u);
+    int s = cur.s0;
+    const int s1 = cur.s1, sfirst = un < 0 ? 0 : unit(un).s0;
     zero();
     // stage s; the loading end is NB stages ahead
     auto stage = [&](bool last) __attribute__((always_inline)) {
       half(h0{}, buf, slot, s & 3);
-      // the next stage has landed, and once every wave is here none reads this one's buffer any more: refill it
-      wait_loads_or<(NB - 2) * kLoads, kStores>(stores);
-      stores = 0;
-      barrier_lds();
       ++s;
       const int sn = last ? sfirst : s;  // the next stage: of this unit, or the next one's first
       const int on = last || (sn & 3) == 0 ? 1 : 0;
       buf = buf + 1 == NB ? 0 : buf + 1;
-      slot = slot + on == NB ? 0 : slot + on;
-      load_scales();
+      slot = slot + on == kSlots ? 0 : slot + on;
+      // the next stage has landed, and once every wave is here none reads this one's buffer any more: refill it
+      wait_loads_or<(NB - 2) * kLoads, kStores>(stores);
+      stores = 0;
+      barrier_lds();
       half(h1{}, buf, slot, sn & 3);
       advance();
     };
@@ -344,14 +380,16 @@ __global__ __launch_bounds__(64 * W, OCC * W / 4) void k_gemm_mx(const GemmArgs 
     while (s < s1 - NB) stage(false);
     next_unit();  // the loading end goes on into the next unit
 #pragma clang loop unroll(disable)
+    while (s < s1 - NB + kLag) stage(false);
+    next_scale_unit();
+#pragma clang loop unroll(disable)
     while (s < s1) stage(s + 1 == s1);
-    const int p = u % a.tiles;
-    const int m0 = p % a.tiles_m * BM, n0 = p / a.tiles_m * BN;
+    const int m0 = cur.tm * BM, n0 = cur.tn * BN, sp = PART ? scalar(u / a.tiles) : 0;
     if (m0 + BM <= a.M && n0 + BN <= a.N && a.wide) {
-      store(yes{}, m0, n0, u / a.tiles);
+      store(yes{}, m0, n0, sp);
       stores = 1;
     } else {
-      store(no{}, m0, n0, u / a.tiles);
+      store(no{}, m0, n0, sp);
     }
   }
   wait_loads<0>();  // no load into LDS outlives the workgroup
@@ -425,18 +463,31 @@ __global__ __launch_bounds__(256) void k_gemm_mx_reduce(const float* __restrict_
   }
 }
 
+// The output tile and the parts of K. A tile's time for a given K in a whole round of the chip, in that of 256 x 256 tiles (one
+// workgroup per compute unit); the smaller ones run two per unit, the second figure is for a unit with one. Measured
+// (us, e4m3 / e2m1 rows): 4,096 x 19,456 x 2,560, 5 rounds of 256 x 256 159 / 115, 7 of 192 x 256 176 / 131, 128 x 256
+// 176 / 128, 128 x 128 217 / 148; 4,096 x 2,560 x 9,728 in one round of 160 256 x 256 tiles 88 / 60, of 220 192 x 256
+// ones 81 / 58; 4,096 x 6,144 x 2,560 256 x 256 63 / 46, 128 x 256 52 / 43; 1,000 x 2,560 x 9,728 128 x 128 32 / 27, 64 x 64
+// 45 / 43; 77 x 6,144 x 2,560 64 x 64 8.4 / 8.3, 128 x 128 11 / 10; 77 x 19,456 x 2,560 128 x 128 11.6 / 10.5, 64 x 64 15.5 / 15.
+// K is split only where 64 x 64 tiles would leave half the chip idle for 64 stages and more (77 x 2,560 x 9,728, 80 tiles,
+// in 4 parts 15.1 / 14.9 with their sum, whole 24.8 / 22.1; 256 x 2,560 x 4,096, 160 tiles of 32 stages, whole 12.9 / 11.7,
+// in 2 15.4 / 15.0).
 struct GemmPlan {
-  int bm, splits;
+  int bm, bn, splits;
 };
-
-// The output tile and the parts of K.
 GemmPlan plan_of(int64_t M, int64_t N, int64_t KT, int cus) {
-  auto tiles = [&](int64_t b) { return (M + b - 1) / b * ((N + b - 1) / b); };
-  if (tiles(256) >= cus / 2) return {256, 1};
-  if (tiles(128) >= cus / 2) return {128, 1};
+  auto tiles = [&](int64_t bm, int64_t bn) { return (M + bm - 1) / bm * ((N + bn - 1) / bn); };
+  auto cost = [&](int64_t t, double pair, double one) {
+    return pair * (double)(t / (2 * cus)) + (t % (2 * cus) == 0 ? 0.0 : t % (2 * cus) <= cus ? one : pair);
+  };
+  const int shape[5][2] = {{256, 256}, {192, 256}, {128, 256}, {128, 128}, {64, 64}};
+  const double c[5] = {cost(tiles(256, 256), 2.0, 1.0), cost(tiles(192, 256), 1.66, 0.83), cost(tiles(128, 256), 1.09, 0.58),
+                       cost(tiles(128, 128), 0.62, 0.36), cost(tiles(64, 64), 0.30, 0.22)};
+  const int best = static_cast<int>(std::min_element(c, c + 5) - c);
   int splits = 1;
-  while (splits < 8 && tiles(64) * splits * 2 <= 2 * cus && KT / (2 * splits) >= 8) splits *= 2;
-  return {64, splits};
+  if (best == 4 && KT >= 64 && tiles(64, 64) <= cus / 2)
+    while (splits < 8 && tiles(64, 64) * splits <= cus && KT / (2 * splits) >= 16) splits *= 2;
+  return {shape[best][0], shape[best][1], splits};
 }
 
 int cu_count(int* cus) {
@@ -447,26 +498,35 @@ int cu_count(int* cus) {
              : KRQ_EHIP;
 }
 
-template <int ELEM, int BM, int W, int OCC, int NB, bool PART>
+template <int ELEM, int BM, int BN, int W, int OCC, int NB, bool PART>
 void launch(const GemmArgs& g, int cus, hipStream_t s) {
   GemmArgs a = g;
   a.tiles_m = (a.M + BM - 1) / BM;
-  a.tiles = a.tiles_m * ((a.N + BM - 1) / BM);
+  a.tiles = a.tiles_m * ((a.N + BN - 1) / BN);
   const int64_t units = (int64_t)a.tiles * a.splits, slots = (int64_t)cus * OCC;
-  hipLaunchKernelGGL((k_gemm_mx<ELEM, BM, BM, W, OCC, NB, PART>), dim3(static_cast<unsigned>(std::min(units, slots))), dim3(64 * W),
+  hipLaunchKernelGGL((k_gemm_mx<ELEM, BM, BN, W, OCC, NB, PART>), dim3(static_cast<unsigned>(std::min(units, slots))), dim3(64 * W),
                      0, s, a);
 }
 
 template <int ELEM>
 void launch_plan(const GemmArgs& a, const GemmPlan& p, int cus, hipStream_t s) {
-  constexpr int D = ELEM == KRQ_MX_E2M1 ? 1 : 0;  // e2m1 stages are shorter: one buffer more
+  constexpr int D = ELEM == KRQ_MX_E2M1 ? 1 : 0;  // e2m1 stages are smaller: one buffer more
   if (a.KT < kMinStages) {
     const int tm = (a.M + 127) / 128;
     hipLaunchKernelGGL((k_gemm_mx_short<ELEM>), dim3(static_cast<unsigned>(tm * ((a.N + 127) / 128))), dim3(256), 0, s, a, tm);
-  } else if (p.bm == 256) launch<ELEM, 256, 8, 1, 2 + D, false>(a, cus, s);
-  else if (p.bm == 128) launch<ELEM, 128, 4, 2, 2 + D, false>(a, cus, s);
-  else if (p.splits == 1) launch<ELEM, 64, 4, 2, 4, false>(a, cus, s);
-  else launch<ELEM, 64, 4, 2, 4, true>(a, cus, s);
+  } else if (p.bm == 256) {
+    launch<ELEM, 256, 256, 8, 1, 3 + D, false>(a, cus, s);
+  } else if (p.bm == 192) {
+    launch<ELEM, 192, 256, 8, 1, 3 + D, false>(a, cus, s);
+  } else if (p.bm == 128 && p.bn == 256) {
+    launch<ELEM, 128, 256, 4, 2, 2, false>(a, cus, s);
+  } else if (p.bm == 128) {
+    launch<ELEM, 128, 128, 4, 2, 3 + D, false>(a, cus, s);
+  } else if (p.splits == 1) {
+    launch<ELEM, 64, 64, 4, 2, 4, false>(a, cus, s);
+  } else {
+    launch<ELEM, 64, 64, 4, 2, 4, true>(a, cus, s);
+  }
 }
 
 }  // namespace

@@ -251,7 +251,13 @@ def test_outputs_end_where_they_should(dev):
 # ------------------------------------------------------------------------------------------ prefill product
 @pytest.mark.parametrize("elem", ["e4m3", "e2m1"])
 @pytest.mark.parametrize("M,N,K", [(1, 1, 32), (33, 17, 160), (77, 6144, 512), (128, 128, 128), (129, 257, 2880), (300, 1000, 1056),
-                                   (64, 2560, 4096), (257, 256, 9728), (520, 768, 640), (1000, 2560, 2560), (2049, 304, 512)])
+                                   (64, 2560, 4096), (257, 256, 9728), (520, 768, 640), (1000, 2560, 2560), (2049, 304, 512),
+                                   # every output tile on 256 compute units, several tiles per workgroup, groups of one stage:
+                                   # 256 x 256, 192 x 256, 128 x 256 (and N not of whole 16-byte pieces), 128 x 128, 64 x 64
+                                   (4096, 4096, 640), (4000, 2560, 544), (4000, 6100, 640), (4000, 6104, 640), (500, 2560, 2176),
+                                   (700, 1100, 1152),
+                                   # K in parts: whole and ragged columns
+                                   (77, 520, 8224), (40, 99, 16384), (64, 2560, 9728)])
 def test_gemm(dev, M, N, K, elem):
     q, wv = weight(N, K, 3, dev, spread_out=M < 77)
     x = bf((M, K), 4)
