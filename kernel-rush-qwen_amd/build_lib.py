@@ -33,7 +33,7 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17",
 # M = 16 302.5 -> 296.8 us, M = 5 296.6 -> 290.2, the fused layer at M = 16 347.9 -> 342.5. The GEMVs
 # (weight streams, bound by HBM) measured the same with it and M = 1 0.3% slower, so they keep the load.
 PRELOAD = ["-mllvm", "-amdgpu-kernarg-preload-count=16"]
-FILE_FLAGS = {"quant.hip": PRELOAD, "fused_fp8.hip": PRELOAD}
+FILE_FLAGS = {"quant.hip": PRELOAD, "fused_fp8.hip": PRELOAD, "mx_quant.hip": PRELOAD}
 
 
 def _run(cmd):

@@ -73,13 +73,6 @@ KRQ_DEV void wait_loads_or(int more) {
       : "memory", "scc");
 }
 
-// workgroup barrier for LDS accesses (the direct loads are waited for explicitly)
-KRQ_DEV void barrier_lds() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
-
 // LDS reads issued up to product U of NP, of NR in all: spread over the first half of the products, so that the rest of
 // them cover the last reads' latency
 template <int NP, int NR>

@@ -387,7 +387,7 @@ int64_t mxfp4_cand_bytes(int64_t M, int64_t V) { return (krq_lmhead_ws_bytes(M, 
 }  // namespace
 
 extern "C" int64_t krq_lmhead_mxfp4_ws_bytes(int x_kind, int elem, int64_t M, int64_t V, int64_t K) {
-  const int64_t rows = krq_gemv_mxfp4_ws_bytes(x_kind, elem, M, K);
+  const int64_t rows = krq_gemv_mxfp4_ws_bytes(x_kind, elem, M, K, 1);
   return rows < 0 || V < 1 ? -1 : mxfp4_cand_bytes(M, V) + rows;
 }
 

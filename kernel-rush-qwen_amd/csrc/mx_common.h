@@ -82,6 +82,13 @@ KRQ_DEV uint2 mx_quant8_e4m3(uint4 v, uint32_t c) {
   return make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
 }
 
+// workgroup barrier for LDS accesses alone: loads from memory stay in flight across it
+KRQ_DEV void barrier_lds() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // Rows rounded into a workspace: elements, then scales, each on 256 bytes.
 inline int64_t mx_rows_scale_at(int elem, int64_t M, int64_t K) { return (krq_mx_tiled_bytes(M, K, elem) + 255) & ~(int64_t)255; }
 inline int64_t mx_rows_bytes(int elem, int64_t M, int64_t K) { return mx_rows_scale_at(elem, M, K) + krq_mx_scale_bytes(M, K); }

@@ -82,7 +82,7 @@ EXPORTS = {
     "krq_embed_mxfp4": (_i32, [_vp, _i32, _i64, _vp, _vp, _i64, _i64, _f32, _vp, _vp]),
     "krq_gemv_mxfp4": (_i32, [_vp, _vp, _i32, _i32, _i64, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp, _i64, _vp,
                               _vp]),
-    "krq_gemv_mxfp4_ws_bytes": (_i64, [_i32, _i32, _i64, _i64]),
+    "krq_gemv_mxfp4_ws_bytes": (_i64, [_i32, _i32, _i64, _i64, _i32]),
     "krq_gemm_mxfp4": (_i32, [_vp, _vp, _i32, _i32, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "krq_gemm_mxfp4_ws_bytes": (_i64, [_i32, _i32, _i64, _i64, _i64]),
     "krq_lmhead_mxfp4_ws_bytes": (_i64, [_i32, _i32, _i64, _i64, _i64]),

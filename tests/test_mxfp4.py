@@ -118,7 +118,7 @@ def test_c_entry_points_refuse_before_any_launch():
     refuse("krq_dequant_mx", b"element type", p, p, 5, 16, 64, p, z)
     refuse("krq_dequant_mx", b"16 bytes", p, p, 1, 16, 64, odd, z)
     refuse("krq_embed_mxfp4", b"indices", p, 1, 0, p, p, 16, 64, 1.0, p, z)
-    refuse("krq_embed_mxfp4", b"indices", p, 1, 1 << 40, p, p, 16, 64, 1.0, p, z)
+    refuse("krq_embed_mxfp4", b"indices", p, 1, 1 << 39, p, p, 16, 64, 1.0, p, z)
     refuse("krq_embed_mxfp4", b"multiple of 32", p, 1, 4, p, p, 16, 40, 1.0, p, z)
     gemv = lambda needle, x=p, xs=p, kind=1, elem=1, ld=0, w=p, M=4, N=64, K=1024, split=1, mode=0, ws=z, nb=0, out=p: refuse(
         "krq_gemv_mxfp4", needle, x, xs, kind, elem, ld, w, p, M, N, K, split, mode, ws, nb, out, z)
@@ -163,9 +163,11 @@ def test_c_entry_points_refuse_before_any_launch():
     head(b"workspace", nb=8)
     head(b"workspace", M=33)
     lib = L.lib()
-    assert lib.krq_gemv_mxfp4_ws_bytes(0, 1, 8, 64) == lib.krq_gemv_mxfp4_ws_bytes(1, 1, 32, 64) == 0
-    assert lib.krq_gemv_mxfp4_ws_bytes(0, 1, 9, 64) == 2048 + 256 and lib.krq_gemv_mxfp4_ws_bytes(0, 0, 32, 64) == 2 * 1024 + 512
-    assert lib.krq_gemv_mxfp4_ws_bytes(0, 1, 33, 64) == lib.krq_gemm_mxfp4_ws_bytes(0, 3, 40, 64, 64) == -1
+    assert lib.krq_gemv_mxfp4_ws_bytes(0, 1, 8, 64, 1) == lib.krq_gemv_mxfp4_ws_bytes(1, 1, 32, 64, 1) == 0
+    assert lib.krq_gemv_mxfp4_ws_bytes(0, 1, 9, 64, 1) == 2048 + 256 and lib.krq_gemv_mxfp4_ws_bytes(0, 0, 32, 64, 1) == 2 * 1024 + 512
+    assert lib.krq_gemv_mxfp4_ws_bytes(0, 1, 1, 10240, 1) == lib.krq_gemv_mxfp4_ws_bytes(0, 1, 8, 16384, 2) == 0
+    assert lib.krq_gemv_mxfp4_ws_bytes(0, 1, 1, 10272, 1) > 0 and lib.krq_gemv_mxfp4_ws_bytes(0, 1, 1, 64, 0) == -1
+    assert lib.krq_gemv_mxfp4_ws_bytes(0, 1, 33, 64, 1) == lib.krq_gemm_mxfp4_ws_bytes(0, 3, 40, 64, 64) == -1
     assert lib.krq_lmhead_mxfp4_ws_bytes(0, 1, 1, 1024, 64) == 512 and lib.krq_lmhead_mxfp4_ws_bytes(0, 1, 0, 1024, 64) == -1
 
 
