@@ -419,7 +419,7 @@ int krq_unpack_fp8(const void* w8_tiled, int64_t N, int64_t K, void* w8_rowmajor
 /* element types of MX blocks, and the activation kinds of krq_gemv_mxfp4 */
 #define KRQ_MX_E2M1 0
 #define KRQ_MX_E4M3 1
-#define KRQ_MX_X_BF16 0     /* bf16 rows; up to KRQ_MX_BF16_ROWS of 10,240 k are rounded in the kernel, others into ws first */
+#define KRQ_MX_X_BF16 0     /* bf16 rows; a few are rounded in the kernel (one of 10,240 k, KRQ_MX_BF16_ROWS of 5,120), others into ws first */
 #define KRQ_MX_X_TILED 1    /* rows from krq_quant_mx_rows, with their scales */
 #define KRQ_MX_BF16_ROWS 8
 
@@ -453,7 +453,7 @@ int krq_embed_mxfp4(const void* ids, int ids_64, int64_t T, const void* w4, cons
  * MXFP4 skinny GEMM / GEMV, M <= 32 (krq_gemv_fp8 on MX blocks; no reference counterpart):
  *   y[m,n] = sum_k x[m,k] w[n,k] over the blocks' values, fp32 accumulation
  * x_kind KRQ_MX_X_BF16: x bf16 [M, K] (rows ldx elements apart, on 16 bytes), rounded to blocks of elem in the
- * kernel, or above KRQ_MX_BF16_ROWS or 10,240 k a split by a launch before; KRQ_MX_X_TILED: x and x_scale from krq_quant_mx_rows
+ * kernel or by a launch before; KRQ_MX_X_TILED: x and x_scale from krq_quant_mx_rows
  * (ldx unused). Products of e2m1 pairs are exact; beside an e4m3 operand the matrix instruction keeps 13 bits
  * below the largest product of a block.
  * w_tiled / w_scale: mx tiled e2m1 [N, K]. mode KRQ_OUT_BF16 -> bf16 [M, N] (split 1); KRQ_OUT_PARTIAL -> fp32

@@ -17,8 +17,14 @@ using namespace krq;
 namespace {
 
 constexpr int kHeldWaves = 10, kStreamWaves = 8;
+// the held kernel's waves with MT row tiles of operands (two: 64 registers of e4m3 operands a group)
+constexpr int held_waves(int MT) { return MT == 1 ? kHeldWaves : 8; }
 constexpr int kMxSplitMax = 64;
-constexpr int kHeldMost = 1024;  // workgroups of a held launch
+// A held launch has a workgroup per set up to 512 sets, above that at most one per compute unit (a few more sets each than
+// units would leave some units with twice the work). us, M = 1 on cold weights: 6,144 x 2,560 (384 sets) in 192 workgroups
+// 4.58, 384 4.14; SwiGLU over 19,456 x 2,560 (608) in 203 7.57, 304 10.4, 608 9.3; 18,000 x 6,400 (563) in 188 13.7, 282 17.0,
+// 563 15.4; the lm head (4,748) in 250 39.5, 475 40.6, 950 45.0.
+constexpr int kHeldOnce = 512, kHeldMost = 256;
 
 // acc += A (16 rows) . B (16 weight rows) over 128 k, scale byte t of sa and sb (t a constant after unrolling). A: e2m1 or
 // e4m3, B: e2m1.
@@ -40,10 +46,11 @@ struct MxArgs {
   const uint8_t* w;    // tiles
   const uint8_t* ws;   // their scales
   void* out;           // bf16 [M, NO], fp32 [splits][M][NO], or the logits (may be null)
-  Best* cand;          // argmax candidates [M][row blocks]
+  Best* cand;          // argmax candidates [M][workgroups][row blocks of a set]
   int64_t ldx;         // bf16 rows' stride
   int64_t NO;          // output columns
-  int M, K, KT, groups, nrb, sets;  // nrb: row blocks of the output; sets of P of them
+  int M, K, KT, groups, nrb, sets, nw;  // nrb: row blocks of the output; sets of P of them; waves (the block's size, which
+                                        // the compiler would load from memory behind every load in flight)
 };
 
 // MODE: KRQ_OUT_BF16, KRQ_OUT_PARTIAL (blockIdx.y: the split), KRQ_OUT_SWIGLU, kOutArgmax.
@@ -54,37 +61,70 @@ KRQ_DEV int row_block(const MxArgs& a, int set, int p) {
 }
 
 // Sums the waves' accumulators of a set, red [nw][P][MT][256], in wave order and writes its outputs; every thread of the
-// workgroup calls it.
+// workgroup calls it, and takes the same rows and columns of each set. kOutArgmax: best holds the thread's largest
+// logits so far (its columns come in rising order), for at least kArgmaxWaves waves.
+constexpr int kArgmaxWaves = 4;
 template <int MT, int MODE, int P>
-KRQ_DEV void finish(const MxArgs& a, const float* red, int nw, int set, int sp) {
+constexpr int best_count() { return MODE == kOutArgmax ? P * MT * 256 / (64 * kArgmaxWaves) : 1; }
+
+template <int MT, int MODE, int P>
+KRQ_DEV void finish(const MxArgs& a, const float* red, int set, int sp, Best* best) {
   constexpr int PO = MODE == KRQ_OUT_SWIGLU ? 1 : P;  // output row blocks
-  for (int v = threadIdx.x; v < PO * MT * 256; v += blockDim.x) {
-    const int p = v / (MT * 256), e = v % (MT * 256);
-    const int m = 16 * (e >> 8) + 4 * ((e >> 4) & 3) + ((e >> 6) & 3);
-    const int64_t n = ((int64_t)set * PO + p) * 16 + (e & 15);
-    const bool real = m < a.M && n < a.NO;
+  static_assert(PO <= 2, "sets of one or two row blocks");
+  const int rows = 16 * a.M;  // values of a row block: row v / 16, column v % 16
+  auto one = [&](int v, Best* bst) {
+    const int p = PO == 2 && v >= rows ? 1 : 0, w = v - p * rows, m = w >> 4;
+    const int e = 256 * (m >> 4) + 64 * (m & 3) + 16 * ((m >> 2) & 3) + (w & 15);  // its place in an accumulator
+    const int64_t n = ((int64_t)set * PO + p) * 16 + (w & 15);
+    if (n >= a.NO) return;
     float y = 0.0f, up = 0.0f;
-    for (int w = 0; w < nw; ++w) {
-      y += red[(w * P + p) * MT * 256 + e];
-      if (MODE == KRQ_OUT_SWIGLU) up += red[(w * P + 1) * MT * 256 + e];
+    for (int i = 0; i < a.nw; ++i) {
+      y += red[(i * P + p) * MT * 256 + e];
+      if (MODE == KRQ_OUT_SWIGLU) up += red[(i * P + 1) * MT * 256 + e];
     }
     if constexpr (MODE == kOutArgmax) {
-      Best b{-INFINITY, 0x7fffffff};
-      if (real) {
-        const uint16_t yb = f32_to_bf16(y);
-        if (a.out) static_cast<uint16_t*>(a.out)[(int64_t)m * a.NO + n] = yb;
-        b = Best{bf16_to_f32(yb), static_cast<int>(n)};
-      }
+      const uint16_t yb = f32_to_bf16(y);
+      if (a.out) static_cast<uint16_t*>(a.out)[(int64_t)m * a.NO + n] = yb;
+      const float l = bf16_to_f32(yb);
+      if (better(l, static_cast<int>(n), bst->v, bst->i)) *bst = Best{l, static_cast<int>(n)};
+    } else {
+      if constexpr (MODE == KRQ_OUT_SWIGLU) y = y / (1.0f + expf(-y)) * up;
+      if constexpr (MODE == KRQ_OUT_PARTIAL) static_cast<float*>(a.out)[((int64_t)sp * a.M + m) * a.NO + n] = y;
+      else static_cast<uint16_t*>(a.out)[(int64_t)m * a.NO + n] = f32_to_bf16(y);
+    }
+  };
+  if constexpr (MODE == kOutArgmax) {
+#pragma unroll
+    for (int q = 0; q < best_count<MT, MODE, P>(); ++q) {
+      const int v = static_cast<int>(threadIdx.x) + q * 64 * a.nw;
+      if (v < PO * rows) one(v, &best[q]);
+    }
+  } else {
+    for (int v = threadIdx.x; v < PO * rows; v += 64 * a.nw) one(v, nullptr);
+  }
+}
+
+template <int MT, int MODE, int P>
+KRQ_DEV void no_best(Best* best) {
+#pragma unroll
+  for (int q = 0; q < best_count<MT, MODE, P>(); ++q) best[q] = Best{-INFINITY, 0x7fffffff};
+}
+
+// the threads' largest logits, folded over the sixteen lanes of a row (which share it: 16 divides a row block's values)
+template <int MT, int MODE, int P>
+KRQ_DEV void write_best(const MxArgs& a, Best* best) {
+  if constexpr (MODE == kOutArgmax) {
+#pragma unroll
+    for (int q = 0; q < best_count<MT, MODE, P>(); ++q) {
+      Best b = best[q];
 #pragma unroll
       for (int o = 1; o < 16; o <<= 1) {
         const Best c = shfl_best(b, o);
         if (better(c.v, c.i, b.v, b.i)) b = c;
       }
-      if (real && (e & 15) == 0) a.cand[(int64_t)m * a.nrb + (int64_t)set * PO + p] = b;
-    } else if (real) {
-      if constexpr (MODE == KRQ_OUT_SWIGLU) y = y / (1.0f + expf(-y)) * up;
-      if constexpr (MODE == KRQ_OUT_PARTIAL) static_cast<float*>(a.out)[((int64_t)sp * a.M + m) * a.NO + n] = y;
-      else static_cast<uint16_t*>(a.out)[(int64_t)m * a.NO + n] = f32_to_bf16(y);
+      const int v = static_cast<int>(threadIdx.x) + q * 64 * a.nw, rows = 16 * a.M;
+      if (v < P * rows && (v & 15) == 0)
+        a.cand[((int64_t)((v >= rows ? v - rows : v) >> 4) * gridDim.x + blockIdx.x) * P + (v >= rows ? 1 : 0)] = b;
     }
   }
 }
@@ -94,7 +134,7 @@ KRQ_DEV void finish(const MxArgs& a, const float* red, int nw, int set, int sp) 
 // block, and the wave's own region of LDS turns them into operands, without a launch or a barrier before the product.
 // Lanes of rows past the last hold zeros (or, XSRC 1, the row: nobody reads their sums).
 template <int ELEM, int XSRC, int MT, int MODE, int P, int GW>
-__global__ __launch_bounds__(kHeldWaves * 64) void k_gemv_mx_held(const MxArgs a) {
+__global__ __launch_bounds__(held_waves(MT) * 64) void k_gemv_mx_held(const MxArgs a) {
   static_assert(XSRC == 0 || MT == 1, "rows rounded here: one row tile");
   static_assert(MODE != KRQ_OUT_SWIGLU || P == 2, "SwiGLU: a gate and an up row block");
   constexpr int AB = ELEM == KRQ_MX_E2M1 ? 1 : 2;  // 16-byte loads per activation tile
@@ -103,7 +143,7 @@ __global__ __launch_bounds__(kHeldWaves * 64) void k_gemv_mx_held(const MxArgs a
   // sums [2][waves][P][MT][256]; at first the rows' regions, per wave kRows x (a group's elements, linear in k; 16 scale bytes)
   extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), nw = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), nw = a.nw;
   const int splits = gridDim.y, sp = blockIdx.y;
   const int g0 = a.groups * sp / splits, g1 = a.groups * (sp + 1) / splits;  // this split's groups
   const int n = (a.sets - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
@@ -200,6 +240,8 @@ __global__ __launch_bounds__(kHeldWaves * 64) void k_gemv_mx_held(const MxArgs a
   }
 
   float* red = reinterpret_cast<float*>(smem);
+  Best best[best_count<MT, MODE, P>()];
+  no_best<MT, MODE, P>(best);
   auto consume = [&](int d, int i) __attribute__((always_inline)) {
     v4f acc[P][MT];
 #pragma unroll
@@ -230,7 +272,7 @@ __global__ __launch_bounds__(kHeldWaves * 64) void k_gemv_mx_held(const MxArgs a
   };
   auto sums = [&](int i) {
     barrier_lds();
-    finish<MT, MODE, P>(a, red + (i & 1) * nw * P * MT * 256, nw, static_cast<int>(blockIdx.x + i * gridDim.x), sp);
+    finish<MT, MODE, P>(a, red + (i & 1) * nw * P * MT * 256, static_cast<int>(blockIdx.x + i * gridDim.x), sp, best);
   };
   int i = 0;
   if constexpr (D == 2) {
@@ -265,6 +307,7 @@ __global__ __launch_bounds__(kHeldWaves * 64) void k_gemv_mx_held(const MxArgs a
     consume(0, i);
     sums(i);
   }
+  write_best<MT, MODE, P>(a, best);
 }
 
 // MT row tiles of activations beside every set's weights; U groups of a wave in flight.
@@ -273,7 +316,7 @@ __global__ __launch_bounds__(kStreamWaves * 64) void k_gemv_mx_stream(const MxAr
   extern __shared__ __align__(16) uint8_t smem[];  // sums [waves][P][MT][256]
   constexpr int AB = ELEM == KRQ_MX_E2M1 ? 1 : 2;
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), nw = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), nw = a.nw;
   const int splits = gridDim.y, sp = blockIdx.y;
   const int g0 = a.groups * sp / splits, g1 = a.groups * (sp + 1) / splits;
   const int jc = g0 + wave < g1 ? (g1 - g0 - wave + nw - 1) / nw : 0;  // this wave's groups
@@ -340,52 +383,62 @@ __global__ __launch_bounds__(kStreamWaves * 64) void k_gemv_mx_stream(const MxAr
 #pragma unroll
       for (int q = 0; q < 4; ++q) red[((wave * P + p) * MT + mt) * 256 + q * 64 + lane] = acc[p][mt][q];
   barrier_lds();
-  finish<MT, MODE, P>(a, red, nw, blockIdx.x, sp);
+  Best best[best_count<MT, MODE, P>()];
+  no_best<MT, MODE, P>(best);
+  finish<MT, MODE, P>(a, red, blockIdx.x, sp, best);
+  write_best<MT, MODE, P>(a, best);
 }
 
 int sets_of(const MxArgs& a, int mode, int P) { return mode == KRQ_OUT_SWIGLU ? a.nrb : (a.nrb + P - 1) / P; }
 
 template <int ELEM, int XSRC, int MT, int MODE, int P, int GW>
-void launch_held(MxArgs a, int splits, int nw, int most, hipStream_t s) {
+int launch_held(MxArgs a, int splits, int nw, hipStream_t s) {
   a.sets = sets_of(a, MODE, P);
+  a.nw = nw;
+  const int most = a.sets * splits <= kHeldOnce ? a.sets : kHeldMost / splits + 1;
   const int rounds = (a.sets + most - 1) / most, blocks = (a.sets + rounds - 1) / rounds;  // as many sets for each
   constexpr size_t row = (ELEM == KRQ_MX_E2M1 ? 256 : 512) + 16;
   const size_t smem = std::max((size_t)2 * nw * P * MT * 1024, XSRC > 0 ? nw * (XSRC == 4 ? 4 : 1) * row : 0);
   hipLaunchKernelGGL((k_gemv_mx_held<ELEM, XSRC, MT, MODE, P, GW>), dim3(blocks, splits), dim3(64 * nw), smem, s, a);
+  return blocks;
 }
 
 template <int ELEM, int MT, int MODE, int P, int U>
-void launch_stream(MxArgs a, int splits, int nw, hipStream_t s) {
+int launch_stream(MxArgs a, int splits, int nw, hipStream_t s) {
   a.sets = sets_of(a, MODE, P);
+  a.nw = nw;
   hipLaunchKernelGGL((k_gemv_mx_stream<ELEM, MT, MODE, P, U>), dim3(a.sets, splits), dim3(64 * nw), (size_t)nw * P * MT * 1024, s, a);
+  return a.sets;
 }
 
+// Launches a mode; returns the workgroups of a split.
 template <int ELEM, int MODE, int P>
-void launch_mode(const MxArgs& a, bool bf16, int splits, hipStream_t s) {
+int launch_mode(const MxArgs& a, bool bf16, int splits, hipStream_t s) {
   const int per = (a.groups + splits - 1) / splits;  // groups of the longest split
-  const int gw = (per + kHeldWaves - 1) / kHeldWaves, nw = (per + gw - 1) / gw, most = getenv("KRQ_MOST") ? atoi(getenv("KRQ_MOST")) : kHeldMost;
-  if (gw == 1 && a.M > 16) return launch_held<ELEM, 0, 2, MODE, P, 1>(a, splits, nw, most, s);
+  const int gw = (per + kHeldWaves - 1) / kHeldWaves, least = MODE == kOutArgmax ? kArgmaxWaves : 1;
+  const int nw = std::max((per + gw - 1) / gw, least);
+  if (a.M > 16 && per <= held_waves(2)) return launch_held<ELEM, 0, 2, MODE, P, 1>(a, splits, nw, s);
   if (gw <= 2 && a.M <= 16) {
     if (bf16 && a.M == 1)
-      return gw == 1 ? launch_held<ELEM, 1, 1, MODE, P, 1>(a, splits, nw, most, s) : launch_held<ELEM, 1, 1, MODE, P, 2>(a, splits, nw, most, s);
-    if (bf16)
-      return gw == 1 ? launch_held<ELEM, 4, 1, MODE, P, 1>(a, splits, nw, most, s) : launch_held<ELEM, 4, 1, MODE, P, 2>(a, splits, nw, most, s);
-    return gw == 1 ? launch_held<ELEM, 0, 1, MODE, P, 1>(a, splits, nw, most, s) : launch_held<ELEM, 0, 1, MODE, P, 2>(a, splits, nw, most, s);
+      return gw == 1 ? launch_held<ELEM, 1, 1, MODE, P, 1>(a, splits, nw, s) : launch_held<ELEM, 1, 1, MODE, P, 2>(a, splits, nw, s);
+    if (bf16) return launch_held<ELEM, 4, 1, MODE, P, 1>(a, splits, nw, s);
+    return gw == 1 ? launch_held<ELEM, 0, 1, MODE, P, 1>(a, splits, nw, s) : launch_held<ELEM, 0, 1, MODE, P, 2>(a, splits, nw, s);
   }
-  const int ns = std::min(per, kStreamWaves);
-  if (a.M <= 16) launch_stream<ELEM, 1, MODE, P, 2>(a, splits, ns, s);
-  else launch_stream<ELEM, 2, MODE, P, 1>(a, splits, ns, s);
+  const int ns = std::max(std::min(per, kStreamWaves), least);
+  return a.M <= 16 ? launch_stream<ELEM, 1, MODE, P, 2>(a, splits, ns, s) : launch_stream<ELEM, 2, MODE, P, 1>(a, splits, ns, s);
 }
 
 template <int MODE, int P>
-void launch_elem(const MxArgs& a, int elem, bool bf16, int splits, hipStream_t s) {
-  if (elem == KRQ_MX_E2M1) launch_mode<KRQ_MX_E2M1, MODE, P>(a, bf16, splits, s);
-  else launch_mode<KRQ_MX_E4M3, MODE, P>(a, bf16, splits, s);
+int launch_elem(const MxArgs& a, int elem, bool bf16, int splits, hipStream_t s) {
+  return elem == KRQ_MX_E2M1 ? launch_mode<KRQ_MX_E2M1, MODE, P>(a, bf16, splits, s) : launch_mode<KRQ_MX_E4M3, MODE, P>(a, bf16, splits, s);
 }
 
-// bf16 rows that a launch rounds itself: few of them, and a K whose operands its waves hold
+// bf16 rows that a launch rounds itself: one whose groups its waves hold, or a few over one group per wave. Rounded before /
+// in the launch, us: SwiGLU over 19,456 x 2,560, M = 5 10.4 / 8.8, M = 8 10.4 / 8.8; 2,560 x 9,728, M = 1 9.0 / 5.2, M = 5
+// (two groups per wave) 9.2 / 11.3.
 bool rounds_rows(int64_t M, int64_t K, int split) {
-  return M <= KRQ_MX_BF16_ROWS && (mx_groups(K) + split - 1) / split <= 2 * kHeldWaves;
+  const int64_t per = (mx_groups(K) + split - 1) / split;
+  return M == 1 ? per <= 2 * kHeldWaves : M <= KRQ_MX_BF16_ROWS && per <= kHeldWaves;
 }
 
 }  // namespace
@@ -395,7 +448,7 @@ namespace krq {
 // The checks and the launch of every product on MXFP4 weights of at most 32 rows (kOutArgmax: the head's).
 int gemv_mx_run(const char* what, const void* x, const void* x_scale, int x_kind, int elem, int64_t ldx, const void* w,
                 const void* w_scale, int64_t M, int64_t N, int64_t K, int split, int mode, void* ws, int64_t ws_bytes, void* out,
-                Best* cand, void* stream) {
+                Best* cand, int64_t* cands, void* stream) {
   KRQ_REQUIRE(x && w && w_scale && (out || mode == kOutArgmax), "%s: null pointer", what);
   KRQ_REQUIRE(elem == KRQ_MX_E2M1 || elem == KRQ_MX_E4M3, "%s: bad element type %d", what, elem);
   KRQ_REQUIRE(x_kind == KRQ_MX_X_BF16 || x_kind == KRQ_MX_X_TILED, "%s: bad x_kind %d", what, x_kind);
@@ -433,12 +486,12 @@ int gemv_mx_run(const char* what, const void* x, const void* x_scale, int x_kind
   a.KT = static_cast<int>(mx_tiles(K));
   a.groups = groups;
   a.nrb = static_cast<int>((a.NO + 15) / 16);
-  a.sets = 0;
+  a.sets = a.nw = 0;
   hipStream_t s = (hipStream_t)stream;
   const bool wide = a.nrb >= 1024;  // enough row blocks for pairs
   if (mode == KRQ_OUT_SWIGLU) launch_elem<KRQ_OUT_SWIGLU, 2>(a, elem, bf16, split, s);
   else if (mode == KRQ_OUT_PARTIAL) launch_elem<KRQ_OUT_PARTIAL, 1>(a, elem, bf16, split, s);
-  else if (mode == kOutArgmax) launch_elem<kOutArgmax, 2>(a, elem, bf16, split, s);
+  else if (mode == kOutArgmax) *cands = 2 * launch_elem<kOutArgmax, 2>(a, elem, bf16, split, s);
   else if (wide) launch_elem<KRQ_OUT_BF16, 2>(a, elem, bf16, split, s);
   else launch_elem<KRQ_OUT_BF16, 1>(a, elem, bf16, split, s);
   return krq_check_launch(what);
@@ -456,5 +509,5 @@ extern "C" int krq_gemv_mxfp4(const void* x, const void* x_scale, int x_kind, in
                               void* out, void* stream) {
   KRQ_REQUIRE(mode == KRQ_OUT_BF16 || mode == KRQ_OUT_PARTIAL || mode == KRQ_OUT_SWIGLU, "gemv_mxfp4: bad mode %d", mode);
   return gemv_mx_run("gemv_mxfp4", x, x_scale, x_kind, elem, ldx, w_tiled, w_scale, M, N, K, split, mode, ws, ws_bytes, out, nullptr,
-                     stream);
+                     nullptr, stream);
 }

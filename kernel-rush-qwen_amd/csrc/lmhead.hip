@@ -383,7 +383,7 @@ extern "C" int krq_lmhead_argmax(const void* h, const float* h_scale, int h_per_
 }
 
 namespace {
-int64_t mxfp4_cand_bytes(int64_t M, int64_t V) { return (krq_lmhead_ws_bytes(M, V) + 255) & ~(int64_t)255; }
+int64_t mxfp4_cand_bytes(int64_t M, int64_t V) { return ((V / 16 + 2) * M * (int64_t)sizeof(Best) + 255) & ~(int64_t)255; }
 }  // namespace
 
 extern "C" int64_t krq_lmhead_mxfp4_ws_bytes(int x_kind, int elem, int64_t M, int64_t V, int64_t K) {
@@ -399,11 +399,12 @@ extern "C" int krq_lmhead_argmax_mxfp4(const void* h, const void* h_scale, int x
   const int64_t need = krq_lmhead_mxfp4_ws_bytes(x_kind, elem, M, V, K), cand = mxfp4_cand_bytes(M, V);
   KRQ_REQUIRE(need >= 0 && ws_bytes >= need, "lmhead_argmax_mxfp4: M=%lld, workspace of %lld bytes", (long long)M,
               (long long)ws_bytes);
+  int64_t cands = 0;
   const int rc = gemv_mx_run("lmhead_argmax_mxfp4", h, h_scale, x_kind, elem, ldh, w_tiled, w_scale, M, V, K, 1, kOutArgmax,
-                             (uint8_t*)ws + cand, ws_bytes - cand, logits, reinterpret_cast<Best*>(ws), stream);
+                             (uint8_t*)ws + cand, ws_bytes - cand, logits, reinterpret_cast<Best*>(ws), &cands, stream);
   if (rc != KRQ_OK) return rc;
   hipLaunchKernelGGL(k_argmax_fold, dim3(static_cast<unsigned>(M)), dim3(kFoldThreads), 0, (hipStream_t)stream,
-                     reinterpret_cast<const Best*>(ws), V / 16, static_cast<int>(M), idx_out);
+                     reinterpret_cast<const Best*>(ws), cands, static_cast<int>(M), idx_out);
   return krq_check_launch("lmhead_argmax_mxfp4");
 }
 

@@ -94,9 +94,9 @@ inline int64_t mx_rows_scale_at(int elem, int64_t M, int64_t K) { return (krq_mx
 inline int64_t mx_rows_bytes(int elem, int64_t M, int64_t K) { return mx_rows_scale_at(elem, M, K) + krq_mx_scale_bytes(M, K); }
 
 // The checks and the launch of every product on MXFP4 weights of at most 32 rows (gemv_mxfp4.hip; kOutArgmax:
-// the lm head's, its candidates to cand).
+// the lm head's, *cands candidates of each row to cand [M][*cands], at most 2 more than row blocks).
 int gemv_mx_run(const char* what, const void* x, const void* x_scale, int x_kind, int elem, int64_t ldx, const void* w,
                 const void* w_scale, int64_t M, int64_t N, int64_t K, int split, int mode, void* ws, int64_t ws_bytes, void* out,
-                Best* cand, void* stream);
+                Best* cand, int64_t* cands, void* stream);
 
 }  // namespace krq

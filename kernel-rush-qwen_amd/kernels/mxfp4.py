@@ -22,7 +22,7 @@ from . import _lib as L
 ELEMS = {"e2m1": L.MX_E2M1, "e4m3": L.MX_E4M3}
 DECODE_MAX_ROWS = 32  # rows of the skinny kernels
 BLOCK = 32
-HELD_MAX_K = 10240  # (a split's) k that the skinny kernels hold as operands, and round themselves for few rows
+ROW_MAX_K = 10240  # up to here the skinny kernels round a single bf16 row themselves, without a workspace
 _HERE = contextlib.nullcontext()
 
 
@@ -208,7 +208,7 @@ def _decode(x, q, split, mode, elem):
     if M == 0:
         return out
     ws, nbytes = None, 0
-    if kind == L.MX_X_BF16 and (M > L.MX_BF16_ROWS or K > HELD_MAX_K):
+    if kind == L.MX_X_BF16 and (M > 1 or K > ROW_MAX_K):
         nbytes = L.lib().krq_gemv_mxfp4_ws_bytes(kind, e, M, K, split)
         ws = t.new_empty((nbytes,), dtype=torch.uint8) if nbytes > 0 else None
     _call(out, "krq_gemv_mxfp4", p, scale, kind, e, ld, q.tiled.data_ptr(), q.tiled_scale.data_ptr(), M, N, K, split, mode,

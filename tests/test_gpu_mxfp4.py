@@ -165,7 +165,12 @@ def test_gemv(dev, M, N, K, elem):
 
 @pytest.mark.parametrize("M,N,K,split", [(1, 2560, 4096, 1), (3, 2560, 9728, 1), (32, 2560, 9728, 1), (16, 6144, 2560, 1),
                                          (1, 6144, 2560, 2), (5, 2560, 9728, 4), (32, 2560, 4096, 8), (20, 100, 1056, 3),
-                                         (7, 48, 16384, 1), (12, 48, 16384, 5), (1, 16, 33 * 512 + 96, 34)])
+                                         (7, 48, 16384, 1), (12, 48, 16384, 5), (1, 16, 33 * 512 + 96, 34),
+                                         # every place of the rows and the weights: one or several row blocks per workgroup,
+                                         # one or two groups per wave, operands beside the weights
+                                         (1, 18000, 1056, 1), (8, 16400, 2560, 1), (16, 17000, 5632, 1), (32, 16500, 2080, 1),
+                                         (1, 9000, 10240, 1), (3, 100, 5152, 1), (20, 10000, 4096, 1), (32, 300, 4608, 1),
+                                         (16, 96, 10272, 1), (1, 9000, 6016, 2), (32, 64, 12288, 3)])
 def test_gemv_large_and_split(dev, M, N, K, split):
     q, wv = weight(N, K, 1, dev)
     x = bf((M, K), 2)
@@ -282,7 +287,7 @@ def test_empty_rows(dev):
 
 
 # ------------------------------------------------------------------------------------------ lm head
-@pytest.mark.parametrize("M,V,K", [(1, 16, 32), (1, 151936, 512), (5, 4112, 2560), (8, 1024, 160), (9, 32000, 1024), (16, 4096, 2880),
+@pytest.mark.parametrize("M,V,K", [(1, 16, 32), (1, 70000, 512), (5, 4112, 2560), (1, 16400, 2560), (32, 20000, 2560), (2, 9008, 6400), (20, 4096, 6400), (16, 1040, 10752), (7, 48, 512), (8, 1024, 160), (9, 32000, 1024), (16, 4096, 2880),
                                    (32, 2048, 544)])
 def test_head(dev, M, V, K):
     q, wv = weight(V, K, 7, dev)

@@ -163,12 +163,13 @@ def test_c_entry_points_refuse_before_any_launch():
     head(b"workspace", nb=8)
     head(b"workspace", M=33)
     lib = L.lib()
-    assert lib.krq_gemv_mxfp4_ws_bytes(0, 1, 8, 64, 1) == lib.krq_gemv_mxfp4_ws_bytes(1, 1, 32, 64, 1) == 0
+    assert lib.krq_gemv_mxfp4_ws_bytes(0, 1, 8, 5120, 1) == lib.krq_gemv_mxfp4_ws_bytes(1, 1, 32, 64, 1) == 0
     assert lib.krq_gemv_mxfp4_ws_bytes(0, 1, 9, 64, 1) == 2048 + 256 and lib.krq_gemv_mxfp4_ws_bytes(0, 0, 32, 64, 1) == 2 * 1024 + 512
-    assert lib.krq_gemv_mxfp4_ws_bytes(0, 1, 1, 10240, 1) == lib.krq_gemv_mxfp4_ws_bytes(0, 1, 8, 16384, 2) == 0
+    assert lib.krq_gemv_mxfp4_ws_bytes(0, 1, 1, 10240, 1) == lib.krq_gemv_mxfp4_ws_bytes(0, 1, 8, 10240, 2) == 0
+    assert lib.krq_gemv_mxfp4_ws_bytes(0, 1, 2, 5152, 1) > 0
     assert lib.krq_gemv_mxfp4_ws_bytes(0, 1, 1, 10272, 1) > 0 and lib.krq_gemv_mxfp4_ws_bytes(0, 1, 1, 64, 0) == -1
     assert lib.krq_gemv_mxfp4_ws_bytes(0, 1, 33, 64, 1) == lib.krq_gemm_mxfp4_ws_bytes(0, 3, 40, 64, 64) == -1
-    assert lib.krq_lmhead_mxfp4_ws_bytes(0, 1, 1, 1024, 64) == 512 and lib.krq_lmhead_mxfp4_ws_bytes(0, 1, 0, 1024, 64) == -1
+    assert lib.krq_lmhead_mxfp4_ws_bytes(0, 1, 1, 1024, 64) == 768 and lib.krq_lmhead_mxfp4_ws_bytes(0, 1, 0, 1024, 64) == -1
 
 
 def _q(N=64, K=64, device="cpu"):
