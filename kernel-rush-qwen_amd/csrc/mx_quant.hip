@@ -142,15 +142,15 @@ __global__ __launch_bounds__(256) void k_mx_dequant(const uint8_t* __restrict__ 
   }
 }
 
-// Rows of a packed table: out[i] = bf16(w[ids[i]] * mult), the product in fp32 (w is exact in it). Eight values
-// per thread; an index outside the table gives a row of NaN.
+// Rows of a packed table: out[i] = bf16(w[ids[i]] * mult), the product in fp32 (w is exact in it). A wave takes 512 k of a
+// row, eight values per lane, and a workgroup four rows; an index outside the table gives a row of NaN.
 template <typename ID>
 __global__ __launch_bounds__(256) void k_mx_embed(const ID* __restrict__ ids, const uint8_t* __restrict__ q,
                                                   const uint8_t* __restrict__ scale, uint16_t* __restrict__ out, int64_t N,
                                                   int64_t T, int K, float mult) {
-  const int c = blockIdx.x * 256 + threadIdx.x;  // the row's eight values 8 c .. 8 c + 7
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63);  // the row's eight values 8 c .. 8 c + 7
   if (8 * c >= K) return;
-  for (int64_t i = blockIdx.y; i < T; i += gridDim.y) {
+  for (int64_t i = blockIdx.y * (int64_t)4 + (threadIdx.x >> 6); i < T; i += (int64_t)gridDim.y * 4) {
     const int64_t id = ids[i];
     const bool real = id >= 0 && id < N;
     const int64_t row = real ? id : 0;
@@ -246,7 +246,7 @@ extern "C" int krq_embed_mxfp4(const void* ids, int ids_64, int64_t T, const voi
   if (const int rc = mx_shape("embed_mxfp4", N, K)) return rc;
   KRQ_REQUIRE(T >= 1 && T <= 0x7fffffffffll, "embed_mxfp4: %lld indices", (long long)T);
   KRQ_REQUIRE(aligned16(w4) && aligned16(out), "embed_mxfp4: w4 and out must start on 16 bytes");
-  const dim3 grid(static_cast<unsigned>((K / 8 + 255) / 256), static_cast<unsigned>(std::min<int64_t>(T, kGridY)));
+  const dim3 grid(static_cast<unsigned>(mx_groups(K)), static_cast<unsigned>(std::min<int64_t>((T + 3) / 4, kGridY)));
   if (ids_64)
     hipLaunchKernelGGL((k_mx_embed<int64_t>), grid, dim3(256), 0, (hipStream_t)stream, (const int64_t*)ids, (const uint8_t*)w4,
                        (const uint8_t*)scale, (uint16_t*)out, N, T, (int)K, mult);

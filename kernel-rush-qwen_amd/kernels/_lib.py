@@ -110,15 +110,19 @@ def lib():
     return _lib
 
 
+def fail(name, rc):
+    """Raise what the status rc of entry point `name` stands for: ValueError for KRQ_EINVAL, else RuntimeError."""
+    msg = (lib().krq_last_error() or b"").decode(errors="replace")
+    if rc == KRQ_EINVAL:
+        raise ValueError(f"{name}: {msg}")
+    raise RuntimeError(f"{name} failed ({rc}): {msg}")
+
+
 def call(name, *args):
     """Call a status-returning entry point; map KRQ_EINVAL to ValueError, others to RuntimeError."""
-    L = lib()
-    rc = getattr(L, name)(*args)
+    rc = getattr(lib(), name)(*args)
     if rc != KRQ_OK:
-        msg = (L.krq_last_error() or b"").decode(errors="replace")
-        if rc == KRQ_EINVAL:
-            raise ValueError(f"{name}: {msg}")
-        raise RuntimeError(f"{name} failed ({rc}): {msg}")
+        fail(name, rc)
 
 
 def ptr(t):

@@ -68,8 +68,9 @@ def _mxfp4_head(h, q, return_logits):
     idx = t.new_empty((M,), dtype=torch.int64)
     logits = t.new_empty((M, V), dtype=torch.bfloat16) if return_logits else None
     ws = t.new_empty((L.lib().krq_lmhead_mxfp4_ws_bytes(kind, e, M, V, K),), dtype=torch.uint8)
-    _mxfp4._call(t, "krq_lmhead_argmax_mxfp4", p, scale, kind, e, ld, q.tiled.data_ptr(), q.tiled_scale.data_ptr(), M, V, K,
-                 L.ptr(logits), ws.data_ptr(), ws.numel(), idx.data_ptr())
+    dev, w, wscale = q.operand
+    _mxfp4._call(dev, "krq_lmhead_argmax_mxfp4", p, scale, kind, e, ld, w, wscale, M, V, K, L.ptr(logits), ws.data_ptr(), ws.numel(),
+                 idx.data_ptr())
     return (idx, logits) if return_logits else idx
 
 

@@ -35,6 +35,8 @@ class MXFP4Weight(tuple):
         self = super().__new__(cls, (w4, scale))
         self.tiled, self.tiled_scale = tiled, tiled_scale
         self.shape = (w4.shape[0], 2 * w4.shape[1])
+        # what every product on this weight passes on: its device and the addresses of its own tiles
+        self.operand = (tiled.get_device(), tiled.data_ptr(), tiled_scale.data_ptr())
         return self
 
 
@@ -62,14 +64,26 @@ def _elem(elem):
     return ELEMS[elem]
 
 
-def _call(t, name, *args):
-    """L.call on t's device and torch's current stream of it."""
-    dev = t.get_device()
-    if dev == torch._C._cuda_getDevice():
-        L.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+_cuda = torch._C
+
+
+def _call(dev, name, *args):
+    """L.call on device dev (made current for it where it is not) and torch's current stream of it. A call on a
+    few rows is host work as much as a launch (a product of one row 8.1 us, 3.6 of them the kernel's; 5.9 with
+    the library's function taken once and no Stream or device objects made)."""
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(L.lib(), name)
+    if dev == _cuda._cuda_getDevice():
+        rc = fn(*args, _cuda._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            L.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+            rc = fn(*args, _cuda._cuda_getCurrentRawStream(dev))
+    if rc != L.KRQ_OK:
+        L.fail(name, rc)
+
+
+_functions = {}
 
 
 def _same_device(first, *tensors):
@@ -83,20 +97,21 @@ def _bf16_rows(x, what):
     """(x, row stride): x [M, K] bf16 as the kernels read it, rows of consecutive values that start on 16 bytes."""
     if not x.is_cuda:
         L.require_device(x)
-    if x.dtype != torch.bfloat16 or x.dim() != 2:
-        raise ValueError(f"expected bf16 {what}, got {x.dtype} {tuple(x.shape)}")
-    M, K = x.shape
+    shape = x.shape
+    if x.dtype is not torch.bfloat16 or len(shape) != 2:
+        raise ValueError(f"expected bf16 {what}, got {x.dtype} {tuple(shape)}")
+    K = ld = shape[1]
     if K == 0 or K % BLOCK:
         raise ValueError(f"{what}: K={K} must be a positive multiple of {BLOCK}")
-    if x.is_contiguous():
-        ld = K
-    else:
+    if not x.is_contiguous():
         ld, unit = x.stride()
-        if M == 1 and unit == 1:
+        if shape[0] == 1 and unit == 1:
             ld = K
         elif unit != 1 or ld < K or ld % 8:
             x, ld = x.contiguous(), K
-    return (x if x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format), ld if x.data_ptr() % 16 == 0 else K)
+    if x.data_ptr() % 16:
+        x, ld = x.clone(memory_format=torch.contiguous_format), K
+    return x, ld
 
 
 def _tiles(M, K, elem, device):
@@ -115,7 +130,7 @@ def quantize(w):
     w4 = torch.empty((N, K // 2), device=w.device, dtype=torch.uint8)
     scale = torch.empty((N, K // BLOCK), device=w.device, dtype=torch.uint8)
     tiled, tscale = _tiles(N, K, L.MX_E2M1, w.device)
-    _call(w, "krq_quant_mxfp4", L.ptr(w), N, K, ld, L.ptr(w4), L.ptr(scale), L.ptr(tiled), L.ptr(tscale))
+    _call(w.get_device(), "krq_quant_mxfp4", L.ptr(w), N, K, ld, L.ptr(w4), L.ptr(scale), L.ptr(tiled), L.ptr(tscale))
     return MXFP4Weight(w4, scale, tiled, tscale)
 
 
@@ -133,7 +148,7 @@ def pack(w4, scale):
     if w4.data_ptr() % 16:
         w4 = w4.clone()
     tiled, tscale = _tiles(N, K, L.MX_E2M1, w4.device)
-    _call(w4, "krq_pack_mxfp4", L.ptr(w4), L.ptr(scale), N, K, L.ptr(tiled), L.ptr(tscale))
+    _call(w4.get_device(), "krq_pack_mxfp4", L.ptr(w4), L.ptr(scale), N, K, L.ptr(tiled), L.ptr(tscale))
     return MXFP4Weight(w4, scale, tiled, tscale)
 
 
@@ -154,7 +169,7 @@ def dequantize(q):
         data, scale = t.data_ptr(), q.tiled_scale.data_ptr()
     out = t.new_empty((M, K), dtype=torch.bfloat16)
     if M:
-        _call(out, "krq_dequant_mx", data, scale, elem, M, K, out.data_ptr())
+        _call(out.get_device(), "krq_dequant_mx", data, scale, elem, M, K, out.data_ptr())
     return out
 
 
@@ -170,24 +185,26 @@ def quant_rows(x, elem="e4m3"):
     at = lib.krq_mx_tiled_bytes(M, K, e)  # (whole KiB)
     data = x.new_empty((at + lib.krq_mx_scale_bytes(M, K),), dtype=torch.uint8)
     p = data.data_ptr()
-    _call(x, "krq_quant_mx_rows", x.data_ptr(), M, K, ld, e, p, p + at)
+    _call(x.get_device(), "krq_quant_mx_rows", x.data_ptr(), M, K, ld, e, p, p + at)
     return MXRows(data, at, (M, K), elem)
 
 
 def _operand(x, q, elem):
-    """(the tensor that keeps x's memory, its address, its scales', x_kind, elem, row stride, M) of bf16 rows or MXRows."""
+    """(the tensor that keeps x's memory, its address, its scales', x_kind, element type, row stride, M) of bf16 rows or
+    MXRows that multiply q."""
     N, K = _weight(q)
     if x.shape[-1] != K:
         raise ValueError(f"x {tuple(x.shape)} and w [{N}, {K}] do not match")
     if isinstance(x, MXRows):
-        t, (M, _), ld, kind, elem = x.data, x.shape, 0, L.MX_X_TILED, x.elem
-        scale = t.data_ptr() + x.scale_at
+        t, M, ld, kind, elem = x.data, x.shape[0], 0, L.MX_X_TILED, x.elem
+        p = t.data_ptr()
+        scale = p + x.scale_at
     else:
         t, ld = _bf16_rows(x, "rows [M, K]")
-        M, scale, kind = t.shape[0], None, L.MX_X_BF16
-    if t.get_device() != q.tiled.get_device():
+        M, p, scale, kind = t.shape[0], t.data_ptr(), None, L.MX_X_BF16
+    if t.get_device() != q.operand[0]:
         _same_device(t, q.tiled)
-    return t, t.data_ptr(), scale, kind, _elem(elem), ld, M
+    return t, p, scale, kind, ELEMS[elem] if elem in ELEMS else _elem(elem), ld, M
 
 
 def _decode(x, q, split, mode, elem):
@@ -199,20 +216,23 @@ def _decode(x, q, split, mode, elem):
         if split < 1:
             raise ValueError(f"split={split}")
         out = t.new_empty((split, M, N), dtype=torch.float32)
-    elif mode == L.OUT_SWIGLU:
-        if N % 32:
-            raise ValueError(f"SwiGLU needs w = [gate; up] of 2 I rows with I a multiple of 16, got N={N}")
-        out = t.new_empty((M, N // 2), dtype=torch.bfloat16)
     else:
-        out = t.new_empty((M, N), dtype=torch.bfloat16)
+        if mode == L.OUT_SWIGLU:
+            if N % 32:
+                raise ValueError(f"SwiGLU needs w = [gate; up] of 2 I rows with I a multiple of 16, got N={N}")
+            cols = N // 2
+        else:
+            cols = N
+        out = t.new_empty((M, cols)) if kind == L.MX_X_BF16 else t.new_empty((M, cols), dtype=torch.bfloat16)
     if M == 0:
         return out
     ws, nbytes = None, 0
     if kind == L.MX_X_BF16 and (M > 1 or K > ROW_MAX_K):
         nbytes = L.lib().krq_gemv_mxfp4_ws_bytes(kind, e, M, K, split)
-        ws = t.new_empty((nbytes,), dtype=torch.uint8) if nbytes > 0 else None
-    _call(out, "krq_gemv_mxfp4", p, scale, kind, e, ld, q.tiled.data_ptr(), q.tiled_scale.data_ptr(), M, N, K, split, mode,
-          L.ptr(ws), nbytes, out.data_ptr())
+        if nbytes > 0:
+            ws = t.new_empty((nbytes,), dtype=torch.uint8)
+    dev, w, wscale = q.operand
+    _call(dev, "krq_gemv_mxfp4", p, scale, kind, e, ld, w, wscale, M, N, K, split, mode, L.ptr(ws), nbytes, out.data_ptr())
     return out
 
 
@@ -239,13 +259,13 @@ def gemm_mxfp4(x, q, elem="e4m3"):
     out = t.new_empty((M, N), dtype=torch.bfloat16)
     if M == 0:
         return out
-    with torch.cuda.device(t.get_device()) if t.get_device() != torch._C._cuda_getDevice() else _HERE:
+    dev, w, wscale = q.operand
+    with torch.cuda.device(dev) if dev != _cuda._cuda_getDevice() else _HERE:  # (the plan is the current device's)
         nbytes = L.lib().krq_gemm_mxfp4_ws_bytes(kind, e, M, N, K)
     if nbytes < 0:
         raise RuntimeError("krq_gemm_mxfp4_ws_bytes: device query failed")
     ws = t.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
-    _call(out, "krq_gemm_mxfp4", p, scale, kind, e, ld, q.tiled.data_ptr(), q.tiled_scale.data_ptr(), M, N, K, L.ptr(ws), nbytes,
-          out.data_ptr())
+    _call(dev, "krq_gemm_mxfp4", p, scale, kind, e, ld, w, wscale, M, N, K, L.ptr(ws), nbytes, out.data_ptr())
     return out
 
 
@@ -267,6 +287,6 @@ def embedding(ids, q, scale=1.0):
     out = w4.new_empty((*ids.shape, K), dtype=torch.bfloat16)
     n = ids.numel()
     if n:
-        _call(out, "krq_embed_mxfp4", ids.data_ptr(), int(ids.dtype == torch.int64), n, w4.data_ptr(), scale_codes.data_ptr(), N, K,
+        _call(out.get_device(), "krq_embed_mxfp4", ids.data_ptr(), int(ids.dtype == torch.int64), n, w4.data_ptr(), scale_codes.data_ptr(), N, K,
               scale, out.data_ptr())
     return out
