@@ -2,13 +2,13 @@
 // tiles of mx_common.h, fp32 accumulation on v_mfma_scale_f32_32x32x64_f8f6f4.
 //
 // Persistent workgroups of W waves own BM x BN outputs, each wave BM / 2 x 2 BN / W of them, in 32 x 32 pieces. The
-// stream of stages (a stage: 128 k, one tile of every row block) runs on from one output tile into the next:
+// stream of stages (a stage: T times 128 k, T tiles of every row block) runs on from one output tile into the next:
 // direct loads bring a stage into one of NB LDS buffers, NB stages ahead of its use. A tile is stored in
 // lane order, so each load copies one whole KiB, and each 16-byte LDS read takes runs of 256 bytes: no padding, no
 // swizzle, no bank conflict, and no address arithmetic per lane. The scale bytes come a group of four stages at
 // a time into a ring of their own, from which every product reads its byte.
 //
-// Fragment of 32 rows, half h of the stage (64 k): lane l holds row l % 32, that is row r = l % 16 of row block
+// Fragment of 32 rows, half h of a tile (64 k): lane l holds row l % 32, that is row r = l % 16 of row block
 // (l / 16) % 2, with c = l / 32
 //   e2m1: k = 64 h + 32 c + 0..31, the 16 bytes of tile lane 16 (2 h + c) + r;
 //   e4m3: k = 64 h + 16 c + 0..15 and 32 more, the bytes of tile lanes 16 c + r and 16 (c + 2) + r of KiB h;
@@ -92,7 +92,7 @@ KRQ_DEV void interleave() {
 
 struct GemmArgs {
   const uint8_t *x, *xs, *w, *ws;
-  int M, N, KT, groups, mbs, nbs;  // mbs, nbs: row blocks of x and w
+  int M, N, KT, KS, groups, mbs, nbs;  // KT tiles of K in KS stages; mbs, nbs: row blocks of x and w
   int tiles_m, tiles, splits;
   int wide;                        // out's rows start on 16 bytes: N % 8 == 0
   float* part;                     // fp32 [splits][M][N] (PART)
@@ -100,17 +100,19 @@ struct GemmArgs {
 };
 
 // PART: a work unit is (tile, split) and writes its fp32 sums to plane `split` of part; else bf16 to out.
-template <int ELEM, int BM, int BN, int W, int OCC, int NB, bool PART>
+template <int ELEM, int BM, int BN, int W, int OCC, int NB, int T, bool PART>
 __global__ __launch_bounds__(64 * W, OCC * W / 4) void k_gemm_mx(const GemmArgs a) {
   constexpr int AB = ELEM == KRQ_MX_E2M1 ? 1 : 2;          // KiB per activation tile
-  constexpr int kA = BM / 16 * AB * 1024, kB = BN / 16 * 1024, kStage = kA + kB;
-  constexpr int QA = (kA / 1024 + W - 1) / W, QB = (kB / 1024 + W - 1) / W, kLoads = QA + QB;  // loads per wave per stage
+  constexpr int kA = BM / 16 * AB * 1024, kB = BN / 16 * 1024, kTile = kA + kB, kStage = T * kTile;
+  constexpr int QA = (kA / 1024 + W - 1) / W, QB = (kB / 1024 + W - 1) / W, kLoads = T * (QA + QB);  // loads per wave per stage
   constexpr int kScale = (BM + BN) / 16 * 256;             // scale bytes of a group
   constexpr int kSl = (kScale / 1024 + W - 1) / W;             // loads per wave per group (some twice)
   constexpr int FI = BM / 64, FJ = BN / (16 * W);          // 32-row fragments of a wave
-  constexpr int NP = FI * FJ, NR = FI * AB + FJ + FI + FJ; // products and LDS reads per half stage
+  constexpr int NP = FI * FJ, NF = FI * AB + FJ;           // products of a half tile, LDS reads of its elements
+  constexpr int HT = 2 * T, kG = 4 / T;                    // half tiles of a stage; stages of a scale group
+  typedef std::conditional_t<T == 1, uint8_t, uint16_t> scale_t;  // a block's scales in a stage
   constexpr int kStores = PART ? NP * 4 : NP * 2;
-  static_assert(NB >= 2 && NB <= 4 && BM % 64 == 0 && BN % (16 * W) == 0, "tile shape");
+  static_assert(NB >= 2 && NB <= 4 && (T == 1 || T == 2) && BM % 64 == 0 && BN % (16 * W) == 0, "tile shape");
   // Scales are loaded for the stage kLag before the tiles' (three buffers and more: they still come a whole stage early),
   // so that a slot can be filled again when all of the next kSlots groups (of one stage at least each) lie ahead of it.
   constexpr int kLag = NB > 2 ? 1 : 0, kSlots = NB - kLag;
@@ -136,22 +138,22 @@ __global__ __launch_bounds__(64 * W, OCC * W / 4) void k_gemm_mx(const GemmArgs 
   };
   auto unit = [&](int u) {
     const int sp = scalar(u / a.tiles), p = u - sp * a.tiles, tn = scalar(p / a.tiles_m);
-    return Unit{p - tn * a.tiles_m, tn, PART ? scalar(static_cast<int>((int64_t)a.KT * sp / a.splits)) : 0,
-                PART ? scalar(static_cast<int>((int64_t)a.KT * (sp + 1) / a.splits)) : a.KT};
+    return Unit{p - tn * a.tiles_m, tn, PART ? scalar(static_cast<int>((int64_t)a.KS * sp / a.splits)) : 0,
+                PART ? scalar(static_cast<int>((int64_t)a.KS * (sp + 1) / a.splits)) : a.KS};
   };
 
   // ---- the stream's loading end: stage ls of ls1 of unit lk, into buffer lb ----
   int lk = 0, ls = 0, ls1 = 0, lstep = 1, lb = 0;
   int cs = 0, cstep = 1, cslot = kSlots - 1, cnew = 1;  // the scales' stage; cnew: the first of a unit
   const uint8_t *xb = a.x, *wb = a.w, *xsb = a.xs, *wsb = a.ws;  // the unit's tiles, at stage ls; its scales
-  uint32_t off[kLoads], soff[kSl];
+  uint32_t off[QA + QB], soff[kSl];
   auto load_unit = [&](int u) {
     const Unit un = unit(u);
     const int mb0 = un.tm * (BM / 16), nb0 = un.tn * (BN / 16);
     ls = un.s0;
     ls1 = un.s1;
-    xb = a.x + ((int64_t)mb0 * a.KT + ls) * (1024 * AB);
-    wb = a.w + ((int64_t)nb0 * a.KT + ls) * 1024;
+    xb = a.x + ((int64_t)mb0 * a.KT + ls * T) * (1024 * AB);
+    wb = a.w + ((int64_t)nb0 * a.KT + ls * T) * 1024;
     int ln = lane;  // (opaque: computed here per unit, not kept live across units)
     asm volatile("" : "+v"(ln));
 #pragma unroll
@@ -182,25 +184,28 @@ __global__ __launch_bounds__(64 * W, OCC * W / 4) void k_gemm_mx(const GemmArgs 
   const uint32_t l0 = lds_at(ring), sl0 = lds_at(sring);
   // the scales of the scales' stage, where it begins a group
   auto load_scales = [&]() {
-    const int on = cstep & (cnew | ((cs & 3) == 0 ? 1 : 0));
+    const int on = cstep & (cnew | ((cs & (kG - 1)) == 0 ? 1 : 0));
     cslot += on;
     cslot = cslot == kSlots ? 0 : cslot;
 #pragma unroll
     for (int q = 0; q < kSl; ++q) {
       const int li = (wave + W * q) % (kScale / 1024);
-      load_lds_if(on, (li < BM / 64 ? xsb : wsb) + (int64_t)(cs >> 2) * 256, soff[q], sl0 + cslot * kScale + li * 1024);
+      load_lds_if(on, (li < BM / 64 ? xsb : wsb) + (int64_t)(cs / kG) * 256, soff[q], sl0 + cslot * kScale + li * 1024);
     }
     cnew = 0;
     cs += cstep;
   };
-  auto load_tile = [&](int q) {
-    load_lds(q < QA ? xb : wb, off[q], l0 + lb * kStage + (q < QA ? (wave + W * q) % (kA / 1024) * 1024 : kA + (wave + W * (q - QA)) % (kB / 1024) * 1024));
+  auto load_tile = [&](int i) {
+    const int t = i / (QA + QB), q = i % (QA + QB);
+    load_lds(q < QA ? xb + t * (1024 * AB) : wb + t * 1024, off[q],
+             l0 + lb * kStage + t * kTile +
+                 (q < QA ? (wave + W * q) % (kA / 1024) * 1024 : kA + (wave + W * (q - QA)) % (kB / 1024) * 1024));
   };
   auto advance = [&]() {  // past the loaded stage
     lb = lb + 1 == NB ? 0 : lb + 1;
     ls += lstep;
-    xb += lstep * (1024 * AB);
-    wb += lstep * 1024;
+    xb += lstep * (T * 1024 * AB);
+    wb += lstep * (T * 1024);
   };
   // Behind the stream's last stage its loads repeat (lstep 0), into buffers that nobody reads any more, so that every stage
   // issues as many.
@@ -212,8 +217,8 @@ __global__ __launch_bounds__(64 * W, OCC * W / 4) void k_gemm_mx(const GemmArgs 
       lstep = 0;
       --ls;
       ls1 = 0x7fffffff;
-      xb -= 1024 * AB;
-      wb -= 1024;
+      xb -= T * 1024 * AB;
+      wb -= T * 1024;
     }
   };
   auto next_scale_unit = [&]() {  // (after next_unit)
@@ -237,23 +242,25 @@ __global__ __launch_bounds__(64 * W, OCC * W / 4) void k_gemm_mx(const GemmArgs 
   const int los = (hi * 64 + 16 * c + r) * 4;
   uint4 fa[2][FI][AB], fb[2][FJ];
   uint32_t sa[2][FI], sb[2][FJ];
-  // read n of the fragments of half h, stage byte t, buffer b, slot sl, into register set h
-  auto read = [&](int n, int h, int b, int sl, int t) {
-    const uint8_t* pa = ring + b * kStage + wmb * (1024 * AB) + loa;
-    const uint8_t* pb = ring + b * kStage + kA + wnb * 1024 + lo;
+  // read n of half tile H of the stage in buffer b, its scales in slot sl at byte t: elements, then (tile 0: the stage's) scales,
+  // into register set H % 2
+  auto read = [&](auto H_c, int n, int b, int sl, int t) __attribute__((always_inline)) {
+    constexpr int H = decltype(H_c)::value, h = H & 1;
+    const uint8_t* pa = ring + b * kStage + (H >> 1) * kTile + wmb * (1024 * AB) + loa;
+    const uint8_t* pb = ring + b * kStage + (H >> 1) * kTile + kA + wnb * 1024 + lo;
     const uint8_t* ps = sring + sl * kScale + los + t + 128 * h;  // (block 2 h + c)
     if (n < FI * AB) {
       const int f = n / AB, e = n % AB;
       fa[h][f][e] = *reinterpret_cast<const uint4*>(pa + f * (2048 * AB) + (AB == 2 ? 1024 * h + 512 * e : 512 * h));
-    } else if (n < FI * AB + FJ) {
+    } else if (n < NF) {
       const int f = n - FI * AB;
       fb[h][f] = *reinterpret_cast<const uint4*>(pb + f * 2048 + 512 * h);
-    } else if (n < FI * AB + FJ + FI) {
-      const int f = n - FI * AB - FJ;
-      sa[h][f] = ps[(wmb + 2 * f) * 256];
+    } else if (n < NF + FI) {
+      const int f = n - NF;
+      sa[h][f] = *reinterpret_cast<const scale_t*>(ps + (wmb + 2 * f) * 256);
     } else {
-      const int f = n - FI * AB - FJ - FI;
-      sb[h][f] = ps[(BM / 16 + wnb + 2 * f) * 256];
+      const int f = n - NF - FI;
+      sb[h][f] = *reinterpret_cast<const scale_t*>(ps + (BM / 16 + wnb + 2 * f) * 256);
     }
   };
   v16f acc[FI][FJ];
@@ -265,30 +272,30 @@ __global__ __launch_bounds__(64 * W, OCC * W / 4) void k_gemm_mx(const GemmArgs 
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
   };
-  // half h of a stage: its products, each followed by its share of the reads of the next half (half 1 - h of buffer b, ...;
-  // behind the stream's last stage they read what nobody uses) and, h = 1, of the loads of the stage at the loading end
-  auto half = [&](auto h_c, int b, int sl, int t) __attribute__((always_inline)) {
-    constexpr int h = decltype(h_c)::value;
+  // half tile H of a stage: its products, each followed by its share of the reads of the next half tile (of buffer b, ...; behind
+  // the stream's last stage they read what nobody uses) and, the stage's last, of the loads of the stage at the loading end
+  auto half = [&](auto H_c, int b, int sl, int t) __attribute__((always_inline)) {
+    constexpr int H = decltype(H_c)::value, h = H & 1, next = (H + 1) % HT;
+    constexpr int NR = NF + (next < 2 ? FI + FJ : 0);
 #pragma unroll
     for (int u = 0; u < NP; ++u) {
       const int i = u / FJ, j = u % FJ;
       acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
           pack_v8i(fb[h][j], zero4()), AB == 2 ? pack_v8i(fa[h][i][0], fa[h][i][AB - 1]) : pack_v8i(fa[h][i][0], zero4()),
-          acc[i][j], 4, ELEM == KRQ_MX_E2M1 ? 4 : 0, 0, static_cast<int>(sb[h][j]), 0, static_cast<int>(sa[h][i]));
-      if (h == 1) {
+          acc[i][j], 4, ELEM == KRQ_MX_E2M1 ? 4 : 0, H >> 1, static_cast<int>(sb[h][j]), H >> 1, static_cast<int>(sa[h][i]));
+      if (H == HT - 1) {
         if (u == 0) load_scales();
 #pragma unroll
         for (int q = u * kLoads / NP; q < (u + 1) * kLoads / NP; ++q) load_tile(q);
       }
 #pragma unroll
-      for (int n = reads_to<NP, NR>(u); n < reads_to<NP, NR>(u + 1); ++n) read(n, 1 - h, b, sl, t);
+      for (int n = reads_to<NP, NR>(u); n < reads_to<NP, NR>(u + 1); ++n)
+        read(std::integral_constant<int, next>{}, n, b, sl, t);
     }
     interleave<0, NP, NR>();
   };
   using yes = std::true_type;
   using no = std::false_type;
-  using h0 = std::integral_constant<int, 0>;
-  using h1 = std::integral_constant<int, 1>;
 
   // A lane's four adjacent columns of a row are 8 bytes in bf16; lanes l and l + 32 exchange halves of two such pieces
   // (v_permlane32_swap), so that each stores 16 bytes. FULL: every row and column lies in the output.
@@ -345,7 +352,7 @@ __global__ __launch_bounds__(64 * W, OCC * W / 4) void k_gemm_mx(const GemmArgs 
   wait_loads<(NB - 1) * kLoads>();
   barrier_lds();
 #pragma unroll
-  for (int n = 0; n < NR; ++n) read(n, 0, 0, 0, unit(unit_of(0)).s0 & 3);
+  for (int n = 0; n < NF + FI + FJ; ++n) read(std::integral_constant<int, 0>{}, n, 0, 0, unit(unit_of(0)).s0 % kG * T);
   int buf = 0, slot = 0;
   int stores = 0;  // the last tile's kStores stores per lane are younger than the next stage's loads
   for (int k = 0, u = unit_of(0), un; u >= 0; ++k, u = un) {
@@ -356,17 +363,22 @@ __global__ __launch_bounds__(64 * W, OCC * W / 4) void k_gemm_mx(const GemmArgs 
     zero();
     // stage s; the loading end is NB stages ahead
     auto stage = [&](bool last) __attribute__((always_inline)) {
-      half(h0{}, buf, slot, s & 3);
+      const int t = s % kG * T;
+      half(std::integral_constant<int, 0>{}, buf, slot, t);
+      if constexpr (T == 2) {
+        half(std::integral_constant<int, 1>{}, buf, slot, t);
+        half(std::integral_constant<int, 2>{}, buf, slot, t);
+      }
       ++s;
       const int sn = last ? sfirst : s;  // the next stage: of this unit, or the next one's first
-      const int on = last || (sn & 3) == 0 ? 1 : 0;
+      const int on = last || sn % kG == 0 ? 1 : 0;
       buf = buf + 1 == NB ? 0 : buf + 1;
       slot = slot + on == kSlots ? 0 : slot + on;
       // the next stage has landed, and once every wave is here none reads this one's buffer any more: refill it
       wait_loads_or<(NB - 2) * kLoads, kStores>(stores);
       stores = 0;
       barrier_lds();
-      half(h1{}, buf, slot, sn & 3);
+      half(std::integral_constant<int, HT - 1>{}, buf, slot, sn % kG * T);
       advance();
     };
 #pragma clang loop unroll(disable)
@@ -491,34 +503,48 @@ int cu_count(int* cus) {
              : KRQ_EHIP;
 }
 
-template <int ELEM, int BM, int BN, int W, int OCC, int NB, bool PART>
+template <int ELEM, int BM, int BN, int W, int OCC, int NB, int T, bool PART>
 void launch(const GemmArgs& g, int cus, hipStream_t s) {
   GemmArgs a = g;
+  a.KS = a.KT / T;
   a.tiles_m = (a.M + BM - 1) / BM;
   a.tiles = a.tiles_m * ((a.N + BN - 1) / BN);
   const int64_t units = (int64_t)a.tiles * a.splits, slots = (int64_t)cus * OCC;
-  hipLaunchKernelGGL((k_gemm_mx<ELEM, BM, BN, W, OCC, NB, PART>), dim3(static_cast<unsigned>(std::min(units, slots))), dim3(64 * W),
+  hipLaunchKernelGGL((k_gemm_mx<ELEM, BM, BN, W, OCC, NB, T, PART>), dim3(static_cast<unsigned>(std::min(units, slots))), dim3(64 * W),
                      0, s, a);
 }
 
+// Two tiles a stage (an even number of tiles, and stages for the buffers) where a stage of one is too short for its
+// barrier and its scalar work: 64 x 64 outputs (us, one / two: 77 x 6,144 x 2,560 8.5 / 7.8, 256 x 2,560 x 4,096 11.4 / 9.3),
+// and e2m1 rows in 256 x 256 (4,096 x 19,456 x 2,560 117.9 / 114.1) and in 128 x 128 with one workgroup per unit, which
+// then takes the unit's whole LDS (1,000 x 2,560 x 9,728 29.7 / 25.0; e4m3 rows 35.2 / 37.4).
 template <int ELEM>
 void launch_plan(const GemmArgs& a, const GemmPlan& p, int cus, hipStream_t s) {
-  constexpr int D = ELEM == KRQ_MX_E2M1 ? 1 : 0;  // e2m1 stages are smaller: one buffer more
+  constexpr bool E2 = ELEM == KRQ_MX_E2M1;
+  constexpr int D = E2 ? 1 : 0;  // e2m1 stages are smaller: one buffer more
+  const bool pairs = a.KT % 2 == 0 && a.KT / 2 / p.splits >= 4;
+  const int64_t tiles = (int64_t)((a.M + p.bm - 1) / p.bm) * ((a.N + p.bn - 1) / p.bn);
   if (a.KT < kMinStages) {
     const int tm = (a.M + 127) / 128;
     hipLaunchKernelGGL((k_gemm_mx_short<ELEM>), dim3(static_cast<unsigned>(tm * ((a.N + 127) / 128))), dim3(256), 0, s, a, tm);
   } else if (p.bm == 256) {
-    launch<ELEM, 256, 256, 8, 1, 3 + D, false>(a, cus, s);
+    if constexpr (E2)
+      if (pairs) return launch<ELEM, 256, 256, 8, 1, 2, 2, false>(a, cus, s);
+    launch<ELEM, 256, 256, 8, 1, 3 + D, 1, false>(a, cus, s);
   } else if (p.bm == 192) {
-    launch<ELEM, 192, 256, 8, 1, 3 + D, false>(a, cus, s);
+    launch<ELEM, 192, 256, 8, 1, 3 + D, 1, false>(a, cus, s);
   } else if (p.bm == 128 && p.bn == 256) {
-    launch<ELEM, 128, 256, 4, 2, 2, false>(a, cus, s);
+    launch<ELEM, 128, 256, 4, 2, 2, 1, false>(a, cus, s);
   } else if (p.bm == 128) {
-    launch<ELEM, 128, 128, 4, 2, 3 + D, false>(a, cus, s);
+    if constexpr (E2)
+      if (pairs && tiles <= cus) return launch<ELEM, 128, 128, 4, 1, 4, 2, false>(a, cus, s);
+    launch<ELEM, 128, 128, 4, 2, 3 + D, 1, false>(a, cus, s);
   } else if (p.splits == 1) {
-    launch<ELEM, 64, 64, 4, 2, 4, false>(a, cus, s);
+    if (pairs) launch<ELEM, 64, 64, 4, 2, 3 + D, 2, false>(a, cus, s);
+    else launch<ELEM, 64, 64, 4, 2, 4, 1, false>(a, cus, s);
   } else {
-    launch<ELEM, 64, 64, 4, 2, 4, true>(a, cus, s);
+    if (pairs) launch<ELEM, 64, 64, 4, 2, 3 + D, 2, true>(a, cus, s);
+    else launch<ELEM, 64, 64, 4, 2, 4, 1, true>(a, cus, s);
   }
 }
 

@@ -262,7 +262,9 @@ def test_outputs_end_where_they_should(dev):
                                    (4096, 4096, 640), (4000, 2560, 544), (4000, 6100, 640), (4000, 6104, 640), (500, 2560, 2176),
                                    (700, 1100, 1152),
                                    # K in parts: whole and ragged columns
-                                   (77, 520, 8224), (40, 99, 16384), (64, 2560, 9728)])
+                                   (77, 520, 8224), (40, 99, 16384), (64, 2560, 9728), (77, 520, 8320),
+                                   # odd and even numbers of tiles of K: one and two a stage
+                                   (4096, 4096, 1024), (1000, 2560, 1024), (1000, 2560, 1152), (200, 640, 1280), (200, 640, 1184)])
 def test_gemm(dev, M, N, K, elem):
     q, wv = weight(N, K, 3, dev, spread_out=M < 77)
     x = bf((M, K), 4)
