@@ -111,7 +111,7 @@ __global__ __launch_bounds__(64 * W, OCC * W / 4) void k_gemm_mx(const GemmArgs 
   constexpr int NP = FI * FJ, NF = FI * AB + FJ;           // products of a half tile, LDS reads of its elements
   constexpr int HT = 2 * T, kG = 4 / T;                    // half tiles of a stage; stages of a scale group
   typedef std::conditional_t<T == 1, uint8_t, uint16_t> scale_t;  // a block's scales in a stage
-  constexpr int kStores = PART ? NP * 4 : NP * 2;
+  constexpr int kStores = PART ? NP * 4 : NP * 2, JP = FJ % 2 == 0 ? 2 : 1;
   static_assert(NB >= 2 && NB <= 4 && (T == 1 || T == 2) && BM % 64 == 0 && BN % (16 * W) == 0, "tile shape");
   // Scales are loaded for the stage kLag before the tiles' (three buffers and more: they still come a whole stage early),
   // so that a slot can be filled again when all of the next kSlots groups (of one stage at least each) lie ahead of it.
@@ -297,8 +297,11 @@ __global__ __launch_bounds__(64 * W, OCC * W / 4) void k_gemm_mx(const GemmArgs 
   using yes = std::true_type;
   using no = std::false_type;
 
-  // A lane's four adjacent columns of a row are 8 bytes in bf16; lanes l and l + 32 exchange halves of two such pieces
-  // (v_permlane32_swap), so that each stores 16 bytes. FULL: every row and column lies in the output.
+  // A lane ends with four adjacent columns (8 bytes in bf16) of row l % 32 in every eighth column. Exchanges turn that into
+  // whole lines: lanes l and l + 32 (v_permlane32_swap) make 16 bytes each, odd and even sixteens (v_permlane16_swap) 64 bytes of
+  // sixteen rows per store, and lanes l and l ^ 8 of two 32-column pieces (DPP) 128 bytes of eight rows (against
+  // stores of 32 bytes of thirty-two rows: 4,096 x 19,456 x 2,560, e2m1 rows, 117.2 -> 114.4 us; without its stores, whose
+  // 159 MB all units write at once, it takes 92). FULL: every row and column lies in the output.
   auto store = [&](auto full_c, int m0, int n0, int sp) {
     constexpr bool FULL = decltype(full_c)::value;
     int le = lane;  // (opaque: addresses are computed here, not hoisted out of the stream and kept)
@@ -324,18 +327,55 @@ __global__ __launch_bounds__(64 * W, OCC * W / 4) void k_gemm_mx(const GemmArgs 
             }
           }
         } else if (FULL || a.wide) {
+          if (j % JP == 0) {
+            uint32_t x[JP][4], y[JP][4];  // rows 0 .. 15 and 16 .. 31 of the pieces
 #pragma unroll
-          for (int g = 0; g < 4; g += 2) {
-            uint32_t v[4];
+            for (int q = 0; q < JP; ++q) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              v[e] = pack_bf16x2(acc[i][j][4 * g + 2 * e], acc[i][j][4 * g + 2 * e + 1]);
-            // (v[0], v[1]: columns 4 c .. of piece g; v[2], v[3]: of piece g + 1)
-            const auto s0 = __builtin_amdgcn_permlane32_swap(v[0], v[2], false, false);
-            const auto s1 = __builtin_amdgcn_permlane32_swap(v[1], v[3], false, false);
-            const int col = n + 8 * (g + ce);
-            if (FULL || (m < a.M && col < a.N))
-              *reinterpret_cast<uint4*>(a.out + (int64_t)m * a.N + col) = make_uint4(s0[0], s1[0], s0[1], s1[1]);
+              for (int g = 0; g < 2; ++g) {
+                const v16f& c16 = acc[i][j + q];
+                const auto lo = __builtin_amdgcn_permlane32_swap(pack_bf16x2(c16[8 * g], c16[8 * g + 1]),
+                                                                 pack_bf16x2(c16[8 * g + 4], c16[8 * g + 5]), false, false);
+                const auto hi = __builtin_amdgcn_permlane32_swap(pack_bf16x2(c16[8 * g + 2], c16[8 * g + 3]),
+                                                                 pack_bf16x2(c16[8 * g + 6], c16[8 * g + 7]), false, false);
+                uint32_t* o = g == 0 ? x[q] : y[q];
+                o[0] = lo[0];
+                o[1] = hi[0];
+                o[2] = lo[1];
+                o[3] = hi[1];
+              }
+#pragma unroll
+              for (int d = 0; d < 4; ++d) {
+                const auto w = __builtin_amdgcn_permlane16_swap(x[q][d], y[q][d], false, false);
+                x[q][d] = w[0];
+                y[q][d] = w[1];
+              }
+            }
+            // sixteen l / 16 now holds columns 8 ((l / 32) + 2 ((l / 16) % 2)) .. + 7
+            const int r16 = le & 15, col = n + 8 * (ce + 2 * ((le >> 4) & 1));
+            auto put = [&](int row, int cc, const uint32_t* v) {
+              if (FULL || (row < a.M && cc < a.N))
+                *reinterpret_cast<uint4*>(a.out + (int64_t)row * a.N + cc) = make_uint4(v[0], v[1], v[2], v[3]);
+            };
+            const int row0 = m0 + 16 * wmb + 32 * i;
+            if constexpr (JP == 2) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                uint32_t u[4], v[4];
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                  const uint32_t p0 = h == 0 ? x[0][d] : y[0][d], p1 = h == 0 ? x[JP - 1][d] : y[JP - 1][d];
+                  u[d] = take_ror8<0xc>(p0, p1);
+                  v[d] = take_ror8<0x3>(p1, p0);
+                }
+                const int row = row0 + 16 * h + (r16 & 7), cc = col + 32 * (r16 >> 3);
+                put(row, cc, u);
+                put(row + 8, cc, v);
+              }
+            } else {
+              put(row0 + r16, col, x[0]);
+              put(row0 + 16 + r16, col, y[0]);
+            }
           }
         } else if (m < a.M) {
 #pragma unroll

@@ -425,7 +425,9 @@ int launch_mode(const MxArgs& a, bool bf16, int splits, hipStream_t s) {
     return gw == 1 ? launch_held<ELEM, 0, 1, MODE, P, 1>(a, splits, nw, s) : launch_held<ELEM, 0, 1, MODE, P, 2>(a, splits, nw, s);
   }
   const int ns = std::max(std::min(per, kStreamWaves), least);
-  return a.M <= 16 ? launch_stream<ELEM, 1, MODE, P, 2>(a, splits, ns, s) : launch_stream<ELEM, 2, MODE, P, 1>(a, splits, ns, s);
+  // (two row tiles and single row blocks: two groups in flight 12.45 -> 11.1 us at 2,560 x 16,384, M = 32; with pairs of row
+  // blocks registers run out, 15.2 -> 16.7 for SwiGLU over 16,384 x 6,144)
+  return a.M <= 16 ? launch_stream<ELEM, 1, MODE, P, 2>(a, splits, ns, s) : launch_stream<ELEM, 2, MODE, P, P == 1 ? 2 : 1>(a, splits, ns, s);
 }
 
 template <int MODE, int P>
