@@ -24,6 +24,9 @@ using namespace krq;
 namespace {
 
 typedef float v16f __attribute__((ext_vector_type(16)));
+// 16 bytes at any element's address (rows of an odd N start anywhere; global stores take any address)
+typedef v4u v4u_any __attribute__((aligned(2)));
+typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
 
 // 32-bit LDS address of a pointer into a __shared__ array, wave-uniform
 KRQ_DEV uint32_t lds_at(const uint8_t* p) {
@@ -94,7 +97,6 @@ struct GemmArgs {
   const uint8_t *x, *xs, *w, *ws;
   int M, N, KT, KS, groups, mbs, nbs;  // KT tiles of K in KS stages; mbs, nbs: row blocks of x and w
   int tiles_m, tiles, splits;
-  int wide;                        // out's rows start on 16 bytes: N % 8 == 0
   float* part;                     // fp32 [splits][M][N] (PART)
   uint16_t* out;
 };
@@ -317,16 +319,17 @@ __global__ __launch_bounds__(64 * W, OCC * W / 4) void k_gemm_mx(const GemmArgs 
           float* p = a.part + ((int64_t)sp * a.M + m) * a.N + n + 4 * ce;
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            if (FULL || (a.wide && m < a.M && n + 8 * g + 4 * ce < a.N)) {
-              *reinterpret_cast<float4*>(p + 8 * g) =
-                  make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
-            } else if (!a.wide && m < a.M) {
+            const int left = a.N - (n + 8 * g + 4 * ce);  // columns from here on
+            if (FULL || (m < a.M && left >= 4)) {
+              *reinterpret_cast<v4f_any*>(p + 8 * g) =
+                  v4f{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+            } else if (m < a.M) {
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                if (n + 8 * g + 4 * ce + e < a.N) p[8 * g + e] = acc[i][j][4 * g + e];
+                if (e < left) p[8 * g + e] = acc[i][j][4 * g + e];
             }
           }
-        } else if (FULL || a.wide) {
+        } else {
           if (j % JP == 0) {
             uint32_t x[JP][4], y[JP][4];  // rows 0 .. 15 and 16 .. 31 of the pieces
 #pragma unroll
@@ -354,8 +357,14 @@ __global__ __launch_bounds__(64 * W, OCC * W / 4) void k_gemm_mx(const GemmArgs 
             // sixteen l / 16 now holds columns 8 ((l / 32) + 2 ((l / 16) % 2)) .. + 7
             const int r16 = le & 15, col = n + 8 * (ce + 2 * ((le >> 4) & 1));
             auto put = [&](int row, int cc, const uint32_t* v) {
-              if (FULL || (row < a.M && cc < a.N))
-                *reinterpret_cast<uint4*>(a.out + (int64_t)row * a.N + cc) = make_uint4(v[0], v[1], v[2], v[3]);
+              uint16_t* o = a.out + (int64_t)row * a.N + cc;
+              if (FULL || (row < a.M && cc + 8 <= a.N)) {
+                *reinterpret_cast<v4u_any*>(o) = v4u{v[0], v[1], v[2], v[3]};
+              } else if (row < a.M) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  if (cc + e < a.N) o[e] = static_cast<uint16_t>(v[e >> 1] >> (16 * (e & 1)));
+              }
             };
             const int row0 = m0 + 16 * wmb + 32 * i;
             if constexpr (JP == 2) {
@@ -376,12 +385,6 @@ __global__ __launch_bounds__(64 * W, OCC * W / 4) void k_gemm_mx(const GemmArgs 
               put(row0 + r16, col, x[0]);
               put(row0 + 16 + r16, col, y[0]);
             }
-          }
-        } else if (m < a.M) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int col = n + 8 * (e >> 2) + 4 * ce + (e & 3);
-            if (col < a.N) a.out[(int64_t)m * a.N + col] = f32_to_bf16(acc[i][j][e]);
           }
         }
       }
@@ -430,7 +433,7 @@ __global__ __launch_bounds__(64 * W, OCC * W / 4) void k_gemm_mx(const GemmArgs 
 #pragma clang loop unroll(disable)
     while (s < s1) stage(s + 1 == s1);
     const int m0 = cur.tm * BM, n0 = cur.tn * BN, sp = PART ? scalar(u / a.tiles) : 0;
-    if (m0 + BM <= a.M && n0 + BN <= a.N && a.wide) {
+    if (m0 + BM <= a.M && n0 + BN <= a.N) {
       store(yes{}, m0, n0, sp);
       stores = 1;
     } else {
@@ -636,7 +639,6 @@ extern "C" int krq_gemm_mxfp4(const void* x, const void* x_scale, int x_kind, in
   a.mbs = static_cast<int>((M + 15) / 16);
   a.nbs = static_cast<int>((N + 15) / 16);
   a.splits = p.splits;
-  a.wide = N % 8 == 0 && aligned16(out);
   a.part = (float*)((uint8_t*)ws + rows);
   a.out = (uint16_t*)out;
   hipStream_t s = (hipStream_t)stream;

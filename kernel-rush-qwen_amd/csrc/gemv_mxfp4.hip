@@ -395,7 +395,7 @@ template <int ELEM, int XSRC, int MT, int MODE, int P, int GW>
 int launch_held(MxArgs a, int splits, int nw, hipStream_t s) {
   a.sets = sets_of(a, MODE, P);
   a.nw = nw;
-  const int most = a.sets * splits <= kHeldOnce ? a.sets : kHeldMost / splits + 1;
+  const int most = (int64_t)a.sets * splits <= kHeldOnce ? a.sets : kHeldMost / splits + 1;
   const int rounds = (a.sets + most - 1) / most, blocks = (a.sets + rounds - 1) / rounds;  // as many sets for each
   constexpr size_t row = (ELEM == KRQ_MX_E2M1 ? 256 : 512) + 16;
   const size_t smem = std::max((size_t)2 * nw * P * MT * 1024, XSRC > 0 ? nw * (XSRC == 4 ? 4 : 1) * row : 0);

@@ -288,5 +288,5 @@ def embedding(ids, q, scale=1.0):
     n = ids.numel()
     if n:
         _call(out.get_device(), "krq_embed_mxfp4", ids.data_ptr(), int(ids.dtype == torch.int64), n, w4.data_ptr(), scale_codes.data_ptr(), N, K,
-              scale, out.data_ptr())
+              float(scale), out.data_ptr())
     return out

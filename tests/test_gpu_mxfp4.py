@@ -170,7 +170,8 @@ def test_gemv(dev, M, N, K, elem):
                                          # one or two groups per wave, operands beside the weights
                                          (1, 18000, 1056, 1), (8, 16400, 2560, 1), (16, 17000, 5632, 1), (32, 16500, 2080, 1),
                                          (1, 9000, 10240, 1), (3, 100, 5152, 1), (20, 10000, 4096, 1), (32, 300, 4608, 1),
-                                         (16, 96, 10272, 1), (1, 9000, 6016, 2), (32, 64, 12288, 3)])
+                                         (16, 96, 10272, 1), (1, 9000, 6016, 2), (32, 64, 12288, 3),
+                                         (32, 16500, 4096, 1), (9, 48, 32, 1)])
 def test_gemv_large_and_split(dev, M, N, K, split):
     q, wv = weight(N, K, 1, dev)
     x = bf((M, K), 2)
@@ -286,6 +287,42 @@ def test_empty_rows(dev):
         X.quantize(none)
     with pytest.raises(ValueError):
         lmhead.lm_head_argmax(none, q)
+
+
+# ------------------------------------------------------------------------------------------ sizes past 32 bits
+def test_far_offsets(dev):
+    """2.2 million rows of 4,096: 18 GB of bf16, 4.5 GB of codes and of tiles, more row blocks than the second axis of a
+    grid. The last rows are what they are on their own."""
+    N, K = 2_200_003, 4096
+    w = torch.empty((N, K), device=dev, dtype=torch.bfloat16).normal_(0, 0.02, generator=torch.Generator(device=dev).manual_seed(1))
+    tail = w[-115:].clone()
+    q, small = X.quantize(w), X.quantize(tail)
+    assert torch.equal(q[0][-115:], small[0]) and torch.equal(q[1][-115:], small[1])
+    p = X.pack(q[0], q[1])
+    assert torch.equal(p.tiled[-(1 << 20):], q.tiled[-(1 << 20):]) and torch.equal(p.tiled_scale[-(1 << 20):], q.tiled_scale[-(1 << 20):])
+    del p, w
+    want = X.dequantize(small)
+    assert torch.equal(X.dequantize(q)[-115:], want)
+    ids = torch.arange(N - 115, N, device=dev)
+    assert torch.equal(X.embedding(ids, q), want)
+    for M in (1, 20):
+        x = bf((M, K), M).to(dev)
+        assert torch.equal(X.linear_mxfp4(x, q)[:, -115:], X.linear_mxfp4(x, small))
+
+
+def test_far_rows(dev):
+    """600,001 rows through the prefill product: 9.8 GB of output; and more rows than a grid's second axis of row blocks."""
+    M, N, K = 600_001, 8192, 512
+    q = X.quantize(bf((N, K), 1, 0.02).to(dev))
+    x = torch.empty((M, K), device=dev, dtype=torch.bfloat16).normal_(generator=torch.Generator(device=dev).manual_seed(2))
+    for elem in ("e4m3", "e2m1"):
+        y = X.linear_mxfp4(x, q, elem)
+        assert torch.equal(y[-77:], X.linear_mxfp4(x[-77:].clone(), q, elem)) and torch.equal(y[:77], X.linear_mxfp4(x[:77].clone(), q, elem))
+        del y
+    x = x.view(-1, 32)[:1_100_000]
+    assert torch.equal(X.dequantize(X.quant_rows(x))[-99:], X.dequantize(X.quant_rows(x[-99:].clone())))
+    ids = torch.randint(8192, (300_001,), device=dev)
+    assert torch.equal(X.embedding(ids, q)[-99:], X.embedding(ids[-99:].clone(), q))
 
 
 # ------------------------------------------------------------------------------------------ lm head
