@@ -181,9 +181,9 @@ def quant_rows(x, elem="e4m3"):
     e = _elem(elem)
     if M == 0:
         return MXRows(x.new_empty((0,), dtype=torch.uint8), 0, (0, K), elem)
-    lib = L.lib()
-    at = lib.krq_mx_tiled_bytes(M, K, e)  # (whole KiB)
-    data = x.new_empty((at + lib.krq_mx_scale_bytes(M, K),), dtype=torch.uint8)
+    mb = (M + 15) >> 4  # krq_mx_tiled_bytes and krq_mx_scale_bytes: tiles of 1 or 2 KiB, 256 bytes of scales per four tiles
+    at = (mb * ((K + 127) >> 7)) << (10 + e)
+    data = x.new_empty((at + (mb * ((K + 511) >> 9) << 8),), dtype=torch.uint8)
     p = data.data_ptr()
     _call(x.get_device(), "krq_quant_mx_rows", x.data_ptr(), M, K, ld, e, p, p + at)
     return MXRows(data, at, (M, K), elem)

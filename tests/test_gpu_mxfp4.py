@@ -238,6 +238,17 @@ def test_nan_stays_in_its_row_and_column(dev, M):
     check(torch.from_numpy(np.where(bad, ref, y)), ref, E, "rest")
 
 
+@pytest.mark.parametrize("ex,ew", [(60, -70), (-110, 100), (100, -20), (-60, -40)])
+def test_scales_far_from_one(dev, ex, ew):
+    K, N = 544, 48
+    w, x = bf((N, K), 1) * 2.0 ** ew, bf((40, K), 2) * 2.0 ** ex
+    q = X.quantize(w.to(dev))
+    ref, E = reference(rounded(x, "e4m3"), rounded(w, "e2m1"))
+    check(X.linear_mxfp4(x.to(dev), q), ref, E, "gemm")
+    for M in (1, 6, 20):
+        check(X.linear_mxfp4(x[:M].to(dev), q), ref[:M], E[:M], M)
+
+
 def test_outputs_end_where_they_should(dev):
     """Through the C ABI into larger buffers: nothing behind the last row is touched."""
     M, N, K = 19, 37, 544
