@@ -30,7 +30,7 @@
  *               64 + 16 g .. + 15 in the second. Scales: [ceil(rows / 16)][ceil(K / 512)][64 lanes], 4
  *               bytes a lane, byte t of lane 16 g + r that of row r, k = 512 s + 128 t + 32 g .. + 31.
  *               Rows past the last and k past K hold zeros. krq_mx_tiled_bytes / krq_mx_scale_bytes
- *               give the sizes.
+ *               give the sizes; both start on 16 bytes.
  *   partials  - split-K output: fp32 [split, M, N]; the consumer sums slices 0..split-1 in that
  *               order and rounds once to bf16 (reference engine/kernels/ops.py:29-39).
  */
@@ -429,7 +429,7 @@ int64_t krq_mx_scale_bytes(int64_t M, int64_t K);
 
 /*
  * MXFP4 weight quantizer (the 4-bit counterpart of krq_quant_fp8_rows; no reference counterpart):
- * w bf16 [N, K], rows ldw elements apart, to e2m1 blocks: w4 [N, K / 2] (element 2 i in the low half of
+ * w bf16 [N, K], rows ldw elements apart, to e2m1 blocks: w4 [N, K / 2] on 16 bytes (element 2 i in the low half of
  * byte i) and scale [N, K / 32] row-major, and the same in the mx tiled layout. K % 32 == 0; w and its
  * rows start on 16 bytes.
  */

@@ -8,6 +8,11 @@
 // k_gemv_mx_held: each wave holds its groups' activation operands in registers (GW groups, MT row tiles) for the whole launch, and the
 // workgroup walks over sets of P row blocks (SwiGLU: a gate block and its up block), the next set's weights in flight.
 // k_gemv_mx_stream: longer rows, more of them; activation tiles are loaded beside the weights.
+//
+// Large launches are bound by the weights' read (the head at one row, 151,936 x 2,560: 33.4 us, 6.2 TB/s, the card's read rate;
+// at 16 38.2), small ones by a launch and a round trip to memory (2,560 x 4,096, M = 1: 3.4 us; SwiGLU over 19,456 x 2,560, M = 5:
+// 8.7, of which 1.3 round the rows), the streaming ones by the rows that every workgroup reads again from L2 (2,560 x
+// 9,728, M = 32: 8.5 us, 311 KB of rows beside 83 KB of weights).
 #include <algorithm>
 
 #include "mx_common.h"
@@ -147,7 +152,7 @@ __global__ __launch_bounds__(held_waves(MT) * 64) void k_gemv_mx_held(const MxAr
   const int splits = gridDim.y, sp = blockIdx.y;
   const int g0 = a.groups * sp / splits, g1 = a.groups * (sp + 1) / splits;  // this split's groups
   const int n = (a.sets - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
-  // group j of the wave (past the split's last: it again, its operands zero)
+  // group j of the wave (past the split's last: it again, to load from; its products are skipped)
   auto group_of = [&](int j) { return min(g0 + wave + j * nw, g1 - 1); };
 
   uint4 av[GW][MT][4 * AB];
@@ -391,6 +396,10 @@ __global__ __launch_bounds__(kStreamWaves * 64) void k_gemv_mx_stream(const MxAr
 
 int sets_of(const MxArgs& a, int mode, int P) { return mode == KRQ_OUT_SWIGLU ? a.nrb : (a.nrb + P - 1) / P; }
 
+// Row blocks of a set: the head takes pairs (151,936 x 2,560, single / pairs, us a call: M = 1 44.5 / 37.9, M = 16 55.3 / 46.3,
+// M = 32 101 / 58), the other outputs single ones (19,456 x 2,560, M = 16 7.5 / 8.5; 65,536 x 2,560, M = 1 17.1 / 17.0).
+constexpr int set_blocks(int mode) { return mode == KRQ_OUT_SWIGLU || mode == kOutArgmax ? 2 : 1; }
+
 template <int ELEM, int XSRC, int MT, int MODE, int P, int GW>
 int launch_held(MxArgs a, int splits, int nw, hipStream_t s) {
   a.sets = sets_of(a, MODE, P);
@@ -400,7 +409,7 @@ int launch_held(MxArgs a, int splits, int nw, hipStream_t s) {
   constexpr size_t row = (ELEM == KRQ_MX_E2M1 ? 256 : 512) + 16;
   const size_t smem = std::max((size_t)2 * nw * P * MT * 1024, XSRC > 0 ? nw * (XSRC == 4 ? 4 : 1) * row : 0);
   hipLaunchKernelGGL((k_gemv_mx_held<ELEM, XSRC, MT, MODE, P, GW>), dim3(blocks, splits), dim3(64 * nw), smem, s, a);
-  return blocks;
+  return blocks * P;
 }
 
 template <int ELEM, int MT, int MODE, int P, int U>
@@ -408,21 +417,27 @@ int launch_stream(MxArgs a, int splits, int nw, hipStream_t s) {
   a.sets = sets_of(a, MODE, P);
   a.nw = nw;
   hipLaunchKernelGGL((k_gemv_mx_stream<ELEM, MT, MODE, P, U>), dim3(a.sets, splits), dim3(64 * nw), (size_t)nw * P * MT * 1024, s, a);
-  return a.sets;
+  return a.sets * P;
 }
 
-// Launches a mode; returns the workgroups of a split.
-template <int ELEM, int MODE, int P>
+// Launches a mode; returns the row blocks that a split's workgroups take at a time (the head's candidates of a row). One row tile of
+// at most 20 groups a split is held, more streams (stream / held, us a call: 2,560 x 9,728, M = 1 9.3 / 5.2, M = 16 9.4 / 9.1;
+// SwiGLU over 19,456 x 6,400, M = 1 21.0 / 14.2).
+template <int ELEM, int MODE>
 int launch_mode(const MxArgs& a, bool bf16, int splits, hipStream_t s) {
   const int per = (a.groups + splits - 1) / splits;  // groups of the longest split
   const int gw = (per + kHeldWaves - 1) / kHeldWaves, least = MODE == kOutArgmax ? kArgmaxWaves : 1;
   const int nw = std::max((per + gw - 1) / gw, least);
+  constexpr int P = set_blocks(MODE);
+  // the head with two groups a wave: single row blocks, of which two sets are in flight (50,000 x 6,400, pairs / single, us a
+  // call: M = 1 37.6 / 32.4, M = 16 45.8 / 38.3)
+  constexpr int P2 = MODE == kOutArgmax ? 1 : P;
   if (a.M > 16 && per <= held_waves(2)) return launch_held<ELEM, 0, 2, MODE, P, 1>(a, splits, nw, s);
   if (gw <= 2 && a.M <= 16) {
     if (bf16 && a.M == 1)
-      return gw == 1 ? launch_held<ELEM, 1, 1, MODE, P, 1>(a, splits, nw, s) : launch_held<ELEM, 1, 1, MODE, P, 2>(a, splits, nw, s);
+      return gw == 1 ? launch_held<ELEM, 1, 1, MODE, P, 1>(a, splits, nw, s) : launch_held<ELEM, 1, 1, MODE, P2, 2>(a, splits, nw, s);
     if (bf16) return launch_held<ELEM, 4, 1, MODE, P, 1>(a, splits, nw, s);
-    return gw == 1 ? launch_held<ELEM, 0, 1, MODE, P, 1>(a, splits, nw, s) : launch_held<ELEM, 0, 1, MODE, P, 2>(a, splits, nw, s);
+    return gw == 1 ? launch_held<ELEM, 0, 1, MODE, P, 1>(a, splits, nw, s) : launch_held<ELEM, 0, 1, MODE, P2, 2>(a, splits, nw, s);
   }
   const int ns = std::max(std::min(per, kStreamWaves), least);
   // (two row tiles and single row blocks: two groups in flight 12.45 -> 11.1 us at 2,560 x 16,384, M = 32; with pairs of row
@@ -430,9 +445,9 @@ int launch_mode(const MxArgs& a, bool bf16, int splits, hipStream_t s) {
   return a.M <= 16 ? launch_stream<ELEM, 1, MODE, P, 2>(a, splits, ns, s) : launch_stream<ELEM, 2, MODE, P, P == 1 ? 2 : 1>(a, splits, ns, s);
 }
 
-template <int MODE, int P>
+template <int MODE>
 int launch_elem(const MxArgs& a, int elem, bool bf16, int splits, hipStream_t s) {
-  return elem == KRQ_MX_E2M1 ? launch_mode<KRQ_MX_E2M1, MODE, P>(a, bf16, splits, s) : launch_mode<KRQ_MX_E4M3, MODE, P>(a, bf16, splits, s);
+  return elem == KRQ_MX_E2M1 ? launch_mode<KRQ_MX_E2M1, MODE>(a, bf16, splits, s) : launch_mode<KRQ_MX_E4M3, MODE>(a, bf16, splits, s);
 }
 
 // bf16 rows that a launch rounds itself: one whose groups its waves hold, or a few over one group per wave. Rounded before /
@@ -461,7 +476,8 @@ int gemv_mx_run(const char* what, const void* x, const void* x_scale, int x_kind
   const int64_t rows = x_kind == KRQ_MX_X_BF16 && !bf16 ? mx_rows_bytes(elem, M, K) : 0;
   KRQ_REQUIRE(x_kind == KRQ_MX_X_BF16 || x_scale, "%s: tiled rows need their scales", what);
   KRQ_REQUIRE(x_kind != KRQ_MX_X_BF16 || (ldx >= K && ldx % 8 == 0), "%s: rows of x must start on 16 bytes (ldx=%lld)", what, (long long)ldx);
-  KRQ_REQUIRE(aligned16(x) && aligned16(w) && aligned16(ws), "%s: x, w and ws must start on 16 bytes", what);
+  KRQ_REQUIRE(aligned16(x) && aligned16(x_scale) && aligned16(w) && aligned16(w_scale) && aligned16(ws),
+              "%s: x, w, their scales and ws must start on 16 bytes", what);
   KRQ_REQUIRE(rows == 0 || (ws && ws_bytes >= rows), "%s: bf16 rows need a workspace of %lld bytes", what, (long long)rows);
   const int groups = static_cast<int>(mx_groups(K));
   KRQ_REQUIRE(split >= 1 && split <= groups && split <= kMxSplitMax, "%s: split=%d of %d groups of 512", what, split, groups);
@@ -490,12 +506,10 @@ int gemv_mx_run(const char* what, const void* x, const void* x_scale, int x_kind
   a.nrb = static_cast<int>((a.NO + 15) / 16);
   a.sets = a.nw = 0;
   hipStream_t s = (hipStream_t)stream;
-  const bool wide = a.nrb >= 1024;  // enough row blocks for pairs
-  if (mode == KRQ_OUT_SWIGLU) launch_elem<KRQ_OUT_SWIGLU, 2>(a, elem, bf16, split, s);
-  else if (mode == KRQ_OUT_PARTIAL) launch_elem<KRQ_OUT_PARTIAL, 1>(a, elem, bf16, split, s);
-  else if (mode == kOutArgmax) *cands = 2 * launch_elem<kOutArgmax, 2>(a, elem, bf16, split, s);
-  else if (wide) launch_elem<KRQ_OUT_BF16, 2>(a, elem, bf16, split, s);
-  else launch_elem<KRQ_OUT_BF16, 1>(a, elem, bf16, split, s);
+  if (mode == KRQ_OUT_SWIGLU) launch_elem<KRQ_OUT_SWIGLU>(a, elem, bf16, split, s);
+  else if (mode == KRQ_OUT_PARTIAL) launch_elem<KRQ_OUT_PARTIAL>(a, elem, bf16, split, s);
+  else if (mode == kOutArgmax) *cands = launch_elem<kOutArgmax>(a, elem, bf16, split, s);
+  else launch_elem<KRQ_OUT_BF16>(a, elem, bf16, split, s);
   return krq_check_launch(what);
 }
 

@@ -12,7 +12,8 @@ FP8 heads take the activation scaling of the weight's form:
       engine.py:504-505): exactly linear_fp8(h, lm8) followed by torch.argmax (engine.py:989,
       :1022) - one ActScale over all of h (at M == 1 the same as per token, so inside the GEMV),
       or the given ActScale / SharedScale `a`.
-MXFP4 heads take h in e4m3 blocks (mxfp4.quant_rows), rounded inside the GEMV up to eight rows.
+MXFP4 heads take h in e4m3 blocks (mxfp4.quant_rows), rounded inside the GEMV where it takes bf16 rows
+(one of up to 10,240 k, eight of up to 5,120), else by a launch before it.
 """
 
 import torch
@@ -68,9 +69,8 @@ def _mxfp4_head(h, q, return_logits):
     idx = t.new_empty((M,), dtype=torch.int64)
     logits = t.new_empty((M, V), dtype=torch.bfloat16) if return_logits else None
     ws = t.new_empty((L.lib().krq_lmhead_mxfp4_ws_bytes(kind, e, M, V, K),), dtype=torch.uint8)
-    dev, w, wscale = q.operand
-    _mxfp4._call(dev, "krq_lmhead_argmax_mxfp4", p, scale, kind, e, ld, w, wscale, M, V, K, L.ptr(logits), ws.data_ptr(), ws.numel(),
-                 idx.data_ptr())
+    _mxfp4._call(t.get_device(), "krq_lmhead_argmax_mxfp4", p, scale, kind, e, ld, q.tiled.data_ptr(), q.tiled_scale.data_ptr(), M, V, K,
+                 L.ptr(logits), ws.data_ptr(), ws.numel(), idx.data_ptr())
     return (idx, logits) if return_logits else idx
 
 

@@ -35,8 +35,6 @@ class MXFP4Weight(tuple):
         self = super().__new__(cls, (w4, scale))
         self.tiled, self.tiled_scale = tiled, tiled_scale
         self.shape = (w4.shape[0], 2 * w4.shape[1])
-        # what every product on this weight passes on: its device and the addresses of its own tiles
-        self.operand = (tiled.get_device(), tiled.data_ptr(), tiled_scale.data_ptr())
         return self
 
 
@@ -69,7 +67,7 @@ _cuda = torch._C
 
 def _call(dev, name, *args):
     """L.call on device dev (made current for it where it is not) and torch's current stream of it. A call on a
-    few rows is host work as much as a launch (a product of one row 8.1 us, 3.6 of them the kernel's; 5.9 with
+    few rows is host work as much as a launch (a product of one row 8.1 us, 3.4 of them the kernel's; 6.1 with
     the library's function taken once and no Stream or device objects made)."""
     fn = _functions.get(name)
     if fn is None:
@@ -202,7 +200,7 @@ def _operand(x, q, elem):
     else:
         t, ld = _bf16_rows(x, "rows [M, K]")
         M, p, scale, kind = t.shape[0], t.data_ptr(), None, L.MX_X_BF16
-    if t.get_device() != q.operand[0]:
+    if t.get_device() != q.tiled.get_device():
         _same_device(t, q.tiled)
     return t, p, scale, kind, ELEMS[elem] if elem in ELEMS else _elem(elem), ld, M
 
@@ -231,8 +229,8 @@ def _decode(x, q, split, mode, elem):
         nbytes = L.lib().krq_gemv_mxfp4_ws_bytes(kind, e, M, K, split)
         if nbytes > 0:
             ws = t.new_empty((nbytes,), dtype=torch.uint8)
-    dev, w, wscale = q.operand
-    _call(dev, "krq_gemv_mxfp4", p, scale, kind, e, ld, w, wscale, M, N, K, split, mode, L.ptr(ws), nbytes, out.data_ptr())
+    _call(t.get_device(), "krq_gemv_mxfp4", p, scale, kind, e, ld, q.tiled.data_ptr(), q.tiled_scale.data_ptr(), M, N, K, split, mode,
+          L.ptr(ws), nbytes, out.data_ptr())
     return out
 
 
@@ -259,13 +257,14 @@ def gemm_mxfp4(x, q, elem="e4m3"):
     out = t.new_empty((M, N), dtype=torch.bfloat16)
     if M == 0:
         return out
-    dev, w, wscale = q.operand
+    dev = t.get_device()
     with torch.cuda.device(dev) if dev != _cuda._cuda_getDevice() else _HERE:  # (the plan is the current device's)
         nbytes = L.lib().krq_gemm_mxfp4_ws_bytes(kind, e, M, N, K)
     if nbytes < 0:
         raise RuntimeError("krq_gemm_mxfp4_ws_bytes: device query failed")
     ws = t.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
-    _call(dev, "krq_gemm_mxfp4", p, scale, kind, e, ld, w, wscale, M, N, K, L.ptr(ws), nbytes, out.data_ptr())
+    _call(dev, "krq_gemm_mxfp4", p, scale, kind, e, ld, q.tiled.data_ptr(), q.tiled_scale.data_ptr(), M, N, K, L.ptr(ws), nbytes,
+          out.data_ptr())
     return out
 
 

@@ -203,7 +203,8 @@ def swiglu_check(y, xv, wv, elem="e4m3"):
 
 
 @pytest.mark.parametrize("elem", ["e4m3", "e2m1"])
-@pytest.mark.parametrize("M,I,K", [(1, 16, 32), (1, 9728, 2560), (3, 48, 160), (8, 80, 1056), (9, 64, 2880), (16, 1024, 2560), (32, 112, 544)])
+@pytest.mark.parametrize("M,I,K", [(1, 16, 32), (1, 9728, 2560), (3, 48, 160), (8, 80, 1056), (9, 64, 2880), (16, 1024, 2560), (32, 112, 544),
+                                   (32, 48, 4096), (17, 32, 4640), (2, 80, 9728)])
 def test_gemv_swiglu(dev, M, I, K, elem):
     q, wv = weight(2 * I, K, 4, dev)
     x = bf((M, K), 5)
@@ -338,7 +339,7 @@ def test_far_rows(dev):
 
 # ------------------------------------------------------------------------------------------ lm head
 @pytest.mark.parametrize("M,V,K", [(1, 16, 32), (1, 70000, 512), (5, 4112, 2560), (1, 16400, 2560), (32, 20000, 2560), (2, 9008, 6400), (20, 4096, 6400), (16, 1040, 10752), (7, 48, 512), (8, 1024, 160), (9, 32000, 1024), (16, 4096, 2880),
-                                   (32, 2048, 544)])
+                                   (32, 2048, 544), (32, 4112, 4096), (25, 1040, 5120), (1, 33008, 5632), (16, 9008, 10240), (1, 1040, 10272)])
 def test_head(dev, M, V, K):
     q, wv = weight(V, K, 7, dev)
     h = bf((M, K), 8)
@@ -492,6 +493,16 @@ def test_refusals_on_the_device(dev):
                  lambda: lmhead.lm_head_argmax(bf((33, 96), 1).to(dev), q)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_tiles_that_moved(dev):
+    """A weight whose tiles were copied elsewhere is read from there."""
+    q, _ = weight(80, 2880, 2, dev)
+    x = bf((3, 2880), 3).to(dev)
+    want = [X.gemv_mxfp4(x, q), X.gemm_mxfp4(x, q), lmhead.lm_head_argmax(x, q)]
+    q.tiled, q.tiled_scale = q.tiled.clone(), q.tiled_scale.clone()
+    for a, b in zip([X.gemv_mxfp4(x, q), X.gemm_mxfp4(x, q), lmhead.lm_head_argmax(x, q)], want):
+        assert torch.equal(a, b)
 
 
 def test_tensors_of_the_cpu_are_refused(dev):

@@ -172,6 +172,21 @@ def test_c_entry_points_refuse_before_any_launch():
     assert lib.krq_lmhead_mxfp4_ws_bytes(0, 1, 1, 1024, 64) == 768 and lib.krq_lmhead_mxfp4_ws_bytes(0, 1, 0, 1024, 64) == -1
 
 
+def test_tiles_and_scales_off_their_alignment_are_refused():
+    p, odd, z = ctypes.c_void_p(4096), ctypes.c_void_p(4100), None
+    one_odd = lambda n: [[odd if i == j else p for i in range(n)] for j in range(n)]
+    calls = [("krq_quant_mxfp4", [p, 16, 64, 64, w4, p, t, ts, z]) for w4, t, ts in one_odd(3)]
+    calls += [("krq_quant_mx_rows", [p, 16, 64, 64, 1, t, ts, z]) for t, ts in one_odd(2)]
+    calls += [("krq_pack_mxfp4", [w4, p, 16, 64, t, ts, z]) for w4, t, ts in one_odd(3)]
+    calls += [("krq_dequant_mx", [t, ts, 1, 16, 64, out, z]) for t, ts, out in one_odd(3)]
+    calls += [("krq_gemv_mxfp4", [x, xs, 1, 1, 0, w, ws, 4, 64, 1024, 1, 0, z, 0, p, z]) for x, xs, w, ws in one_odd(4)]
+    calls += [("krq_gemm_mxfp4", [x, xs, 1, 1, 0, w, ws, 40, 64, 1024, z, 0, p, z]) for x, xs, w, ws in one_odd(4)]
+    calls += [("krq_lmhead_argmax_mxfp4", [x, xs, 1, 1, 0, w, ws, 4, 64, 1024, z, p, 1 << 20, p, z]) for x, xs, w, ws in one_odd(4)]
+    for name, args in calls:
+        assert getattr(L.lib(), name)(*args) == L.KRQ_EINVAL, (name, args)
+        assert b"16 bytes" in L.lib().krq_last_error(), (name, args)
+
+
 def _q(N=64, K=64, device="cpu"):
     u8 = lambda *s: torch.zeros(s, dtype=torch.uint8, device=device)
     return X.MXFP4Weight(u8(N, K // 2), u8(N, K // 32), u8(L.lib().krq_mx_tiled_bytes(N, K, 0)), u8(L.lib().krq_mx_scale_bytes(N, K)))
