@@ -8,6 +8,7 @@
 // k_gemv_mx_held: each wave holds its groups' activation operands in registers (GW groups, MT row tiles) for the whole launch, and the
 // workgroup walks over sets of P row blocks (SwiGLU: a gate block and its up block), the next set's weights in flight.
 // k_gemv_mx_stream: longer rows, more of them; activation tiles are loaded beside the weights.
+// k_gemv_mx_wide: many row blocks of not too long rows; the operands lie in LDS, a wave takes whole row blocks.
 //
 // Large launches are bound by the weights' read (the head at one row, 151,936 x 2,560: 33.4 us, 6.2 TB/s, the card's read rate;
 // at 16 38.2), small ones by a launch and a round trip to memory (2,560 x 4,096, M = 1: 3.4 us; SwiGLU over 19,456 x 2,560, M = 5:
@@ -43,6 +44,19 @@ template <int ELEM>
 KRQ_DEV v4f mx_mfma(int t, v8i a, uint4 b, v4f acc, uint32_t sa, uint32_t sb) {
   return t == 0 ? mx_mfma<ELEM, 0>(a, b, acc, sa, sb) : t == 1 ? mx_mfma<ELEM, 1>(a, b, acc, sa, sb)
          : t == 2 ? mx_mfma<ELEM, 2>(a, b, acc, sa, sb) : mx_mfma<ELEM, 3>(a, b, acc, sa, sb);
+}
+
+// The same with the weights first: a lane's sums are four columns of a row.
+template <int ELEM, int T>
+KRQ_DEV v4f mx_mfma_w(uint4 w, v8i x, v4f acc, uint32_t sw, uint32_t sx) {
+  constexpr int fx = ELEM == KRQ_MX_E2M1 ? 4 : 0;
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(pack_v8i(w, zero4()), x, acc, 4, fx, T, static_cast<int>(sw), T,
+                                                          static_cast<int>(sx));
+}
+template <int ELEM>
+KRQ_DEV v4f mx_mfma_w(int t, uint4 w, v8i x, v4f acc, uint32_t sw, uint32_t sx) {
+  return t == 0 ? mx_mfma_w<ELEM, 0>(w, x, acc, sw, sx) : t == 1 ? mx_mfma_w<ELEM, 1>(w, x, acc, sw, sx)
+         : t == 2 ? mx_mfma_w<ELEM, 2>(w, x, acc, sw, sx) : mx_mfma_w<ELEM, 3>(w, x, acc, sw, sx);
 }
 
 struct MxArgs {
@@ -396,6 +410,188 @@ __global__ __launch_bounds__(kStreamWaves * 64) void k_gemv_mx_stream(const MxAr
 
 int sets_of(const MxArgs& a, int mode, int P) { return mode == KRQ_OUT_SWIGLU ? a.nrb : (a.nrb + P - 1) / P; }
 
+typedef uint32_t v2u_any __attribute__((ext_vector_type(2), aligned(2)));  // 8 bytes at any element's address
+
+// Many row blocks: the rows (bf16 ones rounded by every workgroup for itself) stay in LDS as operands, and a wave takes whole row
+// blocks, so that it waits for nothing but its own weights, of which four groups are in flight on from row block to row block;
+// no sums meet and no barrier holds the stream. Padding to whole groups is zero. Weights are the first operand here: a lane ends
+// with four adjacent columns of row lane % 16. One workgroup per compute unit. us a call: 65,536 x 2,560, M = 16 21.6 (held) -> 17.8,
+// M = 32 26.0 -> 22.4; 151,936 x 2,560, M = 1 42.3 -> 35.3 (5.9 TB/s); the head, M = 16 46.8 -> 42.4, M = 32 58.5 -> 50.2. Pairs of
+// row blocks 45.4 and 53.4, sixteen waves with two groups each 45.0 and 51.7.
+constexpr int kWideWaves = 8, kWideFlight = 4, kWideGroups = 7;  // (more groups: takes_wide)
+template <int ELEM, bool BF16, int MT, int MODE>
+__global__ __launch_bounds__(kWideWaves * 64) void k_gemv_mx_wide(const MxArgs a) {
+  static_assert(!BF16 || MT == 1, "more than sixteen rows come rounded");
+  static_assert(MODE == KRQ_OUT_BF16 || MODE == kOutArgmax, "outputs of a row block are final");
+  constexpr int AB = ELEM == KRQ_MX_E2M1 ? 1 : 2, TB = 1024 * AB, W = kWideWaves, U = kWideFlight, B = 4;
+  __shared__ __align__(16) uint8_t lx[MT * kWideGroups * 4 * TB];
+  __shared__ __align__(16) uint8_t lsc[MT * kWideGroups * 256];
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int G = a.groups, tiles = MT * G * 4;
+  const int first = static_cast<int>(blockIdx.x) * W + wave, stride = static_cast<int>(gridDim.x) * W;
+  const int total = first < a.nrb ? ((a.nrb - first + stride - 1) / stride) * G : 0;  // this wave's groups
+
+  // tile i of the rows: row tile i / (4 G), tile i % (4 G) of it; lanes as k_mx_quant's
+  const int kc = 8 * r, b = kc >> 5;
+  uint4 xv[B][BF16 ? 4 : AB];
+  auto load_rows = [&](int i0) {
+#pragma unroll
+    for (int q = 0; q < B; ++q) {
+      const int i = min(i0 + q * W, tiles - 1), mt = i / (4 * G), t = i - mt * 4 * G;
+      if constexpr (BF16) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          xv[q][j] = ld16(a.x + 2 * (min(16 * mt + 4 * j + g, a.M - 1) * a.ldx + min(kMxTile * t + kc, a.K - 8)));
+      } else {
+#pragma unroll
+        for (int h = 0; h < AB; ++h) xv[q][h] = ld16(a.x + (((int64_t)mt * a.KT + min(t, a.KT - 1)) * (64 * AB) + lane) * 16 + 1024 * h);
+      }
+    }
+  };
+  auto keep_rows = [&](int i0) {
+#pragma unroll
+    for (int q = 0; q < B; ++q) {
+      const int i = i0 + q * W;
+      if (i >= tiles) break;
+      const int mt = i / (4 * G), t = i - mt * 4 * G;
+      if constexpr (BF16) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int row = 4 * j + g;
+          const uint4 v = sel4(16 * mt + row < a.M && kMxTile * t + kc < a.K, xv[q][j]);
+          const uint32_t code = mx_code<ELEM>(quad_absmax(v));
+          if ((lane & 3) == 0) lsc[(((i >> 2) * 64) + 16 * b + row) * 4 + (i & 3)] = static_cast<uint8_t>(code);
+          if constexpr (ELEM == KRQ_MX_E2M1)
+            *reinterpret_cast<uint32_t*>(lx + i * TB + 16 * (16 * b + row) + 4 * (lane & 3)) = mx_quant8_e2m1(v, code);
+          else
+            *reinterpret_cast<uint2*>(lx + i * TB + 1024 * (kc >> 6) + 16 * (16 * ((kc & 63) >> 4) + row) + (kc & 15)) =
+                mx_quant8_e4m3(v, code);
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < AB; ++h) *reinterpret_cast<uint4*>(lx + i * TB + 1024 * h + 16 * lane) = sel4(t < a.KT, xv[q][h]);
+      }
+    }
+  };
+
+  uint4 wv[U][4];
+  uint32_t wsc[U];
+  int lrb = first, lg = 0;  // the loading end
+  auto load = [&](int u) {
+    const int64_t rb = min(lrb, a.nrb - 1);
+    wsc[u] = *reinterpret_cast<const uint32_t*>(a.ws + ((rb * G + lg) * 64 + lane) * 4);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) wv[u][t] = ld16nt(a.w + ((rb * a.KT + min(4 * lg + t, a.KT - 1)) * 64 + lane) * 16);
+    if (++lg == G) {
+      lg = 0;
+      lrb += stride;
+    }
+  };
+  load_rows(wave);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int u = 0; u < U; ++u) load(u);  // (past the last: the last row block)
+  __builtin_amdgcn_sched_barrier(0);
+  keep_rows(wave);
+  for (int i = wave + B * W; i < tiles; i += B * W) {
+    load_rows(i);
+    keep_rows(i);
+  }
+  if constexpr (!BF16)
+    for (int i = threadIdx.x; i < MT * G * 64; i += 64 * W)
+      *reinterpret_cast<uint32_t*>(lsc + 4 * i) = *reinterpret_cast<const uint32_t*>(a.xs + (int64_t)4 * i);
+  barrier_lds();
+
+  v4f acc[MT];
+  Best best[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    acc[mt] = v4f{0.f, 0.f, 0.f, 0.f};
+    best[mt] = Best{-INFINITY, 0x7fffffff};
+  }
+  int crb = first, cg = 0;  // the consuming end
+  auto consume = [&](int u) __attribute__((always_inline)) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const uint32_t sx = *reinterpret_cast<const uint32_t*>(lsc + ((mt * G + cg) * 64 + lane) * 4);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const uint8_t* q = lx + ((mt * G + cg) * 4 + t) * TB + 16 * lane;
+        const v8i x = pack_v8i(*reinterpret_cast<const uint4*>(q), AB == 2 ? *reinterpret_cast<const uint4*>(q + 1024 * (AB - 1)) : zero4());
+        acc[mt] = mx_mfma_w<ELEM>(t, wv[u][t], x, acc[mt], wsc[u], sx);
+      }
+    }
+    if (++cg < G) return;
+    cg = 0;
+    const int64_t n = (int64_t)crb * 16 + 4 * g;
+    crb += stride;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const int m = 16 * mt + r;
+      const uint32_t y[2] = {pack_bf16x2(acc[mt][0], acc[mt][1]), pack_bf16x2(acc[mt][2], acc[mt][3])};
+      acc[mt] = v4f{0.f, 0.f, 0.f, 0.f};
+      uint16_t* o = static_cast<uint16_t*>(a.out) + m * a.NO + n;
+      if (m < a.M && n + 4 <= a.NO) {
+        if (MODE == KRQ_OUT_BF16 || a.out) *reinterpret_cast<v2u_any*>(o) = v2u_any{y[0], y[1]};
+        if constexpr (MODE == kOutArgmax) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float l = as_f32(e & 1 ? y[e >> 1] & 0xffff0000u : y[e >> 1] << 16);
+            if (better(l, static_cast<int>(n) + e, best[mt].v, best[mt].i)) best[mt] = Best{l, static_cast<int>(n) + e};
+          }
+        }
+      } else if (MODE == KRQ_OUT_BF16 && m < a.M) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < a.NO) o[e] = static_cast<uint16_t>(y[e >> 1] >> (16 * (e & 1)));
+      }
+    }
+  };
+  int i = 0;
+  for (; i + 2 * U <= total; i += U) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      consume(u);
+      load(u);
+    }
+  }
+  const int rem = total - i;  // fewer than 2 U groups
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (u < rem) {
+      consume(u);
+      if (U + u < rem) load(u);
+    }
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (U + u < rem) consume(u);
+
+  if constexpr (MODE == kOutArgmax) {  // over the lanes of a row, then over the waves
+    __syncthreads();
+    Best* red = reinterpret_cast<Best*>(lx);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      Best t = best[mt];
+#pragma unroll
+      for (int o = 16; o < 64; o <<= 1) {
+        const Best c = shfl_best(t, o);
+        if (better(c.v, c.i, t.v, t.i)) t = c;
+      }
+      if (lane < 16) red[wave * (16 * MT) + 16 * mt + lane] = t;
+    }
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < a.M) {
+      Best t = red[threadIdx.x];
+      for (int w = 1; w < W; ++w) {
+        const Best c = red[w * (16 * MT) + threadIdx.x];
+        if (better(c.v, c.i, t.v, t.i)) t = c;
+      }
+      a.cand[(int64_t)threadIdx.x * gridDim.x + blockIdx.x] = t;
+    }
+  }
+}
+
 // Row blocks of a set: the head takes pairs (151,936 x 2,560, single / pairs, us a call: M = 1 44.5 / 37.9, M = 16 55.3 / 46.3,
 // M = 32 101 / 58), the other outputs single ones (19,456 x 2,560, M = 16 7.5 / 8.5; 65,536 x 2,560, M = 1 17.1 / 17.0).
 constexpr int set_blocks(int mode) { return mode == KRQ_OUT_SWIGLU || mode == kOutArgmax ? 2 : 1; }
@@ -445,8 +641,30 @@ int launch_mode(const MxArgs& a, bool bf16, int splits, hipStream_t s) {
   return a.M <= 16 ? launch_stream<ELEM, 1, MODE, P, 2>(a, splits, ns, s) : launch_stream<ELEM, 2, MODE, P, P == 1 ? 2 : 1>(a, splits, ns, s);
 }
 
+// Where k_gemv_mx_wide takes a product: up to seven groups (65,536 x 4,096, held / wide, us a call: M = 5 27.0 / 28.1, M = 16
+// 29.6 / 28.7, M = 32 32.6 / 35.4; the head over 64,000 x 3,584, M = 16 31.3 / 27.4), plain outputs from 32,768 columns (M = 5,
+// K = 2,560: 16,384 8.4 / 8.6, 32,768 12.0 / 10.7), for a few rows from 65,536 (M = 4, K = 2,048: 32,768 9.4 / 9.7, 65,536
+// 15.3 / 14.7), the head from 9 rows and 16,000 columns (16,000 x 2,560, M = 16 16.9 / 13.4, M = 32 22.0 / 18.4; fewer rows:
+// 65,536 x 2,048, M = 4 17.8 / 18.5).
+bool takes_wide(int64_t M, int64_t N, int64_t K, int mode) {
+  if (mx_groups(K) > kWideGroups) return false;
+  return mode == kOutArgmax ? M > 8 && N >= 16000 : mode == KRQ_OUT_BF16 && N >= (M > 4 ? 32768 : 65536);
+}
+
+template <int ELEM, int MODE>
+int launch_wide(const MxArgs& a, bool bf16, hipStream_t s) {
+  const int blocks = std::min((a.nrb + kWideWaves - 1) / kWideWaves, kHeldMost);
+  const dim3 block(64 * kWideWaves);
+  if (a.M > 16) hipLaunchKernelGGL((k_gemv_mx_wide<ELEM, false, 2, MODE>), dim3(blocks), block, 0, s, a);
+  else if (bf16) hipLaunchKernelGGL((k_gemv_mx_wide<ELEM, true, 1, MODE>), dim3(blocks), block, 0, s, a);
+  else hipLaunchKernelGGL((k_gemv_mx_wide<ELEM, false, 1, MODE>), dim3(blocks), block, 0, s, a);
+  return blocks;
+}
+
 template <int MODE>
-int launch_elem(const MxArgs& a, int elem, bool bf16, int splits, hipStream_t s) {
+int launch_elem(const MxArgs& a, int elem, bool bf16, bool wide, int splits, hipStream_t s) {
+  if constexpr (MODE == KRQ_OUT_BF16 || MODE == kOutArgmax)
+    if (wide) return elem == KRQ_MX_E2M1 ? launch_wide<KRQ_MX_E2M1, MODE>(a, bf16, s) : launch_wide<KRQ_MX_E4M3, MODE>(a, bf16, s);
   return elem == KRQ_MX_E2M1 ? launch_mode<KRQ_MX_E2M1, MODE>(a, bf16, splits, s) : launch_mode<KRQ_MX_E4M3, MODE>(a, bf16, splits, s);
 }
 
@@ -472,8 +690,7 @@ int gemv_mx_run(const char* what, const void* x, const void* x_scale, int x_kind
   KRQ_REQUIRE(M >= 1 && M <= 32, "%s: M=%lld outside 1..32", what, (long long)M);
   KRQ_REQUIRE(N >= 1 && N <= 0x7fffffff - 64 && K >= kMxBlock && K % kMxBlock == 0 && K <= 0x3fffffff, "%s: shape N=%lld K=%lld (K a multiple of 32)", what,
               (long long)N, (long long)K);
-  const bool bf16 = x_kind == KRQ_MX_X_BF16 && split >= 1 && rounds_rows(M, K, split);
-  const int64_t rows = x_kind == KRQ_MX_X_BF16 && !bf16 ? mx_rows_bytes(elem, M, K) : 0;
+  const int64_t rows = krq_gemv_mxfp4_ws_bytes(x_kind, elem, M, K, std::max(split, 1));
   KRQ_REQUIRE(x_kind == KRQ_MX_X_BF16 || x_scale, "%s: tiled rows need their scales", what);
   KRQ_REQUIRE(x_kind != KRQ_MX_X_BF16 || (ldx >= K && ldx % 8 == 0), "%s: rows of x must start on 16 bytes (ldx=%lld)", what, (long long)ldx);
   KRQ_REQUIRE(aligned16(x) && aligned16(x_scale) && aligned16(w) && aligned16(w_scale) && aligned16(ws),
@@ -484,7 +701,8 @@ int gemv_mx_run(const char* what, const void* x, const void* x_scale, int x_kind
   KRQ_REQUIRE(split == 1 || mode == KRQ_OUT_PARTIAL, "%s: split=%d needs the partials output", what, split);
   const bool swiglu = mode == KRQ_OUT_SWIGLU;
   KRQ_REQUIRE(!swiglu || N % 32 == 0, "%s: SwiGLU needs N=%lld = 2 I with I %% 16 == 0", what, (long long)N);
-  if (rows) {
+  const bool wide = takes_wide(M, N, K, mode), bf16 = x_kind == KRQ_MX_X_BF16 && (rows == 0 || (wide && M <= 16));
+  if (rows && !bf16) {
     uint8_t* sc = (uint8_t*)ws + mx_rows_scale_at(elem, M, K);
     if (const int rc = krq_quant_mx_rows(x, M, K, ldx, elem, ws, sc, stream)) return rc;
     x = ws;
@@ -506,10 +724,10 @@ int gemv_mx_run(const char* what, const void* x, const void* x_scale, int x_kind
   a.nrb = static_cast<int>((a.NO + 15) / 16);
   a.sets = a.nw = 0;
   hipStream_t s = (hipStream_t)stream;
-  if (mode == KRQ_OUT_SWIGLU) launch_elem<KRQ_OUT_SWIGLU>(a, elem, bf16, split, s);
-  else if (mode == KRQ_OUT_PARTIAL) launch_elem<KRQ_OUT_PARTIAL>(a, elem, bf16, split, s);
-  else if (mode == kOutArgmax) *cands = launch_elem<kOutArgmax>(a, elem, bf16, split, s);
-  else launch_elem<KRQ_OUT_BF16>(a, elem, bf16, split, s);
+  if (mode == KRQ_OUT_SWIGLU) launch_elem<KRQ_OUT_SWIGLU>(a, elem, bf16, wide, split, s);
+  else if (mode == KRQ_OUT_PARTIAL) launch_elem<KRQ_OUT_PARTIAL>(a, elem, bf16, wide, split, s);
+  else if (mode == kOutArgmax) *cands = launch_elem<kOutArgmax>(a, elem, bf16, wide, split, s);
+  else launch_elem<KRQ_OUT_BF16>(a, elem, bf16, wide, split, s);
   return krq_check_launch(what);
 }
 

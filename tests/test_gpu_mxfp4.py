@@ -250,6 +250,31 @@ def test_scales_far_from_one(dev, ex, ew):
         check(X.linear_mxfp4(x[:M].to(dev), q), ref[:M], E[:M], M)
 
 
+@pytest.mark.parametrize("elem", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("M,N,K", [(1, 65536, 64), (4, 65549, 544), (1, 70003, 1056), (5, 32768, 32), (8, 32770, 3552), (16, 33001, 96),
+                                   (16, 32784, 2560), (17, 32769, 1184), (32, 32800, 3584), (32, 50002, 160)])
+def test_gemv_many_columns(dev, M, N, K, elem):
+    """Enough row blocks for a wave to take whole ones, odd columns and ends of K, rows of NaN among them; equal to nothing but
+    the reference behind the last row."""
+    w, x = bf((N, K), N, 0.05), bf((M, K), M)
+    x[M // 2, K // 2] = float("inf")
+    w[32001, K - 1] = float("nan")
+    q = X.quantize(w.to(dev))
+    xv, wv = rounded(x, elem), rounded(w, "e2m1")
+    bad = np.zeros((M, N), bool)
+    bad[M // 2], bad[:, 32001] = True, True
+    ref, E = reference(np.nan_to_num(xv), np.nan_to_num(wv))
+    for src in (x.to(dev), X.quant_rows(x.to(dev), elem)):
+        y = X.gemv_mxfp4(src, q, elem=elem).double().cpu().numpy()
+        assert np.array_equal(np.isnan(y), bad)
+        check(torch.from_numpy(np.where(bad, ref, y)), ref, E, (M, N, K, elem))
+    rows = X.quant_rows(x.to(dev), elem)
+    out = torch.full((M + 3, N), 7.0, device=dev, dtype=torch.bfloat16)
+    L.call("krq_gemv_mxfp4", L.ptr(rows.tiled), L.ptr(rows.tiled_scale), L.MX_X_TILED, X.ELEMS[elem], 0, L.ptr(q.tiled),
+           L.ptr(q.tiled_scale), M, N, K, 1, L.OUT_BF16, None, 0, L.ptr(out), L.stream(out))
+    assert out[M:].eq(7).all() and torch.equal(out[:M].nan_to_num(), X.gemv_mxfp4(rows, q).nan_to_num())
+
+
 def test_outputs_end_where_they_should(dev):
     """Through the C ABI into larger buffers: nothing behind the last row is touched."""
     M, N, K = 19, 37, 544
@@ -322,6 +347,19 @@ def test_far_offsets(dev):
         assert torch.equal(X.linear_mxfp4(x, q)[:, -115:], X.linear_mxfp4(x, small))
 
 
+def test_far_columns(dev):
+    """3,000,017 columns of K = 1,632: 2.5 GB of tiles under waves that take whole row blocks."""
+    N, K = 3_000_017, 1632
+    at = N - 17 - 80_000 + 16
+    w = torch.empty((N, K), device=dev, dtype=torch.bfloat16).normal_(0, 0.02, generator=torch.Generator(device=dev).manual_seed(4))
+    q, small = X.quantize(w), X.quantize(w[at:])
+    del w
+    assert at % 16 == 0
+    for M in (3, 16, 32):
+        x = bf((M, K), M).to(dev)
+        assert torch.equal(X.linear_mxfp4(x, q)[:, at:], X.linear_mxfp4(x, small))
+
+
 def test_far_rows(dev):
     """600,001 rows through the prefill product: 9.8 GB of output; and more rows than a grid's second axis of row blocks."""
     M, N, K = 600_001, 8192, 512
@@ -339,7 +377,8 @@ def test_far_rows(dev):
 
 # ------------------------------------------------------------------------------------------ lm head
 @pytest.mark.parametrize("M,V,K", [(1, 16, 32), (1, 70000, 512), (5, 4112, 2560), (1, 16400, 2560), (32, 20000, 2560), (2, 9008, 6400), (20, 4096, 6400), (16, 1040, 10752), (7, 48, 512), (8, 1024, 160), (9, 32000, 1024), (16, 4096, 2880),
-                                   (32, 2048, 544), (32, 4112, 4096), (25, 1040, 5120), (1, 33008, 5632), (16, 9008, 10240), (1, 1040, 10272)])
+                                   (32, 2048, 544), (32, 4112, 4096), (25, 1040, 5120), (1, 33008, 5632), (16, 9008, 10240), (1, 1040, 10272),
+                                   (9, 16000, 32), (16, 17008, 3552), (32, 16400, 3552), (24, 40000, 160), (17, 16016, 1024)])
 def test_head(dev, M, V, K):
     q, wv = weight(V, K, 7, dev)
     h = bf((M, K), 8)
@@ -363,6 +402,12 @@ def test_head_ties_and_nan(dev, M):
     assert idx.tolist() == [36] * M
     w[5000, 7] = float("nan")
     assert lmhead.lm_head_argmax(h.to(dev), X.quantize(w.to(dev))).tolist() == [5000] * M
+    w = torch.cat([w[:, :256], w[:, :256]])  # more row blocks: the ties at 36, 37, 4095, 8200 and 8208 further on, the NaN twice
+    assert lmhead.lm_head_argmax(h[:, :256].to(dev), X.quantize(w.to(dev))).tolist() == [5000] * M
+    tied = bf((V, 256), 3, 0.02)
+    tied = torch.cat([tied, tied])
+    tied[[36, 37, 4095, 8200, 8244, 16000]] = best[:256]
+    assert lmhead.lm_head_argmax(h[:, :256].to(dev), X.quantize(tied.to(dev))).tolist() == [36] * M
     with pytest.raises(ValueError, match="ActScale"):
         lmhead.lm_head_argmax(h.to(dev), X.quantize(w.to(dev)), a=fp8.ActScale(h.to(dev)))
 
