@@ -11,7 +11,7 @@
 // k_gemv_mx_wide: many row blocks of not too long rows; the operands lie in LDS, a wave takes whole row blocks.
 //
 // Large launches are bound by the weights' read (the head at one row, 151,936 x 2,560: 33.4 us, 6.2 TB/s, the card's read rate;
-// at 16 38.2), small ones by a launch and a round trip to memory (2,560 x 4,096, M = 1: 3.4 us; SwiGLU over 19,456 x 2,560, M = 5:
+// at 16 36.6), small ones by a launch and a round trip to memory (2,560 x 4,096, M = 1: 3.4 us; SwiGLU over 19,456 x 2,560, M = 5:
 // 8.7, of which 1.3 round the rows), the streaming ones by the rows that every workgroup reads again from L2 (2,560 x
 // 9,728, M = 32: 8.5 us, 311 KB of rows beside 83 KB of weights).
 #include <algorithm>
