@@ -419,7 +419,7 @@ int krq_unpack_fp8(const void* w8_tiled, int64_t N, int64_t K, void* w8_rowmajor
 /* element types of MX blocks, and the activation kinds of krq_gemv_mxfp4 */
 #define KRQ_MX_E2M1 0
 #define KRQ_MX_E4M3 1
-#define KRQ_MX_X_BF16 0     /* bf16 rows; a few are rounded in the kernel (one of 10,240 k, KRQ_MX_BF16_ROWS of 5,120), others into ws first */
+#define KRQ_MX_X_BF16 0     /* bf16 rows; a few are rounded in the kernel (one of 10,240 k, KRQ_MX_BF16_ROWS of 5,120), others need ws */
 #define KRQ_MX_X_TILED 1    /* rows from krq_quant_mx_rows, with their scales */
 #define KRQ_MX_BF16_ROWS 8
 

@@ -13,8 +13,6 @@ The kernels read operands in the tiled layout of include/krq.h ("mx tiled"). K i
 are any.
 """
 
-import contextlib
-
 import torch
 
 from . import _lib as L
@@ -22,8 +20,8 @@ from . import _lib as L
 ELEMS = {"e2m1": L.MX_E2M1, "e4m3": L.MX_E4M3}
 DECODE_MAX_ROWS = 32  # rows of the skinny kernels
 BLOCK = 32
-ROW_MAX_K = 10240  # up to here the skinny kernels round a single bf16 row themselves, without a workspace
-_HERE = contextlib.nullcontext()
+ROW_MAX_K = 10240  # up to here the skinny kernels round a single bf16 row themselves, without a workspace,
+ROWS_MAX_K = 5120  # and up to here L.MX_BF16_ROWS of them
 
 
 class MXFP4Weight(tuple):
@@ -167,8 +165,16 @@ def dequantize(q):
         data, scale = t.data_ptr(), q.tiled_scale.data_ptr()
     out = t.new_empty((M, K), dtype=torch.bfloat16)
     if M:
-        _call(out.get_device(), "krq_dequant_mx", data, scale, elem, M, K, out.data_ptr())
+        _call(t.get_device(), "krq_dequant_mx", data, scale, elem, M, K, out.data_ptr())
     return out
+
+
+def _rows_bytes(M, K, e):
+    """(where the scales start, the size) of M tiled rows: krq_mx_tiled_bytes and krq_mx_scale_bytes, tiles of 1 or 2 KiB
+    and 256 bytes of scales per four of them, without two calls."""
+    mb = (M + 15) >> 4
+    at = (mb * ((K + 127) >> 7)) << (10 + e)
+    return at, at + (mb * ((K + 511) >> 9) << 8)
 
 
 def quant_rows(x, elem="e4m3"):
@@ -179,9 +185,8 @@ def quant_rows(x, elem="e4m3"):
     e = _elem(elem)
     if M == 0:
         return MXRows(x.new_empty((0,), dtype=torch.uint8), 0, (0, K), elem)
-    mb = (M + 15) >> 4  # krq_mx_tiled_bytes and krq_mx_scale_bytes: tiles of 1 or 2 KiB, 256 bytes of scales per four tiles
-    at = (mb * ((K + 127) >> 7)) << (10 + e)
-    data = x.new_empty((at + (mb * ((K + 511) >> 9) << 8),), dtype=torch.uint8)
+    at, nbytes = _rows_bytes(M, K, e)
+    data = x.new_empty((nbytes,), dtype=torch.uint8)
     p = data.data_ptr()
     _call(x.get_device(), "krq_quant_mx_rows", x.data_ptr(), M, K, ld, e, p, p + at)
     return MXRows(data, at, (M, K), elem)
@@ -225,8 +230,9 @@ def _decode(x, q, split, mode, elem):
     if M == 0:
         return out
     ws, nbytes = None, 0
-    if kind == L.MX_X_BF16 and (M > 1 or K > ROW_MAX_K):
-        nbytes = L.lib().krq_gemv_mxfp4_ws_bytes(kind, e, M, K, split)
+    if kind == L.MX_X_BF16 and K > (ROW_MAX_K if M == 1 else ROWS_MAX_K if M <= L.MX_BF16_ROWS else 0):
+        # (more rows always need room for the rounded ones)
+        nbytes = _rows_bytes(M, K, e)[1] if M > L.MX_BF16_ROWS else L.lib().krq_gemv_mxfp4_ws_bytes(kind, e, M, K, split)
         if nbytes > 0:
             ws = t.new_empty((nbytes,), dtype=torch.uint8)
     _call(t.get_device(), "krq_gemv_mxfp4", p, scale, kind, e, ld, q.tiled.data_ptr(), q.tiled_scale.data_ptr(), M, N, K, split, mode,
@@ -258,8 +264,11 @@ def gemm_mxfp4(x, q, elem="e4m3"):
     if M == 0:
         return out
     dev = t.get_device()
-    with torch.cuda.device(dev) if dev != _cuda._cuda_getDevice() else _HERE:  # (the plan is the current device's)
+    if dev == _cuda._cuda_getDevice():
         nbytes = L.lib().krq_gemm_mxfp4_ws_bytes(kind, e, M, N, K)
+    else:
+        with torch.cuda.device(dev):  # (the plan is the current device's)
+            nbytes = L.lib().krq_gemm_mxfp4_ws_bytes(kind, e, M, N, K)
     if nbytes < 0:
         raise RuntimeError("krq_gemm_mxfp4_ws_bytes: device query failed")
     ws = t.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
@@ -281,11 +290,13 @@ def embedding(ids, q, scale=1.0):
     if ids.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"ids must be int64 or int32, got {ids.dtype}")
     w4, scale_codes = q
-    _same_device(ids, w4)
+    dev = w4.get_device()
+    if dev < 0 or ids.get_device() != dev:
+        _same_device(ids, w4)
     ids = ids.contiguous()
     out = w4.new_empty((*ids.shape, K), dtype=torch.bfloat16)
     n = ids.numel()
     if n:
-        _call(out.get_device(), "krq_embed_mxfp4", ids.data_ptr(), int(ids.dtype == torch.int64), n, w4.data_ptr(), scale_codes.data_ptr(), N, K,
+        _call(dev, "krq_embed_mxfp4", ids.data_ptr(), ids.dtype is torch.int64, n, w4.data_ptr(), scale_codes.data_ptr(), N, K,
               float(scale), out.data_ptr())
     return out

@@ -187,6 +187,19 @@ def test_tiles_and_scales_off_their_alignment_are_refused():
         assert b"16 bytes" in L.lib().krq_last_error(), (name, args)
 
 
+def test_sizes_known_without_a_call():
+    lib = L.lib()
+    for M, K in [(1, 32), (16, 512), (17, 544), (32, 9728), (1000, 2560)]:
+        for e in (0, 1):
+            at, n = X._rows_bytes(M, K, e)
+            assert at == lib.krq_mx_tiled_bytes(M, K, e) and n - at == lib.krq_mx_scale_bytes(M, K)
+            if L.MX_BF16_ROWS < M <= 32:
+                assert n == lib.krq_gemv_mxfp4_ws_bytes(0, e, M, K, 1) == lib.krq_gemv_mxfp4_ws_bytes(0, e, M, K, 2)
+    for split in (1, 2, 3):
+        assert lib.krq_gemv_mxfp4_ws_bytes(0, 1, L.MX_BF16_ROWS, X.ROWS_MAX_K, split) == 0
+        assert lib.krq_gemv_mxfp4_ws_bytes(0, 1, 1, X.ROW_MAX_K, split) == 0
+
+
 def _q(N=64, K=64, device="cpu"):
     u8 = lambda *s: torch.zeros(s, dtype=torch.uint8, device=device)
     return X.MXFP4Weight(u8(N, K // 2), u8(N, K // 32), u8(L.lib().krq_mx_tiled_bytes(N, K, 0)), u8(L.lib().krq_mx_scale_bytes(N, K)))
