@@ -17,7 +17,7 @@
 //
 // Large products are bound by the matrix cores at the card's power and by the burst of every round's stores: 4,096 x 19,456 x
 // 2,560 with e4m3 rows takes 158 to 183 us (the cores 64% busy; 128 without loads, LDS reads and stores), 8,192^3 392 us (2.8
-// PFLOP/s; e2m1 rows 251). Small ones are bound by the loads' latency (1,000 x 2,560 x 9,728, e2m1 rows: 160 tiles on 256 units,
+// PFLOP/s; e2m1 rows 251). Small ones are bound by their loads (1,000 x 2,560 x 9,728, e2m1 rows: 160 tiles on 256 units,
 // 25.4 us, 19 without loads; 77 x 6,144 x 2,560: 7.9).
 #include <algorithm>
 #include <type_traits>
