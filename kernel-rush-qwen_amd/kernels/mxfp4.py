@@ -83,6 +83,7 @@ _functions = {}
 
 
 def _same_device(first, *tensors):
+    """Refuses tensors of the host, whose addresses a kernel would read as its own, and of two devices."""
     L.require_device(first, *tensors)
     for t in tensors:
         if t.get_device() != first.get_device():
@@ -158,10 +159,12 @@ def dequantize(q):
     """The bf16 values an MXFP4Weight or MXRows stands for, [N, K] or [M, K] (its tiled copy's)."""
     if isinstance(q, MXRows):
         (M, K), elem, t = q.shape, ELEMS[q.elem], q.data
+        _same_device(t)
         data = t.data_ptr()
         scale = data + q.scale_at
     else:
         (M, K), elem, t = _weight(q), L.MX_E2M1, q.tiled
+        _same_device(t, q.tiled_scale)
         data, scale = t.data_ptr(), q.tiled_scale.data_ptr()
     out = t.new_empty((M, K), dtype=torch.bfloat16)
     if M:
@@ -205,8 +208,9 @@ def _operand(x, q, elem):
     else:
         t, ld = _bf16_rows(x, "rows [M, K]")
         M, p, scale, kind = t.shape[0], t.data_ptr(), None, L.MX_X_BF16
-    if t.get_device() != q.tiled.get_device():
-        _same_device(t, q.tiled)
+    dev = t.get_device()
+    if dev < 0 or q.tiled.get_device() != dev or q.tiled_scale.get_device() != dev:
+        _same_device(t, q.tiled, q.tiled_scale)
     return t, p, scale, kind, ELEMS[elem] if elem in ELEMS else _elem(elem), ld, M
 
 
@@ -291,8 +295,8 @@ def embedding(ids, q, scale=1.0):
         raise ValueError(f"ids must be int64 or int32, got {ids.dtype}")
     w4, scale_codes = q
     dev = w4.get_device()
-    if dev < 0 or ids.get_device() != dev:
-        _same_device(ids, w4)
+    if dev < 0 or ids.get_device() != dev or scale_codes.get_device() != dev:
+        _same_device(ids, w4, scale_codes)
     ids = ids.contiguous()
     out = w4.new_empty((*ids.shape, K), dtype=torch.bfloat16)
     n = ids.numel()

@@ -1,0 +1,88 @@
+"""Calls of kernels.mxfp4 that end before anything is launched, without a GPU: the library's entry points are
+replaced by a list of what would have been called."""
+
+import pytest
+import torch
+
+from kernels import _lib as L
+from kernels import mxfp4 as X
+
+
+def u8(*shape):
+    return torch.zeros(shape, dtype=torch.uint8)
+
+
+def weight(N=64, K=64):
+    """An MXFP4Weight of zeros in host memory."""
+    return X.MXFP4Weight(u8(N, K // 2), u8(N, K // 32), u8(L.lib().krq_mx_tiled_bytes(N, K, 0)), u8(L.lib().krq_mx_scale_bytes(N, K)))
+
+
+def rows(M=4, K=64, elem="e4m3"):
+    """MXRows of zeros in host memory."""
+    at, size = X._rows_bytes(M, K, X.ELEMS[elem])
+    return X.MXRows(u8(size), at, (M, K), elem)
+
+
+@pytest.fixture
+def launched(monkeypatch):
+    seen = []
+    monkeypatch.setattr(X, "_call", lambda dev, name, *args: seen.append((dev, name, args)))
+    return seen
+
+
+class OnDevice:
+    """A stand-in for a tensor on device `dev`, as far as the checks look at one."""
+
+    def __init__(self, t, dev):
+        self.t, self.dev, self.device, self.is_cuda = t, dev, f"cuda:{dev}", True
+
+    def get_device(self):
+        return self.dev
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+
+@pytest.mark.parametrize("call", [
+    lambda q, r: X.dequantize(q),
+    lambda q, r: X.dequantize(r),
+    lambda q, r: X.gemv_mxfp4(r, q),
+    lambda q, r: X.gemv_mxfp4(r, q, 2),
+    lambda q, r: X.gemv_swiglu_mxfp4(r, q),
+    lambda q, r: X.gemm_mxfp4(r, q),
+    lambda q, r: X.linear_mxfp4(r, q),
+    lambda q, r: X.embedding(torch.zeros(2, dtype=torch.int64), q),
+])
+def test_weights_and_rows_of_the_host_are_refused(launched, call):
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        call(weight(64, 1024), rows(4, 1024))
+    assert not launched
+
+
+@pytest.mark.parametrize("what", ["tiled", "tiled_scale"])
+@pytest.mark.parametrize("where", ["host", "other"])
+def test_every_part_of_a_weight_is_on_the_rows_device(launched, what, where):
+    """A weight of which one tensor stayed behind, or went to another device."""
+    q, r = weight(), rows()
+    r.data = OnDevice(r.data, 0)
+    for name in ("tiled", "tiled_scale"):
+        t = getattr(q, name)
+        if name != what:
+            setattr(q, name, OnDevice(t, 0))
+        elif where == "other":
+            setattr(q, name, OnDevice(t, 1))
+    err = RuntimeError if where == "host" else ValueError
+    for call in (lambda: X.dequantize(q), lambda: X.linear_mxfp4(r, q), lambda: X.gemm_mxfp4(r, q), lambda: X.gemv_swiglu_mxfp4(r, q)):
+        with pytest.raises(err, match="ROCm device|tensors on cuda"):
+            call()
+    assert not launched
+
+
+@pytest.mark.parametrize("where", ["host", "other"])
+def test_the_embeddings_scales_are_on_the_codes_device(launched, where):
+    q, ids = weight(), torch.zeros(2, dtype=torch.int64)
+    scale = q[1] if where == "host" else OnDevice(q[1], 1)
+    moved = X.MXFP4Weight(OnDevice(q[0], 0), scale, q.tiled, q.tiled_scale)
+    with pytest.raises(RuntimeError if where == "host" else ValueError, match="ROCm device|tensors on cuda"):
+        X.embedding(OnDevice(ids, 0), moved)
+    assert not launched
