@@ -77,17 +77,19 @@ def _mxfp4_head(h, q, return_logits):
 def lm_head_argmax(h, w, return_logits=False, h_layout="auto", a=None):
     """h [M, K] bf16 (M <= 32); w the tied embedding, bf16 [V, K], an FP8Weight from
     fp8.quantize (per channel) or fp8.quantize_weight (per tensor), or an MXFP4Weight from mxfp4.quantize
-    (h in e4m3 blocks). Returns int64 [M] token ids,
+    (h in e4m3 blocks, or MXRows as mxfp4.quant_rows rounded them). Returns int64 [M] token ids,
     or (ids, bf16 logits [M, V]) with return_logits=True. h_layout ("auto", "tiled" or
     "rowmajor"): how a per-channel FP8 head's per-token rows are laid out at M > 1 (the same
     operands either way); "auto" takes tiled rows from fp8.TILED_MIN_ROWS, and from TILED_MIN_ROWS
     where the launch that shares them in LDS runs and they start on 16 bytes. a: an ActScale / SharedScale for the FP8 head's activations (as
     linear_fp8 takes), instead of the scaling described in the module docstring."""
-    L.require_device(h)
+    mx = isinstance(w, _mxfp4.MXFP4Weight)
+    if not mx:  # (an MXFP4 head's h may be MXRows: checked with the weight)
+        L.require_device(h)
     M, K = h.shape
     if M > 32:
         raise ValueError(f"lm_head_argmax: M={M} > 32")
-    if isinstance(w, _mxfp4.MXFP4Weight):
+    if mx:
         if a is not None:
             raise ValueError("an MXFP4 head scales h by blocks: it takes no ActScale / SharedScale")
         return _mxfp4_head(h, w, return_logits)

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from kernels import _lib as L
+from kernels import lmhead
 from kernels import mxfp4 as X
 
 
@@ -85,4 +86,19 @@ def test_the_embeddings_scales_are_on_the_codes_device(launched, where):
     moved = X.MXFP4Weight(OnDevice(q[0], 0), scale, q.tiled, q.tiled_scale)
     with pytest.raises(RuntimeError if where == "host" else ValueError, match="ROCm device|tensors on cuda"):
         X.embedding(OnDevice(ids, 0), moved)
+    assert not launched
+
+
+@pytest.mark.parametrize("M", [1, 32])
+@pytest.mark.parametrize("elem", ["e4m3", "e2m1"])
+def test_the_head_takes_rounded_rows(launched, M, elem):
+    """MXRows reach the head's checks as every other product's: here those of where they lie and of how many they are."""
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        lmhead.lm_head_argmax(rows(M, elem=elem), weight())
+    with pytest.raises(ValueError, match="33 > 32"):
+        lmhead.lm_head_argmax(rows(33, elem=elem), weight())
+    with pytest.raises(ValueError, match="ActScale"):
+        lmhead.lm_head_argmax(rows(M, elem=elem), weight(), a=object())
+    with pytest.raises(ValueError, match="do not match"):
+        lmhead.lm_head_argmax(rows(M, 96, elem), weight())
     assert not launched
