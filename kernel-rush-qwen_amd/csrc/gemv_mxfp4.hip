@@ -30,6 +30,9 @@ constexpr int kMxSplitMax = 64;
 // units would leave some units with twice the work). us, M = 1 on cold weights: 6,144 x 2,560 (384 sets) in 192 workgroups
 // 4.58, 384 4.14; SwiGLU over 19,456 x 2,560 (608) in 203 7.57, 304 10.4, 608 9.3; 18,000 x 6,400 (563) in 188 13.7, 282 17.0,
 // 563 15.4; the lm head (4,748) in 250 39.5, 475 40.6, 950 45.0.
+// One over the units, 257 against 171 (513 sets) or 205 (1,025): the head over 16,416 x 2,560, M = 4 13.4 / 10.8, over 32,800 19.3 /
+// 14.3, SwiGLU over 32,800 x 2,560 13.8 / 10.3, 8,208 x 10,240 in two splits 12.3 / 9.8; a plain product, whose workgroups are small
+// enough for two to a unit, 8,208 x 2,560 5.0 / 5.3.
 constexpr int kHeldOnce = 512, kHeldMost = 256;
 
 // acc += A (16 rows) . B (16 weight rows) over 128 k, scale byte t of sa and sb (t a constant after unrolling). A: e2m1 or
@@ -600,7 +603,7 @@ template <int ELEM, int XSRC, int MT, int MODE, int P, int GW>
 int launch_held(MxArgs a, int splits, int nw, hipStream_t s) {
   a.sets = sets_of(a, MODE, P);
   a.nw = nw;
-  const int most = (int64_t)a.sets * splits <= kHeldOnce ? a.sets : kHeldMost / splits + 1;
+  const int most = (int64_t)a.sets * splits <= kHeldOnce ? a.sets : std::max(1, kHeldMost / splits);
   const int rounds = (a.sets + most - 1) / most, blocks = (a.sets + rounds - 1) / rounds;  // as many sets for each
   constexpr size_t row = (ELEM == KRQ_MX_E2M1 ? 256 : 512) + 16;
   const size_t smem = std::max((size_t)2 * nw * P * MT * 1024, XSRC > 0 ? nw * (XSRC == 4 ? 4 : 1) * row : 0);

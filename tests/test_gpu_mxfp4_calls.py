@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 import torch
 
+from kernels import _lib as L
 from kernels import lmhead
 from kernels import mxfp4 as X
 from test_gpu_mxfp4 import bf, check, reference, rounded, weight
@@ -28,3 +29,20 @@ def test_head_of_rounded_rows(dev, M, V, K, elem):
     assert torch.equal(lmhead.lm_head_argmax(rows, q), idx)
     if elem == "e4m3":
         check(lmhead.lm_head_argmax(h.to(dev), q, return_logits=True)[1], ref, E, "bf16 rows")
+
+
+@pytest.mark.parametrize("sets", [513, 514, 771, 1025, 1027, 1281])
+def test_a_long_launch_has_a_workgroup_per_compute_unit_at_most(dev, sets):
+    """The head's candidates, one per workgroup and row block of a pair, counted in its workspace: no more than two for each
+    of 256 compute units, where one unit with a second workgroup would take twice as long as the others. They still cover
+    every column."""
+    V, K = 32 * sets, 512
+    q, _ = weight(V, K, 3, dev)
+    h = bf((1, K), 4).to(dev)
+    nbytes = L.lib().krq_lmhead_mxfp4_ws_bytes(L.MX_X_BF16, L.MX_E4M3, 1, V, K)
+    ws = torch.full((nbytes // 8,), 0x5A5A5A5A5A5A5A5A, device=dev, dtype=torch.int64)
+    logits, idx = torch.empty((1, V), device=dev, dtype=torch.bfloat16), torch.empty((1,), device=dev, dtype=torch.int64)
+    L.call("krq_lmhead_argmax_mxfp4", L.ptr(h), None, L.MX_X_BF16, L.MX_E4M3, K, L.ptr(q.tiled), L.ptr(q.tiled_scale), 1, V, K, L.ptr(logits),
+           L.ptr(ws), nbytes, L.ptr(idx), L.stream(h))
+    assert 0 < int(ws.ne(0x5A5A5A5A5A5A5A5A).sum()) <= 2 * 256
+    assert idx.item() == int(torch.argmax(logits.float().cpu(), -1))
