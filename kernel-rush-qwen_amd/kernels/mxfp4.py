@@ -35,6 +35,9 @@ class MXFP4Weight(tuple):
         self.shape = (w4.shape[0], 2 * w4.shape[1])
         return self
 
+    def __getnewargs__(self):  # (copies and pickles make a new one of these)
+        return self[0], self[1], self.tiled, self.tiled_scale
+
 
 class MXRows:
     """Activation rows [M, K] in MX blocks of `elem`, tiled (quant_rows): `data` uint8, the elements, then

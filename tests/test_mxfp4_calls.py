@@ -1,6 +1,10 @@
 """Calls of kernels.mxfp4 that end before anything is launched, without a GPU: the library's entry points are
 replaced by a list of what would have been called."""
 
+import copy
+import io
+import pickle
+
 import pytest
 import torch
 
@@ -102,3 +106,24 @@ def test_the_head_takes_rounded_rows(launched, M, elem):
     with pytest.raises(ValueError, match="do not match"):
         lmhead.lm_head_argmax(rows(M, 96, elem), weight())
     assert not launched
+
+
+def _saved(q):
+    f = io.BytesIO()
+    torch.save(q, f)
+    f.seek(0)
+    return torch.load(f, weights_only=False)  # (written just above)
+
+
+@pytest.mark.parametrize("again", [copy.copy, copy.deepcopy, lambda q: pickle.loads(pickle.dumps(q)),
+                                   lambda q: pickle.loads(pickle.dumps(q, protocol=2)), _saved,
+                                   lambda q: copy.deepcopy({"layer": [q]})["layer"][0]])
+def test_copies_and_pickles_of_a_weight(again):
+    q = weight(17, 544)
+    parts = (q[0], q[1], q.tiled, q.tiled_scale)
+    for i, t in enumerate(parts):
+        t.random_(256, generator=torch.Generator().manual_seed(i))
+    p = again(q)
+    assert type(p) is X.MXFP4Weight and len(p) == 2 and p.shape == (17, 544)
+    for a, b in zip(parts, (p[0], p[1], p.tiled, p.tiled_scale)):
+        assert torch.equal(a, b) and (a.data_ptr() == b.data_ptr()) == (again is copy.copy)
