@@ -103,6 +103,7 @@ class PersistentMLP:
             raise ValueError(f"PersistentMLP: weights {w_gu.shape} / {w_down.shape} do not match H={H}, I={I}")
         if self.chained or self.one_launch:
             raise ValueError("PersistentMLP: MXFP4 weights run as two launches")
+        _mxfp4._check_split(S, I)  # (before the first launch)
         h2 = _fp8._rows(h)
         if h2.shape[0] != self.M:
             raise ValueError(f"PersistentMLP built for M={self.M}, called with M={h2.shape[0]}")

@@ -22,6 +22,7 @@ DECODE_MAX_ROWS = 32  # rows of the skinny kernels
 BLOCK = 32
 ROW_MAX_K = 10240  # up to here the skinny kernels round a single bf16 row themselves, without a workspace,
 ROWS_MAX_K = 5120  # and up to here L.MX_BF16_ROWS of them
+GROUP, SPLIT_MAX = 512, 64  # k of a group, the unit that split-K shares out; the most parts
 
 
 class MXFP4Weight(tuple):
@@ -217,14 +218,19 @@ def _operand(x, q, elem):
     return t, p, scale, kind, ELEMS[elem] if elem in ELEMS else _elem(elem), ld, M
 
 
+def _check_split(split, K):
+    """Refuses a split that some part of K would have no group for."""
+    if not 1 <= split <= min(-(-K // GROUP), SPLIT_MAX):
+        raise ValueError(f"split={split} of {-(-K // GROUP)} groups of {GROUP} (K={K}), at most {SPLIT_MAX}")
+
+
 def _decode(x, q, split, mode, elem):
     t, p, scale, kind, e, ld, M = _operand(x, q, elem)
     N, K = q.shape
     if M > DECODE_MAX_ROWS:
         raise ValueError(f"M={M} > {DECODE_MAX_ROWS} rows: use gemm_mxfp4 or linear_mxfp4")
     if mode == L.OUT_PARTIAL:
-        if split < 1:
-            raise ValueError(f"split={split}")
+        _check_split(split, K)
         out = t.new_empty((split, M, N), dtype=torch.float32)
     else:
         if mode == L.OUT_SWIGLU:
@@ -251,7 +257,7 @@ def gemv_mxfp4(x, q, split=1, elem="e4m3"):
     """MXFP4 counterpart of fp8.gemv_fp8: x [M, K] bf16 (M <= 32; rounded to blocks of elem) or MXRows, q an
     MXFP4Weight [N, K]. split == 1: bf16 [M, N]. split > 1: fp32 partials [split, M, N] whose in-order sum is
     the product; split s covers the groups of 512 k [s G / split, (s + 1) G / split), G = ceil(K / 512), so
-    split <= G."""
+    split <= G, and at most 64."""
     return _decode(x, q, split, L.OUT_BF16 if split == 1 else L.OUT_PARTIAL, elem)
 
 

@@ -11,6 +11,7 @@ import torch
 from kernels import _lib as L
 from kernels import lmhead
 from kernels import mxfp4 as X
+from kernels.mlp import PersistentMLP
 
 
 def u8(*shape):
@@ -127,3 +128,27 @@ def test_copies_and_pickles_of_a_weight(again):
     assert type(p) is X.MXFP4Weight and len(p) == 2 and p.shape == (17, 544)
     for a, b in zip(parts, (p[0], p[1], p.tiled, p.tiled_scale)):
         assert torch.equal(a, b) and (a.data_ptr() == b.data_ptr()) == (again is copy.copy)
+
+
+@pytest.mark.parametrize("K,split", [(64, 2), (1024, 3), (1024, 0), (1024, -1), (40960, 65), (1 << 20, 1 << 20)])
+def test_a_split_without_groups_is_refused_before_its_output_is_made(monkeypatch, launched, K, split):
+    """With a tensor on the device the partials would be allocated next: split [M, N] planes of them."""
+    r, q = rows(4, K), weight(16, K)
+    made = []
+    data = OnDevice(r.data, 0)
+    data.new_empty = lambda *a, **k: made.append(a)
+    r.data, q.tiled, q.tiled_scale = data, OnDevice(q.tiled, 0), OnDevice(q.tiled_scale, 0)
+    with pytest.raises(ValueError, match=f"split={split}"):
+        X._decode(r, q, split, L.OUT_PARTIAL, "e4m3")
+    assert not launched and not made
+
+
+def test_the_mlp_refuses_a_split_before_its_first_launch(monkeypatch, launched):
+    """I = 1,024 is two groups; split = 4 is one that FP8 weights take."""
+    H, I = 512, 1024
+    mlp = PersistentMLP(1, H, I, "cpu", split=4)
+    monkeypatch.setattr(X, "gemv_swiglu_mxfp4", lambda *a: launched.append(a))
+    monkeypatch.setattr("kernels.fp8._rows", lambda h: h)
+    with pytest.raises(ValueError, match="split=4 of 2 groups"):
+        mlp(torch.zeros(1, H, dtype=torch.bfloat16), weight(2 * I, H), weight(H, I))
+    assert not launched and mlp.act is None
