@@ -156,12 +156,16 @@ __global__ __launch_bounds__(256) void k_mx_embed(const ID* __restrict__ ids, co
     const bool real = id >= 0 && id < N;
     const int64_t row = real ? id : 0;
     const uint32_t o = *reinterpret_cast<const uint32_t*>(q + row * (K >> 1) + 4 * c);
-    const float s = mx_scale(scale[row * (K >> 5) + (c >> 2)]);
+    // Codes 253 and 254: 4 (or 2) times the scale passes fp32 where its product with mult need not. 2^8 of the scale is kept back
+    // until then; the product before is normal for every mult, so that it is rounded as the whole one.
+    const uint32_t code = scale[row * (K >> 5) + (c >> 2)];
+    const bool far = code == 253u || code == 254u;
+    const float s = mx_scale(far ? code - 8 : code), rest = far ? 256.0f : 1.0f;
     const uint4 v = mx_dequant8_e2m1(o, 1.0f);
     uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      w[j] = pack_bf16x2(as_f32(w[j] << 16) * s * mult, as_f32(w[j] & 0xffff0000u) * s * mult);
+      w[j] = pack_bf16x2(as_f32(w[j] << 16) * s * mult * rest, as_f32(w[j] & 0xffff0000u) * s * mult * rest);
     *reinterpret_cast<uint4*>(out + i * K + 8 * c) = real ? make_uint4(w[0], w[1], w[2], w[3]) : kNaN8;
   }
 }

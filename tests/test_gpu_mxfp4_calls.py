@@ -8,6 +8,7 @@ import torch
 from kernels import _lib as L
 from kernels import lmhead
 from kernels import mxfp4 as X
+from oracle import mx as MX
 from test_gpu_mxfp4 import bf, check, reference, rounded, weight
 
 pytestmark = pytest.mark.gpu
@@ -46,3 +47,18 @@ def test_a_long_launch_has_a_workgroup_per_compute_unit_at_most(dev, sets):
            L.ptr(ws), nbytes, L.ptr(idx), L.stream(h))
     assert 0 < int(ws.ne(0x5A5A5A5A5A5A5A5A).sum()) <= 2 * 256
     assert idx.item() == int(torch.argmax(logits.float().cpu(), -1))
+
+
+@pytest.mark.parametrize("mult", [1.0, 0.5, 0.25, 2.0 ** -8, 50.596442562694074, 3.0e-38, 2.0 ** -140, 2.0 ** -149, 2.0 ** 100, -1.0, 0.0])
+def test_embedding_of_every_scale(dev, mult):
+    """Every element under every scale code, a row each, times multipliers from the smallest to large ones: the value times mult in
+    64 bits, then the one rounding of fp32 and that of bf16. Codes 253 and 254 hold values beyond fp32 whose products are not."""
+    K = 32
+    codes = np.tile(np.arange(16, dtype=np.uint8), (256, K // 16))
+    scale = np.arange(256, dtype=np.uint8)[:, None].copy()
+    q = X.pack(torch.from_numpy(MX.pack4(codes)).to(dev), torch.from_numpy(scale).to(dev))
+    y = X.embedding(torch.arange(256, device=dev), q, mult).cpu()
+    v = torch.from_numpy(MX.values(codes, scale, "e2m1")) * float(np.float32(mult))
+    want = v.float().bfloat16()
+    assert torch.equal(y.isnan(), want.isnan()) and want[255].isnan().all()
+    assert torch.equal(y.nan_to_num(0), want.nan_to_num(0))
