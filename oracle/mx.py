@@ -84,3 +84,24 @@ def tile(codes, scale, elem):
     s[:M, :K // 32] = scale
     s = s.reshape(mb, 16, ks, 4, 4).transpose(0, 2, 4, 1, 3)  # row block, group, g, r, tile
     return np.ascontiguousarray(data).reshape(-1), np.ascontiguousarray(s).reshape(-1)
+
+
+def norm_limit(xv, wv, elem, step):
+    """How far the outputs of a product of rounded rows xv [M, K] and weights wv [N, K] may be from xv wv^T in the 2-norm over
+    all of them, for data whose products have independent signs. A bound on one element has to allow for every rounding of its
+    sum to fall one way; over many outputs they do not, and a product that is lost everywhere, or sums kept in too few
+    bits, show here. In the 2-norm, R^2 = sum_k x^2 w^2 of an output, which is what the square of its sum, and of every
+    partial sum at most, amounts to on average:
+      output       half a step `step` of the value: step |y|
+      accumulator  ceil(K / 128) + 16 results (instructions; additions of waves and parts), each of at most four fp32
+                   sums that are off by a step 2^-23 of a partial sum: (ceil(K / 128) + 16) 2^-21 R, all of them one way
+      e4m3         a product loses less than u = 2^-13 max|x| max|w| of its block, in the direction of its own sign: the squares
+                   of the block's 32 losses add up, sqrt(sum_b 32 u_b^2)"""
+    M, K = xv.shape
+    y = np.linalg.norm(xv @ wv.T)
+    R = np.sqrt(((xv ** 2) @ (wv ** 2).T).sum())
+    cut = 0.0
+    if elem == "e4m3":
+        top = lambda v: (np.abs(v).reshape(len(v), -1, 32).max(-1)) ** 2
+        cut = 2.0 ** -13 * np.sqrt(32 * (top(xv) @ top(wv).T).sum())
+    return step * y + (-(-K // 128) + 16) * 2.0 ** -21 * R + cut

@@ -62,3 +62,28 @@ def test_embedding_of_every_scale(dev, mult):
     want = v.float().bfloat16()
     assert torch.equal(y.isnan(), want.isnan()) and want[255].isnan().all()
     assert torch.equal(y.nan_to_num(0), want.nan_to_num(0))
+
+
+@pytest.mark.parametrize("elem", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("M", [1, 6, 12, 20, 40])
+def test_products_under_every_pair_of_scales(dev, M, elem):
+    """One element of a row against weights of every scale code: a product of two values is exact, in bf16 too, from 2^-126 up to
+    the largest bf16 value and is infinite above it; below 2^-126 it is off by less than that at most."""
+    K = 32
+    g = np.random.default_rng(5)
+    codes = g.integers(0, 16, (255, K)).astype(np.uint8)
+    scale = np.arange(255, dtype=np.uint8)[:, None].copy()
+    q = X.pack(torch.from_numpy(MX.pack4(codes)).to(dev), torch.from_numpy(scale).to(dev))
+    wv = MX.values(codes, scale, "e2m1")
+    for start in range(-126, 121, M):
+        x = torch.zeros(M, K)
+        for m in range(M):
+            x[m, (7 * m + start) % K] = 1.5 * 2.0 ** min(start + m, 121) * (-1) ** m
+        x = x.bfloat16()
+        with np.errstate(over="ignore"):
+            want = torch.from_numpy(rounded(x, elem) @ wv.T).float().bfloat16().double().numpy()
+        for src in (x.to(dev), X.quant_rows(x.to(dev), elem)):
+            y = X.linear_mxfp4(src, q, elem).double().cpu().numpy()
+            with np.errstate(invalid="ignore"):  # (infinity less itself)
+                bad = ~((y == want) | (np.abs(y - want) < 2.0 ** -126))
+            assert not bad.any(), (start, np.argwhere(bad)[:4], y[bad][:4], want[bad][:4])
