@@ -419,7 +419,8 @@ int krq_unpack_fp8(const void* w8_tiled, int64_t N, int64_t K, void* w8_rowmajor
 /* element types of MX blocks, and the activation kinds of krq_gemv_mxfp4 */
 #define KRQ_MX_E2M1 0
 #define KRQ_MX_E4M3 1
-#define KRQ_MX_X_BF16 0     /* bf16 rows; a few are rounded in the kernel (one of 10,240 k, KRQ_MX_BF16_ROWS of 5,120), others need ws */
+#define KRQ_MX_X_BF16 0     /* bf16 rows; rounded in the product's launch are one of up to 10,240 k a split, KRQ_MX_BF16_ROWS of up to 5,120
+                               and, over many columns, 16 of up to 3,584; others are rounded into ws by a launch before */
 #define KRQ_MX_X_TILED 1    /* rows from krq_quant_mx_rows, with their scales */
 #define KRQ_MX_BF16_ROWS 8
 
@@ -460,7 +461,8 @@ int krq_embed_mxfp4(const void* ids, int ids_64, int64_t T, const void* w4, cons
  * [split, M, N], split s the sum over the groups of 512 k [s G / split, (s + 1) G / split), G = ceil(K / 512),
  * split <= min(G, 64); KRQ_OUT_SWIGLU (w = [gate; up], N = 2 I, I % 16 == 0) -> bf16 [M, I] =
  * bf16(silu(g) * u) from the fp32 g and u. K % 32 == 0, any N. ws: krq_gemv_mxfp4_ws_bytes(x_kind, elem, M, K,
- * split) bytes on 16 (may be NULL for 0; overwritten, not to be shared by calls that overlap).
+ * split) bytes on 16, enough for every N (may be NULL for 0, and where the rows are rounded in the launch; overwritten, not to be
+ * shared by calls that overlap).
  */
 int krq_gemv_mxfp4(const void* x, const void* x_scale, int x_kind, int elem, int64_t ldx, const void* w_tiled,
                    const void* w_scale, int64_t M, int64_t N, int64_t K, int split, int mode, void* ws, int64_t ws_bytes,

@@ -671,7 +671,8 @@ int launch_elem(const MxArgs& a, int elem, bool bf16, bool wide, int splits, hip
   return elem == KRQ_MX_E2M1 ? launch_mode<KRQ_MX_E2M1, MODE>(a, bf16, splits, s) : launch_mode<KRQ_MX_E4M3, MODE>(a, bf16, splits, s);
 }
 
-// bf16 rows that a launch rounds itself: one whose groups its waves hold, or a few over one group per wave. Rounded before /
+// bf16 rows that a launch of any N rounds itself (k_gemv_mx_wide: up to sixteen): one whose groups its waves hold, or a few over
+// one group per wave. Rounded before /
 // in the launch, us: SwiGLU over 19,456 x 2,560, M = 5 10.4 / 8.8, M = 8 10.4 / 8.8; 2,560 x 9,728, M = 1 9.0 / 5.2, M = 5
 // (two groups per wave) 9.2 / 11.3.
 bool rounds_rows(int64_t M, int64_t K, int split) {
@@ -683,6 +684,11 @@ bool rounds_rows(int64_t M, int64_t K, int split) {
 
 namespace krq {
 
+int64_t gemv_mx_rows_bytes(int x_kind, int elem, int64_t M, int64_t N, int64_t K, int split, int mode) {
+  const bool in_launch = rounds_rows(M, K, split) || (M <= 16 && takes_wide(M, N, K, mode));
+  return x_kind == KRQ_MX_X_BF16 && !in_launch ? mx_rows_bytes(elem, M, K) : 0;
+}
+
 // The checks and the launch of every product on MXFP4 weights of at most 32 rows (kOutArgmax: the head's).
 int gemv_mx_run(const char* what, const void* x, const void* x_scale, int x_kind, int elem, int64_t ldx, const void* w,
                 const void* w_scale, int64_t M, int64_t N, int64_t K, int split, int mode, void* ws, int64_t ws_bytes, void* out,
@@ -693,7 +699,7 @@ int gemv_mx_run(const char* what, const void* x, const void* x_scale, int x_kind
   KRQ_REQUIRE(M >= 1 && M <= 32, "%s: M=%lld outside 1..32", what, (long long)M);
   KRQ_REQUIRE(N >= 1 && N <= 0x7fffffff - 64 && K >= kMxBlock && K % kMxBlock == 0 && K <= 0x3fffffff, "%s: shape N=%lld K=%lld (K a multiple of 32)", what,
               (long long)N, (long long)K);
-  const int64_t rows = krq_gemv_mxfp4_ws_bytes(x_kind, elem, M, K, std::max(split, 1));
+  const int64_t rows = gemv_mx_rows_bytes(x_kind, elem, M, N, K, std::max(split, 1), mode);
   KRQ_REQUIRE(x_kind == KRQ_MX_X_BF16 || x_scale, "%s: tiled rows need their scales", what);
   KRQ_REQUIRE(x_kind != KRQ_MX_X_BF16 || (ldx >= K && ldx % 8 == 0), "%s: rows of x must start on 16 bytes (ldx=%lld)", what, (long long)ldx);
   KRQ_REQUIRE(aligned16(x) && aligned16(x_scale) && aligned16(w) && aligned16(w_scale) && aligned16(ws),
@@ -704,8 +710,8 @@ int gemv_mx_run(const char* what, const void* x, const void* x_scale, int x_kind
   KRQ_REQUIRE(split == 1 || mode == KRQ_OUT_PARTIAL, "%s: split=%d needs the partials output", what, split);
   const bool swiglu = mode == KRQ_OUT_SWIGLU;
   KRQ_REQUIRE(!swiglu || N % 32 == 0, "%s: SwiGLU needs N=%lld = 2 I with I %% 16 == 0", what, (long long)N);
-  const bool wide = takes_wide(M, N, K, mode), bf16 = x_kind == KRQ_MX_X_BF16 && (rows == 0 || (wide && M <= 16));
-  if (rows && !bf16) {
+  const bool wide = takes_wide(M, N, K, mode), bf16 = x_kind == KRQ_MX_X_BF16 && rows == 0;
+  if (rows) {
     uint8_t* sc = (uint8_t*)ws + mx_rows_scale_at(elem, M, K);
     if (const int rc = krq_quant_mx_rows(x, M, K, ldx, elem, ws, sc, stream)) return rc;
     x = ws;

@@ -391,8 +391,8 @@ int64_t mxfp4_cand_bytes(int64_t M, int64_t V) { return ((V / 16 + 2) * M * (int
 }  // namespace
 
 extern "C" int64_t krq_lmhead_mxfp4_ws_bytes(int x_kind, int elem, int64_t M, int64_t V, int64_t K) {
-  const int64_t rows = krq_gemv_mxfp4_ws_bytes(x_kind, elem, M, K, 1);
-  return rows < 0 || V < 1 ? -1 : mxfp4_cand_bytes(M, V) + rows;
+  if (krq_gemv_mxfp4_ws_bytes(x_kind, elem, M, K, 1) < 0 || V < 1) return -1;  // (bad arguments)
+  return mxfp4_cand_bytes(M, V) + gemv_mx_rows_bytes(x_kind, elem, M, V, K, 1, kOutArgmax);
 }
 
 extern "C" int krq_lmhead_argmax_mxfp4(const void* h, const void* h_scale, int x_kind, int elem, int64_t ldh,

@@ -93,6 +93,9 @@ KRQ_DEV void barrier_lds() {
 inline int64_t mx_rows_scale_at(int elem, int64_t M, int64_t K) { return (krq_mx_tiled_bytes(M, K, elem) + 255) & ~(int64_t)255; }
 inline int64_t mx_rows_bytes(int elem, int64_t M, int64_t K) { return mx_rows_scale_at(elem, M, K) + krq_mx_scale_bytes(M, K); }
 
+// Bytes of workspace that gemv_mx_run takes: room for the rounded rows where they are not rounded in the launch.
+int64_t gemv_mx_rows_bytes(int x_kind, int elem, int64_t M, int64_t N, int64_t K, int split, int mode);
+
 // The checks and the launch of every product on MXFP4 weights of at most 32 rows (gemv_mxfp4.hip; kOutArgmax:
 // the lm head's, *cands candidates of each row to cand [M][*cands], at most 2 more than row blocks).
 int gemv_mx_run(const char* what, const void* x, const void* x_scale, int x_kind, int elem, int64_t ldx, const void* w,

@@ -12,8 +12,9 @@ FP8 heads take the activation scaling of the weight's form:
       engine.py:504-505): exactly linear_fp8(h, lm8) followed by torch.argmax (engine.py:989,
       :1022) - one ActScale over all of h (at M == 1 the same as per token, so inside the GEMV),
       or the given ActScale / SharedScale `a`.
-MXFP4 heads take h in e4m3 blocks (mxfp4.quant_rows), rounded inside the GEMV where it takes bf16 rows
-(one of up to 10,240 k, eight of up to 5,120), else by a launch before it.
+MXFP4 heads take h in e4m3 blocks, rounded inside the GEMV where it takes bf16 rows (one of up to 10,240 k, eight of
+up to 5,120, sixteen of up to 3,584 under 16,000 or more columns), else by a launch before it, or as
+mxfp4.quant_rows rounded them.
 """
 
 import torch

@@ -152,3 +152,27 @@ def test_the_mlp_refuses_a_split_before_its_first_launch(monkeypatch, launched):
     with pytest.raises(ValueError, match="split=4 of 2 groups"):
         mlp(torch.zeros(1, H, dtype=torch.bfloat16), weight(2 * I, H), weight(H, I))
     assert not launched and mlp.act is None
+
+
+@pytest.mark.parametrize("M,V,K,asked", [(8, 151936, 2560, 0), (9, 151936, 2560, 0), (16, 16000, 3584, 0), (16, 15984, 2560, 1), (17, 151936, 2560, 1),
+                                         (16, 151936, 3616, 1), (2, 16, 5152, 1), (1, 16, 10240, 0), (1, 16, 10272, 1)])
+def test_the_head_asks_for_room_for_the_rows_only_where_they_are_rounded_before(M, V, K, asked):
+    lib = L.lib()
+    for e in (L.MX_E2M1, L.MX_E4M3):
+        cands = lib.krq_lmhead_mxfp4_ws_bytes(L.MX_X_TILED, e, M, V, K)
+        assert lib.krq_lmhead_mxfp4_ws_bytes(L.MX_X_BF16, e, M, V, K) - cands == asked * X._rows_bytes(M, K, e)[1]
+
+
+def test_workspaces_are_the_librarys_at_every_size(monkeypatch):
+    """The wrapper knows without a call which rows need no workspace, and most sizes of others: as the library says, everywhere."""
+    sizes = []
+    monkeypatch.setattr(X, "_call", lambda dev, name, *a: sizes.append(a[13]))
+    lib = L.lib()
+    for K in range(32, 12001, 32):
+        q = X.MXFP4Weight(u8(16, K // 2), u8(16, K // 32), OnDevice(u8(16), 0), OnDevice(u8(16), 0))
+        for M in (1, 2, 8, 9, 16, 17, 32):
+            x = OnDevice(torch.empty((M, K), dtype=torch.bfloat16), 0)
+            for split in {1, 2, 3, -(-K // 512)}:
+                if split <= -(-K // 512):
+                    X._decode(x, q, split, L.OUT_PARTIAL, "e4m3" if K % 64 else "e2m1")
+                    assert sizes.pop() == lib.krq_gemv_mxfp4_ws_bytes(L.MX_X_BF16, int(K % 64 != 0), M, K, split), (M, K, split)
