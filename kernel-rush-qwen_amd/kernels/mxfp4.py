@@ -32,9 +32,26 @@ class MXFP4Weight(tuple):
 
     def __new__(cls, w4, scale, tiled, tiled_scale):
         self = super().__new__(cls, (w4, scale))
-        self.tiled, self.tiled_scale = tiled, tiled_scale
         self.shape = (w4.shape[0], 2 * w4.shape[1])
+        N, K = self.shape
+        if N < 1 or K < BLOCK or K % BLOCK or tuple(scale.shape) != (N, K // BLOCK):
+            raise ValueError(f"MXFP4Weight: w4 {tuple(w4.shape)} and scale {tuple(scale.shape)} do not match")
+        cls._check("w4", w4, N * K // 2)
+        cls._check("scale", scale, N * K // BLOCK)
+        self.tiled, self.tiled_scale = tiled, tiled_scale
         return self
+
+    @staticmethod
+    def _check(name, t, size):
+        if t.dtype != torch.uint8 or t.numel() != size or not t.is_contiguous():
+            raise ValueError(f"MXFP4Weight: {name} must be {size} contiguous bytes, got {t.dtype} {tuple(t.shape)}")
+
+    def __setattr__(self, name, value):  # (the kernels read as many bytes as the shape needs)
+        if name == "tiled":
+            self._check(name, value, L.lib().krq_mx_tiled_bytes(*self.shape, L.MX_E2M1))
+        elif name == "tiled_scale":
+            self._check(name, value, L.lib().krq_mx_scale_bytes(*self.shape))
+        super().__setattr__(name, value)
 
     def __getnewargs__(self):  # (copies and pickles make a new one of these)
         return self[0], self[1], self.tiled, self.tiled_scale

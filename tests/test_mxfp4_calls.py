@@ -169,10 +169,28 @@ def test_workspaces_are_the_librarys_at_every_size(monkeypatch):
     monkeypatch.setattr(X, "_call", lambda dev, name, *a: sizes.append(a[13]))
     lib = L.lib()
     for K in range(32, 12001, 32):
-        q = X.MXFP4Weight(u8(16, K // 2), u8(16, K // 32), OnDevice(u8(16), 0), OnDevice(u8(16), 0))
+        q = weight(16, K)
+        q.tiled, q.tiled_scale = OnDevice(q.tiled, 0), OnDevice(q.tiled_scale, 0)
         for M in (1, 2, 8, 9, 16, 17, 32):
             x = OnDevice(torch.empty((M, K), dtype=torch.bfloat16), 0)
             for split in {1, 2, 3, -(-K // 512)}:
                 if split <= -(-K // 512):
                     X._decode(x, q, split, L.OUT_PARTIAL, "e4m3" if K % 64 else "e2m1")
                     assert sizes.pop() == lib.krq_gemv_mxfp4_ws_bytes(L.MX_X_BF16, int(K % 64 != 0), M, K, split), (M, K, split)
+
+
+def test_parts_that_do_not_match_make_no_weight():
+    """A weight's tiles and codes hold the bytes that its shape says the kernels read, when it is made and when they are replaced."""
+    q = weight(17, 544)
+    w4, scale, t, ts = q[0], q[1], q.tiled, q.tiled_scale
+    for bad in ((w4[:16], scale, t, ts), (w4, scale[:, :16], t, ts), (w4, scale, t[:-1], ts), (w4, scale, t, ts[:256]), (w4, scale, ts, t),
+                (w4, scale, t.view(torch.int16), ts), (w4, scale, t, ts.float()), (w4.int(), scale, t, ts), (w4.t().contiguous().t(), scale, t, ts),
+                (w4[:1].expand(17, -1), scale, t, ts), (w4, scale, t[:1].expand(t.numel()), ts), (u8(0, 272), u8(0, 17), u8(0), u8(0)),
+                (u8(17, 24), u8(17, 1), t, ts)):
+        with pytest.raises(ValueError, match="MXFP4Weight"):
+            X.MXFP4Weight(*bad)
+    for name, value in (("tiled", t[:1024]), ("tiled", t.float()), ("tiled_scale", ts[:-4]), ("tiled_scale", t)):
+        with pytest.raises(ValueError, match=name):
+            setattr(q, name, value)
+    assert q.tiled is t and q.tiled_scale is ts
+    q.tiled, q.tiled_scale = t.clone(), ts.clone()
