@@ -1,6 +1,7 @@
 """Microscaled 4-bit weights (MXFP4, OCP MX v1.0) on MI355X: quantizers, the decode and prefill products
-on the matrix cores' scaled instructions, and the embedding lookup of a packed table. The 4-bit
-counterpart of kernels.fp8 (the reference has none): 4.25 bits a weight, no calibration.
+on the matrix cores' scaled instructions, and the embedding lookup of a quantized table. The 4-bit
+counterpart of kernels.fp8 (the reference has none): a product reads 4.25 bits a weight; no calibration. A weight
+keeps its codes and scales twice, row-major and tiled, 8.5 bits in memory.
 
 A row is cut into blocks of 32 values along K with one E8M0 scale each, a power of two:
   scale   c = max(0, floor(log2(max|v|)) + 127 - emax), standing for 2^(c - 127); emax 2 (e2m1), 8 (e4m3)
@@ -9,8 +10,9 @@ A block with a NaN or an infinity has scale 255, NaN: every value of it, and eve
 NaN. Weights are e2m1; activation rows are rounded per call to e4m3 blocks (the default) or to e2m1 blocks
 (elem="e2m1": half the bytes and twice the matrix rate in prefill, 4-bit accuracy):
   linear_mxfp4 et al.  y = bf16(sum_k x[m, k] w[n, k]) over the rounded values, accumulated in fp32
-The kernels read operands in the tiled layout of include/krq.h ("mx tiled"). K is a multiple of 32; N and M
-are any.
+The products read operands in the tiled layout of include/krq.h ("mx tiled"), the embedding the row-major one. K is a
+multiple of 32, N any. M is any in gemm_mxfp4 and linear_mxfp4; the decode products gemv_mxfp4 and gemv_swiglu_mxfp4 take at
+most 32 rows (the FP8 ones go on in chunks), whose split-K shares out groups of 512 k.
 """
 
 import torch
@@ -279,9 +281,9 @@ def gemv_mxfp4(x, q, split=1, elem="e4m3"):
 
 
 def gemv_swiglu_mxfp4(x, q, elem="e4m3"):
-    """MXFP4 counterpart of fp8.gemv_swiglu_fp8: q packs w_gu [2I, K] = [gate; up], I % 16 == 0. Returns
-    bf16(silu(g) * u) [M, I] from the fp32 g and u (one rounding, where the FP8 form rounds g, silu(g) and
-    u first as the reference's does)."""
+    """MXFP4 counterpart of fp8.gemv_swiglu_fp8 for x of at most 32 rows: q packs w_gu [2I, K] = [gate; up], I % 16 == 0.
+    Returns bf16(silu(g) * u) [M, I] from the fp32 g and u (one rounding, where the FP8 form rounds g, silu(g) and
+    u first as the reference's does). More rows: silu(g) * u of the halves that linear_mxfp4 gives."""
     return _decode(x, q, 1, L.OUT_SWIGLU, elem)
 
 
@@ -313,9 +315,9 @@ def linear_mxfp4(x, q, elem="e4m3"):
 
 
 def embedding(ids, q, scale=1.0):
-    """Rows of the packed table q [N, K] by index, times scale (a model's embedding multiplier): bf16
-    [*ids.shape, K] = bf16(w[id] * scale) from the row-major codes, so a model with tied embeddings keeps one
-    packed table for this and the lm head. ids int64 or int32; an index outside [0, N) gives a row of NaN."""
+    """Rows of the quantized table q [N, K] by index, times scale (a model's embedding multiplier): bf16
+    [*ids.shape, K] = bf16(w[id] * scale) from the row-major codes. A model with tied embeddings passes one MXFP4Weight
+    here and to the lm head, which reads its tiled copy. ids int64 or int32; an index outside [0, N) gives a row of NaN."""
     N, K = _weight(q)
     if ids.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"ids must be int64 or int32, got {ids.dtype}")
