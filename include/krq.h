@@ -489,6 +489,48 @@ int krq_lmhead_argmax_mxfp4(const void* h, const void* h_scale, int x_kind, int 
                             const void* w_scale, int64_t M, int64_t V, int64_t K, void* logits, void* ws, int64_t ws_bytes,
                             int64_t* idx_out, void* stream);
 
+/*
+ * Residual addition and RMSNorm with the rows rounded for the next product (reference engine/kernels/ops.py:42-79, then
+ * the casts of engine/kernels/fp8.py:38-56):
+ *   d = bf16(p_0 + p_1 + ..), r = bf16(x + d), rstd = fp32(1 / sqrt(sum(r^2) / K + eps)) from an fp64 sum,
+ *   h = bf16(bf16(r * rstd) * ln)
+ * x bf16 [M, K], rows ldx elements apart. delta: NULL (r = x; res unused), split = 0: bf16 [M, K], rows ldd apart, or
+ * split >= 1: fp32 [split][M][K], rows ldd and slices `slice` elements apart. Rows start on 16 bytes. res: bf16 [M, K],
+ * may be x or a bf16 delta where those are contiguous. h: bf16 [M, K], or NULL where out holds the rows.
+ *   KRQ_NORM_ROWS             h alone
+ *   KRQ_NORM_FP8_TOKEN        out e4m3 [M, K], out_scale fp32 [M]: krq_quant_rows of h; _TILED: krq_quant_rows_tiled
+ *   KRQ_NORM_FP8_GIVEN        out e4m3 [M, K] = e4m3(clamp(h * inv[0])): krq_cast_fp8; _TILED: krq_cast_fp8_tiled
+ *   KRQ_NORM_MX_E4M3 / E2M1   out, out_scale: krq_quant_mx_rows of h
+ * K a multiple of 16 (MX 32, _TILED 64), at most 16384; M from 1.
+ */
+#define KRQ_NORM_ROWS 0
+#define KRQ_NORM_FP8_TOKEN 1
+#define KRQ_NORM_FP8_TOKEN_TILED 2
+#define KRQ_NORM_FP8_GIVEN 3
+#define KRQ_NORM_FP8_GIVEN_TILED 4
+#define KRQ_NORM_MX_E4M3 5
+#define KRQ_NORM_MX_E2M1 6
+int krq_add_rmsnorm(const void* x, int64_t ldx, const void* delta, int split, int64_t ldd, int64_t slice, const void* ln,
+                    float eps, int64_t M, int64_t K, int out_kind, const float* inv, void* res, void* h, void* out,
+                    void* out_scale, void* stream);
+
+/*
+ * Low-rank adapters of many requests beside one shared projection (no reference counterpart):
+ *   out[m, n] = y[m, n] + scales[i] * sum_r B[n, r] * (sum_k A[r, k] x[m, k]),  i = ids[m]
+ * x bf16 [M, K], rows ldx apart, on 16 bytes. ids [M] int64 (ids_64 != 0) or int32: negative adds nothing, slots or more
+ * gives a row of NaN. The projection has `parts` parts of parts_n[p] columns (a host array), N their sum, with a
+ * pair of factors each: a bf16 [slots][parts][rank][K]; b bf16 [slots][N * rank], of which slot i uses the first N * r as
+ * [N][r], r = ranks[i] rounded up to 16 (zeros past ranks[i]); ranks int32 [slots], at most rank, 0 for an empty slot;
+ * scales fp32 [slots] (all on the device). rank a multiple of 16 up to 256, parts up to 8, K a multiple of 16.
+ * y, out: bf16, or fp32 with fp32 != 0, rows ldy and ldo apart; out may be y.
+ * Sums in fp32, rounded once. ws: krq_lora_ws_bytes(M, K, parts, rank) bytes on 16 (overwritten; calls that overlap must
+ * not share it).
+ */
+int krq_lora_add(const void* x, int64_t ldx, const void* ids, int ids_64, const void* a, const void* b, const int32_t* ranks,
+                 const float* scales, int64_t slots, int64_t M, int64_t K, const int64_t* parts_n, int parts, int rank,
+                 const void* y, int64_t ldy, void* out, int64_t ldo, int fp32, void* ws, int64_t ws_bytes, void* stream);
+int64_t krq_lora_ws_bytes(int64_t M, int64_t K, int parts, int rank);
+
 const char* krq_version(void);
 const char* krq_last_error(void);
 

@@ -22,7 +22,7 @@ BUILD = os.path.join(HERE, "_build")
 OUT = os.path.join(HERE, "kernels", "libkrq.so")
 TIMELINE_OUT = os.path.join(HERE, "kernels", "libkrq_timeline.so")
 SOURCES = ["quant.hip", "gemv_fp8.hip", "gemv_bf16.hip", "lmhead.hip", "mlp.hip", "fused_gemv.hip", "fused_fp8.hip", "gemm_fp8.hip",
-           "mx_quant.hip", "gemv_mxfp4.hip", "gemm_mxfp4.hip"]
+           "mx_quant.hip", "gemv_mxfp4.hip", "gemm_mxfp4.hip", "norm.hip", "lora.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 in the generated code.
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17",
@@ -33,7 +33,7 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17",
 # M = 16 302.5 -> 296.8 us, M = 5 296.6 -> 290.2, the fused layer at M = 16 347.9 -> 342.5. The GEMVs
 # (weight streams, bound by HBM) measured the same with it and M = 1 0.3% slower, so they keep the load.
 PRELOAD = ["-mllvm", "-amdgpu-kernarg-preload-count=16"]
-FILE_FLAGS = {"quant.hip": PRELOAD, "fused_fp8.hip": PRELOAD, "mx_quant.hip": PRELOAD}
+FILE_FLAGS = {"quant.hip": PRELOAD, "fused_fp8.hip": PRELOAD, "mx_quant.hip": PRELOAD, "norm.hip": PRELOAD}
 
 
 def _run(cmd):

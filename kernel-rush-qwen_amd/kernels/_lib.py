@@ -21,6 +21,7 @@ ALGO_AUTO, ALGO_MFMA, ALGO_VALU = 0, 1, 2
 X_FP8, X_BF16_DYN, X_BF16_STATIC, X_FP8_TILED = 0, 1, 2, 3
 MX_E2M1, MX_E4M3 = 0, 1
 MX_X_BF16, MX_X_TILED, MX_BF16_ROWS = 0, 1, 8
+NORM_ROWS, NORM_FP8_TOKEN, NORM_FP8_TOKEN_TILED, NORM_FP8_GIVEN, NORM_FP8_GIVEN_TILED, NORM_MX_E4M3, NORM_MX_E2M1 = range(7)
 LMHEAD_SCRATCH_BYTES = 4194304  # KRQ_LMHEAD_SCRATCH_BYTES
 
 _vp, _i64, _i32, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
@@ -88,6 +89,10 @@ EXPORTS = {
     "krq_lmhead_mxfp4_ws_bytes": (_i64, [_i32, _i32, _i64, _i64, _i64]),
     "krq_lmhead_argmax_mxfp4": (_i32, [_vp, _vp, _i32, _i32, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp,
                                        _vp]),
+    "krq_add_rmsnorm": (_i32, [_vp, _i64, _vp, _i32, _i64, _i64, _vp, _f32, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "krq_lora_ws_bytes": (_i64, [_i64, _i64, _i32, _i32]),
+    "krq_lora_add": (_i32, [_vp, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i32, _i32, _vp, _i64, _vp, _i64,
+                            _i32, _vp, _i64, _vp]),
     "krq_version": (ctypes.c_char_p, []),
     "krq_last_error": (ctypes.c_char_p, []),
 }

@@ -1,0 +1,142 @@
+"""Low-rank adapters of many requests at once, beside one shared projection (HIP kernels k_lora_down and k_lora_up of
+libkrq.so; the reference has no counterpart):
+
+  out[m] = y[m] + s_i B_i (A_i x[m]),   i = ids[m]
+
+y [M, N] is what linear_fp8, gemv, gemv_fp8 or linear_mxfp4 gave for the rows x [M, K] (the bf16 rows, as norm.add_rmsnorm
+or add_rmsnorm_fp8(with_h=True) writes them), bf16 or fp32; a split-K product's partials take the adapters in one of
+them: add(p[0], x, adapters, ids, out=p[0]). Every row names its adapter, in any order, or none; sums are fp32, the result
+is rounded once. A projection fused from several (QKV, [gate; up]) has one pair of factors per part. Decode and
+prefill take the same call, two launches; rows and ids may change between replays of a captured one.
+"""
+
+import torch
+
+from . import _lib as L
+from . import mxfp4 as _mx
+
+MAX_PARTS, MAX_RANK = 8, 256
+
+
+class Adapters:
+    """The adapters of one projection [N, K], in `slots` slots of up to `rank` ranks (rounded up to 16).
+    K % 16 == 0; n: N, or the columns of each part of a fused projection in order (at most 8 parts).
+    A slot holds a pair of factors for every part, with a rank of its own: a call reads what the slots in use hold, not
+    `rank`. Slots start empty (rank 0), and an empty slot adds nothing. load and clear write into the same memory on the current stream, so
+    that captured calls see them; they must not run beside a call that reads the slot."""
+
+    def __init__(self, K, n, rank, slots, device):
+        self.parts = [int(n)] if isinstance(n, int) else [int(p) for p in n]
+        self.K, self.N, self.slots = int(K), sum(self.parts), int(slots)
+        if self.K < 16 or self.K % 16:
+            raise ValueError(f"K={K} must be a positive multiple of 16")
+        if not 1 <= len(self.parts) <= MAX_PARTS or min(self.parts) < 1:
+            raise ValueError(f"n={n}: 1 to {MAX_PARTS} parts of positive size")
+        if not 1 <= rank <= MAX_RANK:
+            raise ValueError(f"rank={rank} (1 to {MAX_RANK})")
+        if not 1 <= self.slots < 1 << 24:
+            raise ValueError(f"slots={slots}")
+        self.rank = (int(rank) + 15) // 16 * 16
+        # a slot's A: [parts, rank, K] with zeros past its own rank; its B: [N, its rank rounded up to 16], packed
+        self.a = torch.zeros((self.slots, len(self.parts), self.rank, self.K), device=device, dtype=torch.bfloat16)
+        self.b = torch.zeros((self.slots, self.N * self.rank), device=device, dtype=torch.bfloat16)
+        self.ranks = torch.zeros((self.slots,), device=device, dtype=torch.int32)
+        self.scales = torch.zeros((self.slots,), device=device, dtype=torch.float32)
+        self._n = (L.ctypes.c_int64 * len(self.parts))(*self.parts)
+
+    def _slot(self, slot):
+        if not 0 <= slot < self.slots:
+            raise ValueError(f"slot {slot} of {self.slots}")
+        return slot
+
+    @torch.no_grad()
+    def load(self, slot, pairs, scale=1.0):
+        """Put an adapter into a slot: pairs, for each part its (A [r, K], B [part's columns, r]), rounded to bf16, or None where the
+        adapter leaves the part alone; a single (A, B) for a projection of one part. Parts may differ in r, which is at most
+        the rank the Adapters were made for (each then takes the largest's memory). scale: the adapter's alpha / r."""
+        slot = self._slot(slot)
+        if len(self.parts) == 1 and len(pairs) == 2 and all(isinstance(t, torch.Tensor) for t in pairs):
+            pairs = [pairs]
+        if len(pairs) != len(self.parts):
+            raise ValueError(f"{len(pairs)} pairs for {len(self.parts)} parts")
+        rank = 0
+        for p, n in zip(pairs, self.parts):
+            if p is not None:
+                a, b = p
+                if a.dim() != 2 or b.dim() != 2 or a.shape[1] != self.K or b.shape[0] != n or a.shape[0] != b.shape[1]:
+                    raise ValueError(f"A {tuple(a.shape)} and B {tuple(b.shape)} do not match [r, {self.K}] and [{n}, r]")
+                if not 1 <= a.shape[0] <= self.rank:
+                    raise ValueError(f"rank {a.shape[0]} (1 to {self.rank})")
+                rank = max(rank, a.shape[0])
+        r16 = (rank + 15) // 16 * 16
+        self.a[slot].zero_()
+        packed = self.b[slot, :self.N * r16].view(self.N, r16)
+        packed.zero_()
+        at = 0
+        for i, (p, n) in enumerate(zip(pairs, self.parts)):
+            if p is not None:
+                a, b = p
+                self.a[slot, i, :a.shape[0]].copy_(a)
+                packed[at:at + n, :a.shape[0]].copy_(b)
+            at += n
+        self.scales[slot] = float(scale)
+        self.ranks[slot] = rank
+
+    @torch.no_grad()
+    def clear(self, slot):
+        """Empty a slot."""
+        self.ranks[self._slot(slot)] = 0
+
+
+def _rows(t, what, dtypes, cols):
+    if t.dim() != 2 or t.dtype not in dtypes or t.shape[1] != cols:
+        raise ValueError(f"{what} must be {' or '.join(str(d) for d in dtypes)} [M, {cols}], got {t.dtype} {tuple(t.shape)}")
+    ld = t.stride(0) if t.shape[0] > 1 else cols
+    return ld if (cols == 1 or t.stride(1) == 1) and ld >= cols else None
+
+
+def _extent(t, ld):
+    return t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * ld + t.shape[1]) * t.element_size()
+
+
+def add(y, x, adapters, ids, out=None):
+    """y [M, N] bf16 or fp32, x [M, K] bf16, ids [M] int32 or int64 (a slot of adapters for each row; negative: none) ->
+    y plus every row's adapter's product, in y's type. out: where it goes (default a new tensor; y itself adds in place).
+    An id past the last slot gives a row of NaN. Rows of y, x and out may lie apart; x's are copied where they do not start on 16 bytes."""
+    ad = adapters
+    L.require_device(y, x, ids, out)
+    dev = x.get_device()
+    if y.get_device() != dev or ids.get_device() != dev or ad.a.get_device() != dev or (out is not None and out.get_device() != dev):
+        raise ValueError(f"tensors on {x.device}, {y.device}, {ids.device}, {ad.a.device}")
+    ldx = _rows(x, "x", (torch.bfloat16,), ad.K)
+    M = x.shape[0]
+    ldy = _rows(y, "y", (torch.bfloat16, torch.float32), ad.N)
+    if ids.dtype not in (torch.int32, torch.int64) or tuple(ids.shape) != (M,) or y.shape[0] != M:
+        raise ValueError(f"ids {ids.dtype} {tuple(ids.shape)}, x {tuple(x.shape)} and y {tuple(y.shape)} do not match")
+    if ldx is None or ldx % 8 or x.data_ptr() % 16:
+        x, ldx = x.clone(memory_format=torch.contiguous_format), ad.K
+    ids = ids.contiguous()
+    if out is None:
+        out, ldo = torch.empty((M, ad.N), device=y.device, dtype=y.dtype), ad.N
+    else:
+        ldo = _rows(out, "out", (y.dtype,), ad.N)
+        if ldo is None or out.shape[0] != M:
+            raise ValueError(f"out must be [{M}, {ad.N}] with rows of consecutive values, got {tuple(out.shape)} strides {out.stride()}")
+    if ldy is None:
+        if out is y:
+            raise ValueError("y must have rows of consecutive values to be added to in place")
+        y, ldy = y.contiguous(), ad.N
+    if M == 0:
+        return out
+    for t, ld in ((y, ldy), (x, ldx)):
+        if t is y and out.data_ptr() == y.data_ptr() and ldo == ldy:
+            continue
+        (a0, a1), (b0, b1) = _extent(out, ldo), _extent(t, ld)
+        if a0 < b1 and b0 < a1:
+            raise ValueError("out overlaps an input (it may be y itself)")
+    nbytes = L.lib().krq_lora_ws_bytes(M, ad.K, len(ad.parts), ad.rank)
+    ws = torch.empty((max(nbytes, 1),), device=x.device, dtype=torch.uint8)
+    _mx._call(dev, "krq_lora_add", x.data_ptr(), ldx, ids.data_ptr(), ids.dtype is torch.int64, ad.a.data_ptr(), ad.b.data_ptr(),
+              ad.ranks.data_ptr(), ad.scales.data_ptr(), ad.slots, M, ad.K, ad._n, len(ad.parts), ad.rank, y.data_ptr(), ldy,
+              out.data_ptr(), ldo, y.dtype is torch.float32, ws.data_ptr(), nbytes)
+    return out
