@@ -531,6 +531,29 @@ int krq_lora_add(const void* x, int64_t ldx, const void* ids, int ids_64, const 
                  const void* y, int64_t ldy, void* out, int64_t ldo, int fp32, void* ws, int64_t ws_bytes, void* stream);
 int64_t krq_lora_ws_bytes(int64_t M, int64_t K, int parts, int rank);
 
+/*
+ * Beam search's selection behind the lm head (reference engine/engine.py:1021-1022 takes the argmax): for every batch entry b
+ * the n largest of
+ *   v[w, t] = scores[b, w] + (logits[b W + w, t] - lse[b W + w]),  lse = log sum_t exp(logits)
+ * over its W beams and V tokens, in order, with v in fp64; ties to the lower beam, then (equal logits of a beam) to the lower token.
+ * A beam whose logits are all -inf, or whose score is -inf, has v = -inf; one with a NaN or +inf among its logits, or as
+ * its score, NaN, which counts as largest. logits bf16, or fp32 with fp32 != 0, [B W, V], rows ld apart; scores fp32 [B, W].
+ * out_scores fp32 [B, n] (v rounded), out_beams and out_tokens int64 [B, n]. W and n up to 64, n <= W V, V up to 2^20,
+ * B W up to 65535. ws: krq_beam_select_ws_bytes bytes on 16 (overwritten; calls that overlap must not share it).
+ */
+int krq_beam_select(const void* logits, int fp32, int64_t ld, const float* scores, int64_t B, int64_t W, int64_t V, int64_t n,
+                    void* ws, int64_t ws_bytes, float* out_scores, int64_t* out_beams, int64_t* out_tokens, void* stream);
+int64_t krq_beam_select_ws_bytes(int64_t B, int64_t W, int64_t V, int64_t n, int fp32);
+/*
+ * States in the order of the chosen beams, in place: each of `count` (up to 64; states is a host array) is memory
+ * [outer][B * W][mid][S][dbytes], and row b W + w gets the positions s < lengths[b] of row b W + beams[b, w] as they were
+ * before; later positions stay (lengths NULL: all S move). beams [B, W] and lengths [B] on the device, int64 (beams_64,
+ * lengths_64 != 0) or int32. A beam outside [0, W) leaves its row as it is; a length is taken as at least 0 and at most S.
+ * States must not overlap. W up to 64, B up to 2^20.
+ */
+int krq_beam_reorder(void* const* states, int count, int64_t outer, int64_t B, int64_t W, int64_t mid, int64_t S, int64_t dbytes,
+                     const void* beams, int beams_64, const void* lengths, int lengths_64, void* stream);
+
 const char* krq_version(void);
 const char* krq_last_error(void);
 

@@ -1,0 +1,418 @@
+// Beam search's step behind the lm head: the n best continuations of every batch entry's beams, and the states put in
+// their order.
+//
+// Selection. v[w, t] = score[w] + (logit[w, t] - lse[w]), lse[w] = log sum_t exp(logit[w, t]); the n largest v of an
+// entry's W beams, ties to the lower beam, then to the lower token. Within a beam v goes as the logit, so the logits are
+// read once, by k_beam_rows: a workgroup takes a chunk of a row, keeps it in registers, and leaves the chunk's largest
+// value, its sum of exponentials and its n largest logits (with tokens, in order). k_beam_pick then takes a batch
+// entry: lse and the merged n of every row, and the merge of the rows by v in fp64 (candidates of two beams can lie
+// closer than fp32 tells apart).
+//
+// The n largest of a chunk. A logit and its token make one 64-bit key, all of them different: the logit's bits in an
+// order that compares as unsigned (NaN over everything), then the token's complement. The n-th largest of the 64 lanes'
+// largest keys, found bit by bit with ballots, has n keys at or above it, and only n lanes of a wave reach it: the keys
+// that do (n to a few n) go to LDS, and each finds its place by counting the larger ones. Equal logits cost nothing
+// extra, whatever their number.
+//
+// Bound by the read of the logits from a few rows on; by the two launches' latencies below.
+#include <algorithm>
+
+#include "gemv_common.h"
+
+using namespace krq;
+
+namespace {
+
+constexpr int kBeamMax = 64, kBeamThreads = 256, kPickThreads = 1024, kPickWaves = kPickThreads / 64;
+constexpr uint32_t kOrdInf = 0xff800000u, kOrdNegInf = 0x007fffffu;
+
+// fp32 bits in an order that compares as unsigned: NaN on top, -0 as +0
+KRQ_DEV uint32_t ord_of(float f) {
+  if (f != f) return 0xffffffffu;
+  const uint32_t u = as_u32(f + 0.0f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+KRQ_DEV float of_ord(uint32_t o) { return as_f32(o & 0x80000000u ? o & 0x7fffffffu : ~o); }  // (not of a NaN's)
+KRQ_DEV uint64_t ord_of_f64(double f) {
+  if (f != f) return ~0ull;
+  const uint64_t u = __builtin_bit_cast(uint64_t, f + 0.0);
+  return u >> 63 ? ~u : u | 1ull << 63;
+}
+KRQ_DEV uint32_t hi32(uint64_t k) { return static_cast<uint32_t>(k >> 32); }
+
+// The n-th largest of the wave's 64 keys (different but for zeros): its upper half bit by bit, then among the lanes that
+// share that the lower.
+KRQ_DEV uint64_t nth_key(uint64_t key, int n) {
+  const uint32_t hi = hi32(key), lo = static_cast<uint32_t>(key);
+  uint32_t t = 0;
+#pragma unroll
+  for (int b = 31; b >= 0; --b) {
+    const uint32_t c = t | 1u << b;
+    if (__popcll(__ballot(hi >= c)) >= n) t = c;
+  }
+  const int more = __popcll(__ballot(hi > t));
+  const uint64_t tied = __ballot(hi == t);
+  uint32_t u = 0;
+  if (__popcll(tied) > 1) {
+#pragma unroll
+    for (int b = 31; b >= 0; --b) {
+      const uint32_t c = u | 1u << b;
+      if (more + __popcll(__ballot(hi == t && lo >= c)) >= n) u = c;
+    }
+  } else {
+    u = __builtin_amdgcn_readlane(static_cast<int>(lo), __builtin_ctzll(tied | 1ull << 63));
+  }
+  return static_cast<uint64_t>(t) << 32 | u;
+}
+
+struct RowStat {
+  uint32_t top;  // ord_of the chunk's largest value
+  float sum;     // sum of exp(value - largest)
+};
+
+// 16 bytes of logits that start on any of them (an odd vocabulary's rows): chunks and threads take the same tokens wherever
+// a row starts, so that equal rows have equal sums.
+typedef unsigned int v4u_on2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned int v4u_on4 __attribute__((ext_vector_type(4), aligned(4)));
+KRQ_DEV v4u ld16_any(const uint16_t* p) { return *reinterpret_cast<const v4u_on2*>(p); }
+KRQ_DEV v4u ld16_any(const float* p) { return *reinterpret_cast<const v4u_on4*>(p); }
+
+template <typename T, int NV>
+__global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const T* __restrict__ logits, int64_t ld, int64_t V, int n, int chunks,
+                                                            RowStat* __restrict__ stat, uint64_t* __restrict__ cand) {
+  constexpr int VEC = 16 / sizeof(T), P = NV * VEC, CH = P * kBeamThreads;
+  extern __shared__ uint64_t list[];  // [4 n P]
+  __shared__ uint32_t tops[4];
+  __shared__ float sums[4];
+  __shared__ uint64_t nth[4];
+  __shared__ int count;
+  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, c = blockIdx.x;
+  const int64_t row = blockIdx.y;
+  const T* r = logits + row * ld;
+  const int64_t base = (int64_t)c * CH;
+  uint32_t o[P];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int64_t e = base + (v * kBeamThreads + tid) * VEC;
+    if (e + VEC <= V) {
+      const v4u a = ld16_any(r + e);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 2) {
+          o[v * VEC + 2 * i] = ord_of(as_f32(a[i] << 16));
+          o[v * VEC + 2 * i + 1] = ord_of(as_f32(a[i] & 0xffff0000u));
+        } else {
+          o[v * VEC + i] = ord_of(as_f32(a[i]));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        o[v * VEC + i] = 0;
+        if (e + i < V) {
+          if constexpr (sizeof(T) == 2) o[v * VEC + i] = ord_of(bf16_to_f32(r[e + i]));
+          else o[v * VEC + i] = ord_of(r[e + i]);
+        }
+      }
+    }
+  }
+  auto token = [&](int i) { return static_cast<uint32_t>(base + ((i / VEC) * kBeamThreads + tid) * VEC + i % VEC); };
+  uint64_t best = 0;  // (elements come in the order of their tokens: the first of the largest is the lowest)
+  uint32_t top = 0;
+  int at = 0;
+#pragma unroll
+  for (int i = 0; i < P; ++i)
+    if (o[i] > top) top = o[i], at = i;
+  if (top) best = static_cast<uint64_t>(top) << 32 | static_cast<uint32_t>(~token(at));
+  const uint64_t t = nth_key(best, n);
+  const uint32_t wt = wave_max_u32_dpp(top);
+  if (lane == 0) tops[w] = wt, nth[w] = t;
+  if (tid == 0) count = 0;
+  __syncthreads();
+  uint32_t m = tops[0];
+  uint64_t least = nth[0];
+#pragma unroll
+  for (int i = 1; i < 4; ++i) m = umax32(m, tops[i]), least = nth[i] > least ? nth[i] : least;
+  float s = 0.0f;
+  if (m > kOrdNegInf && m < kOrdInf) {
+    const float mx = of_ord(m);
+#pragma unroll
+    for (int i = 0; i < P; ++i) s += o[i] ? __expf(of_ord(o[i]) - mx) : 0.0f;
+  }
+  s = wave_sum(s);
+  if (lane == 0) sums[w] = s;
+  const uint32_t lh = hi32(least);
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    if (o[i] >= lh && o[i]) {
+      const uint64_t key = static_cast<uint64_t>(o[i]) << 32 | static_cast<uint32_t>(~token(i));
+      if (key >= least) list[atomicAdd(&count, 1)] = key;  // (at most n lanes of a wave, P keys each)
+    }
+  }
+  __syncthreads();
+  const int have = count;
+  uint64_t* out = cand + (row * chunks + c) * n;
+  for (int i = tid; i < have; i += kBeamThreads) {
+    const uint64_t key = list[i];
+    int rank = 0;
+    for (int j = 0; j < have; ++j) rank += list[j] > key;
+    if (rank < n) out[rank] = key;
+  }
+  for (int i = have + tid; i < n; i += kBeamThreads) out[i] = 0;  // (the chunk has fewer)
+  if (tid == 0) stat[row * chunks + c] = RowStat{m, (sums[0] + sums[1]) + (sums[2] + sums[3])};
+}
+
+// One batch entry. A wave merges a row at a time; then every row's sorted candidates meet in LDS, where each finds its
+// place by a binary search in the other rows.
+__global__ __launch_bounds__(kPickThreads) void k_beam_pick(const RowStat* __restrict__ stat, const uint64_t* __restrict__ cand,
+                                                            const float* __restrict__ scores, int64_t V, int W, int n, int chunks,
+                                                            int lists, float* __restrict__ out_scores,
+                                                            int64_t* __restrict__ out_beams, int64_t* __restrict__ out_tokens) {
+  extern __shared__ uint64_t mem[];  // values [W][n], tokens [W][n] (32 bits), a list for each of `lists` waves [n * per]
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int64_t b = blockIdx.x;
+  const int total = chunks * n, per = (total + 63) >> 6, len = static_cast<int>(min((int64_t)n, V));
+  uint64_t* vals = mem;
+  uint32_t* toks = reinterpret_cast<uint32_t*>(mem + W * n);
+  uint64_t* list = mem + W * n + (W * n + 1) / 2 + (int64_t)wave * n * per;
+  for (int w = wave; wave < lists && w < W; w += lists) {
+    const int64_t row = b * W + w;
+    const RowStat* st = stat + row * chunks;
+    const float score = scores[row];
+    uint32_t top = 0;
+    for (int c = lane; c < chunks; c += 64) top = umax32(top, st[c].top);
+    top = wave_max_u32_dpp(top);
+    // the kind of the row: v of all its candidates, where that is one value
+    const bool bad = top >= kOrdInf || !(score < __builtin_inff());
+    const bool dead = top == kOrdNegInf || score == -__builtin_inff();
+    if (bad || dead) {
+      for (int i = lane; i < len; i += 64) vals[w * n + i] = bad ? ~0ull : ord_of_f64(-__builtin_inf()), toks[w * n + i] = i;
+      continue;
+    }
+    const float mx = of_ord(top);
+    double s = 0.0;
+    for (int c = lane; c < chunks; c += 64) {
+      const RowStat q = st[c];
+      if (q.top > kOrdNegInf) s += q.sum * exp((double)of_ord(q.top) - (double)mx);
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
+    const double lse = (double)mx + log(s);
+    const uint64_t* rc = cand + row * total;
+    uint64_t best = 0;
+    for (int i = lane; i < total; i += 64) best = rc[i] > best ? rc[i] : best;
+    const uint64_t least = nth_key(best, n);
+    int have = 0;
+    for (int i0 = 0; i0 < total; i0 += 64) {
+      const uint64_t key = i0 + lane < total ? rc[i0 + lane] : 0;
+      const bool in = key && key >= least;
+      const uint64_t mask = __ballot(in);
+      if (in) list[have + __popcll(mask & ((1ull << lane) - 1))] = key;
+      have += __popcll(mask);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (int i = lane; i < have; i += 64) {
+      const uint64_t key = list[i];
+      int rank = 0;
+      for (int j = 0; j < have; ++j) rank += list[j] > key;
+      if (rank < len) {
+        vals[w * n + rank] = ord_of_f64((double)score + ((double)of_ord(hi32(key)) - lse));
+        toks[w * n + rank] = ~static_cast<uint32_t>(key);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  __syncthreads();
+  for (int i = tid; i < W * len; i += kPickThreads) {
+    const int w = i / len, p = i % len;
+    const uint64_t v = vals[w * n + p];
+    int rank = p;
+    for (int q = 0; q < W && rank < n; ++q) {
+      if (q == w) continue;
+      int lo = 0, hi = len;  // how many of row q come before: larger, or equal in a lower beam
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        const uint64_t u = vals[q * n + mid];
+        if (u > v || (u == v && q < w)) lo = mid + 1;
+        else hi = mid;
+      }
+      rank += lo;
+    }
+    if (rank < n) {
+      const int64_t at = b * n + rank;
+      out_scores[at] = v == ~0ull ? __builtin_nanf("")
+                                  : static_cast<float>(__builtin_bit_cast(double, v >> 63 ? v & ~(1ull << 63) : ~v));
+      out_beams[at] = w;
+      out_tokens[at] = toks[w * n + p];
+    }
+  }
+}
+
+struct SelectPlan {
+  int nv, chunks;
+  int64_t stat_bytes, bytes;
+};
+
+// Chunks of 32 values a thread, or of 8 where the rows would not fill the chip.
+SelectPlan select_plan(int64_t rows, int64_t V, int n, int esize) {
+  SelectPlan p;
+  const int vec = 16 / esize;
+  const int64_t most = (V + 32 * kBeamThreads - 1) / (32 * kBeamThreads);
+  const int values = rows * most >= 512 || most > 32 ? 32 : 8;
+  p.nv = values / vec;
+  p.chunks = static_cast<int>((V + values * kBeamThreads - 1) / (values * kBeamThreads));
+  p.stat_bytes = (rows * p.chunks * (int64_t)sizeof(RowStat) + 15) / 16 * 16;
+  p.bytes = p.stat_bytes + rows * p.chunks * n * (int64_t)sizeof(uint64_t);
+  return p;
+}
+
+// The waves of k_beam_pick that merge rows side by side, by the LDS that their lists take beside the rows', and that LDS.
+constexpr size_t kPickLds = 128 * 1024;
+int pick_lists(int W, int n, int chunks, size_t* lds) {
+  const size_t rows = sizeof(uint64_t) * (W * n + (W * n + 1) / 2), list = sizeof(uint64_t) * n * ((chunks * n + 63) / 64);
+  const int lists = static_cast<int>(std::min<size_t>((kPickLds - rows) / list, std::min(W, kPickWaves)));
+  *lds = rows + lists * list;
+  return lists;
+}
+// (48 KiB of rows and a list of 66 KiB at the most: the largest W, n and vocabulary)
+constexpr int64_t kVocabMax = 1 << 20;
+
+bool select_fits(int64_t B, int64_t W, int64_t V, int64_t n) {
+  return B >= 1 && W >= 1 && W <= kBeamMax && n >= 1 && n <= kBeamMax && V >= 1 && V <= kVocabMax && n <= W * V && B * W <= 65535;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Reordering. States are [outer][B W][mid][S][d] in memory; row b W + w takes the positions s < length[b] of row b W +
+// beams[b, w]. A thread owns the same unit of bytes in all W rows of an entry: it reads the sources of the rows that
+// change, then writes those, so that the work is done in place with no second copy, whatever the order.
+// ---------------------------------------------------------------------------------------------
+constexpr int kReorderStates = 64, kReorderThreads = 256;
+
+struct ReorderArgs {
+  void* state[kReorderStates];
+  const void* beams;
+  const void* lengths;
+  int64_t outer, mid, span, dbytes, S;  // span: S * dbytes
+  int B, W, blocks, beams64, lengths64;
+};
+
+template <typename U, int WM>
+__global__ __launch_bounds__(kReorderThreads) void k_beam_reorder(ReorderArgs a) {
+  const int64_t block = blockIdx.x % a.blocks;
+  int64_t at = blockIdx.x / a.blocks;
+  const int64_t h = at % a.mid;
+  at /= a.mid;
+  const int b = static_cast<int>(at % a.B);
+  const int64_t o = at / a.B;
+  int64_t len = a.span;
+  if (a.lengths) {
+    const int64_t l = a.lengths64 ? static_cast<const int64_t*>(a.lengths)[b] : static_cast<const int32_t*>(a.lengths)[b];
+    len = min(max(l, (int64_t)0), a.S) * a.dbytes;
+  }
+  const int64_t byte = (block * kReorderThreads + threadIdx.x) * (int64_t)sizeof(U);
+  if (byte >= len) return;
+  const int64_t row = a.mid * a.span;  // bytes between two rows
+  uint8_t* base = static_cast<uint8_t*>(a.state[blockIdx.y]) + ((o * a.B + b) * a.W * a.mid + h) * a.span + byte;
+  U v[WM];
+  uint64_t moved = 0;
+#pragma unroll
+  for (int w = 0; w < WM; ++w) {
+    if (w < a.W) {
+      const int64_t p = a.beams64 ? static_cast<const int64_t*>(a.beams)[b * a.W + w] : static_cast<const int32_t*>(a.beams)[b * a.W + w];
+      if (p != w && p >= 0 && p < a.W) {
+        v[w] = *reinterpret_cast<const U*>(base + p * row);
+        moved |= 1ull << w;
+      }
+    }
+  }
+#pragma unroll
+  for (int w = 0; w < WM; ++w)
+    if (moved >> w & 1) *reinterpret_cast<U*>(base + w * row) = v[w];
+}
+
+template <typename U>
+void launch_reorder(const ReorderArgs& a, int states, hipStream_t s) {
+  ReorderArgs r = a;
+  const int64_t unit = (int64_t)kReorderThreads * sizeof(U);
+  r.blocks = static_cast<int>((a.span + unit - 1) / unit);
+  const dim3 grid(static_cast<unsigned>(r.blocks * a.outer * a.B * a.mid), states);
+  if (a.W <= 4) hipLaunchKernelGGL((k_beam_reorder<U, 4>), grid, dim3(kReorderThreads), 0, s, r);
+  else if (a.W <= 8) hipLaunchKernelGGL((k_beam_reorder<U, 8>), grid, dim3(kReorderThreads), 0, s, r);
+  else if (a.W <= 16) hipLaunchKernelGGL((k_beam_reorder<U, 16>), grid, dim3(kReorderThreads), 0, s, r);
+  else if constexpr (sizeof(U) <= 4) hipLaunchKernelGGL((k_beam_reorder<U, kBeamMax>), grid, dim3(kReorderThreads), 0, s, r);
+}
+
+}  // namespace
+
+extern "C" int64_t krq_beam_select_ws_bytes(int64_t B, int64_t W, int64_t V, int64_t n, int fp32) {
+  if (!select_fits(B, W, V, n)) return -1;
+  return select_plan(B * W, V, static_cast<int>(n), fp32 ? 4 : 2).bytes;
+}
+
+extern "C" int krq_beam_select(const void* logits, int fp32, int64_t ld, const float* scores, int64_t B, int64_t W, int64_t V, int64_t n,
+                               void* ws, int64_t ws_bytes, float* out_scores, int64_t* out_beams, int64_t* out_tokens, void* stream) {
+  KRQ_REQUIRE(logits && scores && ws && out_scores && out_beams && out_tokens, "beam_select: null pointer");
+  KRQ_REQUIRE(select_fits(B, W, V, n), "beam_select: %lld x %lld beams, vocabulary %lld, n=%lld (beams and n up to %d, n <= beams * "
+              "vocabulary, rows up to 65535, vocabulary up to 2^20)", (long long)B, (long long)W, (long long)V, (long long)n, kBeamMax);
+  KRQ_REQUIRE(ld >= V, "beam_select: rows of %lld logits %lld apart", (long long)V, (long long)ld);
+  const int esize = fp32 ? 4 : 2;
+  KRQ_REQUIRE(reinterpret_cast<uintptr_t>(logits) % esize == 0 && aligned16(ws), "beam_select: logits or ws not on their alignment");
+  const SelectPlan p = select_plan(B * W, V, static_cast<int>(n), esize);
+  KRQ_REQUIRE(ws_bytes >= p.bytes, "beam_select: ws of %lld bytes, needs %lld", (long long)ws_bytes, (long long)p.bytes);
+  size_t lds;
+  const int lists = pick_lists(static_cast<int>(W), static_cast<int>(n), p.chunks, &lds);
+  RowStat* stat = (RowStat*)ws;
+  uint64_t* cand = (uint64_t*)((uint8_t*)ws + p.stat_bytes);
+  hipStream_t s = (hipStream_t)stream;
+  const dim3 grid(p.chunks, static_cast<unsigned>(B * W));
+  const size_t list = sizeof(uint64_t) * 4 * n * (p.nv * 16 / esize);
+#define KRQ_ROWS(T, NV)                                                                                                       \
+  hipLaunchKernelGGL((k_beam_rows<T, NV>), grid, dim3(kBeamThreads), list, s, (const T*)logits, ld, V, (int)n, p.chunks, stat, cand)
+  if (fp32) {
+    if (p.nv == 8) KRQ_ROWS(float, 8);
+    else KRQ_ROWS(float, 2);
+  } else {
+    if (p.nv == 4) KRQ_ROWS(uint16_t, 4);
+    else KRQ_ROWS(uint16_t, 1);
+  }
+#undef KRQ_ROWS
+  if (const int rc = krq_check_launch("beam_select")) return rc;
+  hipLaunchKernelGGL(k_beam_pick, dim3(static_cast<unsigned>(B)), dim3(kPickThreads), lds, s, stat, cand, scores, V, (int)W, (int)n,
+                     p.chunks, lists, out_scores, out_beams, out_tokens);
+  return krq_check_launch("beam_select");
+}
+
+extern "C" int krq_beam_reorder(void* const* states, int count, int64_t outer, int64_t B, int64_t W, int64_t mid, int64_t S,
+                                int64_t dbytes, const void* beams, int beams_64, const void* lengths, int lengths_64, void* stream) {
+  KRQ_REQUIRE(states && beams && count >= 1 && count <= kReorderStates, "beam_reorder: %d states (1 to %d)", count, kReorderStates);
+  KRQ_REQUIRE(outer >= 1 && B >= 1 && W >= 1 && W <= kBeamMax && mid >= 1 && S >= 1 && dbytes >= 1 && B <= (1 << 20),
+              "beam_reorder: bad shape [%lld][%lld x %lld][%lld][%lld][%lld bytes] (at most %d beams)", (long long)outer, (long long)B,
+              (long long)W, (long long)mid, (long long)S, (long long)dbytes, kBeamMax);
+  ReorderArgs a{};
+  uintptr_t bits = static_cast<uintptr_t>(dbytes);
+  for (int i = 0; i < count; ++i) {
+    KRQ_REQUIRE(states[i], "beam_reorder: null state");
+    a.state[i] = states[i];
+    bits |= reinterpret_cast<uintptr_t>(states[i]);
+  }
+  a.beams = beams;
+  a.lengths = lengths;
+  a.outer = outer;
+  a.mid = mid;
+  a.span = S * dbytes;
+  a.dbytes = dbytes;
+  a.S = S;
+  a.B = static_cast<int>(B);
+  a.W = static_cast<int>(W);
+  a.beams64 = beams_64 != 0;
+  a.lengths64 = lengths_64 != 0;
+  const int unit = bits % 16 == 0 && W <= 16 ? 16 : bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
+  const double blocks = (double)((a.span + (int64_t)kReorderThreads * unit - 1) / ((int64_t)kReorderThreads * unit)) * outer * B * mid;
+  KRQ_REQUIRE(blocks < 2147483647.0, "beam_reorder: a state is too large for one launch");
+  hipStream_t s = (hipStream_t)stream;
+  if (unit == 16) launch_reorder<v4u>(a, count, s);
+  else if (unit == 4) launch_reorder<uint32_t>(a, count, s);
+  else if (unit == 2) launch_reorder<uint16_t>(a, count, s);
+  else launch_reorder<uint8_t>(a, count, s);
+  return krq_check_launch("beam_reorder");
+}
