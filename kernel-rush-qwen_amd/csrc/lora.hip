@@ -3,20 +3,22 @@
 //   out[m, n] = y[m, n] + s_i sum_r B_i[n, r] h[m, r],   h[m, r] = sum_k A_i,p(n)[r, k] x[m, k],   i = ids[m]
 //
 // for the P parts of a fused projection (part p(n) of column n), each with its own factors. Two launches: k_lora_down
-// makes h, k_lora_up adds. A tile of rows may name any adapters in any order: a wave takes the distinct ones of its tile
-// one after the other (or, where rows are few, each by a workgroup of its own), multiplies the whole tile and writes the
-// rows that name it. The rows of a matrix-core operand do not mix, so rows of other adapters cost nothing but the idle
+// makes h, k_lora_up adds. Rows may name any adapters in any order: a tile of 16 takes its distinct ones one after the
+// other (or, where rows are few, each in a workgroup of its own), multiplies the whole tile and writes the rows that
+// name it; from 17 rows, windows of 256 are put in the order of their adapters first. The rows of a matrix-core operand do not mix, so rows of other adapters cost nothing but the idle
 // columns, and a NaN stays in its row.
 //
 // What bounds it: the factors of the adapters in use, read once each, at few rows; x, y and out at many. The products
 // are a few percent of the matrix cores' rate.
 //
-// k order. v_mfma_f32_16x16x32_bf16 adds products over 32 k of which lane group g = lane / 16 holds eight; which eight is
-// free as long as both operands agree. In steps of 64 k, group g takes k = 16 g .. 16 g + 15 of each row: 32 contiguous
-// bytes, so that the four groups read whole 128-byte lines of row-major factors and rows.
+// The down product's operands. v_mfma_f32_16x16x32_bf16 takes 16 bytes of one row per lane; sixteen consecutive lanes have
+// sixteen rows, so that loads of row-major operands touch a line per lane (a launch of 4,096 x 2,560 rows took 11.5 us bound
+// by that). A is kept in lane order, [K / 64][2][64 lanes][8] per 16 ranks, lane 16 g + j its rank j, k = 16 g + 8 e .. + 7 of a
+// step's 64; rows of x are loaded eight lanes to a line and turned through LDS, each wave its own.
 //
-// h is kept in fp32 and enters the second product as the sum of two bf16 (h to 2^-16 at most), so that the sum is rounded once,
-// at the end: the second product takes twice the matrix instructions, which it has to spare.
+// h is kept in fp32 and enters the second product as the sum of two bf16 (to 2^-16; three, to 2^-24, beside an fp32 y), so
+// that the sum is rounded once, at the end: the second product takes two or three times the matrix instructions, which
+// it has to spare.
 #include <algorithm>
 
 #include "mx_common.h"
@@ -25,27 +27,27 @@ using namespace krq;
 
 namespace {
 
-constexpr int kMaxParts = 8, kMaxRank = 256, kMaxSplit = 8;
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
+constexpr int kMaxParts = 8, kMaxRank = 256, kWindow = 256;
+constexpr int kSplitFew = 4, kSplitMany = 2;  // parts of K at most, for up to 256 rows and for more
 
 struct LoraArgs {
   const uint16_t* x;
   const void* ids;
-  const uint16_t* a;     // [slots][P][R][K]
+  const uint16_t* a;     // [slots][P][R / 16][steps][2][64][8]: lane order, zeros past K
   const uint16_t* b;     // [slots][N R], a slot's factors as [N][its rank, rounded up to 16]
   const int32_t* ranks;  // [slots], up to R; 0: none
   const float* scales;   // [slots]
   const void* y;
   void* out;
-  float* h;              // [split][M][P R]
+  int4* place;           // [M] what k_lora_down found at each place: row, id, rank
+  float* h;              // [split][M][P R] by place, times the scale
   int64_t M, K, ldx, ldy, ldo;
-  int slots, P, R, N, split, ids64, slot_ways;
+  int slots, P, R, N, split, ids64, ways;
   int part[kMaxParts + 1], block[kMaxParts + 1];  // first column of each part; first group of column blocks
 };
 
 KRQ_DEV int load_id(const LoraArgs& a, int64_t m) {  // -1: none; slots: out of range
-  int64_t id = a.ids64 ? static_cast<const int64_t*>(a.ids)[m] : static_cast<const int32_t*>(a.ids)[m];
+  const int64_t id = a.ids64 ? static_cast<const int64_t*>(a.ids)[m] : static_cast<const int32_t*>(a.ids)[m];
   return id < 0 ? -1 : id >= a.slots ? a.slots : static_cast<int>(id);
 }
 
@@ -56,11 +58,39 @@ KRQ_DEV int rank_of(const LoraArgs& a, int id) {
 KRQ_DEV v4f mfma32(uint4 a, uint4 b, v4f c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
-KRQ_DEV v4f mfma16(uint2 a, uint2 b, v4f c) {
-  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+// The rows of a workgroup's window (256 rows from w0) by adapter: the key of place i, id + 1 and the row in the window. A
+// window of few runs of the same id, as requests that follow each other make, stays as it is; another is sorted (each row
+// counts the rows before it, half of them in each of two threads), so that a tile of 16 places meets few adapters in
+// whatever order the rows name them. Rows past M are last. Sorting a window costs 3 us of a launch's 8 (4,096 x 2,560), a tile of
+// several adapters as much again for each.
+constexpr int kRunsMax = 12;
+KRQ_DEV void sort_window(const LoraArgs& a, int64_t w0, uint32_t* raw, uint32_t* sorted) {
+  const uint32_t t = threadIdx.x & (kWindow - 1), half = threadIdx.x / kWindow;
+  const uint32_t key = w0 + t < a.M ? static_cast<uint32_t>(load_id(a, w0 + t) + 1) << 8 | t : 0xffffffffu;
+  if (half == 0) raw[t] = key;
+  __syncthreads();
+  const int runs = __syncthreads_count(half == 0 && t > 0 && raw[t - 1] >> 8 != key >> 8);
+  uint32_t place = t;
+  if (runs > kRunsMax) {
+    uint32_t before = 0;
+#pragma unroll 8
+    for (int j = 0; j < kWindow / 2; j += 4) {
+      const uint4 o = *reinterpret_cast<const uint4*>(raw + half * (kWindow / 2) + j);
+      before += o.x < key;
+      before += o.y < key;
+      before += o.z < key;
+      before += o.w < key;
+    }
+    if (half) sorted[t] = before;
+    __syncthreads();
+    if (!half) place = w0 + t < a.M ? before + sorted[t] : t;  // (past M: equal keys, each stays, behind the others)
+    __syncthreads();
+  }
+  if (half == 0) sorted[place] = key;
+  __syncthreads();
 }
 
-// The distinct ids of up to 64 rows, one at a time: `id` is each lane's row's, `left` the lanes not yet taken.
+// The distinct ids of up to 64 places, one at a time: `id` is each lane's place's, `left` the lanes not yet taken.
 KRQ_DEV int next_id(int id, uint64_t& left, uint64_t& same) {
   const int cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
   same = __ballot(id == cur) & left;
@@ -68,276 +98,373 @@ KRQ_DEV int next_id(int id, uint64_t& left, uint64_t& same) {
   return cur;
 }
 
-// h. A workgroup takes MT tiles of 16 rows, TC tiles of 16 ranks (of the P r of the row's adapter) and one of the
-// `split` parts of K, its four waves a quarter of that each, summed in LDS in wave order.
-template <int MT, int TC>
-__global__ __launch_bounds__(256) void k_lora_down(LoraArgs a) {
-  __shared__ float red[4][MT * TC][64 * 4];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, j = lane & 15;
-  const int ways = a.slot_ways;
-  const int64_t m0 = (blockIdx.x / ways) * (int64_t)(16 * MT);
-  const int way = blockIdx.x % ways;
-  const int64_t mine = m0 + (lane & (16 * MT - 1));
-  const int id = load_id(a, min(mine, a.M - 1));
-  uint64_t left = __ballot(mine < a.M && lane < 16 * MT);
+// h. A workgroup takes MT tiles of 16 places, TC tiles of 16 ranks (of the P r of the adapter) and one of the `split`
+// parts of K, its NW waves a part of that each, summed in LDS in wave order. A wave has few steps of 64 k, so that a launch is
+// as long as its chain of loads, ids, ranks, the first NB steps: those of x wait for the row alone, and with TC = 1 those of
+// A for the id alone.
+template <int MT, int TC, int NW, int NB, bool SORT>
+__global__ __launch_bounds__(64 * NW, TC <= 2 ? 4 : 2) void k_lora_down(LoraArgs a) {
+  static_assert(64 * NW == 2 * kWindow);
+  constexpr int kOwn = (TC > 2 ? TC : 2) * MT * 64;  // a wave's LDS: a step of x, then its sums
+  __shared__ uint4 own[NW][kOwn];
+  __shared__ uint32_t sorted[SORT ? kWindow : 1];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, j = lane & 15;
+  // (the tiles' first workgroups before their second ones, which often have nothing to do: blocks go round the XCDs)
+  const uint32_t tiles = gridDim.x / a.ways;
+  const int64_t m0 = (blockIdx.x % tiles) * (int64_t)(16 * MT), w0 = SORT ? m0 / kWindow * kWindow : m0;
+  const int way = blockIdx.x / tiles, slot = lane & (16 * MT - 1);
   // this wave's part of K, in steps of 64
-  const int64_t steps = (a.K + 63) >> 6;
-  const int64_t q0 = blockIdx.z * 4 + w, qn = a.split * 4;
-  const int64_t s0 = steps * q0 / qn, s1 = steps * (q0 + 1) / qn;
-  for (int turn = 0; left; ++turn) {
-    uint64_t same;
-    const int cur = next_id(id, left, same);
-    if (ways > 1 && turn % ways != way) continue;
-    const int per = (rank_of(a, cur) + 15) >> 4, T = a.P * per;
-    const int t0 = blockIdx.y * TC;
-    if (t0 >= T) continue;
-    const uint16_t* ar[TC];
+  const int steps = static_cast<int>((a.K + 63) >> 6), q0 = blockIdx.z * NW + w, qn = a.split * NW;
+  const int s0 = static_cast<int>((int64_t)steps * q0 / qn), s1 = static_cast<int>((int64_t)steps * (q0 + 1) / qn);
+  int id;
+  if constexpr (SORT) {
+    sort_window(a, w0, reinterpret_cast<uint32_t*>(&own[0][0]), sorted);
+    id = static_cast<int>(sorted[m0 - w0 + slot] >> 8) - 1;
+  } else {
+    id = load_id(a, min(m0 + slot, a.M - 1));
+  }
+  const int most = static_cast<int>(min(a.M - w0, (int64_t)kWindow)) - 1;
+  auto row_of = [&](int place) {  // the row in the window of a place of the tile
+    return min(SORT ? static_cast<int>(sorted[m0 - w0 + place] & 255u) : place, most);
+  };
+  // x: lane l takes 16 bytes l % 8 of rows l / 8 and 8 + l / 8 of a tile's 128 of a step
+  const int c = lane & 7, last = static_cast<int>(a.K) - 8 - 8 * c;  // the last 8 k, from this lane's
+  const uint8_t* xw = reinterpret_cast<const uint8_t*>(a.x + w0 * a.ldx);
+  uint32_t xr[MT][2];  // (a window's rows lie within 4 GiB)
 #pragma unroll
-    for (int t = 0; t < TC; ++t) {
-      const int tt = min(t0 + t, T - 1);
-      ar[t] = a.a + (((int64_t)cur * a.P + tt / per) * a.R + 16 * (tt % per) + j) * a.K + 16 * g;
-    }
-    const uint16_t* xr[MT];
+  for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int i = 0; i < MT; ++i) xr[i] = a.x + min(m0 + 16 * i + j, a.M - 1) * a.ldx + 16 * g;
-    v4f acc[MT][TC] = {};
-#pragma unroll 2
-    for (int64_t s = s0; s < s1; ++s) {
-      const bool in = 64 * s + 16 * g < a.K;  // (K is a multiple of 16)
-      uint4 av[TC][2], xv[MT][2];
-#pragma unroll
-      for (int t = 0; t < TC; ++t)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) av[t][e] = in ? ld16(reinterpret_cast<const uint8_t*>(ar[t] + 64 * s + 8 * e)) : zero4();
+    for (int e = 0; e < 2; ++e) xr[i][e] = 2u * (row_of(16 * i + 8 * e + (lane >> 3)) * static_cast<uint32_t>(a.ldx) + 8 * c);
+  uint4 av[NB][TC][2], xv[NB][MT][2];
+  const uint4* ar[TC];
+  auto load_x = [&](int s, int at) {
+    if (s < s1) {
+      const int k = min(64 * s, last);
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) xv[i][e] = in ? ld16(reinterpret_cast<const uint8_t*>(xr[i] + 64 * s + 8 * e)) : zero4();
+        for (int e = 0; e < 2; ++e) {
+          xv[at][i][e] = ld16(xw + (xr[i][e] + 2 * k));
+        }
+    }
+  };
+  auto load_a = [&](int s, int at) {
+    if (s < s1) {
+#pragma unroll
+      for (int t = 0; t < TC; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) av[at][t][e] = ar[t][(2 * s + e) * 64];
+    }
+  };
+  const bool real = m0 + slot < a.M && lane < 16 * MT;
+  uint64_t left = __ballot(real);
+  const int rank = real ? rank_of(a, id) : 0;
+  const float scale = real && id >= 0 && id < a.slots ? a.scales[id] : 0.0f;
+  if (real && w == 0 && way == 0 && blockIdx.y == 0 && blockIdx.z == 0)
+    a.place[m0 + slot] = make_int4(static_cast<int>(w0) + row_of(slot), id, rank, 0);
+  // this workgroup's adapters of the tile: every `ways`-th, from the way-th
+  int turn = -1, first, cur;
+  uint64_t same;
+  auto next = [&]() {
+    while (left) {
+      first = __builtin_ctzll(left);
+      cur = next_id(id, left, same);
+      if (cur >= 0 && cur < a.slots && ++turn % a.ways == way) return true;
+    }
+    return false;
+  };
+  if (!next()) return;
+#pragma unroll
+  for (int u = 0; u < NB; ++u) load_x(s0 + u, u);
+  bool fresh = true;
+  do {
+    const int R16 = a.R >> 4;
+    int per = 1, T, t0 = blockIdx.y * TC;
+    auto tile_at = [&](int tile) { return reinterpret_cast<const uint4*>(a.a) + ((int64_t)cur * a.P * R16 + tile) * steps * 128 + lane; };
+    if constexpr (TC == 1) {  // tile blockIdx.y of the bank's, whatever the rank
+      ar[0] = tile_at(t0);
+#pragma unroll
+      for (int u = 0; u < NB; ++u) load_a(s0 + u, u);
+      per = (__builtin_amdgcn_readlane(rank, first) + 15) >> 4;
+      if (t0 % R16 >= per) continue;
+      t0 = t0 / R16 * per + t0 % R16;
+      T = t0 + 1;
+    } else {
+      per = (__builtin_amdgcn_readlane(rank, first) + 15) >> 4;
+      T = a.P * per;
+      if (t0 >= T) continue;
+#pragma unroll
+      for (int t = 0; t < TC; ++t) {
+        const int tt = min(t0 + t, T - 1);
+        ar[t] = tile_at(tt / per * R16 + tt % per);
+      }
+#pragma unroll
+      for (int u = 0; u < NB; ++u) load_a(s0 + u, u);
+    }
+    if (!fresh) {
+#pragma unroll
+      for (int u = 0; u < NB; ++u) load_x(s0 + u, u);
+    }
+    fresh = false;
+    v4f acc[MT][TC] = {};
+    auto multiply = [&](int s, int at) {
+      // slot (row, chunk ^ row % 8): neither the writes nor the reads of a chunk of sixteen rows meet in a bank
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          own[w][i * 128 + (8 * e + (lane >> 3)) * 8 + (c ^ (lane >> 3))] = sel4(64 * s <= last, xv[at][i][e]);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
       for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+        for (int i = 0; i < MT; ++i) {
+          const uint4 xo = own[w][i * 128 + j * 8 + ((2 * g + e) ^ (j & 7))];
 #pragma unroll
-          for (int t = 0; t < TC; ++t) acc[i][t] = mfma32(av[t][e], xv[i][e], acc[i][t]);
+          for (int t = 0; t < TC; ++t) acc[i][t] = mfma32(av[at][t][e], xo, acc[i][t]);
+        }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    };
+    for (int s = s0; s < s1; s += NB) {
+#pragma unroll
+      for (int u = 0; u < NB; ++u)
+        if (s + u < s1) {
+          multiply(s + u, u);
+          load_a(s + u + NB, u);
+          load_x(s + u + NB, u);
+        }
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int t = 0; t < TC; ++t) *reinterpret_cast<v4f*>(&red[w][i * TC + t][4 * lane]) = acc[i][t];
+      for (int t = 0; t < TC; ++t) own[w][(i * TC + t) * 64 + lane] = __builtin_bit_cast(uint4, acc[i][t]);
     __syncthreads();
-    // lane: row j of a tile, ranks 4 g .. 4 g + 3
-    for (int p = w; p < MT * TC; p += 4) {
-      v4f v = *reinterpret_cast<v4f*>(&red[0][p][4 * lane]);
+    // lane: place j of a tile, ranks 4 g .. 4 g + 3
+    const float sc = as_f32(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(as_u32(scale)), first)));
+    for (int p = w; p < MT * TC; p += NW) {
+      v4f v = __builtin_bit_cast(v4f, own[0][p * 64 + lane]);
 #pragma unroll
-      for (int q = 1; q < 4; ++q) v += *reinterpret_cast<v4f*>(&red[q][p][4 * lane]);
+      for (int q = 1; q < NW; ++q) v += __builtin_bit_cast(v4f, own[q][p * 64 + lane]);
+      v *= sc;
       const int i = p / TC, t = t0 + p % TC;
-      if (t < T && (same >> (16 * i + j) & 1)) {
-        const int64_t m = m0 + 16 * i + j;
-        *reinterpret_cast<v4f*>(a.h + (blockIdx.z * a.M + m) * (a.P * a.R) + (t / per) * a.R + 16 * (t % per) + 4 * g) = v;
-      }
+      if (t < T && (same >> (16 * i + j) & 1))
+        *reinterpret_cast<v4f*>(a.h + (blockIdx.z * a.M + m0 + 16 * i + j) * (a.P * a.R) + (t / per) * a.R + 16 * (t % per) + 4 * g) = v;
     }
     __syncthreads();
-  }
+  } while (next());
 }
 
-KRQ_DEV float lo_of(float v, float hi) { return finite_f32(hi) ? v - hi : 0.0f; }
-
-// fp32 as the sum of two bf16: hi rounded, lo the rest rounded (none beside an infinity or a NaN)
-KRQ_DEV void split_bf16(const float* v, int n, uint32_t* hi, uint32_t* lo) {
+// fp32 as the sum of NT bf16: each the rounded rest of those before it (none beside an infinity or a NaN)
+template <int NT>
+KRQ_DEV void split_bf16(float x, float y, uint32_t (&o)[NT]) {
 #pragma unroll
-  for (int i = 0; i < n / 2; ++i) {
-    hi[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
-    lo[i] = pack_bf16x2(lo_of(v[2 * i], as_f32(hi[i] << 16)), lo_of(v[2 * i + 1], as_f32(hi[i] & 0xffff0000u)));
+  for (int i = 0; i < NT; ++i) {
+    o[i] = pack_bf16x2(x, y);
+    const float hx = as_f32(o[i] << 16), hy = as_f32(o[i] & 0xffff0000u);
+    x = finite_f32(hx) ? x - hx : 0.0f;
+    y = finite_f32(hy) ? y - hy : 0.0f;
   }
 }
 
-// Sixteen values of a row at `at`, of which `n` lie in the part (n >= 16: all).
+// A lane's piece of a row: 16 bytes, VEC values, on any address that holds one (rows of an odd number of columns).
+typedef unsigned int v4u_on2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned int v4u_on4 __attribute__((ext_vector_type(4), aligned(4)));
 template <typename T>
-KRQ_DEV void load16(const T* at, int n, bool wide, float* v) {
-  if (wide) {
-    if constexpr (sizeof(T) == 2) {
+struct Piece {
+  static constexpr int VEC = 16 / sizeof(T);
+  v4u u;
+  KRQ_DEV void load(const uint16_t* at) { u = *reinterpret_cast<const v4u_on2*>(at); }
+  KRQ_DEV void load(const float* at) { u = *reinterpret_cast<const v4u_on4*>(at); }
+  KRQ_DEV void store(uint16_t* at) const { *reinterpret_cast<v4u_on2*>(at) = u; }
+  KRQ_DEV void store(float* at) const { *reinterpret_cast<v4u_on4*>(at) = u; }
+  KRQ_DEV void load(const T* at, int n) {  // the first n values
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const uint4 u = ld16(reinterpret_cast<const uint8_t*>(at) + 16 * q);
-        const uint32_t e[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[8 * q + 2 * i] = as_f32(e[i] << 16), v[8 * q + 2 * i + 1] = as_f32(e[i] & 0xffff0000u);
-      }
-    } else {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float4 u = reinterpret_cast<const float4*>(at)[q];
-        v[4 * q] = u.x, v[4 * q + 1] = u.y, v[4 * q + 2] = u.z, v[4 * q + 3] = u.w;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if constexpr (sizeof(T) == 2) v[i] = i < n ? bf16_to_f32(at[i]) : 0.0f;
-      else v[i] = i < n ? at[i] : 0.0f;
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 2)
+        u[i] = (2 * i < n ? at[2 * i] : 0u) | (2 * i + 1 < n ? static_cast<uint32_t>(at[2 * i + 1]) << 16 : 0u);
+      else
+        u[i] = i < n ? as_u32(at[i]) : 0u;
     }
   }
-}
-
-template <typename T>
-KRQ_DEV void store16(T* at, int n, bool wide, const float* v) {
-  if (wide) {
-    if constexpr (sizeof(T) == 2) {
+  KRQ_DEV void store(T* at, int n) const {
 #pragma unroll
-      for (int q = 0; q < 2; ++q)
-        *reinterpret_cast<uint4*>(at + 8 * q) =
-            make_uint4(pack_bf16x2(v[8 * q], v[8 * q + 1]), pack_bf16x2(v[8 * q + 2], v[8 * q + 3]),
-                       pack_bf16x2(v[8 * q + 4], v[8 * q + 5]), pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
-    } else {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) reinterpret_cast<float4*>(at)[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
+    for (int i = 0; i < VEC; ++i)
       if (i < n) {
-        if constexpr (sizeof(T) == 2) at[i] = static_cast<uint16_t>(pack_bf16x2(v[i], v[i]));
-        else at[i] = v[i];
+        if constexpr (sizeof(T) == 2) at[i] = static_cast<uint16_t>(u[i >> 1] >> (16 * (i & 1)));
+        else at[i] = as_f32(u[i]);
       }
   }
-}
+  KRQ_DEV void add(const v4f* acc) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 2)
+        u[i] = pack_bf16x2(as_f32(u[i] << 16) + acc[i >> 1][2 * (i & 1)], as_f32(u[i] & 0xffff0000u) + acc[i >> 1][2 * (i & 1) + 1]);
+      else
+        u[i] = as_u32(as_f32(u[i]) + acc[0][i]);
+    }
+  }
+};
 
-// y + the delta. A wave takes 16 rows and NI blocks of 64 columns of one part; a lane finishes 16 consecutive columns
-// of one row: tile t of a block multiplies the columns 16 (i / 4) + 4 t + i % 4, i = 0 .. 15, so that the four
-// accumulators of a lane are neighbours. ROWS: the workgroup's waves take four row tiles, else four groups of columns.
+// y + the delta. A wave takes 16 places and NI blocks of 64 columns of one part; a lane finishes pieces of 16 bytes of
+// one row, the four lanes of a row 64 contiguous bytes at a time. Of bf16, tile t of a block multiplies the columns
+// 32 (t / 2) + 8 (i / 4) + 4 (t % 2) + i % 4, i = 0 .. 15, so that two accumulators make a piece; of fp32 the columns 16 t + i.
+// ROWS: the workgroup's waves take four tiles of places, else four groups of columns.
 template <typename T, int NI, bool ROWS>
-__global__ __launch_bounds__(256) void k_lora_up(LoraArgs a) {
-  extern __shared__ uint4 stage[];  // h as operands: [wave][R / 32 or less][hi, lo][lane]
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, j = lane & 15;
-  const int ways = a.slot_ways;
+__global__ __launch_bounds__(256, 4) void k_lora_up(LoraArgs a) {
+  constexpr int SP = ROWS ? kSplitMany : kSplitFew;
+  constexpr int NT = sizeof(T) == 2 ? 2 : 3;  // bf16 terms of h: to 2^-16 or 2^-24
+  constexpr int VEC = Piece<T>::VEC, NP = 16 / VEC, TP = 4 / NP;  // pieces of a block, accumulators of a piece
+  extern __shared__ uint4 stage[];  // h as operands: [wave][steps of 32 ranks][NT][lane]
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, j = lane & 15;
   const int units = a.block[a.P], wide_units = ROWS ? units : (units + 3) >> 2;  // (the columns of a row tile first)
   const int64_t at = blockIdx.x / wide_units;
-  const int64_t m0 = ROWS ? (at * 4 + w) * 16 : at / ways * 16;
-  const int way = ROWS ? 0 : static_cast<int>(at % ways);
+  const int64_t m0 = ROWS ? (at * 4 + w) * 16 : at / a.ways * 16;
+  const int way = ROWS ? 0 : static_cast<int>(at % a.ways);
   const int unit = ROWS ? blockIdx.x % wide_units : blockIdx.x % wide_units * 4 + w;
   if (m0 >= a.M || unit >= units) return;
   int p = 0;
   while (unit >= a.block[p + 1]) ++p;
   const int n0 = a.part[p] + (unit - a.block[p]) * 64 * NI, n1 = a.part[p + 1];
-  const int64_t m = m0 + j;
-  const int id = load_id(a, min(m, a.M - 1));
-  uint64_t left = __ballot(m < a.M) & 0xffff;
-  uint4* st = stage + w * ((a.R + 31) / 32) * 128;
-  const T* yr = static_cast<const T*>(a.y) + min(m, a.M - 1) * a.ldy;
-  T* orow = static_cast<T*>(a.out) + min(m, a.M - 1) * a.ldo;
-  constexpr int kVec = 16 / sizeof(T);
-  const bool even = a.ldy % kVec == 0 && a.ldo % kVec == 0 && n0 % kVec == 0 &&
-                    (reinterpret_cast<uintptr_t>(a.y) | reinterpret_cast<uintptr_t>(a.out)) % 16 == 0;
+  const int64_t pc = min(m0 + j, a.M - 1);  // the lane's place
+  const float* hr = a.h + pc * (a.P * a.R) + p * a.R;
+  const int64_t slice = a.M * (a.P * a.R);
+  // a step of 32 ranks of h, 8 g .. 8 g + 7 of them in this lane; the first waits for nothing
+  auto load_h = [&](int s, v4f (&f)[SP][2]) {
+    const int r = min(32 * s + 8 * g, a.R - 8);
+#pragma unroll
+    for (int q = 0; q < SP; ++q)
+      if (q < a.split)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) f[q][e] = *reinterpret_cast<const v4f*>(hr + q * slice + r + 4 * e);
+  };
+  v4f f[SP][2];
+  load_h(0, f);
+  const int4 place = a.place[pc];
+  const int id = place.y;
+  uint64_t left = __ballot(m0 + j < a.M) & 0xffff;
+  uint4* st = stage + w * ((a.R + 31) / 32) * NT * 64 + lane;
+  const T* yr = static_cast<const T*>(a.y) + (int64_t)place.x * a.ldy;
+  T* orow = static_cast<T*>(a.out) + (int64_t)place.x * a.ldo;
+  bool fresh = true;  // f holds the first step
   for (int turn = 0; left; ++turn) {
     uint64_t same;
-    const int cur = next_id(id, left, same);
-    if (ways > 1 && turn % ways != way) continue;
+    const int first = __builtin_ctzll(left), cur = next_id(id, left, same);
+    if (!ROWS && turn % a.ways != way) continue;
     const bool me = same >> j & 1;
-    const int rank = rank_of(a, cur), r16 = (rank + 15) & ~15, full = r16 >> 5;
-    const bool tail = r16 & 16;
+    const int rank = __builtin_amdgcn_readlane(place.z, first), r16 = (rank + 15) & ~15;
     if (r16 == 0 && cur < a.slots && a.out == a.y) continue;
-    // this row's h, summed over the parts of K in order, times the adapter's scale
-    if (r16) {
-      const float scale = a.scales[cur];
-      const int64_t slice = a.M * (a.P * a.R);
-      const float* hr = a.h + m * (a.P * a.R) + p * a.R;
-      for (int s = 0; s < full; ++s) {
-        float v[8] = {};
-        if (me) {
-          for (int q = 0; q < a.split; ++q) {
-            const float4* f = reinterpret_cast<const float4*>(hr + q * slice + 32 * s + 8 * g);
-            const float4 f0 = f[0], f1 = f[1];
-            v[0] += f0.x; v[1] += f0.y; v[2] += f0.z; v[3] += f0.w;
-            v[4] += f1.x; v[5] += f1.y; v[6] += f1.z; v[7] += f1.w;
-          }
+    // whole blocks of the wave, all their y in flight before anything else; a last block that the part ends in by itself
+    const int whole = min(NI, (n1 - n0) >> 6);
+    Piece<T> v[NI][NP];
+    if (me) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = 32 * s + 8 * g + i < rank ? v[i] * scale : 0.0f;
+      for (int blk = 0; blk < NI; ++blk)
+        if (blk < whole)
+#pragma unroll
+          for (int q = 0; q < NP; ++q) v[blk][q].load(yr + n0 + VEC * g + 64 * blk + 4 * VEC * q);
+    }
+    // this place's h, summed over the parts of K in order, in NT terms
+    for (int s = 0; 32 * s < r16; ++s) {
+      if (!(fresh && s == 0)) load_h(s, f);
+      v4f v2[2] = {f[0][0], f[0][1]};
+#pragma unroll
+      for (int q = 1; q < SP; ++q)
+        if (q < a.split) v2[0] += f[q][0], v2[1] += f[q][1];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v2[i >> 2][i & 3] = me && 32 * s + 8 * g + i < rank ? v2[i >> 2][i & 3] : 0.0f;
+      uint32_t o[4][NT];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) split_bf16<NT>(v2[i >> 1][2 * (i & 1)], v2[i >> 1][2 * (i & 1) + 1], o[i]);
+#pragma unroll
+      for (int e = 0; e < NT; ++e) st[(s * NT + e) * 64] = make_uint4(o[0][e], o[1][e], o[2][e], o[3][e]);
+      fresh = false;
+    }
+    const uint16_t* bs = a.b + (int64_t)(r16 ? cur : 0) * a.N * a.R;
+    // the products of a block's 64 columns from column nb, of which the part has `most` + 1
+    const int col = sizeof(T) == 2 ? 8 * (j >> 2) + (j & 3) : j;  // this lane's column of tile 0; of tile t:
+    auto of_tile = [](int t) { return sizeof(T) == 2 ? 32 * (t >> 1) + 4 * (t & 1) : 16 * t; };
+    auto product = [&](int nb, bool edge, int most, v4f* acc) {
+      const uint8_t* base = reinterpret_cast<const uint8_t*>(bs + (int64_t)nb * r16);
+      auto from = [&](int t, uint32_t r) {  // rank r of the lane's column of tile t
+        return edge ? base + 2u * (min(col + of_tile(t), most) * r16 + r) : base + 2 * of_tile(t) * r16 + 2u * (col * r16 + r);
+      };
+#pragma unroll
+      for (int t = 0; t < 4; ++t) acc[t] = v4f{};
+      for (int s = 0; 32 * s < r16; ++s) {
+        const bool in = 32 * s + 8 * g < r16;  // (an odd 16 ranks: the upper lanes have none)
+        uint4 bv[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) bv[t] = ld16(from(t, in ? 32 * s + 8 * g : 0));
+#pragma unroll
+        for (int t = 0; t < 4; ++t) bv[t] = sel4(in, bv[t]);
+#pragma unroll
+        for (int e = 0; e < NT; ++e) {
+          const uint4 h = st[(s * NT + e) * 64];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) acc[t] = mfma32(bv[t], h, acc[t]);
         }
-        uint32_t hi[4], lo[4];
-        split_bf16(v, 8, hi, lo);
-        st[s * 128 + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        st[s * 128 + 64 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
-      if (tail) {
-        float v[4] = {};
-        if (me) {
-          for (int q = 0; q < a.split; ++q) {
-            const float4 f = *reinterpret_cast<const float4*>(hr + q * slice + 32 * full + 4 * g);
-            v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
-          }
+    };
+    auto finish = [&](Piece<T>& u, const v4f* acc) {
+      if (r16) u.add(acc);
+      if (cur >= a.slots) {
+        constexpr uint32_t nan = sizeof(T) == 2 ? 0x7fc07fc0u : 0x7fc00000u;
+        u.u = v4u{nan, nan, nan, nan};
+      }
+    };
+    v4f acc[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = 32 * full + 4 * g + i < rank ? v[i] * scale : 0.0f;
+    for (int blk = 0; blk < NI; ++blk) {
+      if (blk < whole) {
+        if (r16) product(n0 + 64 * blk, false, 63, acc);
+#pragma unroll
+        for (int q = 0; q < NP; ++q) {
+          finish(v[blk][q], acc + TP * q);
+          if (me) v[blk][q].store(orow + n0 + VEC * g + 64 * blk + 4 * VEC * q);
         }
-        uint32_t hi[2], lo[2];
-        split_bf16(v, 4, hi, lo);
-        st[full * 128 + lane] = make_uint4(hi[0], hi[1], lo[0], lo[1]);
       }
     }
-    const uint16_t* bs = r16 ? a.b + (int64_t)cur * a.N * a.R : a.b;
-#pragma unroll 1
-    for (int blk = 0; blk < NI; ++blk) {
-      const int nb = n0 + 64 * blk;
-      if (nb >= n1) break;
-      const int nl = nb + 16 * g, have = n1 - nl;
-      const bool wide = even && have >= 16;
-      float v[16];
-      if (me) load16(yr + nl, have, wide, v);
-      if (r16) {
-        v4f acc[4] = {};
-        const uint16_t* br[4];
+    const int ne = n0 + 64 * whole;
+    if (whole < NI && ne < n1) {
+      if (r16) product(ne, true, n1 - 1 - ne, acc);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) br[t] = bs + (int64_t)min(nb + 16 * (j >> 2) + 4 * t + (j & 3), n1 - 1) * r16;
-        for (int s = 0; s < full; ++s) {
-          const uint4 hi = st[s * 128 + lane], lo = st[s * 128 + 64 + lane];
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const uint4 bv = ld16(reinterpret_cast<const uint8_t*>(br[t] + 32 * s + 8 * g));
-            acc[t] = mfma32(bv, hi, acc[t]);
-            acc[t] = mfma32(bv, lo, acc[t]);
-          }
-        }
-        if (tail) {
-          const uint4 hl = st[full * 128 + lane];
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const uint2 bv = *reinterpret_cast<const uint2*>(br[t] + 32 * full + 4 * g);
-            acc[t] = mfma16(bv, make_uint2(hl.x, hl.y), acc[t]);
-            acc[t] = mfma16(bv, make_uint2(hl.z, hl.w), acc[t]);
-          }
-        }
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[4 * t + i] += acc[t][i];
+      for (int q = 0; q < NP; ++q) {
+        const int n = ne + VEC * g + 4 * VEC * q;
+        Piece<T> u;
+        if (me) u.load(yr + n, n1 - n);
+        finish(u, acc + TP * q);
+        if (me) u.store(orow + n, n1 - n);
       }
-      if (cur >= a.slots) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = as_f32(0x7fc00000u);
-      }
-      if (me && have > 0) store16(orow + nl, have, wide, v);
     }
   }
 }
 
 struct LoraPlan {
-  int split, mt, ways;
+  int split, mt, tc, ways;
 };
 
-// Few rows: 16-row tiles, K in up to eight parts, the adapters of a tile each in a workgroup of its own (every row may
-// name another one). Many: 64-row tiles, so that a factor is read once for 64 rows, K in as many parts as fill the chip.
+constexpr int kDownWaves = 8;
+
+// Few rows: 16-row tiles; many: 32-row tiles and all ranks of a projection up to 64 together, so that factors and rows are read once. The adapters that a tile meets go to `ways` workgroups, the
+// first of each in parallel. K in as many parts as it takes to fill the chip with two steps of 64 k a wave.
 LoraPlan lora_plan(int64_t M, int64_t K, int P, int R) {
   LoraPlan p;
-  p.mt = M <= 256 ? 1 : 4;
-  const int64_t tiles = (M + 16 * p.mt - 1) / (16 * p.mt);
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kMaxSplit, K / 512));
-  if (p.mt == 1) {
-    p.ways = M <= 64 ? 16 : 4;
-    p.split = static_cast<int>(most);
-  } else {
-    p.ways = 1;
-    p.split = static_cast<int>(std::max<int64_t>(1, std::min(most, 512 / tiles)));
-  }
+  const int T = P * R / 16;
+  p.mt = M <= 256 ? 1 : 2;
+  p.ways = M <= 16 ? static_cast<int>(M) : M <= 256 ? 4 : 2;
+  p.tc = p.mt == 1 ? 1 : (T + (T + 3) / 4 - 1) / ((T + 3) / 4);
+  const int64_t groups = (M + 16 * p.mt - 1) / (16 * p.mt) * ((T + p.tc - 1) / p.tc) * (M <= 16 ? M : 1);
+  const int64_t most = std::max<int64_t>(1, K / (64 * 2 * kDownWaves));
+  p.split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({most, p.mt == 1 ? kSplitFew : kSplitMany, (512 + groups - 1) / groups})));
   return p;
+}
+
+template <int MT, int TC, bool SORT>
+void launch_down(const LoraArgs& a, hipStream_t s) {
+  const int64_t tiles = (a.M + 16 * MT - 1) / (16 * MT);
+  const int T = a.P * a.R / 16;
+  hipLaunchKernelGGL((k_lora_down<MT, TC, kDownWaves, MT == 1 ? 3 : 2, SORT>), dim3((unsigned)(tiles * a.ways), (T + TC - 1) / TC, a.split),
+                     dim3(64 * kDownWaves), 0, s, a);
 }
 
 template <typename T, int NI, bool ROWS>
@@ -345,30 +472,39 @@ void launch_up(const LoraArgs& a, hipStream_t s) {
   LoraArgs u = a;
   u.block[0] = 0;
   for (int p = 0; p < a.P; ++p) u.block[p + 1] = u.block[p] + (a.part[p + 1] - a.part[p] + 64 * NI - 1) / (64 * NI);
-  const int64_t units = u.block[a.P];
-  const int64_t tiles = (a.M + 15) / 16;
-  const dim3 grid(static_cast<unsigned>(ROWS ? units * ((tiles + 3) / 4) : (units + 3) / 4 * tiles * a.slot_ways));
-  const size_t smem = static_cast<size_t>(4) * ((a.R + 31) / 32) * 128 * 16;
+  const int64_t units = u.block[a.P], tiles = (a.M + 15) / 16;
+  const dim3 grid(static_cast<unsigned>(ROWS ? units * ((tiles + 3) / 4) : (units + 3) / 4 * tiles * a.ways));
+  const size_t smem = static_cast<size_t>(4) * ((a.R + 31) / 32) * (sizeof(T) == 2 ? 2 : 3) * 64 * 16;
   hipLaunchKernelGGL((k_lora_up<T, NI, ROWS>), grid, dim3(256), smem, s, u);
 }
+
+template <typename T>
+void launch_up_any(const LoraArgs& a, hipStream_t s) {
+  if (a.M <= 256) launch_up<T, 1, false>(a, s);
+  else launch_up<T, sizeof(T) == 2 ? 4 : 2, true>(a, s);
+}
+
+// places, then h
+int64_t place_bytes(int64_t M) { return (M * (int64_t)sizeof(int4) + 255) / 256 * 256; }
 
 }  // namespace
 
 extern "C" int64_t krq_lora_ws_bytes(int64_t M, int64_t K, int parts, int rank) {
   if (M < 1 || K < 16 || parts < 1 || parts > kMaxParts || rank < 16 || rank > kMaxRank) return -1;
-  return lora_plan(M, K, parts, rank).split * M * parts * rank * (int64_t)sizeof(float);
+  return place_bytes(M) + lora_plan(M, K, parts, rank).split * M * parts * rank * (int64_t)sizeof(float);
 }
 
 extern "C" int krq_lora_add(const void* x, int64_t ldx, const void* ids, int ids_64, const void* a, const void* b, const int32_t* ranks,
                             const float* scales, int64_t slots, int64_t M, int64_t K, const int64_t* parts_n, int parts, int rank,
                             const void* y, int64_t ldy, void* out, int64_t ldo, int fp32, void* ws, int64_t ws_bytes, void* stream) {
   KRQ_REQUIRE(x && ids && a && b && ranks && scales && parts_n && y && out && ws, "lora_add: null pointer");
-  KRQ_REQUIRE(M >= 1 && M <= (1 << 24) && K >= 16 && K % 16 == 0 && K <= (1 << 24), "lora_add: bad shape M=%lld K=%lld (K a multiple of 16)",
+  KRQ_REQUIRE(M >= 1 && M <= (1 << 24) && K >= 16 && K % 16 == 0 && K < (1 << 22), "lora_add: bad shape M=%lld K=%lld (K a multiple of 16)",
               (long long)M, (long long)K);
   KRQ_REQUIRE(parts >= 1 && parts <= kMaxParts, "lora_add: %d parts (at most %d)", parts, kMaxParts);
   KRQ_REQUIRE(rank >= 16 && rank % 16 == 0 && rank <= kMaxRank, "lora_add: rank=%d (a multiple of 16, at most %d)", rank, kMaxRank);
-  KRQ_REQUIRE(slots >= 1 && slots < (1 << 24), "lora_add: %lld slots", (long long)slots);
-  KRQ_REQUIRE(ldx >= K && ldx % 8 == 0 && aligned16(x), "lora_add: rows of x must start on 16 bytes (ldx=%lld)", (long long)ldx);
+  KRQ_REQUIRE(slots >= 1 && slots < (1 << 23), "lora_add: %lld slots", (long long)slots);
+  KRQ_REQUIRE(ldx >= K && ldx % 8 == 0 && ldx < (1 << 22) && aligned16(x), "lora_add: rows of x must start on 16 bytes, less than 2^22 apart (ldx=%lld)",
+              (long long)ldx);
   KRQ_REQUIRE(aligned16(a) && aligned16(b) && aligned16(ws), "lora_add: the factors and ws must start on 16 bytes");
   LoraArgs l{};
   int64_t n = 0;
@@ -393,7 +529,8 @@ extern "C" int krq_lora_add(const void* x, int64_t ldx, const void* ids, int ids
   l.scales = scales;
   l.y = y;
   l.out = out;
-  l.h = (float*)ws;
+  l.place = (int4*)ws;
+  l.h = (float*)((uint8_t*)ws + place_bytes(M));
   l.M = M;
   l.K = K;
   l.ldx = ldx;
@@ -405,21 +542,16 @@ extern "C" int krq_lora_add(const void* x, int64_t ldx, const void* ids, int ids
   l.N = (int)n;
   l.split = plan.split;
   l.ids64 = ids_64 != 0;
-  l.slot_ways = plan.ways;
+  l.ways = plan.ways;
   hipStream_t s = (hipStream_t)stream;
-  const int T = parts * rank / 16;
-  const int64_t tiles = (M + 16 * plan.mt - 1) / (16 * plan.mt);
-  if (plan.mt == 1)
-    hipLaunchKernelGGL((k_lora_down<1, 1>), dim3((unsigned)(tiles * plan.ways), T, plan.split), dim3(256), 0, s, l);
-  else
-    hipLaunchKernelGGL((k_lora_down<4, 4>), dim3((unsigned)tiles, (T + 3) / 4, plan.split), dim3(256), 0, s, l);
+  if (M <= 16) launch_down<1, 1, false>(l, s);
+  else if (plan.mt == 1) launch_down<1, 1, true>(l, s);
+  else if (plan.tc == 1) launch_down<2, 1, true>(l, s);
+  else if (plan.tc == 2) launch_down<2, 2, true>(l, s);
+  else if (plan.tc == 3) launch_down<2, 3, true>(l, s);
+  else launch_down<2, 4, true>(l, s);
   if (const int rc = krq_check_launch("lora_add")) return rc;
-  if (plan.mt == 1) {
-    if (fp32) launch_up<float, 1, false>(l, s);
-    else launch_up<uint16_t, 1, false>(l, s);
-  } else {
-    if (fp32) launch_up<float, 4, true>(l, s);
-    else launch_up<uint16_t, 4, true>(l, s);
-  }
+  if (fp32) launch_up_any<float>(l, s);
+  else launch_up_any<uint16_t>(l, s);
   return krq_check_launch("lora_add");
 }

@@ -15,7 +15,7 @@ import torch
 from . import _lib as L
 from . import mxfp4 as _mx
 
-MAX_PARTS, MAX_RANK = 8, 256
+MAX_PARTS, MAX_RANK, MAX_ROW = 8, 256, 1 << 22
 
 
 class Adapters:
@@ -28,17 +28,19 @@ class Adapters:
     def __init__(self, K, n, rank, slots, device):
         self.parts = [int(n)] if isinstance(n, int) else [int(p) for p in n]
         self.K, self.N, self.slots = int(K), sum(self.parts), int(slots)
-        if self.K < 16 or self.K % 16:
-            raise ValueError(f"K={K} must be a positive multiple of 16")
+        if not 16 <= self.K < MAX_ROW or self.K % 16:
+            raise ValueError(f"K={K} must be a positive multiple of 16 under 2^22")
         if not 1 <= len(self.parts) <= MAX_PARTS or min(self.parts) < 1:
             raise ValueError(f"n={n}: 1 to {MAX_PARTS} parts of positive size")
         if not 1 <= rank <= MAX_RANK:
             raise ValueError(f"rank={rank} (1 to {MAX_RANK})")
-        if not 1 <= self.slots < 1 << 24:
+        if not 1 <= self.slots < 1 << 23:
             raise ValueError(f"slots={slots}")
         self.rank = (int(rank) + 15) // 16 * 16
-        # a slot's A: [parts, rank, K] with zeros past its own rank; its B: [N, its rank rounded up to 16], packed
-        self.a = torch.zeros((self.slots, len(self.parts), self.rank, self.K), device=device, dtype=torch.bfloat16)
+        # a slot's A: for each part, 16 ranks and 64 k the kernel's operands in lane order (lane 16 g + j: rank j, k = 16 g + 8 e
+        # .. + 7), zeros past its rank and past K; its B: [N, its rank rounded up to 16]
+        self.a = torch.zeros((self.slots, len(self.parts), self.rank // 16, -(-self.K // 64), 2, 4, 16, 8), device=device,
+                             dtype=torch.bfloat16)
         self.b = torch.zeros((self.slots, self.N * self.rank), device=device, dtype=torch.bfloat16)
         self.ranks = torch.zeros((self.slots,), device=device, dtype=torch.int32)
         self.scales = torch.zeros((self.slots,), device=device, dtype=torch.float32)
@@ -76,7 +78,10 @@ class Adapters:
         for i, (p, n) in enumerate(zip(pairs, self.parts)):
             if p is not None:
                 a, b = p
-                self.a[slot, i, :a.shape[0]].copy_(a)
+                tiles = a.new_zeros((r16, self.a.shape[3] * 64))
+                tiles[:a.shape[0], :self.K] = a
+                # [rank tile, j, step, g, e, 8] -> [rank tile, step, e, g, j, 8]
+                self.a[slot, i, :r16 // 16] = tiles.view(r16 // 16, 16, -1, 4, 2, 8).permute(0, 2, 4, 3, 1, 5)
                 packed[at:at + n, :a.shape[0]].copy_(b)
             at += n
         self.scales[slot] = float(scale)
@@ -113,7 +118,7 @@ def add(y, x, adapters, ids, out=None):
     ldy = _rows(y, "y", (torch.bfloat16, torch.float32), ad.N)
     if ids.dtype not in (torch.int32, torch.int64) or tuple(ids.shape) != (M,) or y.shape[0] != M:
         raise ValueError(f"ids {ids.dtype} {tuple(ids.shape)}, x {tuple(x.shape)} and y {tuple(y.shape)} do not match")
-    if ldx is None or ldx % 8 or x.data_ptr() % 16:
+    if ldx is None or ldx % 8 or ldx >= MAX_ROW or x.data_ptr() % 16:
         x, ldx = x.clone(memory_format=torch.contiguous_format), ad.K
     ids = ids.contiguous()
     if out is None:

@@ -112,7 +112,7 @@ def test_banks_that_cannot_be(args):
 
 def test_load_checks_its_pairs():
     ad = lora.Adapters(64, (48, 16), 20, 4, "cpu")
-    assert ad.rank == 32 and ad.a.shape == (4, 2, 32, 64) and ad.b.shape == (4, 64 * 32)
+    assert ad.rank == 32 and ad.a.shape == (4, 2, 2, 1, 2, 4, 16, 8) and ad.b.shape == (4, 64 * 32)
 
     def pair(r, n=48, K=64, rb=None):
         return torch.ones(r, K), torch.ones(n, rb or r)
@@ -140,7 +140,10 @@ def test_load_packs_a_slot():
     ad.load(1, [(torch.randn(40, 32), torch.randn(3, 40)), None], 1.0)
     ad.load(1, [(a0, b0), (a1, b1)], 0.5)
     assert ad.ranks.tolist() == [0, 17] and ad.scales.tolist() == [0.0, 0.5]
-    assert torch.equal(ad.a[1, 0, :17], a0) and torch.equal(ad.a[1, 1, :5], a1) and not ad.a[1, 0, 17:].any() and not ad.a[1, 1, 5:].any()
+    want = torch.zeros(2, 48, 64, dtype=BF)
+    want[0, :17, :32], want[1, :5, :32] = a0, a1
+    got = ad.a[1].permute(0, 1, 5, 2, 4, 3, 6).reshape(2, 48, 64)  # [part, rank tile, j | step, g, e, 8]
+    assert torch.equal(got, want)
     b = ad.b[1, :5 * 32].view(5, 32)
     assert torch.equal(b[:3, :17], b0) and torch.equal(b[3:, :5], b1) and not b[:3, 17:].any() and not b[3:, 5:].any()
     ad.clear(1)
@@ -158,7 +161,7 @@ def test_entry_point_refuses():
     odd, q = ctypes.c_void_p(4097), ctypes.c_void_p(8200)
     bad = [dict([(k, None)]) for k in ("x", "ids", "a", "b", "ranks", "scales", "y", "out", "ws")]
     bad += [dict(M=0), dict(M=1 << 25), dict(K=8), dict(K=72), dict(K=1 << 25), dict(parts=0), dict(n=(1,) * 9, parts=9), dict(n=(48, 0)),
-            dict(rank=0), dict(rank=8), dict(rank=272), dict(slots=0), dict(slots=1 << 24), dict(ldx=32), dict(ldx=68), dict(x=q), dict(a=q),
+            dict(rank=0), dict(rank=8), dict(rank=272), dict(slots=0), dict(slots=1 << 23), dict(ldx=32), dict(ldx=68), dict(x=q), dict(a=q),
             dict(b=q), dict(ws=q), dict(ldy=63), dict(ldo=63), dict(y=odd), dict(out=odd), dict(y=q, fp32=1, out=ctypes.c_void_p(4098)),
             dict(ldy=72), dict(nbytes=3 * 2 * 16 * 4 - 1)]
     for kw in bad:
