@@ -8,11 +8,11 @@
 // entry: lse and the merged n of every row, and the merge of the rows by v in fp64 (candidates of two beams can lie
 // closer than fp32 tells apart).
 //
-// The n largest of a chunk. A logit and its token make one 64-bit key, all of them different: the logit's bits in an
-// order that compares as unsigned (NaN over everything), then the token's complement. The n-th largest of the 64 lanes'
-// largest keys, found bit by bit with ballots, has n keys at or above it, and only n lanes of a wave reach it: the keys
-// that do (n to a few n) go to LDS, and each finds its place by counting the larger ones. Equal logits cost nothing
-// extra, whatever their number.
+// The n largest of a chunk. The n-th largest of the 64 lanes' largest values, found by its upper 16 bits with ballots, has n
+// values at or above it, and few more: those go to LDS, and each finds its place by counting the larger ones. Logit and
+// token make one 64-bit key for that, all of them different: the logit's bits in an order that compares as unsigned (NaN over
+// everything), then the token's complement. Where equal logits leave too many (a mask, a coarse type), the n-th largest
+// is taken of the lanes' largest keys instead, which only n lanes of a wave reach.
 //
 // Bound by the read of the logits from a few rows on; by the two launches' latencies below.
 #include <algorithm>
@@ -66,7 +66,7 @@ KRQ_DEV uint64_t nth_key(uint64_t key, int n) {
 }
 
 struct RowStat {
-  uint32_t top;  // ord_of the chunk's largest value
+  uint32_t top;  // ord_of the chunk's largest value, a NaN's where one is among them
   float sum;     // sum of exp(value - largest)
 };
 
@@ -77,99 +77,174 @@ typedef unsigned int v4u_on4 __attribute__((ext_vector_type(4), aligned(4)));
 KRQ_DEV v4u ld16_any(const uint16_t* p) { return *reinterpret_cast<const v4u_on2*>(p); }
 KRQ_DEV v4u ld16_any(const float* p) { return *reinterpret_cast<const v4u_on4*>(p); }
 
+// The largest threshold of 16 upper bits that n of the wave's values reach.
+KRQ_DEV uint32_t nth_upper(uint32_t ord, int n) {
+  uint32_t t = 0;
+#pragma unroll
+  for (int b = 31; b >= 16; --b) {
+    const uint32_t c = t | 1u << b;
+    if (__popcll(__ballot(ord >= c)) >= n) t = c;
+  }
+  return t;
+}
+
+// Sum over the lanes before this one, and over all.
+KRQ_DEV int wave_before(int v, int& all) {
+  const int lane = threadIdx.x & 63;
+  int s = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(s, d, 64);
+    if (lane >= d) s += o;
+  }
+  all = __builtin_amdgcn_readlane(s, 63);
+  return s - v;
+}
+
+constexpr int kFewKeys = 384;  // keys that are ranked as they come
+
 template <typename T, int NV>
 __global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const T* __restrict__ logits, int64_t ld, int64_t V, int n, int chunks,
                                                             RowStat* __restrict__ stat, uint64_t* __restrict__ cand) {
   constexpr int VEC = 16 / sizeof(T), P = NV * VEC, CH = P * kBeamThreads;
-  extern __shared__ uint64_t list[];  // [4 n P]
-  __shared__ uint32_t tops[4];
-  __shared__ float sums[4];
+  extern __shared__ uint64_t list[];  // [max(4 n P, kFewKeys)]
+  __shared__ float tops[4], sums[4];
+  __shared__ uint32_t least[4];
   __shared__ uint64_t nth[4];
-  __shared__ int count;
+  __shared__ int counts[4];
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, c = blockIdx.x;
   const int64_t row = blockIdx.y;
   const T* r = logits + row * ld;
   const int64_t base = (int64_t)c * CH;
-  uint32_t o[P];
-#pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const int64_t e = base + (v * kBeamThreads + tid) * VEC;
-    if (e + VEC <= V) {
-      const v4u a = ld16_any(r + e);
+  const int left = static_cast<int>(min(V - base, (int64_t)CH));  // tokens of the chunk
+  float f[P];  // (places past V hold -inf)
+  auto load = [&](int v, float* o) {
+    const int e = (v * kBeamThreads + tid) * VEC;
+    if (e + VEC <= left) {
+      const v4u a = ld16_any(r + base + e);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(T) == 2) {
-          o[v * VEC + 2 * i] = ord_of(as_f32(a[i] << 16));
-          o[v * VEC + 2 * i + 1] = ord_of(as_f32(a[i] & 0xffff0000u));
-        } else {
-          o[v * VEC + i] = ord_of(as_f32(a[i]));
-        }
+        if constexpr (sizeof(T) == 2) o[2 * i] = as_f32(a[i] << 16), o[2 * i + 1] = as_f32(a[i] & 0xffff0000u);
+        else o[i] = as_f32(a[i]);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        o[v * VEC + i] = 0;
-        if (e + i < V) {
-          if constexpr (sizeof(T) == 2) o[v * VEC + i] = ord_of(bf16_to_f32(r[e + i]));
-          else o[v * VEC + i] = ord_of(r[e + i]);
+        o[i] = -__builtin_inff();
+        if (e + i < left) {
+          if constexpr (sizeof(T) == 2) o[i] = bf16_to_f32(r[base + e + i]);
+          else o[i] = r[base + e + i];
         }
       }
     }
-  }
-  auto token = [&](int i) { return static_cast<uint32_t>(base + ((i / VEC) * kBeamThreads + tid) * VEC + i % VEC); };
-  uint64_t best = 0;  // (elements come in the order of their tokens: the first of the largest is the lowest)
-  uint32_t top = 0;
-  int at = 0;
+  };
 #pragma unroll
-  for (int i = 0; i < P; ++i)
-    if (o[i] > top) top = o[i], at = i;
-  if (top) best = static_cast<uint64_t>(top) << 32 | static_cast<uint32_t>(~token(at));
-  const uint64_t t = nth_key(best, n);
-  const uint32_t wt = wave_max_u32_dpp(top);
-  if (lane == 0) tops[w] = wt, nth[w] = t;
-  if (tid == 0) count = 0;
+  for (int v = 0; v < NV; ++v) load(v, f + v * VEC);
+  auto key_of = [&](int v, int i, float value) {  // of place i of the thread's vector v; 0 past V
+    const int e = (v * kBeamThreads + tid) * VEC + i;
+    return e < left ? static_cast<uint64_t>(ord_of(value)) << 32 | static_cast<uint32_t>(~static_cast<uint32_t>(base + e)) : 0;
+  };
+  float top = f[0];
+#pragma unroll
+  for (int i = 1; i < P; ++i) top = fmaxf(top, f[i]);  // (a NaN shows in the sum)
+  const uint32_t ord = ord_of(top == top ? top : -__builtin_inff());
+  const uint32_t wt = wave_max_u32_dpp(ord), t16 = nth_upper(ord, n);
+  if (lane == 0) tops[w] = of_ord(wt), least[w] = t16;
   __syncthreads();
-  uint32_t m = tops[0];
-  uint64_t least = nth[0];
-#pragma unroll
-  for (int i = 1; i < 4; ++i) m = umax32(m, tops[i]), least = nth[i] > least ? nth[i] : least;
+  const float m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  const uint32_t t = umax32(umax32(least[0], least[1]), umax32(least[2], least[3]));
+  const float tf = t > kOrdNegInf ? of_ord(t) : -__builtin_inff();  // (below that are NaN's bits)
   float s = 0.0f;
-  if (m > kOrdNegInf && m < kOrdInf) {
-    const float mx = of_ord(m);
-#pragma unroll
-    for (int i = 0; i < P; ++i) s += o[i] ? __expf(of_ord(o[i]) - mx) : 0.0f;
-  }
-  s = wave_sum(s);
-  if (lane == 0) sums[w] = s;
-  const uint32_t lh = hi32(least);
+  const float off = m > -__builtin_inff() ? m : 0.0f;
+  int mine = 0;
 #pragma unroll
   for (int i = 0; i < P; ++i) {
-    if (o[i] >= lh && o[i]) {
-      const uint64_t key = static_cast<uint64_t>(o[i]) << 32 | static_cast<uint32_t>(~token(i));
-      if (key >= least) list[atomicAdd(&count, 1)] = key;  // (at most n lanes of a wave, P keys each)
+    s += __builtin_amdgcn_exp2f((f[i] - off) * 1.44269504f);
+    mine += f[i] >= tf;
+  }
+  s = wave_sum(s);
+  int all;
+  int at = wave_before(mine, all);
+  if (lane == 0) sums[w] = s, counts[w] = all;
+  __syncthreads();
+  int have = counts[0] + counts[1] + counts[2] + counts[3];
+  if (have <= kFewKeys) {
+    for (int q = 0; q < w; ++q) at += counts[q];
+    if (mine) {
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+        if (f[i] >= tf) list[at++] = key_of(i / VEC, i % VEC, f[i]);
+    }
+  } else {  // by keys, the logits read again (a launch of equal logits: few registers for it)
+    float o[VEC];
+    uint64_t best = 0;
+#pragma unroll 1
+    for (int v = 0; v < NV; ++v) {
+      load(v, o);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const uint64_t k = key_of(v, i, o[i]);
+        best = k > best ? k : best;
+      }
+    }
+    const uint64_t exact = nth_key(best, n);
+    if (lane == 0) nth[w] = exact;
+    __syncthreads();
+    uint64_t lk = nth[0];
+#pragma unroll
+    for (int q = 1; q < 4; ++q) lk = nth[q] > lk ? nth[q] : lk;
+    mine = 0;
+#pragma unroll 1
+    for (int v = 0; v < NV; ++v) {
+      load(v, o);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const uint64_t k = key_of(v, i, o[i]);
+        mine += k >= lk && k;
+      }
+    }
+    at = wave_before(mine, all);
+    if (lane == 0) counts[w] = all;
+    __syncthreads();
+    have = counts[0] + counts[1] + counts[2] + counts[3];
+    for (int q = 0; q < w; ++q) at += counts[q];
+#pragma unroll 1
+    for (int v = 0; v < NV; ++v) {
+      load(v, o);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const uint64_t k = key_of(v, i, o[i]);
+        if (k >= lk && k) list[at++] = k;  // (at most n lanes of a wave, P keys each)
+      }
     }
   }
   __syncthreads();
-  const int have = count;
   uint64_t* out = cand + (row * chunks + c) * n;
   for (int i = tid; i < have; i += kBeamThreads) {
     const uint64_t key = list[i];
     int rank = 0;
-    for (int j = 0; j < have; ++j) rank += list[j] > key;
+    for (int j = 0; j < have; ++j) rank += list[j] > key || (list[j] == key && j < i);  // (equal: places past V)
     if (rank < n) out[rank] = key;
   }
   for (int i = have + tid; i < n; i += kBeamThreads) out[i] = 0;  // (the chunk has fewer)
-  if (tid == 0) stat[row * chunks + c] = RowStat{m, (sums[0] + sums[1]) + (sums[2] + sums[3])};
+  // a chunk without a finite logit has sum 0, one with a NaN a sum of NaN and with +inf a largest of it
+  if (tid == 0) {
+    const float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    stat[row * chunks + c] = RowStat{sum != sum ? 0xffffffffu : ord_of(m), m > -__builtin_inff() ? sum : 0.0f};
+  }
 }
 
-// One batch entry. A wave merges a row at a time; then every row's sorted candidates meet in LDS, where each finds its
-// place by a binary search in the other rows.
+// One batch entry. A wave merges a row at a time, its keys in registers where they are up to KR a lane; then every row's
+// sorted candidates meet in LDS, where each finds its place: by counting where they are few, else by a binary search in
+// the other rows.
+constexpr int kCounted = 512;
+template <int KR>
 __global__ __launch_bounds__(kPickThreads) void k_beam_pick(const RowStat* __restrict__ stat, const uint64_t* __restrict__ cand,
                                                             const float* __restrict__ scores, int64_t V, int W, int n, int chunks,
                                                             int lists, float* __restrict__ out_scores,
                                                             int64_t* __restrict__ out_beams, int64_t* __restrict__ out_tokens) {
   extern __shared__ uint64_t mem[];  // values [W][n], tokens [W][n] (32 bits), a list for each of `lists` waves [n * per]
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int tid = threadIdx.x, threads = blockDim.x, wave = tid >> 6, lane = tid & 63;
   const int64_t b = blockIdx.x;
   const int total = chunks * n, per = (total + 63) >> 6, len = static_cast<int>(min((int64_t)n, V));
   uint64_t* vals = mem;
@@ -178,9 +253,24 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(const RowStat* __res
   for (int w = wave; wave < lists && w < W; w += lists) {
     const int64_t row = b * W + w;
     const RowStat* st = stat + row * chunks;
+    const uint64_t* rc = cand + row * total;
+    uint64_t k[KR > 0 ? KR : 1];
+    if constexpr (KR > 0) {
+#pragma unroll
+      for (int i = 0; i < KR; ++i) k[i] = lane + 64 * i < total ? rc[lane + 64 * i] : 0;
+    }
+    auto each = [&](auto visit) {  // every key of the row, all lanes together; 0: none
+      if constexpr (KR > 0) {
+#pragma unroll
+        for (int i = 0; i < KR; ++i) visit(k[i]);
+      } else {
+        for (int i = 0; i < total; i += 64) visit(i + lane < total ? rc[i + lane] : 0);
+      }
+    };
     const float score = scores[row];
-    uint32_t top = 0;
-    for (int c = lane; c < chunks; c += 64) top = umax32(top, st[c].top);
+    const RowStat q = lane < chunks ? st[lane] : RowStat{0, 0.0f};
+    uint32_t top = q.top;
+    for (int c = lane + 64; c < chunks; c += 64) top = umax32(top, st[c].top);
     top = wave_max_u32_dpp(top);
     // the kind of the row: v of all its candidates, where that is one value
     const bool bad = top >= kOrdInf || !(score < __builtin_inff());
@@ -190,30 +280,30 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(const RowStat* __res
       continue;
     }
     const float mx = of_ord(top);
-    double s = 0.0;
-    for (int c = lane; c < chunks; c += 64) {
-      const RowStat q = st[c];
-      if (q.top > kOrdNegInf) s += q.sum * exp((double)of_ord(q.top) - (double)mx);
-    }
+    auto part = [&](RowStat r) { return r.top > kOrdNegInf ? r.sum * exp((double)of_ord(r.top) - (double)mx) : 0.0; };
+    double s = part(q);
+    for (int c = lane + 64; c < chunks; c += 64) s += part(st[c]);
 #pragma unroll
     for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
     const double lse = (double)mx + log(s);
-    const uint64_t* rc = cand + row * total;
     uint64_t best = 0;
-    for (int i = lane; i < total; i += 64) best = rc[i] > best ? rc[i] : best;
-    const uint64_t least = nth_key(best, n);
+    each([&](uint64_t key) { best = key > best ? key : best; });
+    uint64_t least = static_cast<uint64_t>(nth_upper(hi32(best), n)) << 32;
     int have = 0;
-    for (int i0 = 0; i0 < total; i0 += 64) {
-      const uint64_t key = i0 + lane < total ? rc[i0 + lane] : 0;
+    each([&](uint64_t key) { have += __popcll(__ballot(key && key >= least)); });
+    if (have > min(n * per, kFewKeys)) least = nth_key(best, n);  // (reached by n lanes' keys, n * per)
+    have = 0;
+    each([&](uint64_t key) {
       const bool in = key && key >= least;
       const uint64_t mask = __ballot(in);
       if (in) list[have + __popcll(mask & ((1ull << lane) - 1))] = key;
       have += __popcll(mask);
-    }
+    });
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     for (int i = lane; i < have; i += 64) {
       const uint64_t key = list[i];
       int rank = 0;
+#pragma unroll 4
       for (int j = 0; j < have; ++j) rank += list[j] > key;
       if (rank < len) {
         vals[w * n + rank] = ord_of_f64((double)score + ((double)of_ord(hi32(key)) - lse));
@@ -223,20 +313,32 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(const RowStat* __res
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
   __syncthreads();
-  for (int i = tid; i < W * len; i += kPickThreads) {
+  for (int i = tid; i < W * len; i += threads) {
     const int w = i / len, p = i % len;
     const uint64_t v = vals[w * n + p];
     int rank = p;
-    for (int q = 0; q < W && rank < n; ++q) {
-      if (q == w) continue;
-      int lo = 0, hi = len;  // how many of row q come before: larger, or equal in a lower beam
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        const uint64_t u = vals[q * n + mid];
-        if (u > v || (u == v && q < w)) lo = mid + 1;
-        else hi = mid;
+    if (W * len <= kCounted) {
+      for (int q = 0; q < W; ++q) {
+        if (q == w) continue;
+        const uint64_t edge = q < w ? v : v + (v != ~0ull);  // of lower beams the equal ones come before too
+        int before = 0;
+#pragma unroll 4
+        for (int j = 0; j < len; ++j) before += vals[q * n + j] >= edge;
+        if (q > w && v == ~0ull) before = 0;
+        rank += before;
       }
-      rank += lo;
+    } else {
+      for (int q = 0; q < W && rank < n; ++q) {
+        if (q == w) continue;
+        int lo = 0, hi = len;
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          const uint64_t u = vals[q * n + mid];
+          if (u > v || (u == v && q < w)) lo = mid + 1;
+          else hi = mid;
+        }
+        rank += lo;
+      }
     }
     if (rank < n) {
       const int64_t at = b * n + rank;
@@ -365,7 +467,7 @@ extern "C" int krq_beam_select(const void* logits, int fp32, int64_t ld, const f
   uint64_t* cand = (uint64_t*)((uint8_t*)ws + p.stat_bytes);
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid(p.chunks, static_cast<unsigned>(B * W));
-  const size_t list = sizeof(uint64_t) * 4 * n * (p.nv * 16 / esize);
+  const size_t list = sizeof(uint64_t) * std::max<int64_t>(4 * n * (p.nv * 16 / esize), kFewKeys);
 #define KRQ_ROWS(T, NV)                                                                                                       \
   hipLaunchKernelGGL((k_beam_rows<T, NV>), grid, dim3(kBeamThreads), list, s, (const T*)logits, ld, V, (int)n, p.chunks, stat, cand)
   if (fp32) {
@@ -377,8 +479,15 @@ extern "C" int krq_beam_select(const void* logits, int fp32, int64_t ld, const f
   }
 #undef KRQ_ROWS
   if (const int rc = krq_check_launch("beam_select")) return rc;
-  hipLaunchKernelGGL(k_beam_pick, dim3(static_cast<unsigned>(B)), dim3(kPickThreads), lds, s, stat, cand, scores, V, (int)W, (int)n,
-                     p.chunks, lists, out_scores, out_beams, out_tokens);
+  const int waves = static_cast<int>(std::max<int64_t>(4, std::min<int64_t>(W, kPickWaves)));
+#define KRQ_PICK(KR)                                                                                                          \
+  hipLaunchKernelGGL(k_beam_pick<KR>, dim3(static_cast<unsigned>(B)), dim3(64 * waves), lds, s, stat, cand, scores, V, (int)W, \
+                     (int)n, p.chunks, lists, out_scores, out_beams, out_tokens)
+  const int64_t keys = p.chunks * n;
+  if (keys <= 5 * 64) KRQ_PICK(5);
+  else if (keys <= 10 * 64) KRQ_PICK(10);
+  else KRQ_PICK(0);
+#undef KRQ_PICK
   return krq_check_launch("beam_select");
 }
 
