@@ -101,13 +101,13 @@ KRQ_DEV int wave_before(int v, int& all) {
   return s - v;
 }
 
-constexpr int kFewKeys = 384;  // keys that are ranked as they come
+constexpr int kFewKeys = 512, kSegKeys = kFewKeys / 4;  // keys that are ranked as they come; of a wave
 
 template <typename T, int NV>
 __global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const T* __restrict__ logits, int64_t ld, int64_t V, int n, int chunks,
                                                             RowStat* __restrict__ stat, uint64_t* __restrict__ cand) {
   constexpr int VEC = 16 / sizeof(T), P = NV * VEC, CH = P * kBeamThreads;
-  extern __shared__ uint64_t list[];  // [max(4 n P, kFewKeys)]
+  extern __shared__ __attribute__((aligned(16))) uint64_t list[];  // [max(4 n P, kFewKeys)]
   __shared__ float tops[4], sums[4];
   __shared__ uint32_t least[4];
   __shared__ uint64_t nth[4];
@@ -118,15 +118,17 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const T* __restrict_
   const int64_t base = (int64_t)c * CH;
   const int left = static_cast<int>(min(V - base, (int64_t)CH));  // tokens of the chunk
   float f[P];  // (places past V hold -inf)
+  auto unpack = [](v4u a, float* o) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 2) o[2 * i] = as_f32(a[i] << 16), o[2 * i + 1] = as_f32(a[i] & 0xffff0000u);
+      else o[i] = as_f32(a[i]);
+    }
+  };
   auto load = [&](int v, float* o) {
     const int e = (v * kBeamThreads + tid) * VEC;
     if (e + VEC <= left) {
-      const v4u a = ld16_any(r + base + e);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(T) == 2) o[2 * i] = as_f32(a[i] << 16), o[2 * i + 1] = as_f32(a[i] & 0xffff0000u);
-        else o[i] = as_f32(a[i]);
-      }
+      unpack(ld16_any(r + base + e), o);
     } else {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
@@ -138,8 +140,16 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const T* __restrict_
       }
     }
   };
+  if (left == CH) {  // (all loads in flight at once: a branch around each would wait for it)
+    v4u a[NV];
 #pragma unroll
-  for (int v = 0; v < NV; ++v) load(v, f + v * VEC);
+    for (int v = 0; v < NV; ++v) a[v] = ld16_any(r + base + (v * kBeamThreads + tid) * VEC);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) unpack(a[v], f + v * VEC);
+  } else {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) load(v, f + v * VEC);
+  }
   auto key_of = [&](int v, int i, float value) {  // of place i of the thread's vector v; 0 past V
     const int e = (v * kBeamThreads + tid) * VEC + i;
     return e < left ? static_cast<uint64_t>(ord_of(value)) << 32 | static_cast<uint32_t>(~static_cast<uint32_t>(base + e)) : 0;
@@ -152,29 +162,66 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const T* __restrict_
   if (lane == 0) tops[w] = of_ord(wt), least[w] = t16;
   __syncthreads();
   const float m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  uint64_t* out = cand + (row * chunks + c) * n;
+  if (m == -__builtin_inff()) {  // masked altogether: its first tokens (with a NaN, its row's candidates are not read)
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < P; ++i) nan |= f[i] != f[i];
+    nan = __syncthreads_or(nan);
+    if (tid < n) out[tid] = tid < left ? static_cast<uint64_t>(kOrdNegInf) << 32 | static_cast<uint32_t>(~static_cast<uint32_t>(base + tid)) : 0;
+    if (tid == 0) stat[row * chunks + c] = RowStat{nan ? 0xffffffffu : kOrdNegInf, 0.0f};
+    return;
+  }
   const uint32_t t = umax32(umax32(least[0], least[1]), umax32(least[2], least[3]));
   const float tf = t > kOrdNegInf ? of_ord(t) : -__builtin_inff();  // (below that are NaN's bits)
-  float s = 0.0f;
-  const float off = m > -__builtin_inff() ? m : 0.0f;
+  // every wave its own part of the list, as far as that goes; the count tells whether it did
+  uint64_t* seg = list + w * kSegKeys;
   int mine = 0;
 #pragma unroll
   for (int i = 0; i < P; ++i) {
-    s += __builtin_amdgcn_exp2f((f[i] - off) * 1.44269504f);
-    mine += f[i] >= tf;
-  }
-  s = wave_sum(s);
-  int all;
-  int at = wave_before(mine, all);
-  if (lane == 0) sums[w] = s, counts[w] = all;
-  __syncthreads();
-  int have = counts[0] + counts[1] + counts[2] + counts[3];
-  if (have <= kFewKeys) {
-    for (int q = 0; q < w; ++q) at += counts[q];
-    if (mine) {
-#pragma unroll
-      for (int i = 0; i < P; ++i)
-        if (f[i] >= tf) list[at++] = key_of(i / VEC, i % VEC, f[i]);
+    const bool in = f[i] >= tf;
+    const uint64_t mask = __ballot(in);
+    if (mask) {
+      const int at = mine + static_cast<int>(__builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32),
+                                                                       __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0)));
+      if (in && at < kSegKeys) seg[at] = key_of(i / VEC, i % VEC, f[i]);  // (0 past V)
+      mine += __popcll(mask);
     }
+  }
+  if (lane == 0 && (mine & 1) && mine < kSegKeys) seg[mine] = 0;  // (read in pairs)
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < P; ++i) s += __builtin_amdgcn_exp2f((f[i] - m) * 1.44269504f);
+  s = wave_sum(s);
+  if (lane == 0) sums[w] = s, counts[w] = mine;
+  __syncthreads();
+  const int most = max(max(counts[0], counts[1]), max(counts[2], counts[3]));
+  int have = counts[0] + counts[1] + counts[2] + counts[3];
+  // (a NaN gives a sum of NaN, and +inf does)
+  if (tid == 0) {
+    const float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    stat[row * chunks + c] = RowStat{sum != sum ? 0xffffffffu : ord_of(m), sum};
+  }
+  if (most <= kSegKeys) {
+    // sixteen of the wave's keys at a time, a quarter of the lanes for each wave's list
+    const int q = lane >> 4, others = counts[q];
+    const ulonglong2* from = reinterpret_cast<const ulonglong2*>(list + q * kSegKeys);
+    for (int i0 = 0; i0 < mine; i0 += 16) {
+      const int i = i0 + (lane & 15);
+      const uint64_t key = i < mine ? seg[i] : 0;
+      int rank = 0;
+#pragma unroll 4
+      for (int j = 0; 2 * j < others; ++j) {
+        const ulonglong2 k2 = from[j];
+        rank += k2.x > key;
+        rank += k2.y > key;
+      }
+      rank += __shfl_xor(rank, 16, 64);
+      rank += __shfl_xor(rank, 32, 64);
+      if (q == 0 && rank < n && key) out[rank] = key;
+    }
+    // (places past V reach the threshold only where it is -inf, as all places do then)
+    for (int i = have + tid; i < n; i += kBeamThreads) out[i] = 0;  // (the chunk has fewer)
   } else {  // by keys, the logits read again (a launch of equal logits: few registers for it)
     float o[VEC];
     uint64_t best = 0;
@@ -203,7 +250,7 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const T* __restrict_
         mine += k >= lk && k;
       }
     }
-    at = wave_before(mine, all);
+    int all, at = wave_before(mine, all);
     if (lane == 0) counts[w] = all;
     __syncthreads();
     have = counts[0] + counts[1] + counts[2] + counts[3];
@@ -217,20 +264,14 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const T* __restrict_
         if (k >= lk && k) list[at++] = k;  // (at most n lanes of a wave, P keys each)
       }
     }
-  }
-  __syncthreads();
-  uint64_t* out = cand + (row * chunks + c) * n;
-  for (int i = tid; i < have; i += kBeamThreads) {
-    const uint64_t key = list[i];
-    int rank = 0;
-    for (int j = 0; j < have; ++j) rank += list[j] > key || (list[j] == key && j < i);  // (equal: places past V)
-    if (rank < n) out[rank] = key;
-  }
-  for (int i = have + tid; i < n; i += kBeamThreads) out[i] = 0;  // (the chunk has fewer)
-  // a chunk without a finite logit has sum 0, one with a NaN a sum of NaN and with +inf a largest of it
-  if (tid == 0) {
-    const float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-    stat[row * chunks + c] = RowStat{sum != sum ? 0xffffffffu : ord_of(m), m > -__builtin_inff() ? sum : 0.0f};
+    __syncthreads();
+    for (int i = tid; i < have; i += kBeamThreads) {
+      const uint64_t key = list[i];
+      int rank = 0;
+      for (int j = 0; j < have; ++j) rank += list[j] > key;
+      if (rank < n) out[rank] = key;
+    }
+    for (int i = have + tid; i < n; i += kBeamThreads) out[i] = 0;
   }
 }
 

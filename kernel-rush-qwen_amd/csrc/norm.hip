@@ -18,7 +18,7 @@ using namespace krq;
 
 namespace {
 
-constexpr int kNormMaxK = 16384;
+constexpr int kNormMaxK = 16384, kPartials = 4;  // partials of a split in flight
 
 enum Src { kSrcNone, kSrcBf16, kSrcPartials };
 enum Out { kOutRows, kOutToken, kOutGiven, kOutMxE4, kOutMxE2 };
@@ -109,10 +109,11 @@ __global__ __launch_bounds__(64 * NW) void k_add_rmsnorm(NormArgs a) {
   __shared__ uint32_t smax[W > 1 && OUT == kOutToken ? NW : 1];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, K = a.K;
   int64_t b = blockIdx.x;
-  if (a.spread) {  // sixteen consecutive blocks' rows share a tile's lines: blocks of one XCD (blockIdx % 8) take them
-    const int64_t q = b >> 7;
-    const int in = static_cast<int>(b & 127);
-    b = (q << 7) + 16 * (in & 7) + (in >> 3);
+  constexpr int kTile = 16 / (NW / W);  // blocks to sixteen rows
+  if (a.spread) {  // sixteen rows share a tile's lines: blocks of one XCD (blockIdx % 8) take them
+    const int64_t q = b / (8 * kTile);
+    const int in = static_cast<int>(b % (8 * kTile));
+    b = q * (8 * kTile) + kTile * (in & 7) + (in >> 3);
   }
   const int64_t m = b * (NW / W) + wave / W;
   if (m >= a.rows) return;  // (whole rows' waves: with W > 1 a workgroup has one row)
@@ -154,43 +155,54 @@ __global__ __launch_bounds__(64 * NW) void k_add_rmsnorm(NormArgs a) {
     return;
   }
 
-  // the row, read once
+  // the row, read once: every load at once, at a clamped address (chunks past K repeat the last and count as zeros)
+  auto chunk = [&](int c) { return min(first + 64 * W * c, n8 - 1); };
   const uint8_t* xr = reinterpret_cast<const uint8_t*>(a.x + m * a.ldx);
+  uint4 l[C];
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int i = first + 64 * W * c;
-    v[c] = i < n8 ? ld16(xr + 16 * i) : zero4();
-  }
-  double ss = 0.0;
+  for (int c = 0; c < C; ++c) v[c] = ld16(xr + 16 * chunk(c));
   if constexpr (SRC == kSrcBf16) {
     const uint8_t* dr = reinterpret_cast<const uint8_t*>(static_cast<const uint16_t*>(a.delta) + m * a.ldd);
     uint4 d[C];
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const int i = first + 64 * W * c;
-      d[c] = i < n8 ? ld16(dr + 16 * i) : zero4();
-    }
+    for (int c = 0; c < C; ++c) d[c] = ld16(dr + 16 * chunk(c));
+#pragma unroll
+    for (int c = 0; c < C; ++c) l[c] = ld16(reinterpret_cast<const uint8_t*>(a.ln) + 16 * chunk(c));
 #pragma unroll
     for (int c = 0; c < C; ++c) v[c] = add8(v[c], d[c]);
   } else if constexpr (SRC == kSrcPartials) {
     const float* dr = static_cast<const float*>(a.delta) + m * a.ldd;
+    v4f sum[C][2];
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const int i = first + 64 * W * c;
-      if (i < n8) {
-        const float4* p = reinterpret_cast<const float4*>(dr + 8 * i);
-        float4 s0 = p[0], s1 = p[1];
-        for (int s = 1; s < a.split; ++s) {
-          const float4* ps = reinterpret_cast<const float4*>(dr + s * a.slice + 8 * i);
-          const float4 t0 = ps[0], t1 = ps[1];
-          s0.x += t0.x; s0.y += t0.y; s0.z += t0.z; s0.w += t0.w;
-          s1.x += t1.x; s1.y += t1.y; s1.z += t1.z; s1.w += t1.w;
-        }
-        v[c] = add8(v[c], make_uint4(pack_bf16x2(s0.x, s0.y), pack_bf16x2(s0.z, s0.w), pack_bf16x2(s1.x, s1.y),
-                                     pack_bf16x2(s1.z, s1.w)));
-      }
+    for (int c = 0; c < C; ++c) l[c] = ld16(reinterpret_cast<const uint8_t*>(a.ln) + 16 * chunk(c));
+    for (int s = 0; s < a.split; s += kPartials) {  // (past the last: loaded again, not added)
+      v4f t[kPartials][C][2];
+#pragma unroll
+      for (int u = 0; u < kPartials; ++u)
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            t[u][c][e] = *reinterpret_cast<const v4f*>(dr + min(s + u, a.split - 1) * a.slice + 8 * chunk(c) + 4 * e);
+#pragma unroll
+      for (int u = 0; u < kPartials; ++u)
+        if (s + u < a.split)
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) sum[c][e] = s + u == 0 ? t[u][c][e] : sum[c][e] + t[u][c][e];
     }
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      v[c] = add8(v[c], make_uint4(pack_bf16x2(sum[c][0][0], sum[c][0][1]), pack_bf16x2(sum[c][0][2], sum[c][0][3]),
+                                   pack_bf16x2(sum[c][1][0], sum[c][1][1]), pack_bf16x2(sum[c][1][2], sum[c][1][3])));
+  } else {
+#pragma unroll
+    for (int c = 0; c < C; ++c) l[c] = ld16(reinterpret_cast<const uint8_t*>(a.ln) + 16 * chunk(c));
   }
+#pragma unroll
+  for (int c = 0; c < C; ++c) v[c] = sel4(first + 64 * W * c < n8, v[c]);
+  double ss = 0.0;
   if (SRC != kSrcNone) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
@@ -214,8 +226,7 @@ __global__ __launch_bounds__(64 * NW) void k_add_rmsnorm(NormArgs a) {
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int i = first + 64 * W * c;
-    const uint4 l = i < n8 ? ld16(reinterpret_cast<const uint8_t*>(a.ln) + 16 * i) : zero4();
-    v[c] = i < n8 ? norm8(v[c], l, rstd) : zero4();
+    v[c] = sel4(i < n8, norm8(v[c], l[c], rstd));
     if (a.h && i < n8) *reinterpret_cast<uint4*>(a.h + m * K + 8 * i) = v[c];
     if constexpr (OUT == kOutToken) am = absmax8(v[c], am);
   }
@@ -257,17 +268,26 @@ void launch(const NormArgs& a, hipStream_t s) {
   constexpr int per = NW / W;
   NormArgs b = a;
   int64_t blocks = (a.rows + per - 1) / per;
-  b.spread = per == 1 && (a.tiled || OUT == kOutMxE4 || OUT == kOutMxE2) && a.rows >= 128;
-  if (b.spread) blocks = (blocks + 127) / 128 * 128;
+  b.spread = (a.tiled || OUT == kOutMxE4 || OUT == kOutMxE2) && a.rows >= 128;
+  if (b.spread) blocks = (blocks + 128 / per - 1) / (128 / per) * (128 / per);
   hipLaunchKernelGGL((k_add_rmsnorm<NW, W, C, SRC, OUT>), dim3(static_cast<unsigned>(blocks)), dim3(64 * NW), 0, s, b);
 }
+
+// Rows by one or two waves each where there are enough rows to fill the chip that way and K leaves those waves no idle
+// chunks, else by eight or sixteen waves, whose loads are all in flight at once. Calls of a graph, per-token scales, a bf16 addend, us, few
+// waves / many: 2,560 x 512 rows 5.0 / 4.9, 1,001 rows 6.5 / 7.5, 2,048 rows 9.1 / -; 4,096 x 1,001 8.7 / 8.5; 5,120 x 1,001 9.6 / 10.6,
+// 4,096 rows 27.4 / 31.2; 8,192 x 1,001 13.1 / 12.6 and 16,384 x 1,001 (four waves) 22.9 / 22.7.
+constexpr int64_t kManyRows = 600, kMoreRows = 1536;
 
 template <int SRC, int OUT>
 void pick(const NormArgs& a, hipStream_t s) {
   const int K = OUT == kOutMxE4 || OUT == kOutMxE2 ? static_cast<int>(mx_groups(a.K)) * kMxGroup : a.K;  // chunks written
-  if (a.rows >= 1024 && K <= 2560) launch<4, 1, 5, SRC, OUT>(a, s);
-  else if (a.rows >= 1024 && K <= 4096) launch<4, 1, 8, SRC, OUT>(a, s);
-  else if (K <= 4096) launch<8, 8, 1, SRC, OUT>(a, s);
+  if constexpr (SRC != kSrcPartials) {  // (partials of many rows: too many registers)
+    if (a.rows >= kManyRows && K <= 2560) return launch<4, 1, 5, SRC, OUT>(a, s);
+    if (a.rows >= kMoreRows && K <= 4096) return launch<4, 1, 8, SRC, OUT>(a, s);
+    if (a.rows >= kManyRows && K > 4096 && K <= 5120) return launch<2, 2, 5, SRC, OUT>(a, s);
+  }
+  if (K <= 4096) launch<8, 8, 1, SRC, OUT>(a, s);
   else if (K <= 8192) launch<8, 8, 2, SRC, OUT>(a, s);
   else launch<16, 16, 2, SRC, OUT>(a, s);
 }
