@@ -8,7 +8,7 @@
 // entry: lse and the merged n of every row, and the merge of the rows by v in fp64 (candidates of two beams can lie
 // closer than fp32 tells apart).
 //
-// The n largest of a chunk. The n-th largest of the 64 lanes' largest values, found by its upper 16 bits with ballots, has n
+// The n largest of a chunk. The n-th largest of 64 groups' largest values, found by its upper 16 bits with ballots, has n
 // values at or above it, and few more: those go to LDS, and each finds its place by counting the larger ones. Logit and
 // token make one 64-bit key for that, all of them different: the logit's bits in an order that compares as unsigned (NaN over
 // everything), then the token's complement. Where equal logits leave too many (a mask, a coarse type), the n-th largest
@@ -108,8 +108,7 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const T* __restrict_
                                                             RowStat* __restrict__ stat, uint64_t* __restrict__ cand) {
   constexpr int VEC = 16 / sizeof(T), P = NV * VEC, CH = P * kBeamThreads;
   extern __shared__ __attribute__((aligned(16))) uint64_t list[];  // [max(4 n P, kFewKeys)]
-  __shared__ float tops[4], sums[4];
-  __shared__ uint32_t least[4];
+  __shared__ float tops[kBeamThreads], sums[4];
   __shared__ uint64_t nth[4];
   __shared__ int counts[4];
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, c = blockIdx.x;
@@ -157,11 +156,13 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const T* __restrict_
   float top = f[0];
 #pragma unroll
   for (int i = 1; i < P; ++i) top = fmaxf(top, f[i]);  // (a NaN shows in the sum)
-  const uint32_t ord = ord_of(top == top ? top : -__builtin_inff());
-  const uint32_t wt = wave_max_u32_dpp(ord), t16 = nth_upper(ord, n);
-  if (lane == 0) tops[w] = of_ord(wt), least[w] = t16;
+  // the largest of the four waves' lanes of a number: the n-th largest of those 64 is reached by n values, and by few more
+  // (of 8,192, for n = 16, by 18 at the mean; the n-th of a wave's own lanes by 70)
+  tops[tid] = top == top ? top : -__builtin_inff();
   __syncthreads();
-  const float m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  top = fmaxf(fmaxf(tops[lane], tops[lane + 64]), fmaxf(tops[lane + 128], tops[lane + 192]));
+  const uint32_t ord = ord_of(top), t = nth_upper(ord, n);
+  const float m = of_ord(wave_max_u32_dpp(ord));
   uint64_t* out = cand + (row * chunks + c) * n;
   if (m == -__builtin_inff()) {  // masked altogether: its first tokens (with a NaN, its row's candidates are not read)
     bool nan = false;
@@ -172,7 +173,6 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const T* __restrict_
     if (tid == 0) stat[row * chunks + c] = RowStat{nan ? 0xffffffffu : kOrdNegInf, 0.0f};
     return;
   }
-  const uint32_t t = umax32(umax32(least[0], least[1]), umax32(least[2], least[3]));
   const float tf = t > kOrdNegInf ? of_ord(t) : -__builtin_inff();  // (below that are NaN's bits)
   // every wave its own part of the list, as far as that goes; the count tells whether it did
   uint64_t* seg = list + w * kSegKeys;
@@ -284,6 +284,7 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(const RowStat* __res
                                                             const float* __restrict__ scores, int64_t V, int W, int n, int chunks,
                                                             int lists, float* __restrict__ out_scores,
                                                             int64_t* __restrict__ out_beams, int64_t* __restrict__ out_tokens) {
+  __shared__ int ranks[kCounted];
   extern __shared__ uint64_t mem[];  // values [W][n], tokens [W][n] (32 bits), a list for each of `lists` waves [n * per]
   const int tid = threadIdx.x, threads = blockDim.x, wave = tid >> 6, lane = tid & 63;
   const int64_t b = blockIdx.x;
@@ -321,12 +322,13 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(const RowStat* __res
       continue;
     }
     const float mx = of_ord(top);
-    auto part = [&](RowStat r) { return r.top > kOrdNegInf ? r.sum * exp((double)of_ord(r.top) - (double)mx) : 0.0; };
+    // (as exact as the sums are: the chunks that matter have small exponents)
+    auto part = [&](RowStat r) {
+      return r.top > kOrdNegInf ? (double)(r.sum * __builtin_amdgcn_exp2f((of_ord(r.top) - mx) * 1.44269504f)) : 0.0;
+    };
     double s = part(q);
     for (int c = lane + 64; c < chunks; c += 64) s += part(st[c]);
-#pragma unroll
-    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
-    const double lse = (double)mx + log(s);
+    const double lse = (double)mx + log(wave_sum_f64(s));
     uint64_t best = 0;
     each([&](uint64_t key) { best = key > best ? key : best; });
     uint64_t least = static_cast<uint64_t>(nth_upper(hi32(best), n)) << 32;
@@ -353,22 +355,45 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(const RowStat* __res
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
-  __syncthreads();
-  for (int i = tid; i < W * len; i += threads) {
+  // the place of a candidate: those of larger v before it, and of equal v those of lower beams and before it in its own,
+  // the order that the rows lie in
+  const int all = W * len;
+  auto put = [&](int i, int rank) {
     const int w = i / len, p = i % len;
-    const uint64_t v = vals[w * n + p];
-    int rank = p;
-    if (W * len <= kCounted) {
-      for (int q = 0; q < W; ++q) {
-        if (q == w) continue;
-        const uint64_t edge = q < w ? v : v + (v != ~0ull);  // of lower beams the equal ones come before too
-        int before = 0;
-#pragma unroll 4
-        for (int j = 0; j < len; ++j) before += vals[q * n + j] >= edge;
-        if (q > w && v == ~0ull) before = 0;
-        rank += before;
+    if (rank < n) {
+      const int64_t at = b * n + rank;
+      const uint64_t v = vals[w * n + p];
+      out_scores[at] = v == ~0ull ? __builtin_nanf("")
+                                  : static_cast<float>(__builtin_bit_cast(double, v >> 63 ? v & ~(1ull << 63) : ~v));
+      out_beams[at] = w;
+      out_tokens[at] = toks[w * n + p];
+    }
+  };
+  if (len == n && all <= kCounted) {  // counted, by several threads for each where there are
+    int* rank = ranks;
+    for (int i = tid; i < all; i += threads) rank[i] = 0;
+    __syncthreads();
+    const int ways = max(threads / all, 1), each = (all + ways - 1) / ways;
+    for (int k = tid; k < all * ways; k += threads) {
+      const int i = k % all, j0 = k / all * each, j1 = min(j0 + each, all);
+      const uint64_t v = vals[i];
+      int before = 0;
+#pragma unroll 8
+      for (int j = j0; j < j1; ++j) {
+        const uint64_t u = vals[j];
+        before += u > v || (u == v && j < i);
       }
-    } else {
+      if (ways == 1) rank[i] = before;
+      else atomicAdd(&rank[i], before);
+    }
+    __syncthreads();
+    for (int i = tid; i < all; i += threads) put(i, rank[i]);
+  } else {
+    __syncthreads();
+    for (int i = tid; i < all; i += threads) {
+      const int w = i / len, p = i % len;
+      const uint64_t v = vals[w * n + p];
+      int rank = p;
       for (int q = 0; q < W && rank < n; ++q) {
         if (q == w) continue;
         int lo = 0, hi = len;
@@ -380,13 +405,7 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(const RowStat* __res
         }
         rank += lo;
       }
-    }
-    if (rank < n) {
-      const int64_t at = b * n + rank;
-      out_scores[at] = v == ~0ull ? __builtin_nanf("")
-                                  : static_cast<float>(__builtin_bit_cast(double, v >> 63 ? v & ~(1ull << 63) : ~v));
-      out_beams[at] = w;
-      out_tokens[at] = toks[w * n + p];
+      put(i, rank);
     }
   }
 }

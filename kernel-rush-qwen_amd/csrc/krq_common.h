@@ -166,6 +166,33 @@ KRQ_DEV float wave_sum(float v) {
   return v;
 }
 
+template <int CTRL>
+KRQ_DEV double dpp_f64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(u), CTRL, 0xf, 0xf, false));
+  const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), CTRL, 0xf, 0xf, false));
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// Sum over the wave, every lane active: wave_sum's butterfly with both halves of a double moved.
+KRQ_DEV double wave_sum_f64(double v) {
+  typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+  auto join = [](uint32_t lo, uint32_t hi) { return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo); };
+  uint64_t u = __builtin_bit_cast(uint64_t, v);
+  u32x2 lo = __builtin_amdgcn_permlane32_swap((uint32_t)u, (uint32_t)u, false, false);
+  u32x2 hi = __builtin_amdgcn_permlane32_swap((uint32_t)(u >> 32), (uint32_t)(u >> 32), false, false);
+  v = join(lo[0], hi[0]) + join(lo[1], hi[1]);
+  u = __builtin_bit_cast(uint64_t, v);
+  lo = __builtin_amdgcn_permlane16_swap((uint32_t)u, (uint32_t)u, false, false);
+  hi = __builtin_amdgcn_permlane16_swap((uint32_t)(u >> 32), (uint32_t)(u >> 32), false, false);
+  v = join(lo[0], hi[0]) + join(lo[1], hi[1]);
+  v += dpp_f64<0x128>(v);                 // row_ror:8
+  v += dpp_f64<0x141>(dpp_f64<0x1B>(v));  // lane ^ 4
+  v += dpp_f64<0x4E>(v);                  // lane ^ 2
+  v += dpp_f64<0xB1>(v);                  // lane ^ 1
+  return v;
+}
+
 // max over a block of NT threads (NT a multiple of 64, at most 1024); every thread gets it.
 template <int NT>
 KRQ_DEV uint32_t block_max_u32(uint32_t v) {

@@ -10,6 +10,9 @@ lm_head_argmax(..., return_logits=True) or any head, with a grammar's or sampler
 Both take device tensors alone, wait for nothing and can be captured.
 """
 
+import functools
+import math
+
 import torch
 
 from . import _lib as L
@@ -26,6 +29,11 @@ def _same_device(first, *tensors):
             raise ValueError(f"tensors on {first.device} and {t.device}")
 
 
+@functools.lru_cache(maxsize=4096)
+def _ws_bytes(B, W, V, n, fp32):
+    return L.lib().krq_beam_select_ws_bytes(B, W, V, n, fp32)
+
+
 def select(logits, scores, n=None):
     """logits [B W, V] (or [B, W, V]) bf16 or fp32, scores [B, W] fp32 (sums of log probabilities so far) -> (scores [B, n]
     fp32, beams [B, n] int64, tokens [B, n] int64): the n (default 2 W) largest of
@@ -34,35 +42,39 @@ def select(logits, scores, n=None):
     never preferred to others; a beam with nothing else, or with the score -inf (a first step's copies), has candidates of -inf. A beam with
     a NaN or +inf among its logits, or as its score, has candidates of NaN, which count as the largest, as in lm_head_argmax. W and n up to
     64, n <= W V, V up to 2^20, B W up to 65,535."""
-    if logits.dtype not in (torch.bfloat16, torch.float32) or logits.dim() not in (2, 3):
-        raise ValueError(f"logits must be bf16 or fp32 [B W, V] or [B, W, V], got {logits.dtype} {tuple(logits.shape)}")
+    fp32 = logits.dtype is torch.float32
+    shape = logits.shape
+    if not (fp32 or logits.dtype is torch.bfloat16) or not 2 <= len(shape) <= 3:
+        raise ValueError(f"logits must be bf16 or fp32 [B W, V] or [B, W, V], got {logits.dtype} {tuple(shape)}")
     if scores.dtype is not torch.float32 or scores.dim() != 2:
         raise ValueError(f"scores must be fp32 [B, W], got {scores.dtype} {tuple(scores.shape)}")
-    _same_device(logits, scores)
+    dev = logits.get_device()
+    if dev < 0 or scores.get_device() != dev:
+        _same_device(logits, scores)
     B, W = scores.shape
-    V = logits.shape[-1]
-    if tuple(logits.shape[:-1]) not in ((B * W,), (B, W)):
-        raise ValueError(f"logits {tuple(logits.shape)} and scores {tuple(scores.shape)} do not match")
+    V = shape[-1]
+    if shape[:-1] != (B * W,) and shape[:-1] != (B, W):
+        raise ValueError(f"logits {tuple(shape)} and scores {tuple(scores.shape)} do not match")
     n = 2 * W if n is None else int(n)
     if not 1 <= W <= MAX_BEAMS or not 1 <= V <= MAX_VOCAB or B * W > MAX_ROWS:
         raise ValueError(f"{B} x {W} beams, vocabulary {V}: at most {MAX_BEAMS} beams, {MAX_ROWS} rows, {MAX_VOCAB} tokens")
     if not 1 <= n <= min(MAX_N, W * V):
         raise ValueError(f"n={n} (1 to {min(MAX_N, W * V)})")
-    if logits.dim() == 3:
+    ld = V
+    if not logits.is_contiguous():
         logits = logits.reshape(B * W, V)
-    ld = logits.stride(0) if B * W > 1 else V
-    if (V > 1 and logits.stride(1) != 1) or ld < V:
-        logits, ld = logits.contiguous(), V
+        ld = logits.stride(0) if B * W > 1 else V
+        if (V > 1 and logits.stride(1) != 1) or ld < V:
+            logits, ld = logits.contiguous(), V
     scores = scores.contiguous()
-    out_scores = torch.empty((B, n), device=logits.device, dtype=torch.float32)
-    out = torch.empty((2, B, n), device=logits.device, dtype=torch.int64)
+    out_scores = scores.new_empty((B, n))
+    beams, tokens = scores.new_empty((2, B, n), dtype=torch.int64).unbind(0)
     if B:
-        fp32 = logits.dtype is torch.float32
-        nbytes = L.lib().krq_beam_select_ws_bytes(B, W, V, n, fp32)
-        ws = torch.empty((nbytes,), device=logits.device, dtype=torch.uint8)
-        _mx._call(logits.get_device(), "krq_beam_select", logits.data_ptr(), fp32, ld, scores.data_ptr(), B, W, V, n, ws.data_ptr(), nbytes,
-                  out_scores.data_ptr(), out[0].data_ptr(), out[1].data_ptr())
-    return out_scores, out[0], out[1]
+        nbytes = _ws_bytes(B, W, V, n, fp32)
+        ws = scores.new_empty((nbytes,), dtype=torch.uint8)
+        _mx._call(dev, "krq_beam_select", logits.data_ptr(), fp32, ld, scores.data_ptr(), B, W, V, n, ws.data_ptr(), nbytes,
+                  out_scores.data_ptr(), beams.data_ptr(), tokens.data_ptr())
+    return out_scores, beams, tokens
 
 
 def reorder(states, beams, dim=0, lengths=None, length_dim=None):
@@ -73,48 +85,55 @@ def reorder(states, beams, dim=0, lengths=None, length_dim=None):
     A beam outside [0, W) leaves its row as it is. Rows whose beam is their own are neither read nor written. One launch for all states
     of a shape (of up to 64). Returns states."""
     many = [states] if isinstance(states, torch.Tensor) else list(states)
-    if beams.dtype not in (torch.int64, torch.int32) or beams.dim() != 2:
-        raise ValueError(f"beams must be int64 or int32 [B, W], got {beams.dtype} {tuple(beams.shape)}")
+    shape, dev = beams.shape, beams.get_device()
+    if not (beams.dtype is torch.int64 or beams.dtype is torch.int32) or len(shape) != 2:
+        raise ValueError(f"beams must be int64 or int32 [B, W], got {beams.dtype} {tuple(shape)}")
     if (lengths is None) != (length_dim is None):
         raise ValueError("lengths and length_dim go together")
-    _same_device(beams, lengths, *many)
-    B, W = beams.shape
+    B, W = shape
     if W > MAX_BEAMS or B > 1 << 20:
         raise ValueError(f"{B} x {W} beams (at most {MAX_BEAMS} beams, 2^20 entries)")
-    if lengths is not None and (lengths.dtype not in (torch.int64, torch.int32) or tuple(lengths.shape) != (B,)):
-        raise ValueError(f"lengths must be int64 or int32 [{B}], got {lengths.dtype} {tuple(lengths.shape)}")
+    if dev < 0 or (lengths is not None and lengths.get_device() != dev):
+        _same_device(beams, lengths)
+    if lengths is not None:
+        if not (lengths.dtype is torch.int64 or lengths.dtype is torch.int32) or lengths.shape != (B,):
+            raise ValueError(f"lengths must be int64 or int32 [{B}], got {lengths.dtype} {tuple(lengths.shape)}")
+        lengths = lengths.contiguous()
+    beams = beams.contiguous()
     groups, spans = {}, []
     for t in many:
-        d = dim + t.dim() if dim < 0 else dim
-        s = t.dim() if length_dim is None else length_dim + t.dim() if length_dim < 0 else length_dim
-        if not 0 <= d < t.dim() or t.shape[d] != B * W or (length_dim is not None and not d < s < t.dim()):
-            raise ValueError(f"state {tuple(t.shape)}: {B} x {W} rows along dim={dim}, positions along length_dim={length_dim} after it")
+        if t.get_device() != dev:
+            _same_device(beams, t)
         if not t.is_contiguous():
             raise ValueError(f"state {tuple(t.shape)} strides {t.stride()}: states are reordered in place and must be contiguous")
-        if t.numel() == 0:
-            continue
-        outer = mid = 1
-        for k in t.shape[:d]:
-            outer *= k
-        for k in t.shape[d + 1:s]:
-            mid *= k
-        if length_dim is None:
-            outer, mid, S, size = outer, 1, 1, mid * t.element_size()
-        else:
-            S, size = t.shape[s], t.element_size()
-            for k in t.shape[s + 1:]:
-                size *= k
-        groups.setdefault((outer, mid, S, size), []).append(t.data_ptr())
-        spans.append((t.data_ptr(), t.numel() * t.element_size()))
-    spans.sort()
-    for (a, size), (b, _) in zip(spans, spans[1:]):
-        if a + size > b:
-            raise ValueError("states overlap: each would be reordered more than once")
-    beams = beams.contiguous()
-    lengths = lengths if lengths is None else lengths.contiguous()
+        size = t.element_size()
+        geometry = _geometry(t.shape, size, B, W, dim, length_dim)
+        size *= t.numel()
+        if size:
+            p = t.data_ptr()
+            groups.setdefault(geometry, []).append(p)
+            spans.append((p, size))
+    if len(spans) > 1:
+        spans.sort()
+        for (a, size), (b, _) in zip(spans, spans[1:]):
+            if a + size > b:
+                raise ValueError("states overlap: each would be reordered more than once")
     for (outer, mid, S, size), ptrs in groups.items():
         for i in range(0, len(ptrs), MAX_STATES):
             part = ptrs[i:i + MAX_STATES]
-            _mx._call(beams.get_device(), "krq_beam_reorder", (L.ctypes.c_void_p * len(part))(*part), len(part), outer, B, W, mid, S, size,
-                      beams.data_ptr(), beams.dtype is torch.int64, L.ptr(lengths), lengths is not None and lengths.dtype is torch.int64)
+            _mx._call(dev, "krq_beam_reorder", (L.ctypes.c_void_p * len(part))(*part), len(part), outer, B, W, mid, S, size, beams.data_ptr(),
+                      beams.dtype is torch.int64, L.ptr(lengths), lengths is not None and lengths.dtype is torch.int64)
     return states
+
+
+@functools.lru_cache(maxsize=4096)
+def _geometry(shape, size, B, W, dim, length_dim):
+    """(entries before the rows, between rows and positions, positions, bytes of a position) of a state of elements of `size` bytes."""
+    d = dim + len(shape) if dim < 0 else dim
+    s = len(shape) if length_dim is None else length_dim + len(shape) if length_dim < 0 else length_dim
+    if not 0 <= d < len(shape) or shape[d] != B * W or (length_dim is not None and not d < s < len(shape)):
+        raise ValueError(f"state {tuple(shape)}: {B} x {W} rows along dim={dim}, positions along length_dim={length_dim} after it")
+    outer, mid = math.prod(shape[:d]), math.prod(shape[d + 1:s])
+    if length_dim is None:
+        return outer, 1, 1, mid * size
+    return outer, mid, shape[s], math.prod(shape[s + 1:]) * size

@@ -10,6 +10,8 @@ is rounded once. A projection fused from several (QKV, [gate; up]) has one pair 
 prefill take the same call, two launches; rows and ids may change between replays of a captured one.
 """
 
+import functools
+
 import torch
 
 from . import _lib as L
@@ -71,19 +73,25 @@ class Adapters:
                     raise ValueError(f"rank {a.shape[0]} (1 to {self.rank})")
                 rank = max(rank, a.shape[0])
         r16 = (rank + 15) // 16 * 16
-        self.a[slot].zero_()
-        packed = self.b[slot, :self.N * r16].view(self.N, r16)
-        packed.zero_()
-        at = 0
+        packed, at = self.b[slot, :self.N * r16].view(self.N, r16), 0
         for i, (p, n) in enumerate(zip(pairs, self.parts)):
-            if p is not None:
-                a, b = p
-                tiles = a.new_zeros((r16, self.a.shape[3] * 64))
-                tiles[:a.shape[0], :self.K] = a
-                # [rank tile, j, step, g, e, 8] -> [rank tile, step, e, g, j, 8]
-                self.a[slot, i, :r16 // 16] = tiles.view(r16 // 16, 16, -1, 4, 2, 8).permute(0, 2, 4, 3, 1, 5)
-                packed[at:at + n, :a.shape[0]].copy_(b)
+            tiles, cols = self.a[slot, i, :r16 // 16], packed[at:at + n]
             at += n
+            if p is None:
+                tiles.zero_()
+                cols.zero_()
+                continue
+            a, b = p
+            r = a.shape[0]
+            if r < r16:
+                cols.zero_()
+            cols[:, :r].copy_(b)
+            if r < r16 or self.K % 64:  # whole tiles
+                whole = torch.zeros((r16, tiles.shape[1] * 64), device=tiles.device, dtype=tiles.dtype)
+                whole[:r, :self.K] = a
+                a = whole
+            # [rank tile, j, step, g, e, 8] -> [rank tile, step, e, g, j, 8]
+            tiles.copy_(a.reshape(r16 // 16, 16, -1, 4, 2, 8).permute(0, 2, 4, 3, 1, 5))
         self.scales[slot] = float(scale)
         self.ranks[slot] = rank
 
@@ -93,9 +101,8 @@ class Adapters:
         self.ranks[self._slot(slot)] = 0
 
 
-def _rows(t, what, dtypes, cols):
-    if t.dim() != 2 or t.dtype not in dtypes or t.shape[1] != cols:
-        raise ValueError(f"{what} must be {' or '.join(str(d) for d in dtypes)} [M, {cols}], got {t.dtype} {tuple(t.shape)}")
+def _ld(t, cols):
+    """The row stride of t [M, cols], None where its rows are not of consecutive values."""
     ld = t.stride(0) if t.shape[0] > 1 else cols
     return ld if (cols == 1 or t.stride(1) == 1) and ld >= cols else None
 
@@ -104,44 +111,57 @@ def _extent(t, ld):
     return t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * ld + t.shape[1]) * t.element_size()
 
 
+@functools.lru_cache(maxsize=4096)
+def _ws_bytes(M, K, parts, rank):
+    return L.lib().krq_lora_ws_bytes(M, K, parts, rank)
+
+
 def add(y, x, adapters, ids, out=None):
     """y [M, N] bf16 or fp32, x [M, K] bf16, ids [M] int32 or int64 (a slot of adapters for each row; negative: none) ->
     y plus every row's adapter's product, in y's type. out: where it goes (default a new tensor; y itself adds in place).
     An id past the last slot gives a row of NaN. Rows of y, x and out may lie apart; x's are copied where they do not start on 16 bytes."""
-    ad = adapters
-    L.require_device(y, x, ids, out)
-    dev = x.get_device()
-    if y.get_device() != dev or ids.get_device() != dev or ad.a.get_device() != dev or (out is not None and out.get_device() != dev):
-        raise ValueError(f"tensors on {x.device}, {y.device}, {ids.device}, {ad.a.device}")
-    ldx = _rows(x, "x", (torch.bfloat16,), ad.K)
-    M = x.shape[0]
-    ldy = _rows(y, "y", (torch.bfloat16, torch.float32), ad.N)
-    if ids.dtype not in (torch.int32, torch.int64) or tuple(ids.shape) != (M,) or y.shape[0] != M:
+    ad, dev = adapters, x.get_device()
+    if dev < 0 or y.get_device() != dev or ids.get_device() != dev or ad.a.get_device() != dev or (
+            out is not None and out.get_device() != dev):
+        L.require_device(y, x, ids, out)
+        raise ValueError(f"tensors on {x.device}, {y.device}, {ids.device}, {ad.a.device}" + ("" if out is None else f", {out.device}"))
+    K, N, M = ad.K, ad.N, x.shape[0]
+    if x.dtype is not torch.bfloat16 or x.shape != (M, K):
+        raise ValueError(f"x must be bf16 [M, {K}], got {x.dtype} {tuple(x.shape)}")
+    fp32 = y.dtype is torch.float32
+    if not (fp32 or y.dtype is torch.bfloat16) or y.dim() != 2 or y.shape[1] != N:
+        raise ValueError(f"y must be bf16 or fp32 [M, {N}], got {y.dtype} {tuple(y.shape)}")
+    wide = ids.dtype is torch.int64
+    if not (wide or ids.dtype is torch.int32) or ids.shape != (M,) or y.shape[0] != M:
         raise ValueError(f"ids {ids.dtype} {tuple(ids.shape)}, x {tuple(x.shape)} and y {tuple(y.shape)} do not match")
-    if ldx is None or ldx % 8 or ldx >= MAX_ROW or x.data_ptr() % 16:
-        x, ldx = x.clone(memory_format=torch.contiguous_format), ad.K
+    ldx, ldy = _ld(x, K), _ld(y, N)
+    if ldx is None or ldx & 7 or ldx >= MAX_ROW or x.data_ptr() & 15:
+        x, ldx = x.clone(memory_format=torch.contiguous_format), K
     ids = ids.contiguous()
     if out is None:
-        out, ldo = torch.empty((M, ad.N), device=y.device, dtype=y.dtype), ad.N
+        if ldy is None:
+            y, ldy = y.contiguous(), N
+        out, ldo = y.new_empty((M, N)), N
     else:
-        ldo = _rows(out, "out", (y.dtype,), ad.N)
-        if ldo is None or out.shape[0] != M:
-            raise ValueError(f"out must be [{M}, {ad.N}] with rows of consecutive values, got {tuple(out.shape)} strides {out.stride()}")
-    if ldy is None:
-        if out is y:
-            raise ValueError("y must have rows of consecutive values to be added to in place")
-        y, ldy = y.contiguous(), ad.N
+        ldo = _ld(out, N) if out.dim() == 2 and out.dtype is y.dtype and out.shape == (M, N) else None
+        if ldo is None:
+            raise ValueError(f"out must be {y.dtype} [{M}, {N}] with rows of consecutive values, got {out.dtype} {tuple(out.shape)} "
+                             f"strides {out.stride()}")
+        if ldy is None:
+            y, ldy = y.contiguous(), N
+        if M:
+            o0, o1 = _extent(out, ldo)
+            for t, ld in ((y, ldy), (x, ldx)):
+                if t is y and o0 == y.data_ptr() and ldo == ldy:
+                    continue
+                a, b = _extent(t, ld)
+                if o0 < b and a < o1:
+                    raise ValueError("out overlaps an input (it may be y itself)")
     if M == 0:
         return out
-    for t, ld in ((y, ldy), (x, ldx)):
-        if t is y and out.data_ptr() == y.data_ptr() and ldo == ldy:
-            continue
-        (a0, a1), (b0, b1) = _extent(out, ldo), _extent(t, ld)
-        if a0 < b1 and b0 < a1:
-            raise ValueError("out overlaps an input (it may be y itself)")
-    nbytes = L.lib().krq_lora_ws_bytes(M, ad.K, len(ad.parts), ad.rank)
-    ws = torch.empty((max(nbytes, 1),), device=x.device, dtype=torch.uint8)
-    _mx._call(dev, "krq_lora_add", x.data_ptr(), ldx, ids.data_ptr(), ids.dtype is torch.int64, ad.a.data_ptr(), ad.b.data_ptr(),
-              ad.ranks.data_ptr(), ad.scales.data_ptr(), ad.slots, M, ad.K, ad._n, len(ad.parts), ad.rank, y.data_ptr(), ldy,
-              out.data_ptr(), ldo, y.dtype is torch.float32, ws.data_ptr(), nbytes)
+    parts = len(ad.parts)
+    nbytes = _ws_bytes(M, K, parts, ad.rank)
+    ws = x.new_empty((max(nbytes, 1),), dtype=torch.uint8)
+    _mx._call(dev, "krq_lora_add", x.data_ptr(), ldx, ids.data_ptr(), wide, ad.a.data_ptr(), ad.b.data_ptr(), ad.ranks.data_ptr(),
+              ad.scales.data_ptr(), ad.slots, M, K, ad._n, parts, ad.rank, y.data_ptr(), ldy, out.data_ptr(), ldo, fp32, ws.data_ptr(), nbytes)
     return out

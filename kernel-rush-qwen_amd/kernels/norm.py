@@ -72,58 +72,79 @@ def _apart(out, t, same):
         raise ValueError("res_out overlaps an input (it may be x itself)")
 
 
-def _launch(x, delta, ln, eps, res_out, kind, inv, h, out, scale):
-    """Checks the operands, makes res, launches; returns res. h, out, scale: functions of the checked x that make them."""
-    L.require_device(x, delta, ln, inv, res_out)
-    for t in (delta, ln, inv, res_out):
-        if t is not None and t.get_device() != x.get_device():
-            raise ValueError(f"tensors on {x.device} and {t.device}")
-    res = x
-    x, ldx = _rows(x, "x")
-    M, K = x.shape
-    if K % 16 or not 16 <= K <= MAX_K:
+def _misplaced(x, *tensors):
+    L.require_device(x, *tensors)
+    raise ValueError("tensors on " + ", ".join(sorted({str(t.device) for t in (x, *tensors) if t is not None})))
+
+
+def _operands(x, delta, ln, res_out):
+    """(x, its row stride, delta, partials or 0, its row and slice strides, ln, res, M, K, device) as the kernel takes them. A
+    call of a few rows is host work as much as a launch: operands that lie as they should are looked at once, by attribute."""
+    dev = x.get_device()
+    if dev < 0 or ln.get_device() != dev or (delta is not None and delta.get_device() != dev) or (
+            res_out is not None and res_out.get_device() != dev):
+        _misplaced(x, delta, ln, res_out)
+    shape = x.shape
+    if x.dtype is not torch.bfloat16 or len(shape) != 2:
+        raise ValueError(f"x must be bf16 [M, K], got {x.dtype} {tuple(shape)}")
+    M, K = shape
+    if K & 15 or not 16 <= K <= MAX_K:
         raise ValueError(f"K={K} must be a multiple of 16 up to {MAX_K}")
-    if ln.dtype is not torch.bfloat16 or tuple(ln.shape) != (K,):
+    if ln.dtype is not torch.bfloat16 or ln.dim() != 1 or ln.shape[0] != K:
         raise ValueError(f"ln must be bf16 [{K}], got {ln.dtype} {tuple(ln.shape)}")
-    ln = ln if ln.is_contiguous() and ln.data_ptr() % 16 == 0 else _own_memory(ln)
-    split = ldd = part = 0
+    res, ldx, split, ldd, part = x, K, 0, 0, 0
+    if not x.is_contiguous() or x.data_ptr() & 15:
+        x, ldx = _rows(x, "x")
+    if not ln.is_contiguous() or ln.data_ptr() & 15:
+        ln = _own_memory(ln)
     if delta is not None:
-        if tuple(delta.shape[-2:]) != (M, K):
-            raise ValueError(f"x {tuple(x.shape)} and delta {tuple(delta.shape)} do not match")
-        if delta.dim() == 2:
-            delta, ldd = _rows(delta, "delta")
+        dshape = delta.shape
+        if dshape[-2:] != shape or not 2 <= len(dshape) <= 3:
+            raise ValueError(f"x {tuple(shape)} and delta {tuple(dshape)} do not match")
+        plain = delta.is_contiguous() and not delta.data_ptr() & 15
+        if len(dshape) == 2:
+            if plain and delta.dtype is torch.bfloat16:
+                ldd = K
+            else:
+                delta, ldd = _rows(delta, "delta")
         else:
-            delta, ldd, part = _partials(delta, M, K)
-            split = delta.shape[0]
+            split = dshape[0]
+            if plain and delta.dtype is torch.float32 and 1 <= split <= SPLIT_MAX:
+                ldd, part = K, M * K
+            else:
+                delta, ldd, part = _partials(delta, M, K)
         if res_out is None:
-            res = torch.empty((M, K), device=x.device, dtype=torch.bfloat16)
+            res = torch.empty_like(x) if ldx == K else x.new_empty(shape)
         else:
             res = res_out
-            if res.dtype is not torch.bfloat16 or tuple(res.shape) != (M, K) or not res.is_contiguous() or res.data_ptr() % 16:
+            if res.dtype is not torch.bfloat16 or res.shape != shape or not res.is_contiguous() or res.data_ptr() & 15:
                 raise ValueError(f"res_out must be contiguous bf16 [{M}, {K}] on 16 bytes, got {res.dtype} {tuple(res.shape)}")
             _apart(res, x, ldx == K)
             _apart(res, delta, split == 0 and ldd == K)
             _apart(res, ln, False)
     elif res_out is not None:
         raise ValueError("res_out without delta: there is no new residual")
-    if M:
-        _mx._call(x.get_device(), "krq_add_rmsnorm", L.ptr(x), ldx, L.ptr(delta), split, ldd, part, L.ptr(ln), float(eps), M, K, kind,
-                  L.ptr(inv), L.ptr(res) if delta is not None else None, h, out, scale)
-    return res
+    return x, ldx, delta, split, ldd, part, ln, res, M, K, dev
 
 
-def _shape(x):
-    if x.dim() != 2:
-        raise ValueError(f"x must be bf16 [M, K], got {x.dtype} {tuple(x.shape)}")
-    return x.shape
+def _launch(operands, eps, kind, inv, h, out, scale):
+    x, ldx, delta, split, ldd, part, ln, res, M, K, dev = operands
+    if M == 0:
+        return
+    if delta is None:
+        _mx._call(dev, "krq_add_rmsnorm", x.data_ptr(), ldx, None, 0, 0, 0, ln.data_ptr(), eps, M, K, kind, inv, None, h, out, scale)
+    else:
+        _mx._call(dev, "krq_add_rmsnorm", x.data_ptr(), ldx, delta.data_ptr(), split, ldd, part, ln.data_ptr(), eps, M, K, kind, inv,
+                  res.data_ptr(), h, out, scale)
 
 
 def add_rmsnorm(x, delta, ln, eps=1e-6, res_out=None):
     """x [M, K] bf16, delta None, bf16 [M, K] or fp32 partials [S, M, K], ln [K] bf16 -> (res, h), both bf16 [M, K].
     res_out: where res goes (contiguous; may be x, whose rows are then replaced); res is x itself where delta is None."""
-    M, K = _shape(x)
-    h = torch.empty((M, K), device=x.device, dtype=torch.bfloat16)
-    return _launch(x, delta, ln, eps, res_out, L.NORM_ROWS, None, L.ptr(h), None, None), h
+    ops = _operands(x, delta, ln, res_out)
+    h = ops[0].new_empty(ops[8:10])
+    _launch(ops, eps, L.NORM_ROWS, None, h.data_ptr(), None, None)
+    return ops[7], h
 
 
 def add_rmsnorm_fp8(x, delta, ln, eps=1e-6, a=None, tiled=False, with_h=False, res_out=None):
@@ -132,37 +153,40 @@ def add_rmsnorm_fp8(x, delta, ln, eps=1e-6, a=None, tiled=False, with_h=False, r
     equal to linear_fp8's cast of h, xs = a.scale. x8 is float8_e4m3fn [M, K] for gemv_fp8(x8, q, split, xs=xs),
     gemm_fp8(x8, q, xs=xs) and their kin; tiled=True (K % 64 == 0): uint8 in the tiled activation layout, padded to
     16 * ceil(M / 16) rows, for gemv_fp8_tiled_launch(x8, xs, q, M, ..) at up to 32 rows."""
-    M, K = _shape(x)
-    if tiled and K % 64:
+    ops = _operands(x, delta, ln, res_out)
+    x, M, K = ops[0], ops[8], ops[9]
+    if not tiled:
+        x8 = x.new_empty((M, K), dtype=torch.float8_e4m3fn)
+    elif K % 64:
         raise ValueError(f"tiled rows need K={K} a multiple of 64")
-    if tiled:
-        x8 = torch.empty(((M + 15) // 16 * 16 * K,), device=x.device, dtype=torch.uint8)
     else:
-        x8 = torch.empty((M, K), device=x.device, dtype=torch.float8_e4m3fn)
+        x8 = x.new_empty(((M + 15) // 16 * 16 * K,), dtype=torch.uint8)
     if a is None:
-        inv, xs = None, torch.empty((M, 1), device=x.device, dtype=torch.float32)
-        kind = L.NORM_FP8_TOKEN_TILED if tiled else L.NORM_FP8_TOKEN
+        inv = None
+        xs = x.new_empty((M, 1), dtype=torch.float32)
+        kind, ps = L.NORM_FP8_TOKEN_TILED if tiled else L.NORM_FP8_TOKEN, xs.data_ptr()
     else:
-        inv, xs = _fp8._one(a.inv), _fp8._one(a.scale)
-        if inv.numel() != 1 or xs.numel() != 1:
-            raise ValueError("a must have one inverse and one scale")
-        kind = L.NORM_FP8_GIVEN_TILED if tiled else L.NORM_FP8_GIVEN
-    h = torch.empty((M, K), device=x.device, dtype=torch.bfloat16) if with_h else None
-    res = _launch(x, delta, ln, eps, res_out, kind, inv, L.ptr(h), L.ptr(x8), None if a is not None else L.ptr(xs))
-    return (res, x8, xs, h) if with_h else (res, x8, xs)
+        one, xs = _fp8._one(a.inv), _fp8._one(a.scale)
+        if one.get_device() != ops[10] or xs.get_device() != ops[10]:
+            _misplaced(x, one, xs)
+        kind, inv, ps = L.NORM_FP8_GIVEN_TILED if tiled else L.NORM_FP8_GIVEN, one.data_ptr(), None
+    h = x.new_empty((M, K)) if with_h else None
+    _launch(ops, eps, kind, inv, h.data_ptr() if with_h else None, x8.data_ptr(), ps)
+    return (ops[7], x8, xs, h) if with_h else (ops[7], x8, xs)
 
 
 def add_rmsnorm_mx(x, delta, ln, eps=1e-6, elem="e4m3", with_h=False, res_out=None):
     """add_rmsnorm with h in MX blocks of elem: (res, rows), or (res, rows, h) with_h; rows is the MXRows of
     mxfp4.quant_rows(h, elem), for every product on an MXFP4Weight. K % 32 == 0."""
-    M, K = _shape(x)
+    ops = _operands(x, delta, ln, res_out)
+    x, M, K = ops[0], ops[8], ops[9]
     if K % _mx.BLOCK:
         raise ValueError(f"MX blocks need K={K} a multiple of {_mx.BLOCK}")
     e = _mx._elem(elem)
     at, nbytes = _mx._rows_bytes(M, K, e)
-    data = torch.empty((nbytes,), device=x.device, dtype=torch.uint8)
-    h = torch.empty((M, K), device=x.device, dtype=torch.bfloat16) if with_h else None
+    data = x.new_empty((nbytes,), dtype=torch.uint8)
+    h = x.new_empty((M, K)) if with_h else None
     p = data.data_ptr()
-    res = _launch(x, delta, ln, eps, res_out, L.NORM_MX_E4M3 if e == L.MX_E4M3 else L.NORM_MX_E2M1, None, L.ptr(h), p, p + at)
+    _launch(ops, eps, L.NORM_MX_E4M3 if e == L.MX_E4M3 else L.NORM_MX_E2M1, None, h.data_ptr() if with_h else None, p, p + at)
     rows = _mx.MXRows(data, at, (M, K), elem)
-    return (res, rows, h) if with_h else (res, rows)
+    return (ops[7], rows, h) if with_h else (ops[7], rows)
