@@ -520,8 +520,10 @@ int krq_add_rmsnorm(const void* x, int64_t ldx, const void* delta, int split, in
  * x bf16 [M, K], rows ldx apart, on 16 bytes. ids [M] int64 (ids_64 != 0) or int32: negative adds nothing, slots or more
  * gives a row of NaN. The projection has `parts` parts of parts_n[p] columns (a host array), N their sum, with a
  * pair of factors each: a bf16 [slots][parts][rank / 16][ceil(K / 64)][2][64][8], in lane order: of 16 ranks and 64 k, entry
- * [e][16 g + j] the k = 16 g + 8 e .. + 7 of rank j, zeros past ranks[i] and past K; b bf16 [slots][N * rank], of which slot i uses the first N * r as
- * [N][r], r = ranks[i] rounded up to 16 (zeros past ranks[i]); ranks int32 [slots], at most rank, 0 for an empty slot;
+ * [e][16 g + j] the k = 16 g + 8 e .. + 7 of rank j, zeros past ranks[i] and past K; b bf16
+ * [slots][tiles * 16 * rank], tiles the sum of ceil(parts_n[p] / 16), of which slot i uses the first tiles * 16 * r, r = ranks[i]
+ * rounded up to 16: of 16 columns of a part and 32 ranks entry [16 g + j] the ranks 8 g .. + 7 of column j, then, for an odd last
+ * 16 ranks, the same in 32 entries (zeros past ranks[i] and past the part); ranks int32 [slots], at most rank, 0 for an empty slot;
  * scales fp32 [slots] (all on the device). rank a multiple of 16 up to 256, parts up to 8, K a multiple of 16.
  * y, out: bf16, or fp32 with fp32 != 0, rows ldy and ldo apart; out may be y.
  * Sums in fp32, rounded once. ws: krq_lora_ws_bytes(M, K, parts, rank) bytes on 16 (overwritten; calls that overlap must

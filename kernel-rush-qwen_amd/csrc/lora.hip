@@ -11,10 +11,12 @@
 // What bounds it: the factors of the adapters in use, read once each, at few rows; x, y and out at many. The products
 // are a few percent of the matrix cores' rate.
 //
-// The down product's operands. v_mfma_f32_16x16x32_bf16 takes 16 bytes of one row per lane; sixteen consecutive lanes have
+// The operands of the factors. v_mfma_f32_16x16x32_bf16 takes 16 bytes of one row per lane; sixteen consecutive lanes have
 // sixteen rows, so that loads of row-major operands touch a line per lane (a launch of 4,096 x 2,560 rows took 11.5 us bound
 // by that). A is kept in lane order, [K / 64][2][64 lanes][8] per 16 ranks, lane 16 g + j its rank j, k = 16 g + 8 e .. + 7 of a
-// step's 64; rows of x are loaded eight lanes to a line and turned through LDS, each wave its own.
+// step's 64; rows of x are loaded eight lanes to a line and turned through LDS, each wave its own. B is kept as [r / 32][64 lanes][8]
+// per 16 columns, lane 16 g + j column j, ranks 8 g .. + 7 of 32, and an odd last 16 ranks in 32 lanes (row-major, 4,096 rows of
+// gate_up with rank 64 took 151 us, KRQ_B64 now).
 //
 // h is kept in fp32 and enters the second product as the sum of two bf16 (to 2^-16; three, to 2^-24, beside an fp32 y), so
 // that the sum is rounded once, at the end: the second product takes two or three times the matrix instructions, which
@@ -34,7 +36,7 @@ struct LoraArgs {
   const uint16_t* x;
   const void* ids;
   const uint16_t* a;     // [slots][P][R / 16][steps][2][64][8]: lane order, zeros past K
-  const uint16_t* b;     // [slots][N R], a slot's factors as [N][its rank, rounded up to 16]
+  const uint16_t* b;     // [slots][tiles 16 R]: for each tile of 16 columns and the slot's rank, rounded up to 16, lane order
   const int32_t* ranks;  // [slots], up to R; 0: none
   const float* scales;   // [slots]
   const void* y;
@@ -42,8 +44,9 @@ struct LoraArgs {
   int4* place;           // [M] what k_lora_down found at each place: row, id, rank
   float* h;              // [split][M][P R] by place, times the scale
   int64_t M, K, ldx, ldy, ldo;
-  int slots, P, R, N, split, ids64, ways;
+  int slots, P, R, split, ids64, ways;
   int part[kMaxParts + 1], block[kMaxParts + 1];  // first column of each part; first group of column blocks
+  int tile[kMaxParts + 1];                        // first tile of 16 columns: every part starts a new one
 };
 
 KRQ_DEV int load_id(const LoraArgs& a, int64_t m) {  // -1: none; slots: out of range
@@ -166,6 +169,14 @@ __global__ __launch_bounds__(64 * NW, TC <= 2 ? 4 : 2) void k_lora_down(LoraArgs
   int turn = -1, first, cur;
   uint64_t same;
   auto next = [&]() {
+    if constexpr (!SORT) {  // one tile and a workgroup for each row: the first row of an adapter takes it
+      const bool mine = left != 0;
+      left = 0;
+      first = way;
+      cur = __builtin_amdgcn_readlane(id, way);
+      same = __ballot(real && id == cur);
+      return mine && cur >= 0 && cur < a.slots && __builtin_ctzll(same) == way;
+    }
     while (left) {
       first = __builtin_ctzll(left);
       cur = next_id(id, left, same);
@@ -348,8 +359,17 @@ __global__ __launch_bounds__(256, 4) void k_lora_up(LoraArgs a) {
   bool fresh = true;  // f holds the first step
   for (int turn = 0; left; ++turn) {
     uint64_t same;
-    const int first = __builtin_ctzll(left), cur = next_id(id, left, same);
-    if (!ROWS && turn % a.ways != way) continue;
+    int first = __builtin_ctzll(left), cur;
+    if (!ROWS && a.M <= 16) {  // one tile and a workgroup for each row
+      first = way;
+      cur = __builtin_amdgcn_readlane(id, way);
+      same = __ballot(id == cur) & left;
+      left = 0;
+      if (__builtin_ctzll(same) != way) return;
+    } else {
+      cur = next_id(id, left, same);
+      if (!ROWS && turn % a.ways != way) continue;
+    }
     const bool me = same >> j & 1;
     const int rank = __builtin_amdgcn_readlane(place.z, first), r16 = (rank + 15) & ~15;
     if (r16 == 0 && cur < a.slots && a.out == a.y) continue;
@@ -379,22 +399,27 @@ __global__ __launch_bounds__(256, 4) void k_lora_up(LoraArgs a) {
       for (int e = 0; e < NT; ++e) st[(s * NT + e) * 64] = make_uint4(o[0][e], o[1][e], o[2][e], o[3][e]);
       fresh = false;
     }
-    const uint16_t* bs = a.b + (int64_t)(r16 ? cur : 0) * a.N * a.R;
-    // the products of a block's 64 columns from column nb, of which the part has `most` + 1
-    const int col = sizeof(T) == 2 ? 8 * (j >> 2) + (j & 3) : j;  // this lane's column of tile 0; of tile t:
-    auto of_tile = [](int t) { return sizeof(T) == 2 ? 32 * (t >> 1) + 4 * (t & 1) : 16 * t; };
-    auto product = [&](int nb, bool edge, int most, v4f* acc) {
-      const uint8_t* base = reinterpret_cast<const uint8_t*>(bs + (int64_t)nb * r16);
-      auto from = [&](int t, uint32_t r) {  // rank r of the lane's column of tile t
-        return edge ? base + 2u * (min(col + of_tile(t), most) * r16 + r) : base + 2 * of_tile(t) * r16 + 2u * (col * r16 + r);
-      };
+    const uint8_t* bs = reinterpret_cast<const uint8_t*>(a.b) + (int64_t)(r16 ? cur : 0) * a.tile[a.P] * (32 * a.R);
+    // the products of the 64 columns of block nb of the part. Column j of the operand of tile t: see above; of fp32 it is the
+    // column j of the factor's tile t, of bf16 it lies in tile 2 (t / 2) + j / 8, there 8 (j / 4 % 2) + 4 (t % 2) + j % 4
+    const int first_tile = a.tile[p] + ((n0 - a.part[p]) >> 4), last_tile = a.tile[p + 1] - 1;
+    const int row = sizeof(T) == 2 ? 8 * ((j >> 2) & 1) + (j & 3) : j, over = sizeof(T) == 2 ? j >> 3 : 0;
+    auto product = [&](int blk, bool edge, v4f* acc) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) acc[t] = v4f{};
+      const int64_t size = 32 * r16;  // bytes of a tile
+      const uint8_t* base = bs + (first_tile + 4 * blk) * size;
+      const int most = last_tile - (first_tile + 4 * blk);
       for (int s = 0; 32 * s < r16; ++s) {
         const bool in = 32 * s + 8 * g < r16;  // (an odd 16 ranks: the upper lanes have none)
+        const uint32_t lane_at = 16u * (16 * (in ? g : 0) + row);
         uint4 bv[4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) bv[t] = ld16(from(t, in ? 32 * s + 8 * g : 0));
+        for (int t = 0; t < 4; ++t) {
+          const int tile = sizeof(T) == 2 ? 2 * (t >> 1) : t, sub = sizeof(T) == 2 ? 64 * (t & 1) : 0;
+          bv[t] = ld16(edge ? base + min(tile + over, most) * size + (1024 * s + sub + lane_at)
+                            : base + tile * size + 1024 * s + sub + (static_cast<uint32_t>(over * size) + lane_at));
+        }
 #pragma unroll
         for (int t = 0; t < 4; ++t) bv[t] = sel4(in, bv[t]);
 #pragma unroll
@@ -416,7 +441,7 @@ __global__ __launch_bounds__(256, 4) void k_lora_up(LoraArgs a) {
 #pragma unroll
     for (int blk = 0; blk < NI; ++blk) {
       if (blk < whole) {
-        if (r16) product(n0 + 64 * blk, false, 63, acc);
+        if (r16) product(blk, false, acc);
 #pragma unroll
         for (int q = 0; q < NP; ++q) {
           finish(v[blk][q], acc + TP * q);
@@ -426,7 +451,7 @@ __global__ __launch_bounds__(256, 4) void k_lora_up(LoraArgs a) {
     }
     const int ne = n0 + 64 * whole;
     if (whole < NI && ne < n1) {
-      if (r16) product(ne, true, n1 - 1 - ne, acc);
+      if (r16) product(whole, true, acc);
 #pragma unroll
       for (int q = 0; q < NP; ++q) {
         const int n = ne + VEC * g + 4 * VEC * q;
@@ -444,15 +469,17 @@ struct LoraPlan {
 };
 
 constexpr int kDownWaves = 8;
+constexpr int64_t kUpGroups = 2000;
 
 // Few rows: 16-row tiles; many: 32-row tiles and all ranks of a projection up to 64 together, so that factors and rows are read once. The adapters that a tile meets go to `ways` workgroups, the
-// first of each in parallel. K in as many parts as it takes to fill the chip with two steps of 64 k a wave.
-LoraPlan lora_plan(int64_t M, int64_t K, int P, int R) {
+// first of each in parallel: about as many as 16 places of ascending ids meet of the bank's slots. K in as many parts as it takes to fill the chip with two steps of 64 k a wave.
+LoraPlan lora_plan(int64_t M, int64_t K, int P, int R, int64_t slots) {
   LoraPlan p;
   const int T = P * R / 16;
   p.mt = M <= 256 ? 1 : 2;
-  p.ways = M <= 16 ? static_cast<int>(M) : M <= 256 ? 4 : 2;
-  p.tc = p.mt == 1 ? 1 : (T + (T + 3) / 4 - 1) / ((T + 3) / 4);
+  p.ways = M <= 16 ? static_cast<int>(M)
+                   : static_cast<int>(std::max<int64_t>(2, std::min<int64_t>({16, slots, slots * 16 / M + 2})));
+  p.tc = p.mt == 2 ? (T + (T + 3) / 4 - 1) / ((T + 3) / 4) : M > 16 && T >= 8 ? 4 : 1;
   const int64_t groups = (M + 16 * p.mt - 1) / (16 * p.mt) * ((T + p.tc - 1) / p.tc) * (M <= 16 ? M : 1);
   const int64_t most = std::max<int64_t>(1, K / (64 * 2 * kDownWaves));
   p.split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({most, p.mt == 1 ? kSplitFew : kSplitMany, (512 + groups - 1) / groups})));
@@ -463,7 +490,7 @@ template <int MT, int TC, bool SORT>
 void launch_down(const LoraArgs& a, hipStream_t s) {
   const int64_t tiles = (a.M + 16 * MT - 1) / (16 * MT);
   const int T = a.P * a.R / 16;
-  hipLaunchKernelGGL((k_lora_down<MT, TC, kDownWaves, MT == 1 ? 3 : 2, SORT>), dim3((unsigned)(tiles * a.ways), (T + TC - 1) / TC, a.split),
+  hipLaunchKernelGGL((k_lora_down<MT, TC, kDownWaves, MT * TC == 1 ? 3 : 2, SORT>), dim3((unsigned)(tiles * a.ways), (T + TC - 1) / TC, a.split),
                      dim3(64 * kDownWaves), 0, s, a);
 }
 
@@ -478,10 +505,17 @@ void launch_up(const LoraArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((k_lora_up<T, NI, ROWS>), grid, dim3(256), smem, s, u);
 }
 
+// Column blocks that a wave of the many-row form takes: as many as leave some thousand workgroups. 777 rows of QKV, us, one / two /
+// four: KRQ_NI
 template <typename T>
 void launch_up_any(const LoraArgs& a, hipStream_t s) {
-  if (a.M <= 256) launch_up<T, 1, false>(a, s);
-  else launch_up<T, sizeof(T) == 2 ? 4 : 2, true>(a, s);
+  if (a.M <= 256) return launch_up<T, 1, false>(a, s);
+  int64_t blocks = 0;
+  for (int p = 0; p < a.P; ++p) blocks += (a.part[p + 1] - a.part[p] + 63) / 64;
+  blocks *= (a.M + 63) / 64;
+  if (blocks < 2 * kUpGroups) return launch_up<T, 1, true>(a, s);
+  if (blocks < 4 * kUpGroups || sizeof(T) == 4) return launch_up<T, 2, true>(a, s);
+  if constexpr (sizeof(T) == 2) launch_up<T, 4, true>(a, s);
 }
 
 // places, then h
@@ -491,7 +525,7 @@ int64_t place_bytes(int64_t M) { return (M * (int64_t)sizeof(int4) + 255) / 256 
 
 extern "C" int64_t krq_lora_ws_bytes(int64_t M, int64_t K, int parts, int rank) {
   if (M < 1 || K < 16 || parts < 1 || parts > kMaxParts || rank < 16 || rank > kMaxRank) return -1;
-  return place_bytes(M) + lora_plan(M, K, parts, rank).split * M * parts * rank * (int64_t)sizeof(float);
+  return place_bytes(M) + lora_plan(M, K, parts, rank, 1).split * M * parts * rank * (int64_t)sizeof(float);
 }
 
 extern "C" int krq_lora_add(const void* x, int64_t ldx, const void* ids, int ids_64, const void* a, const void* b, const int32_t* ranks,
@@ -512,14 +546,15 @@ extern "C" int krq_lora_add(const void* x, int64_t ldx, const void* ids, int ids
     KRQ_REQUIRE(parts_n[p] >= 1 && parts_n[p] <= (1 << 24), "lora_add: part %d of %lld columns", p, (long long)parts_n[p]);
     l.part[p] = static_cast<int>(n);
     n += parts_n[p];
+    l.part[p + 1] = static_cast<int>(n);
+    l.tile[p + 1] = l.tile[p] + static_cast<int>((parts_n[p] + 15) / 16);
   }
-  l.part[parts] = static_cast<int>(n);
   KRQ_REQUIRE(ldy >= n && ldo >= n, "lora_add: rows of %lld columns %lld and %lld apart", (long long)n, (long long)ldy, (long long)ldo);
   const int esize = fp32 ? 4 : 2;
   KRQ_REQUIRE((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(out)) % esize == 0, "lora_add: y and out must start on a value");
   KRQ_REQUIRE(y != out || ldy == ldo, "lora_add: out is y with other rows");
   KRQ_REQUIRE((M + 15) / 16 * (n / 64 + parts) < 0x7fffffff, "lora_add: %lld x %lld is too large", (long long)M, (long long)n);
-  const LoraPlan plan = lora_plan(M, K, parts, rank);
+  const LoraPlan plan = lora_plan(M, K, parts, rank, slots);
   KRQ_REQUIRE(ws_bytes >= krq_lora_ws_bytes(M, K, parts, rank), "lora_add: ws of %lld bytes is too small", (long long)ws_bytes);
   l.x = (const uint16_t*)x;
   l.ids = ids;
@@ -539,13 +574,13 @@ extern "C" int krq_lora_add(const void* x, int64_t ldx, const void* ids, int ids
   l.slots = (int)slots;
   l.P = parts;
   l.R = rank;
-  l.N = (int)n;
   l.split = plan.split;
   l.ids64 = ids_64 != 0;
   l.ways = plan.ways;
   hipStream_t s = (hipStream_t)stream;
   if (M <= 16) launch_down<1, 1, false>(l, s);
-  else if (plan.mt == 1) launch_down<1, 1, true>(l, s);
+  else if (plan.mt == 1 && plan.tc == 1) launch_down<1, 1, true>(l, s);
+  else if (plan.mt == 1) launch_down<1, 4, true>(l, s);
   else if (plan.tc == 1) launch_down<2, 1, true>(l, s);
   else if (plan.tc == 2) launch_down<2, 2, true>(l, s);
   else if (plan.tc == 3) launch_down<2, 3, true>(l, s);

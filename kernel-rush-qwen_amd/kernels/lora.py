@@ -40,10 +40,12 @@ class Adapters:
             raise ValueError(f"slots={slots}")
         self.rank = (int(rank) + 15) // 16 * 16
         # a slot's A: for each part, 16 ranks and 64 k the kernel's operands in lane order (lane 16 g + j: rank j, k = 16 g + 8 e
-        # .. + 7), zeros past its rank and past K; its B: [N, its rank rounded up to 16]
+        # .. + 7), zeros past its rank and past K; its B: for each 16 columns of a part and 32 ranks the same (lane 16 g + j:
+        # column j, ranks 8 g .. + 7; 32 lanes of an odd last 16 ranks), zeros past its rank and past the part
         self.a = torch.zeros((self.slots, len(self.parts), self.rank // 16, -(-self.K // 64), 2, 4, 16, 8), device=device,
                              dtype=torch.bfloat16)
-        self.b = torch.zeros((self.slots, self.N * self.rank), device=device, dtype=torch.bfloat16)
+        self._tiles = [-(-p // 16) for p in self.parts]
+        self.b = torch.zeros((self.slots, sum(self._tiles) * 16 * self.rank), device=device, dtype=torch.bfloat16)
         self.ranks = torch.zeros((self.slots,), device=device, dtype=torch.int32)
         self.scales = torch.zeros((self.slots,), device=device, dtype=torch.float32)
         self._n = (L.ctypes.c_int64 * len(self.parts))(*self.parts)
@@ -73,27 +75,33 @@ class Adapters:
                     raise ValueError(f"rank {a.shape[0]} (1 to {self.rank})")
                 rank = max(rank, a.shape[0])
         r16 = (rank + 15) // 16 * 16
-        packed, at = self.b[slot, :self.N * r16].view(self.N, r16), 0
-        for i, (p, n) in enumerate(zip(pairs, self.parts)):
-            tiles, cols = self.a[slot, i, :r16 // 16], packed[at:at + n]
-            at += n
+        packed = self.b[slot, :sum(self._tiles) * 16 * r16].view(-1, 16 * r16)
+        full = r16 // 32 * 32  # ranks of whole steps
+        for i, (p, n, cols) in enumerate(zip(pairs, self.parts, packed.split(self._tiles))):
+            tiles = self.a[slot, i, :r16 // 16]
             if p is None:
                 tiles.zero_()
                 cols.zero_()
                 continue
-            a, b = p
-            r = a.shape[0]
-            if r < r16:
-                cols.zero_()
-            cols[:, :r].copy_(b)
-            if r < r16 or self.K % 64:  # whole tiles
-                whole = torch.zeros((r16, tiles.shape[1] * 64), device=tiles.device, dtype=tiles.dtype)
-                whole[:r, :self.K] = a
-                a = whole
             # [rank tile, j, step, g, e, 8] -> [rank tile, step, e, g, j, 8]
-            tiles.copy_(a.reshape(r16 // 16, 16, -1, 4, 2, 8).permute(0, 2, 4, 3, 1, 5))
+            a = self._whole(p[0], r16, tiles.shape[1] * 64).view(r16 // 16, 16, -1, 4, 2, 8)
+            tiles.copy_(a.permute(0, 2, 4, 3, 1, 5))
+            # [tile, j, step, g, 8] -> [tile, step, g, j, 8]
+            b = self._whole(p[1], cols.shape[0] * 16, r16).view(-1, 16, r16)
+            if full:
+                cols[:, :16 * full].view(-1, full // 32, 4, 16, 8).copy_(b[:, :, :full].view(-1, 16, full // 32, 4, 8).permute(0, 2, 3, 1, 4))
+            if full < r16:
+                cols[:, 16 * full:].view(-1, 2, 16, 8).copy_(b[:, :, full:].view(-1, 16, 2, 8).permute(0, 2, 1, 3))
         self.scales[slot] = float(scale)
         self.ranks[slot] = rank
+
+    def _whole(self, t, rows, cols):
+        """t in bf16 on the slots' device, with zeros up to [rows, cols]."""
+        if t.shape == (rows, cols):
+            return t.to(self.a.device, torch.bfloat16).contiguous()
+        w = torch.zeros((rows, cols), device=self.a.device, dtype=torch.bfloat16)
+        w[:t.shape[0], :t.shape[1]] = t
+        return w
 
     @torch.no_grad()
     def clear(self, slot):

@@ -144,8 +144,23 @@ def test_load_packs_a_slot():
     want[0, :17, :32], want[1, :5, :32] = a0, a1
     got = ad.a[1, :, :2].permute(0, 1, 5, 2, 4, 3, 6).reshape(2, 32, 64)  # [part, rank tile, j | step, g, e, 8]
     assert torch.equal(got, want)
-    b = ad.b[1, :5 * 32].view(5, 32)
-    assert torch.equal(b[:3, :17], b0) and torch.equal(b[3:, :5], b1) and not b[:3, 17:].any() and not b[3:, 5:].any()
+    for part, (b, n) in enumerate(((b0, 3), (b1, 2))):  # a tile of 16 columns each: [g, j, 8] of 32 ranks
+        want = torch.zeros(16, 32, dtype=BF)
+        want[:n, :b.shape[1]] = b
+        assert torch.equal(ad.b[1].view(-1)[part * 512:(part + 1) * 512].view(4, 16, 8).permute(1, 0, 2).reshape(16, 32), want)
+    ad = lora.Adapters(32, 35, 40, 1, "cpu")  # three tiles; 32 ranks and 16 more
+    b0 = torch.randn(35, 40, generator=g).to(BF)
+    ad.load(0, (torch.randn(40, 32), b0))
+    t = ad.b[0, :3 * 16 * 48].view(3, 16 * 48)
+    got = torch.cat([t[:, :512].view(3, 4, 16, 8).permute(0, 2, 1, 3).reshape(48, 32), t[:, 512:].view(3, 2, 16, 8).permute(0, 2, 1, 3).reshape(48, 16)], 1)
+    want = torch.zeros(48, 48, dtype=BF)
+    want[:35, :40] = b0
+    assert torch.equal(got, want)
+
+
+def test_clear():
+    ad = lora.Adapters(32, (3, 2), 40, 2, "cpu")
+    ad.load(1, [(torch.randn(17, 32), torch.randn(3, 17)), None])
     ad.clear(1)
     assert ad.ranks.tolist() == [0, 0]
 
