@@ -16,7 +16,7 @@
 // by that). A is kept in lane order, [K / 64][2][64 lanes][8] per 16 ranks, lane 16 g + j its rank j, k = 16 g + 8 e .. + 7 of a
 // step's 64; rows of x are loaded eight lanes to a line and turned through LDS, each wave its own. B is kept as [r / 32][64 lanes][8]
 // per 16 columns, lane 16 g + j column j, ranks 8 g .. + 7 of 32, and an odd last 16 ranks in 32 lanes (row-major, 4,096 rows of
-// gate_up with rank 64 took 151 us, KRQ_B64 now).
+// gate_up with rank 64 took 151 us, 119 this way).
 //
 // h is kept in fp32 and enters the second product as the sum of two bf16 (to 2^-16; three, to 2^-24, beside an fp32 y), so
 // that the sum is rounded once, at the end: the second product takes two or three times the matrix instructions, which
@@ -30,7 +30,7 @@ using namespace krq;
 namespace {
 
 constexpr int kMaxParts = 8, kMaxRank = 256, kWindow = 256;
-constexpr int kSplitFew = 4, kSplitMany = 2;  // parts of K at most, for up to 256 rows and for more
+constexpr int kSplitFew = 4, kSplitMany = 2;  // parts of K at most, for up to kFewRows rows and for more
 
 struct LoraArgs {
   const uint16_t* x;
@@ -468,15 +468,18 @@ struct LoraPlan {
   int split, mt, tc, ways;
 };
 
-constexpr int kDownWaves = 8;
+constexpr int kDownWaves = 8, kFewRows = 384;
 constexpr int64_t kUpGroups = 2000;
 
-// Few rows: 16-row tiles; many: 32-row tiles and all ranks of a projection up to 64 together, so that factors and rows are read once. The adapters that a tile meets go to `ways` workgroups, the
-// first of each in parallel: about as many as 16 places of ascending ids meet of the bank's slots. K in as many parts as it takes to fill the chip with two steps of 64 k a wave.
+// Few rows: 16-row tiles; many: 32-row tiles and all ranks of a projection up to 64 together, so that factors and rows are
+// read once. QKV, both launches, us, 16 / 32 rows: 300 rows 11.8 / 13.2, 512 15.2 / 12.9, 777 26.4 / 19.0. The adapters that a tile meets go
+// to `ways` workgroups, the first of each in parallel: about as many as 16 places of ascending ids meet of the bank's slots
+// (17 rows of 16 adapters in any order, us, 4 / 16 ways: 16.7 / 12.0; 64 rows 13.5 / 15.2, 11.6 with 6). K in as many parts as it
+// takes to fill the chip with two steps of 64 k a wave.
 LoraPlan lora_plan(int64_t M, int64_t K, int P, int R, int64_t slots) {
   LoraPlan p;
   const int T = P * R / 16;
-  p.mt = M <= 256 ? 1 : 2;
+  p.mt = M <= kFewRows ? 1 : 2;
   p.ways = M <= 16 ? static_cast<int>(M)
                    : static_cast<int>(std::max<int64_t>(2, std::min<int64_t>({16, slots, slots * 16 / M + 2})));
   p.tc = p.mt == 2 ? (T + (T + 3) / 4 - 1) / ((T + 3) / 4) : M > 16 && T >= 8 ? 4 : 1;
@@ -505,17 +508,15 @@ void launch_up(const LoraArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((k_lora_up<T, NI, ROWS>), grid, dim3(256), smem, s, u);
 }
 
-// Column blocks that a wave of the many-row form takes: as many as leave some thousand workgroups. 777 rows of QKV, us, one / two /
-// four: KRQ_NI
+// Column blocks of 64 that a wave of the many-row form takes: one where that leaves few workgroups, else 512 bytes of a row. Both launches
+// of a graph, us, one / four: 777 rows of QKV 19.2 / 20.8, 2,048 24.1 / 22.7, 4,096 rows of gate_up 126 / 91.6.
 template <typename T>
 void launch_up_any(const LoraArgs& a, hipStream_t s) {
-  if (a.M <= 256) return launch_up<T, 1, false>(a, s);
+  if (a.M <= kFewRows) return launch_up<T, 1, false>(a, s);
   int64_t blocks = 0;
   for (int p = 0; p < a.P; ++p) blocks += (a.part[p + 1] - a.part[p] + 63) / 64;
-  blocks *= (a.M + 63) / 64;
-  if (blocks < 2 * kUpGroups) return launch_up<T, 1, true>(a, s);
-  if (blocks < 4 * kUpGroups || sizeof(T) == 4) return launch_up<T, 2, true>(a, s);
-  if constexpr (sizeof(T) == 2) launch_up<T, 4, true>(a, s);
+  if (blocks * ((a.M + 63) / 64) < kUpGroups) launch_up<T, 1, true>(a, s);
+  else launch_up<T, sizeof(T) == 2 ? 4 : 2, true>(a, s);
 }
 
 // places, then h
