@@ -48,7 +48,17 @@ class Adapters:
         self.b = torch.zeros((self.slots, sum(self._tiles) * 16 * self.rank), device=device, dtype=torch.bfloat16)
         self.ranks = torch.zeros((self.slots,), device=device, dtype=torch.int32)
         self.scales = torch.zeros((self.slots,), device=device, dtype=torch.float32)
-        self._n = (L.ctypes.c_int64 * len(self.parts))(*self.parts)
+        self._set_n()
+
+    def _set_n(self):
+        self._n = (L.ctypes.c_int64 * len(self.parts))(*self.parts)  # the entry point's argument
+
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k != "_n"}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._set_n()
 
     def _slot(self, slot):
         if not 0 <= slot < self.slots:
@@ -74,6 +84,9 @@ class Adapters:
                 if not 1 <= a.shape[0] <= self.rank:
                     raise ValueError(f"rank {a.shape[0]} (1 to {self.rank})")
                 rank = max(rank, a.shape[0])
+        if rank == 0:  # (no part has a pair)
+            self.ranks[slot] = 0
+            return
         r16 = (rank + 15) // 16 * 16
         packed = self.b[slot, :sum(self._tiles) * 16 * r16].view(-1, 16 * r16)
         full = r16 // 32 * 32  # ranks of whole steps

@@ -1,6 +1,8 @@
 """Calls of kernels.lora and krq_lora_add that end before anything is launched, without a GPU."""
 
+import copy
 import ctypes
+import pickle
 
 import pytest
 import torch
@@ -163,6 +165,21 @@ def test_clear():
     ad.load(1, [(torch.randn(17, 32), torch.randn(3, 17)), None])
     ad.clear(1)
     assert ad.ranks.tolist() == [0, 0]
+
+
+def test_load_without_pairs_empties_a_slot():
+    ad = lora.Adapters(32, (3, 2), 40, 2, "cpu")
+    ad.load(1, [(torch.randn(17, 32), torch.randn(3, 17)), None])
+    ad.load(1, [None, None])
+    assert ad.ranks.tolist() == [0, 0]
+
+
+def test_a_bank_can_be_copied():
+    ad = lora.Adapters(32, (3, 2), 40, 2, "cpu")
+    ad.load(1, [(torch.randn(17, 32), torch.randn(3, 17)), None], 0.25)
+    for other in (copy.deepcopy(ad), pickle.loads(pickle.dumps(ad))):
+        assert other.parts == ad.parts and list(other._n) == [3, 2] and other.ranks.tolist() == [0, 17]
+        assert torch.equal(other.a, ad.a) and torch.equal(other.b, ad.b) and other.a.data_ptr() != ad.a.data_ptr()
 
 
 def test_entry_point_refuses():
