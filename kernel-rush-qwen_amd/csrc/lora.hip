@@ -340,8 +340,9 @@ __global__ __launch_bounds__(256, 4) void k_lora_up(LoraArgs a) {
   const float* hr = a.h + pc * (a.P * a.R) + p * a.R;
   const int64_t slice = a.M * (a.P * a.R);
   // a step of 32 ranks of h, 8 g .. 8 g + 7 of them in this lane; the first waits for nothing
-  auto load_h = [&](int s, v4f (&f)[SP][2]) {
-    const int r = min(32 * s + 8 * g, a.R - 8);
+  // (an odd last 16 ranks: the lanes 32 .. 63 have the same as those 32 before them)
+  auto load_h = [&](int s, bool odd, v4f (&f)[SP][2]) {
+    const int r = min(32 * s + 8 * (odd ? g & 1 : g), a.R - 8);
 #pragma unroll
     for (int q = 0; q < SP; ++q)
       if (q < a.split)
@@ -349,7 +350,7 @@ __global__ __launch_bounds__(256, 4) void k_lora_up(LoraArgs a) {
         for (int e = 0; e < 2; ++e) f[q][e] = *reinterpret_cast<const v4f*>(hr + q * slice + r + 4 * e);
   };
   v4f f[SP][2];
-  load_h(0, f);
+  load_h(0, a.R == 16, f);
   const int4 place = a.place[pc];
   const int id = place.y;
   uint64_t left = __ballot(m0 + j < a.M) & 0xffff;
@@ -385,18 +386,23 @@ __global__ __launch_bounds__(256, 4) void k_lora_up(LoraArgs a) {
     }
     // this place's h, summed over the parts of K in order, in NT terms
     for (int s = 0; 32 * s < r16; ++s) {
-      if (!(fresh && s == 0)) load_h(s, f);
+      const bool odd = 32 * s + 16 == r16;
+      if (!(fresh && s == 0 && odd == (a.R == 16))) load_h(s, odd, f);
       v4f v2[2] = {f[0][0], f[0][1]};
 #pragma unroll
       for (int q = 1; q < SP; ++q)
         if (q < a.split) v2[0] += f[q][0], v2[1] += f[q][1];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v2[i >> 2][i & 3] = me && 32 * s + 8 * g + i < rank ? v2[i >> 2][i & 3] : 0.0f;
+      for (int i = 0; i < 8; ++i) v2[i >> 2][i & 3] = me && 32 * s + 8 * (odd ? g & 1 : g) + i < rank ? v2[i >> 2][i & 3] : 0.0f;
       uint32_t o[4][NT];
 #pragma unroll
       for (int i = 0; i < 4; ++i) split_bf16<NT>(v2[i >> 1][2 * (i & 1)], v2[i >> 1][2 * (i & 1) + 1], o[i]);
 #pragma unroll
-      for (int e = 0; e < NT; ++e) st[(s * NT + e) * 64] = make_uint4(o[0][e], o[1][e], o[2][e], o[3][e]);
+      for (int e = 0; e < NT; ++e) {
+        uint4 u = make_uint4(o[0][e], o[1][e], o[2][e], o[3][e]);
+        if (odd && g >= 2) u = e + 1 < NT ? make_uint4(o[0][e + 1 < NT ? e + 1 : e], o[1][e + 1 < NT ? e + 1 : e], o[2][e + 1 < NT ? e + 1 : e], o[3][e + 1 < NT ? e + 1 : e]) : zero4();
+        st[(s * NT + e) * 64] = u;
+      }
       fresh = false;
     }
     const uint8_t* bs = reinterpret_cast<const uint8_t*>(a.b) + (int64_t)(r16 ? cur : 0) * a.tile[a.P] * (32 * a.R);
@@ -411,8 +417,8 @@ __global__ __launch_bounds__(256, 4) void k_lora_up(LoraArgs a) {
       const uint8_t* base = bs + (first_tile + 4 * blk) * size;
       const int most = last_tile - (first_tile + 4 * blk);
       for (int s = 0; 32 * s < r16; ++s) {
-        const bool in = 32 * s + 8 * g < r16;  // (an odd 16 ranks: the upper lanes have none)
-        const uint32_t lane_at = 16u * (16 * (in ? g : 0) + row);
+        const bool odd = 32 * s + 16 == r16;
+        const uint32_t lane_at = 16u * (16 * (odd ? g & 1 : g) + row);
         uint4 bv[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -421,9 +427,8 @@ __global__ __launch_bounds__(256, 4) void k_lora_up(LoraArgs a) {
                             : base + tile * size + 1024 * s + sub + (static_cast<uint32_t>(over * size) + lane_at));
         }
 #pragma unroll
-        for (int t = 0; t < 4; ++t) bv[t] = sel4(in, bv[t]);
-#pragma unroll
         for (int e = 0; e < NT; ++e) {
+          if (odd && e % 2) continue;  // (two terms of 16 ranks in one operand)
           const uint4 h = st[(s * NT + e) * 64];
 #pragma unroll
           for (int t = 0; t < 4; ++t) acc[t] = mfma32(bv[t], h, acc[t]);
