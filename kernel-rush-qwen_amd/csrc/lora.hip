@@ -289,6 +289,8 @@ struct Piece {
   KRQ_DEV void store(uint16_t* at) const { *reinterpret_cast<v4u_on2*>(at) = u; }
   KRQ_DEV void store(float* at) const { *reinterpret_cast<v4u_on4*>(at) = u; }
   KRQ_DEV void load(const T* at, int n) {  // the first n values
+    if (n >= VEC) return load(at);
+    if (n <= 0) return;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (sizeof(T) == 2)
@@ -298,6 +300,7 @@ struct Piece {
     }
   }
   KRQ_DEV void store(T* at, int n) const {
+    if (n >= VEC) return store(at);
 #pragma unroll
     for (int i = 0; i < VEC; ++i)
       if (i < n) {
