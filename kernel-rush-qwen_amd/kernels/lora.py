@@ -162,7 +162,7 @@ def add(y, x, adapters, ids, out=None):
     if out is None:
         if ldy is None:
             y, ldy = y.contiguous(), N
-        out, ldo = y.new_empty((M, N)), N
+        out, ldo = torch.empty_like(y) if ldy == N else y.new_empty((M, N)), N
     else:
         ldo = _ld(out, N) if out.dim() == 2 and out.dtype is y.dtype and out.shape == (M, N) else None
         if ldo is None:
