@@ -173,7 +173,10 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const T* __restrict_
     if (tid == 0) stat[row * chunks + c] = RowStat{nan ? 0xffffffffu : kOrdNegInf, 0.0f};
     return;
   }
-  const float tf = t > kOrdNegInf ? of_ord(t) : -__builtin_inff();  // (below that are NaN's bits)
+  // Fewer than n groups with a finite value (a mask that ends in the chunk): the finite ones are taken, and then the first
+  // masked tokens.
+  const bool few = t <= kOrdNegInf;
+  const float tf = few ? -3.40282347e38f : of_ord(t);
   // every wave its own part of the list, as far as that goes; the count tells whether it did
   uint64_t* seg = list + w * kSegKeys;
   int mine = 0;
@@ -220,7 +223,30 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const T* __restrict_
       rank += __shfl_xor(rank, 32, 64);
       if (q == 0 && rank < n && key) out[rank] = key;
     }
-    // (places past V reach the threshold only where it is -inf, as all places do then)
+    if (few && have < n) {  // n - have masked tokens more, which lie among the first have + n, if the chunk has them
+      __syncthreads();      // (counts are written again)
+      const int span = min(left, have + n);
+      int found = have;
+      for (int i0 = 0; i0 < span; i0 += kBeamThreads) {
+        const int i = i0 + tid;
+        float v = 0.0f;
+        if (i < span) {
+          if constexpr (sizeof(T) == 2) v = bf16_to_f32(r[base + i]);
+          else v = r[base + i];
+        }
+        const bool masked = v == -__builtin_inff();
+        const uint64_t mask = __ballot(masked);
+        if (lane == 0) counts[w] = __popcll(mask);
+        __syncthreads();
+        int at = found + __popcll(mask & ((1ull << lane) - 1));
+        for (int q = 0; q < w; ++q) at += counts[q];
+        if (masked && at < n)
+          out[at] = static_cast<uint64_t>(kOrdNegInf) << 32 | static_cast<uint32_t>(~static_cast<uint32_t>(base + i));
+        found += counts[0] + counts[1] + counts[2] + counts[3];
+        __syncthreads();
+      }
+      have = found;
+    }
     for (int i = have + tid; i < n; i += kBeamThreads) out[i] = 0;  // (the chunk has fewer)
   } else {  // by keys, the logits read again (a launch of equal logits: few registers for it)
     float o[VEC];
@@ -276,15 +302,14 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const T* __restrict_
 }
 
 // One batch entry. A wave merges a row at a time, its keys in registers where they are up to KR a lane; then every row's
-// sorted candidates meet in LDS, where each finds its place: by counting where they are few, else by a binary search in
-// the other rows.
-constexpr int kCounted = 512;
+// sorted candidates meet in LDS, where each finds its place by binary searches in the other rows, by several threads for
+// each where there are (counting all of 260 took 10 us, of 450 19).
 template <int KR>
 __global__ __launch_bounds__(kPickThreads) void k_beam_pick(const RowStat* __restrict__ stat, const uint64_t* __restrict__ cand,
                                                             const float* __restrict__ scores, int64_t V, int W, int n, int chunks,
                                                             int lists, float* __restrict__ out_scores,
                                                             int64_t* __restrict__ out_beams, int64_t* __restrict__ out_tokens) {
-  __shared__ int ranks[kCounted];
+  __shared__ int ranks[kPickThreads];
   extern __shared__ uint64_t mem[];  // values [W][n], tokens [W][n] (32 bits), a list for each of `lists` waves [n * per]
   const int tid = threadIdx.x, threads = blockDim.x, wave = tid >> 6, lane = tid & 63;
   const int64_t b = blockIdx.x;
@@ -369,44 +394,32 @@ __global__ __launch_bounds__(kPickThreads) void k_beam_pick(const RowStat* __res
       out_tokens[at] = toks[w * n + p];
     }
   };
-  if (len == n && all <= kCounted) {  // counted, by several threads for each where there are
-    int* rank = ranks;
-    for (int i = tid; i < all; i += threads) rank[i] = 0;
-    __syncthreads();
-    const int ways = max(threads / all, 1), each = (all + ways - 1) / ways;
-    for (int k = tid; k < all * ways; k += threads) {
-      const int i = k % all, j0 = k / all * each, j1 = min(j0 + each, all);
-      const uint64_t v = vals[i];
-      int before = 0;
-#pragma unroll 8
-      for (int j = j0; j < j1; ++j) {
-        const uint64_t u = vals[j];
-        before += u > v || (u == v && j < i);
+  const int ways = min(max(threads / all, 1), W);
+  auto before = [&](int i, int k) {  // how many come before candidate i in the k-th of `ways` parts of the rows
+    const int w = i / len, p = i % len;
+    const uint64_t v = vals[w * n + p];
+    int rank = 0;
+    for (int q = k; q < W && rank < n; q += ways) {
+      int lo = q == w ? p : 0, hi = q == w ? p : len;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        const uint64_t u = vals[q * n + mid];
+        if (u > v || (u == v && q < w)) lo = mid + 1;
+        else hi = mid;
       }
-      if (ways == 1) rank[i] = before;
-      else atomicAdd(&rank[i], before);
+      rank += lo;
     }
+    return rank;
+  };
+  if (ways > 1) {  // (all < threads <= kPickThreads)
+    for (int i = tid; i < all; i += threads) ranks[i] = 0;
     __syncthreads();
-    for (int i = tid; i < all; i += threads) put(i, rank[i]);
+    for (int k = tid; k < all * ways; k += threads) atomicAdd(&ranks[k % all], before(k % all, k / all));
+    __syncthreads();
+    for (int i = tid; i < all; i += threads) put(i, ranks[i]);
   } else {
     __syncthreads();
-    for (int i = tid; i < all; i += threads) {
-      const int w = i / len, p = i % len;
-      const uint64_t v = vals[w * n + p];
-      int rank = p;
-      for (int q = 0; q < W && rank < n; ++q) {
-        if (q == w) continue;
-        int lo = 0, hi = len;
-        while (lo < hi) {
-          const int mid = (lo + hi) >> 1;
-          const uint64_t u = vals[q * n + mid];
-          if (u > v || (u == v && q < w)) lo = mid + 1;
-          else hi = mid;
-        }
-        rank += lo;
-      }
-      put(i, rank);
-    }
+    for (int i = tid; i < all; i += threads) put(i, before(i, 0));
   }
 }
 
@@ -415,14 +428,17 @@ struct SelectPlan {
   int64_t stat_bytes, bytes;
 };
 
-// Chunks of 32 values a thread, or of 8 where the rows would not fill the chip.
+// Chunks of 32 values a thread; of 8 or 16 where the rows would not fill the chip and the keys that are left still fit
+// k_beam_pick's registers.
+constexpr int kKeysShort = 10 * 64, kKeysLong = 20 * 64;
 SelectPlan select_plan(int64_t rows, int64_t V, int n, int esize) {
   SelectPlan p;
   const int vec = 16 / esize;
-  const int64_t most = (V + 32 * kBeamThreads - 1) / (32 * kBeamThreads);
-  const int values = rows * most >= 512 || most > 32 ? 32 : 8;
+  auto chunks = [&](int values) { return (V + values * kBeamThreads - 1) / (values * kBeamThreads); };
+  const bool many = rows * chunks(32) >= 512;
+  const int values = !many && chunks(8) * n <= kKeysShort ? 8 : !many && chunks(16) * n <= kKeysLong ? 16 : 32;
   p.nv = values / vec;
-  p.chunks = static_cast<int>((V + values * kBeamThreads - 1) / (values * kBeamThreads));
+  p.chunks = static_cast<int>(chunks(values));
   p.stat_bytes = (rows * p.chunks * (int64_t)sizeof(RowStat) + 15) / 16 * 16;
   p.bytes = p.stat_bytes + rows * p.chunks * n * (int64_t)sizeof(uint64_t);
   return p;
@@ -532,9 +548,11 @@ extern "C" int krq_beam_select(const void* logits, int fp32, int64_t ld, const f
   hipLaunchKernelGGL((k_beam_rows<T, NV>), grid, dim3(kBeamThreads), list, s, (const T*)logits, ld, V, (int)n, p.chunks, stat, cand)
   if (fp32) {
     if (p.nv == 8) KRQ_ROWS(float, 8);
+    else if (p.nv == 4) KRQ_ROWS(float, 4);
     else KRQ_ROWS(float, 2);
   } else {
     if (p.nv == 4) KRQ_ROWS(uint16_t, 4);
+    else if (p.nv == 2) KRQ_ROWS(uint16_t, 2);
     else KRQ_ROWS(uint16_t, 1);
   }
 #undef KRQ_ROWS
@@ -545,7 +563,8 @@ extern "C" int krq_beam_select(const void* logits, int fp32, int64_t ld, const f
                      (int)n, p.chunks, lists, out_scores, out_beams, out_tokens)
   const int64_t keys = p.chunks * n;
   if (keys <= 5 * 64) KRQ_PICK(5);
-  else if (keys <= 10 * 64) KRQ_PICK(10);
+  else if (keys <= kKeysShort) KRQ_PICK(10);
+  else if (keys <= kKeysLong) KRQ_PICK(20);
   else KRQ_PICK(0);
 #undef KRQ_PICK
   return krq_check_launch("beam_select");

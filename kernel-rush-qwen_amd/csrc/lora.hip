@@ -44,7 +44,7 @@ struct LoraArgs {
   int4* place;           // [M] what k_lora_down found at each place: row, id, rank
   float* h;              // [split][M][P R] by place, times the scale
   int64_t M, K, ldx, ldy, ldo;
-  int slots, P, R, split, ids64, ways;
+  int slots, P, R, split, ids64, ways, window;
   int part[kMaxParts + 1], block[kMaxParts + 1];  // first column of each part; first group of column blocks
   int tile[kMaxParts + 1];                        // first tile of 16 columns: every part starts a new one
 };
@@ -61,15 +61,16 @@ KRQ_DEV int rank_of(const LoraArgs& a, int id) {
 KRQ_DEV v4f mfma32(uint4 a, uint4 b, v4f c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
-// The rows of a workgroup's window (256 rows from w0) by adapter: the key of place i, id + 1 and the row in the window. A
+// The rows of a workgroup's window (up to 256 rows from w0) by adapter: the key of place i, id + 1 and the row in the window. A
 // window of few runs of the same id, as requests that follow each other make, stays as it is; another is sorted (each row
 // counts the rows before it, half of them in each of two threads), so that a tile of 16 places meets few adapters in
-// whatever order the rows name them. Rows past M are last. Sorting a window costs 3 us of a launch's 8 (4,096 x 2,560), a tile of
-// several adapters as much again for each.
+// whatever order the rows name them. Rows past M are last. 256 rows of QKV, this launch, us: 8
+// runs 5.5, 16 adapters in any order 8.7.
 constexpr int kRunsMax = 12;
 KRQ_DEV void sort_window(const LoraArgs& a, int64_t w0, uint32_t* raw, uint32_t* sorted) {
   const uint32_t t = threadIdx.x & (kWindow - 1), half = threadIdx.x / kWindow;
-  const uint32_t key = w0 + t < a.M ? static_cast<uint32_t>(load_id(a, w0 + t) + 1) << 8 | t : 0xffffffffu;
+  const bool real = t < a.window && w0 + t < a.M;
+  const uint32_t key = real ? static_cast<uint32_t>(load_id(a, w0 + t) + 1) << 8 | t : 0xffffffffu;
   if (half == 0) raw[t] = key;
   __syncthreads();
   const int runs = __syncthreads_count(half == 0 && t > 0 && raw[t - 1] >> 8 != key >> 8);
@@ -86,7 +87,7 @@ KRQ_DEV void sort_window(const LoraArgs& a, int64_t w0, uint32_t* raw, uint32_t*
     }
     if (half) sorted[t] = before;
     __syncthreads();
-    if (!half) place = w0 + t < a.M ? before + sorted[t] : t;  // (past M: equal keys, each stays, behind the others)
+    if (!half) place = real ? before + sorted[t] : t;  // (past M: equal keys, each stays, behind the others)
     __syncthreads();
   }
   if (half == 0) sorted[place] = key;
@@ -114,7 +115,7 @@ __global__ __launch_bounds__(64 * NW, TC <= 2 ? 4 : 2) void k_lora_down(LoraArgs
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, j = lane & 15;
   // (the tiles' first workgroups before their second ones, which often have nothing to do: blocks go round the XCDs)
   const uint32_t tiles = gridDim.x / a.ways;
-  const int64_t m0 = (blockIdx.x % tiles) * (int64_t)(16 * MT), w0 = SORT ? m0 / kWindow * kWindow : m0;
+  const int64_t m0 = (blockIdx.x % tiles) * (int64_t)(16 * MT), w0 = SORT ? m0 / a.window * a.window : m0;
   const int way = blockIdx.x / tiles, slot = lane & (16 * MT - 1);
   // this wave's part of K, in steps of 64
   const int steps = static_cast<int>((a.K + 63) >> 6), q0 = blockIdx.z * NW + w, qn = a.split * NW;
@@ -126,7 +127,7 @@ __global__ __launch_bounds__(64 * NW, TC <= 2 ? 4 : 2) void k_lora_down(LoraArgs
   } else {
     id = load_id(a, min(m0 + slot, a.M - 1));
   }
-  const int most = static_cast<int>(min(a.M - w0, (int64_t)kWindow)) - 1;
+  const int most = static_cast<int>(min(a.M - w0, (int64_t)(SORT ? a.window : 16))) - 1;
   auto row_of = [&](int place) {  // the row in the window of a place of the tile
     return min(SORT ? static_cast<int>(sorted[m0 - w0 + place] & 255u) : place, most);
   };
@@ -489,7 +490,7 @@ LoraPlan lora_plan(int64_t M, int64_t K, int P, int R, int64_t slots) {
   const int T = P * R / 16;
   p.mt = M <= kFewRows ? 1 : 2;
   p.ways = M <= 16 ? static_cast<int>(M)
-                   : static_cast<int>(std::max<int64_t>(2, std::min<int64_t>({16, slots, slots * 16 / M + 2})));
+                   : static_cast<int>(std::max<int64_t>(2, std::min<int64_t>({p.mt == 1 ? 16 : 4, slots, slots * 16 * p.mt / std::min<int64_t>(M, kWindow) + 2})));
   p.tc = p.mt == 2 ? (T + (T + 3) / 4 - 1) / ((T + 3) / 4) : M > 16 && T >= 8 ? 4 : 1;
   const int64_t groups = (M + 16 * p.mt - 1) / (16 * p.mt) * ((T + p.tc - 1) / p.tc) * (M <= 16 ? M : 1);
   const int64_t most = std::max<int64_t>(1, K / (64 * 2 * kDownWaves));
@@ -586,6 +587,9 @@ extern "C" int krq_lora_add(const void* x, int64_t ldx, const void* ids, int ids
   l.split = plan.split;
   l.ids64 = ids_64 != 0;
   l.ways = plan.ways;
+  // windows of one size, so that a short last one has no tile of many adapters
+  const int64_t windows = (M + kWindow - 1) / kWindow;
+  l.window = static_cast<int>(((M + windows - 1) / windows + 31) / 32 * 32);
   hipStream_t s = (hipStream_t)stream;
   if (M <= 16) launch_down<1, 1, false>(l, s);
   else if (plan.mt == 1 && plan.tc == 1) launch_down<1, 1, true>(l, s);

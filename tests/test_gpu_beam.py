@@ -113,6 +113,21 @@ def test_masks(dev, dtype):
     assert got[4].isnan().all() and (beams[4] == 0).all() and got[5].isnan().all()
 
 
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("V,n", [(5000, 64), (5000, 9), (20000, 33)])
+def test_few_tokens_allowed(dev, V, n, dtype):
+    """Masks that leave some tokens, fewer and more than a chunk's threshold needs, among them whole chunks without one."""
+    g = torch.Generator(device=dev).manual_seed(V + n)
+    allowed = (1, 5, n - 1, n, n + 1, 100, 520, 2047)
+    logits = torch.full((len(allowed) * 2, V), -INF, device=dev)
+    for i, k in enumerate(allowed):
+        for row in (2 * i, 2 * i + 1):
+            where = torch.randperm(V if row % 2 else min(V, 2100), generator=g, device=dev)[:k]
+            logits[row, where] = torch.randn(k, generator=g, device=dev) * 2
+    check(logits.to(dtype), -torch.rand(len(allowed), 2, generator=g, device=dev), n)
+    check(logits[4:].to(dtype), torch.zeros(2 * len(allowed) - 4, 1, device=dev), n)
+
+
 def test_extreme_values(dev):
     big = torch.finfo(torch.float32).max
     logits = torch.zeros(2, 3000, device=dev)
