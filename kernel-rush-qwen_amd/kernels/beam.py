@@ -53,7 +53,7 @@ def select(logits, scores, n=None):
         _same_device(logits, scores)
     B, W = scores.shape
     V = shape[-1]
-    if shape[:-1] != (B * W,) and shape[:-1] != (B, W):
+    if shape[0] != (B * W if len(shape) == 2 else B) or (len(shape) == 3 and shape[1] != W):
         raise ValueError(f"logits {tuple(shape)} and scores {tuple(scores.shape)} do not match")
     n = 2 * W if n is None else int(n)
     if not 1 <= W <= MAX_BEAMS or not 1 <= V <= MAX_VOCAB or B * W > MAX_ROWS:
@@ -66,9 +66,11 @@ def select(logits, scores, n=None):
         ld = logits.stride(0) if B * W > 1 else V
         if (V > 1 and logits.stride(1) != 1) or ld < V:
             logits, ld = logits.contiguous(), V
-    scores = scores.contiguous()
+    if not scores.is_contiguous():
+        scores = scores.contiguous()
     out_scores = scores.new_empty((B, n))
-    beams, tokens = scores.new_empty((2, B, n), dtype=torch.int64).unbind(0)
+    beams = scores.new_empty((B, n), dtype=torch.int64)
+    tokens = torch.empty_like(beams)
     if B:
         nbytes = _ws_bytes(B, W, V, n, fp32)
         ws = scores.new_empty((nbytes,), dtype=torch.uint8)

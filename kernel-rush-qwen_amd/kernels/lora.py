@@ -147,18 +147,23 @@ def add(y, x, adapters, ids, out=None):
         L.require_device(y, x, ids, out)
         raise ValueError(f"tensors on {x.device}, {y.device}, {ids.device}, {ad.a.device}" + ("" if out is None else f", {out.device}"))
     K, N, M = ad.K, ad.N, x.shape[0]
-    if x.dtype is not torch.bfloat16 or x.shape != (M, K):
+    if x.dtype is not torch.bfloat16 or x.dim() != 2 or x.shape[1] != K:
         raise ValueError(f"x must be bf16 [M, {K}], got {x.dtype} {tuple(x.shape)}")
     fp32 = y.dtype is torch.float32
-    if not (fp32 or y.dtype is torch.bfloat16) or y.dim() != 2 or y.shape[1] != N:
+    shape = y.shape
+    if not (fp32 or y.dtype is torch.bfloat16) or len(shape) != 2 or shape[1] != N:
         raise ValueError(f"y must be bf16 or fp32 [M, {N}], got {y.dtype} {tuple(y.shape)}")
     wide = ids.dtype is torch.int64
-    if not (wide or ids.dtype is torch.int32) or ids.shape != (M,) or y.shape[0] != M:
+    if not (wide or ids.dtype is torch.int32) or ids.dim() != 1 or ids.shape[0] != M or shape[0] != M:
         raise ValueError(f"ids {ids.dtype} {tuple(ids.shape)}, x {tuple(x.shape)} and y {tuple(y.shape)} do not match")
-    ldx, ldy = _ld(x, K), _ld(y, N)
-    if ldx is None or ldx & 7 or ldx >= MAX_ROW or x.data_ptr() & 15:
+    ldx = K if x.is_contiguous() else _ld(x, K)
+    ldy = N if y.is_contiguous() else _ld(y, N)
+    px = x.data_ptr()
+    if px & 15 or ldx is None or ldx & 7 or ldx >= MAX_ROW:
         x, ldx = x.clone(memory_format=torch.contiguous_format), K
-    ids = ids.contiguous()
+        px = x.data_ptr()
+    if not ids.is_contiguous():
+        ids = ids.contiguous()
     if out is None:
         if ldy is None:
             y, ldy = y.contiguous(), N
@@ -183,6 +188,6 @@ def add(y, x, adapters, ids, out=None):
     parts = len(ad.parts)
     nbytes = _ws_bytes(M, K, parts, ad.rank)
     ws = x.new_empty((max(nbytes, 1),), dtype=torch.uint8)
-    _mx._call(dev, "krq_lora_add", x.data_ptr(), ldx, ids.data_ptr(), wide, ad.a.data_ptr(), ad.b.data_ptr(), ad.ranks.data_ptr(),
+    _mx._call(dev, "krq_lora_add", px, ldx, ids.data_ptr(), wide, ad.a.data_ptr(), ad.b.data_ptr(), ad.ranks.data_ptr(),
               ad.scales.data_ptr(), ad.slots, M, K, ad._n, parts, ad.rank, y.data_ptr(), ldy, out.data_ptr(), ldo, fp32, ws.data_ptr(), nbytes)
     return out
