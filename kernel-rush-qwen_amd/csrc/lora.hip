@@ -5,8 +5,8 @@
 // for the P parts of a fused projection (part p(n) of column n), each with its own factors. Two launches: k_lora_down
 // makes h, k_lora_up adds. Rows may name any adapters in any order: a tile of 16 takes its distinct ones one after the
 // other (or, where rows are few, each in a workgroup of its own), multiplies the whole tile and writes the rows that
-// name it; from 17 rows, windows of 256 are put in the order of their adapters first. The rows of a matrix-core operand do not mix, so rows of other adapters cost nothing but the idle
-// columns, and a NaN stays in its row.
+// name it; from 17 rows, windows of up to 256 are put in the order of their adapters first. The rows of a matrix-core
+// operand do not mix, so rows of other adapters cost nothing but the idle columns, and a NaN stays in its row.
 //
 // What bounds it: the factors of the adapters in use, read once each, at few rows; x, y and out at many. The products
 // are a few percent of the matrix cores' rate.
@@ -61,11 +61,10 @@ KRQ_DEV int rank_of(const LoraArgs& a, int id) {
 KRQ_DEV v4f mfma32(uint4 a, uint4 b, v4f c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
-// The rows of a workgroup's window (up to 256 rows from w0) by adapter: the key of place i, id + 1 and the row in the window. A
-// window of few runs of the same id, as requests that follow each other make, stays as it is; another is sorted (each row
-// counts the rows before it, half of them in each of two threads), so that a tile of 16 places meets few adapters in
-// whatever order the rows name them. Rows past M are last. 256 rows of QKV, this launch, us: 8
-// runs 5.5, 16 adapters in any order 8.7.
+// The rows of a workgroup's window (up to 256 rows from w0) by adapter: the key of place i, id + 1 and the row in the
+// window. A window of few runs of the same id, as requests that follow each other make, stays as it is; another is
+// sorted (each row counts the rows before it, half of them in each of two threads), so that a tile of 16 places meets few
+// adapters in whatever order the rows name them. Rows past M are last.
 constexpr int kRunsMax = 12;
 KRQ_DEV void sort_window(const LoraArgs& a, int64_t w0, uint32_t* raw, uint32_t* sorted) {
   const uint32_t t = threadIdx.x & (kWindow - 1), half = threadIdx.x / kWindow;
@@ -477,24 +476,39 @@ struct LoraPlan {
   int split, mt, tc, ways;
 };
 
-constexpr int kDownWaves = 8, kFewRows = 384;
+constexpr int kDownWaves = 8, kFewRows = 384, kShortTiles = 6600;
 constexpr int64_t kUpGroups = 2000;
 
-// Few rows: 16-row tiles; many: 32-row tiles and all ranks of a projection up to 64 together, so that factors and rows are
-// read once. QKV, both launches, us, 16 / 32 rows: 300 rows 11.8 / 13.2, 512 15.2 / 12.9, 777 26.4 / 19.0. The adapters that a tile meets go
-// to `ways` workgroups, the first of each in parallel: about as many as 16 places of ascending ids meet of the bank's slots
-// (17 rows of 16 adapters in any order, us, 4 / 16 ways: 16.7 / 12.0; 64 rows 13.5 / 15.2, 11.6 with 6). K in as many parts as it
-// takes to fill the chip with two steps of 64 k a wave.
+// The most parts of K: two steps of 64 k for a wave at the least.
+int64_t most_parts(int64_t M, int64_t K) {
+  return std::max<int64_t>(1, std::min<int64_t>(K / (64 * 2 * kDownWaves), M <= kFewRows ? kSplitFew : kSplitMany));
+}
+
+// The first launch's tiles. Rows: 16 at a time, from kShortTiles products of 16 ranks on 32, so that the factors are read half as
+// often (both launches, us, 16 / 32 rows: 1,715 x 4,976, rank 32, 23.5 / 27.9; 3,744 x 464, two parts of rank 24, 21.0 / 18.1).
+// Ranks: up to two tiles of 16 together, or four from kFewRows rows on, so that the rows are read fewer times; one where
+// that would leave the chip empty (186 x 7,056, two parts of rank 32, one / two / four: 18.4 / 17.0 / 18.9). The adapters that a tile
+// meets go to `ways` workgroups, the mean of a bank whose slots are all in use and two more (75 rows of 14 adapters, 1,984 x three
+// parts of rank 32: 14.2, with one way less 16.9). K in as many parts as leave a workgroup for each CU and no second round of
+// them (85 x 8,592, 13 adapters, three parts of rank 24, one / two / four: 22.1 / 18.1 / 19.9).
 LoraPlan lora_plan(int64_t M, int64_t K, int P, int R, int64_t slots) {
   LoraPlan p;
   const int T = P * R / 16;
-  p.mt = M <= kFewRows ? 1 : 2;
-  p.ways = M <= 16 ? static_cast<int>(M)
-                   : static_cast<int>(std::max<int64_t>(2, std::min<int64_t>({p.mt == 1 ? 16 : 4, slots, slots * 16 * p.mt / std::min<int64_t>(M, kWindow) + 2})));
-  p.tc = p.mt == 2 ? (T + (T + 3) / 4 - 1) / ((T + 3) / 4) : M > 16 && T >= 8 ? 4 : 1;
-  const int64_t groups = (M + 16 * p.mt - 1) / (16 * p.mt) * ((T + p.tc - 1) / p.tc) * (M <= 16 ? M : 1);
-  const int64_t most = std::max<int64_t>(1, K / (64 * 2 * kDownWaves));
-  p.split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({most, p.mt == 1 ? kSplitFew : kSplitMany, (512 + groups - 1) / groups})));
+  const int64_t most = most_parts(M, K), window = std::min<int64_t>(M, kWindow);
+  if (M <= 16) {  // a workgroup for each row
+    p.mt = p.tc = 1;
+    p.ways = static_cast<int>(M);
+    p.split = static_cast<int>(std::min<int64_t>(most, (512 + M * T - 1) / (M * T)));
+    return p;
+  }
+  const bool few = M <= kFewRows;
+  p.mt = few || M * T <= kShortTiles ? 1 : 2;
+  p.ways = static_cast<int>(std::min<int64_t>({few ? 16 : 4, slots, (slots * 32 * p.mt + 5 * window) / (2 * window)}));
+  // 16 times the adapters that a tile meets at the mean
+  const int64_t tiles = (M + 16 * p.mt - 1) / (16 * p.mt), met = std::min<int64_t>({16 * slots, 256 * p.mt, 16 + slots * 256 * p.mt / window});
+  const int wide = tiles * T * met < 16 * 64 ? 1 : few ? 2 : 4, groups = (T + wide - 1) / wide;
+  p.tc = (T + groups - 1) / groups;
+  p.split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, 16 * (few ? 192 : 5 * K / 64) / (tiles * groups * met))));
   return p;
 }
 
@@ -535,7 +549,7 @@ int64_t place_bytes(int64_t M) { return (M * (int64_t)sizeof(int4) + 255) / 256 
 
 extern "C" int64_t krq_lora_ws_bytes(int64_t M, int64_t K, int parts, int rank) {
   if (M < 1 || K < 16 || parts < 1 || parts > kMaxParts || rank < 16 || rank > kMaxRank) return -1;
-  return place_bytes(M) + lora_plan(M, K, parts, rank, 1).split * M * parts * rank * (int64_t)sizeof(float);
+  return place_bytes(M) + most_parts(M, K) * M * parts * rank * (int64_t)sizeof(float);
 }
 
 extern "C" int krq_lora_add(const void* x, int64_t ldx, const void* ids, int ids_64, const void* a, const void* b, const int32_t* ranks,
@@ -593,6 +607,8 @@ extern "C" int krq_lora_add(const void* x, int64_t ldx, const void* ids, int ids
   hipStream_t s = (hipStream_t)stream;
   if (M <= 16) launch_down<1, 1, false>(l, s);
   else if (plan.mt == 1 && plan.tc == 1) launch_down<1, 1, true>(l, s);
+  else if (plan.mt == 1 && plan.tc == 2) launch_down<1, 2, true>(l, s);
+  else if (plan.mt == 1 && plan.tc == 3) launch_down<1, 3, true>(l, s);
   else if (plan.mt == 1) launch_down<1, 4, true>(l, s);
   else if (plan.tc == 1) launch_down<2, 1, true>(l, s);
   else if (plan.tc == 2) launch_down<2, 2, true>(l, s);
