@@ -128,6 +128,21 @@ def test_few_tokens_allowed(dev, V, n, dtype):
     check(logits[4:].to(dtype), torch.zeros(2 * len(allowed) - 4, 1, device=dev), n)
 
 
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("left", [1, 20, 130, 255, 256, 511, 512])
+def test_short_last_chunk(dev, left, dtype):
+    """A row's last tokens, behind whole chunks: distinct, equal, masked in part, the largest of the row or none of them."""
+    V = 3 * 8192 + left
+    for n in (1, 19, 64):
+        logits, scores = make(dev, 2, 3, V, dtype, seed=left)
+        logits[0, -left:] += 20
+        logits[1, -left:] = 25
+        logits[2, :-left] = -INF
+        logits[3, -left // 2:] = -INF
+        logits[4, -left:] = -INF
+        check(logits, scores, n)
+
+
 def test_extreme_values(dev):
     big = torch.finfo(torch.float32).max
     logits = torch.zeros(2, 3000, device=dev)
