@@ -524,7 +524,8 @@ int krq_add_rmsnorm(const void* x, int64_t ldx, const void* delta, int split, in
  * [slots][tiles * 16 * rank], tiles the sum of ceil(parts_n[p] / 16), of which slot i uses the first tiles * 16 * r, r = ranks[i]
  * rounded up to 16: of 16 columns of a part and 32 ranks entry [16 g + j] the ranks 8 g .. + 7 of column j, then, for an odd last
  * 16 ranks, the same in 32 entries (zeros past ranks[i] and past the part); ranks int32 [slots], at most rank, 0 for an empty slot;
- * scales fp32 [slots] (all on the device). rank a multiple of 16 up to 256, parts up to 8, K a multiple of 16.
+ * scales fp32 [slots] (all on the device). rank a multiple of 16 up to 256, parts up to 8, K a multiple of 16; K and ldx under
+ * 2^22, slots under 2^23, M and every part's columns up to 2^24.
  * y, out: bf16, or fp32 with fp32 != 0, rows ldy and ldo apart; out may be y.
  * Sums in fp32, rounded once. ws: krq_lora_ws_bytes(M, K, parts, rank) bytes on 16 (overwritten; calls that overlap must
  * not share it).
