@@ -106,6 +106,23 @@ def test_against_the_formula(dev, M, K, parts, ranks, rank, order, dtype):
     assert lora.add(y, x, ad, ids, out=y) is y and torch.equal(got, y)
 
 
+@pytest.mark.parametrize("M,K,parts,ranks,rank", [
+    (777, 2576, [90, 30, 17], [32, 16, 8], 32),      # 16 places, three tiles of ranks of six
+    (1100, 320, [64, 70], [32, 20], 32),             # 16 places, all four
+    (6700, 2064, [66], [16, 9, 3], 16),              # 32 places, one tile of ranks
+    (3400, 1040, [40, 24], [16, 5], 16),             # 32 places, two
+    (2250, 2128, [33, 8, 60], [16, 16, 16, 16], 16),  # three
+    (1700, 6144, [50], [64, 48], 64),                # four, K in two parts
+])
+@pytest.mark.parametrize("order", ["each", "runs"])
+def test_tiles_of_places_and_ranks(dev, M, K, parts, ranks, rank, order):
+    pairs, scales, x, y, ids = make(dev, M, K, parts, ranks, BF, order=order)
+    ad = bank(dev, K, parts, rank, pairs, scales)
+    got = lora.add(y, x, ad, ids)
+    check(got, y, x, pairs, scales, ids, parts)
+    assert torch.equal(got, lora.add(y, x, ad, ids))
+
+
 @pytest.mark.parametrize("M,K,N,r", [(9, 2560, 2560, 16), (400, 4096, 1024, 64)])
 def test_norm_of_the_error(dev, M, K, N, r):
     pairs, scales, x, _, ids = make(dev, M, K, [N], [r] * 3, BF, none=False)
