@@ -578,7 +578,7 @@ extern "C" int krq_beam_select(const void* logits, int fp32, int64_t ld, const f
 extern "C" int krq_beam_reorder(void* const* states, int count, int64_t outer, int64_t B, int64_t W, int64_t mid, int64_t S,
                                 int64_t dbytes, const void* beams, int beams_64, const void* lengths, int lengths_64, void* stream) {
   KRQ_REQUIRE(states && beams && count >= 1 && count <= kReorderStates, "beam_reorder: %d states (1 to %d)", count, kReorderStates);
-  KRQ_REQUIRE(outer >= 1 && B >= 1 && W >= 1 && W <= kBeamMax && mid >= 1 && S >= 1 && dbytes >= 1 && B <= (1 << 20),
+  KRQ_REQUIRE(outer >= 1 && B >= 1 && W >= 1 && W <= kBeamMax && mid >= 1 && S >= 1 && dbytes >= 1 && B <= (1 << 20) && S <= ((int64_t)1 << 40) / dbytes,
               "beam_reorder: bad shape [%lld][%lld x %lld][%lld][%lld][%lld bytes] (at most %d beams)", (long long)outer, (long long)B,
               (long long)W, (long long)mid, (long long)S, (long long)dbytes, kBeamMax);
   ReorderArgs a{};
@@ -601,7 +601,7 @@ extern "C" int krq_beam_reorder(void* const* states, int count, int64_t outer, i
   a.lengths64 = lengths_64 != 0;
   const int unit = bits % 16 == 0 && W <= 16 ? 16 : bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
   const double blocks = (double)((a.span + (int64_t)kReorderThreads * unit - 1) / ((int64_t)kReorderThreads * unit)) * outer * B * mid;
-  KRQ_REQUIRE(blocks < 2147483647.0, "beam_reorder: a state is too large for one launch");
+  KRQ_REQUIRE(blocks * kReorderThreads < 4294967296.0, "beam_reorder: a state is too large for one launch");
   hipStream_t s = (hipStream_t)stream;
   if (unit == 16) launch_reorder<v4u>(a, count, s);
   else if (unit == 4) launch_reorder<uint32_t>(a, count, s);

@@ -577,7 +577,8 @@ extern "C" int krq_lora_add(const void* x, int64_t ldx, const void* ids, int ids
   const int esize = fp32 ? 4 : 2;
   KRQ_REQUIRE((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(out)) % esize == 0, "lora_add: y and out must start on a value");
   KRQ_REQUIRE(y != out || ldy == ldo, "lora_add: out is y with other rows");
-  KRQ_REQUIRE((M + 15) / 16 * (n / 64 + parts) < 0x7fffffff, "lora_add: %lld x %lld is too large", (long long)M, (long long)n);
+  // (the second launch's workgroups at the most: of few rows one for each way, of many a wave has 512 bytes of a row)
+  KRQ_REQUIRE((M <= kFewRows ? (M + 15) / 16 * 16 * (n / 256 + parts) : (M + 63) / 64 * (n / (fp32 ? 128 : 256) + parts)) < (1 << 24), "lora_add: %lld x %lld is too large", (long long)M, (long long)n);
   const LoraPlan plan = lora_plan(M, K, parts, rank, slots);
   KRQ_REQUIRE(ws_bytes >= krq_lora_ws_bytes(M, K, parts, rank), "lora_add: ws of %lld bytes is too small", (long long)ws_bytes);
   l.x = (const uint16_t*)x;

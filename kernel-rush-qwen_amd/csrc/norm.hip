@@ -237,13 +237,15 @@ __global__ __launch_bounds__(64 * NW) void k_add_rmsnorm(NormArgs a) {
 }
 
 template <int NW, int W, int C, int SRC, int OUT>
-void launch(const NormArgs& a, hipStream_t s) {
+int launch(const NormArgs& a, hipStream_t s) {
   constexpr int per = NW / W;
   NormArgs b = a;
   int64_t blocks = (a.rows + per - 1) / per;
   b.spread = (a.tiled || OUT == kOutMxE4 || OUT == kOutMxE2) && a.rows >= 128;
   if (b.spread) blocks = (blocks + 128 / per - 1) / (128 / per) * (128 / per);
+  KRQ_REQUIRE(blocks * (64 * NW) < (int64_t)1 << 32, "add_rmsnorm: %lld rows of K=%d are too many for a launch", (long long)a.M, a.K);
   hipLaunchKernelGGL((k_add_rmsnorm<NW, W, C, SRC, OUT>), dim3(static_cast<unsigned>(blocks)), dim3(64 * NW), 0, s, b);
+  return krq_check_launch("add_rmsnorm");
 }
 
 // Rows by one or two waves each where there are enough rows to fill the chip that way and K leaves those waves no idle
@@ -253,23 +255,22 @@ void launch(const NormArgs& a, hipStream_t s) {
 constexpr int64_t kManyRows = 600, kMoreRows = 1536;
 
 template <int SRC, int OUT>
-void pick(const NormArgs& a, hipStream_t s) {
+int pick(const NormArgs& a, hipStream_t s) {
   const int K = OUT == kOutMxE4 || OUT == kOutMxE2 ? static_cast<int>(mx_groups(a.K)) * kMxGroup : a.K;  // chunks written
   if constexpr (SRC != kSrcPartials) {  // (partials of many rows: too many registers)
     if (a.rows >= kManyRows && K <= 2560) return launch<4, 1, 5, SRC, OUT>(a, s);
     if (a.rows >= kMoreRows && K <= 4096) return launch<4, 1, 8, SRC, OUT>(a, s);
     if (a.rows >= kManyRows && K > 4096 && K <= 5120) return launch<2, 2, 5, SRC, OUT>(a, s);
   }
-  if (K <= 4096) launch<8, 8, 1, SRC, OUT>(a, s);
-  else if (K <= 8192) launch<8, 8, 2, SRC, OUT>(a, s);
-  else launch<16, 16, 2, SRC, OUT>(a, s);
+  if (K <= 4096) return launch<8, 8, 1, SRC, OUT>(a, s);
+  if (K <= 8192) return launch<8, 8, 2, SRC, OUT>(a, s);
+  return launch<16, 16, 2, SRC, OUT>(a, s);
 }
 
 template <int OUT>
-void pick_src(const NormArgs& a, hipStream_t s) {
-  if (!a.delta) pick<kSrcNone, OUT>(a, s);
-  else if (a.split == 0) pick<kSrcBf16, OUT>(a, s);
-  else pick<kSrcPartials, OUT>(a, s);
+int pick_src(const NormArgs& a, hipStream_t s) {
+  if (!a.delta) return pick<kSrcNone, OUT>(a, s);
+  return a.split == 0 ? pick<kSrcBf16, OUT>(a, s) : pick<kSrcPartials, OUT>(a, s);
 }
 
 }  // namespace
@@ -315,10 +316,9 @@ extern "C" int krq_add_rmsnorm(const void* x, int64_t ldx, const void* delta, in
   a.split = split;
   a.tiled = tiled;
   hipStream_t s = (hipStream_t)stream;
-  if (out_kind == KRQ_NORM_ROWS) pick_src<kOutRows>(a, s);
-  else if (given) pick_src<kOutGiven>(a, s);
-  else if (out_kind == KRQ_NORM_MX_E4M3) pick_src<kOutMxE4>(a, s);
-  else if (out_kind == KRQ_NORM_MX_E2M1) pick_src<kOutMxE2>(a, s);
-  else pick_src<kOutToken>(a, s);
-  return krq_check_launch("add_rmsnorm");
+  if (out_kind == KRQ_NORM_ROWS) return pick_src<kOutRows>(a, s);
+  if (given) return pick_src<kOutGiven>(a, s);
+  if (out_kind == KRQ_NORM_MX_E4M3) return pick_src<kOutMxE4>(a, s);
+  if (out_kind == KRQ_NORM_MX_E2M1) return pick_src<kOutMxE2>(a, s);
+  return pick_src<kOutToken>(a, s);
 }

@@ -104,3 +104,11 @@ def test_entry_points_refuse():
                dict(mid=0), dict(S=0), dict(size=0), dict(B=(1 << 20) + 1), dict(outer=1 << 20, mid=1 << 20)]:
         assert reorder(**kw) == L.KRQ_EINVAL, kw
         assert b"beam_reorder" in lib.krq_last_error(), kw
+
+
+def test_more_threads_than_a_launch_has():
+    lib, p = L.lib(), ctypes.c_void_p(4096)
+    states = (ctypes.c_void_p * 1)(4096)
+    for outer, S, size in ((1, 1 << 32, 1), (1 << 10, 1 << 22, 1), (1 << 24, 1, 16), (1, 1 << 36, 16), (1, 1 << 40, 1 << 40)):
+        assert lib.krq_beam_reorder(states, 1, outer, 1, 2, 1, S, size, p, 1, None, 0, None) == L.KRQ_EINVAL
+        assert b"beam_reorder" in lib.krq_last_error()

@@ -202,3 +202,11 @@ def test_entry_point_refuses():
     assert lib.krq_lora_ws_bytes(3, 64, 2, 16) >= 3 * 2 * 16 * 4
     for args in ((0, 64, 2, 16), (3, 8, 2, 16), (3, 64, 0, 16), (3, 64, 9, 16), (3, 64, 2, 8), (3, 64, 2, 300)):
         assert lib.krq_lora_ws_bytes(*args) == -1
+
+
+def test_more_threads_than_a_launch_has():
+    lib, p = L.lib(), ctypes.c_void_p(4096)
+    for M, N, fp32 in ((48, 1 << 27, 0), (384, 1 << 24, 1), (1 << 24, 1 << 14, 0), (1 << 22, 1 << 15, 1)):
+        n = (ctypes.c_int64 * 8)(*[N // 8] * 8)
+        assert lib.krq_lora_add(p, 64, p, 0, p, p, p, p, 4, M, 64, n, 8, 16, p, N, p, N, fp32, p, 1 << 50, None) == L.KRQ_EINVAL
+        assert b"too large" in lib.krq_last_error()

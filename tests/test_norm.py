@@ -114,3 +114,10 @@ def test_entry_point_refuses():
     for kw in bad:
         assert call(**kw) == L.KRQ_EINVAL, kw
         assert b"add_rmsnorm" in lib.krq_last_error(), kw
+
+
+def test_more_threads_than_a_launch_has():
+    lib, p = L.lib(), ctypes.c_void_p(4096)
+    for M, K, split in ((1 << 23, 64, 2), (1 << 26, 64, 0), (1 << 22, 16384, 0)):
+        assert lib.krq_add_rmsnorm(p, K, p, split, K, M * K, p, 1e-6, M, K, 0, None, p, p, None, None, None) == L.KRQ_EINVAL
+        assert b"too many" in lib.krq_last_error()
