@@ -68,12 +68,12 @@ def select(logits, scores, n=None):
             logits, ld = logits.contiguous(), V
     if not scores.is_contiguous():
         scores = scores.contiguous()
-    out_scores = scores.new_empty((B, n))
-    beams = scores.new_empty((B, n), dtype=torch.int64)
+    out_scores = scores.new_empty(B, n)
+    beams = torch.empty_like(out_scores, dtype=torch.int64)
     tokens = torch.empty_like(beams)
     if B:
         nbytes = _ws_bytes(B, W, V, n, fp32)
-        ws = scores.new_empty((nbytes,), dtype=torch.uint8)
+        ws = scores.new_empty((nbytes + 3) // 4)
         _mx._call(dev, "krq_beam_select", logits.data_ptr(), fp32, ld, scores.data_ptr(), B, W, V, n, ws.data_ptr(), nbytes,
                   out_scores.data_ptr(), beams.data_ptr(), tokens.data_ptr())
     return out_scores, beams, tokens

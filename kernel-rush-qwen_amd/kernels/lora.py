@@ -187,7 +187,7 @@ def add(y, x, adapters, ids, out=None):
         return out
     parts = len(ad.parts)
     nbytes = _ws_bytes(M, K, parts, ad.rank)
-    ws = x.new_empty((max(nbytes, 1),), dtype=torch.uint8)
+    ws = x.new_empty((nbytes + 1) // 2)
     _mx._call(dev, "krq_lora_add", px, ldx, ids.data_ptr(), wide, ad.a.data_ptr(), ad.b.data_ptr(), ad.ranks.data_ptr(),
               ad.scales.data_ptr(), ad.slots, M, K, ad._n, parts, ad.rank, y.data_ptr(), ldy, out.data_ptr(), ldo, fp32, ws.data_ptr(), nbytes)
     return out

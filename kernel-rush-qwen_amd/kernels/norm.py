@@ -142,7 +142,7 @@ def add_rmsnorm(x, delta, ln, eps=1e-6, res_out=None):
     """x [M, K] bf16, delta None, bf16 [M, K] or fp32 partials [S, M, K], ln [K] bf16 -> (res, h), both bf16 [M, K].
     res_out: where res goes (contiguous; may be x, whose rows are then replaced); res is x itself where delta is None."""
     ops = _operands(x, delta, ln, res_out)
-    h = ops[0].new_empty(ops[8:10])
+    h = torch.empty_like(ops[0]) if ops[1] == ops[9] else ops[0].new_empty(ops[8:10])
     _launch(ops, eps, L.NORM_ROWS, None, h.data_ptr(), None, None)
     return ops[7], h
 
@@ -156,21 +156,21 @@ def add_rmsnorm_fp8(x, delta, ln, eps=1e-6, a=None, tiled=False, with_h=False, r
     ops = _operands(x, delta, ln, res_out)
     x, M, K = ops[0], ops[8], ops[9]
     if not tiled:
-        x8 = x.new_empty((M, K), dtype=torch.float8_e4m3fn)
+        x8 = torch.empty_like(x, dtype=torch.float8_e4m3fn) if ops[1] == K else x.new_empty(M, K, dtype=torch.float8_e4m3fn)
     elif K % 64:
         raise ValueError(f"tiled rows need K={K} a multiple of 64")
     else:
-        x8 = x.new_empty(((M + 15) // 16 * 16 * K,), dtype=torch.uint8)
+        x8 = x.new_empty((M + 15) // 16 * 16 * K, dtype=torch.uint8)
     if a is None:
         inv = None
-        xs = x.new_empty((M, 1), dtype=torch.float32)
+        xs = x.new_empty(M, 1, dtype=torch.float32)
         kind, ps = L.NORM_FP8_TOKEN_TILED if tiled else L.NORM_FP8_TOKEN, xs.data_ptr()
     else:
         one, xs = _fp8._one(a.inv), _fp8._one(a.scale)
         if one.get_device() != ops[10] or xs.get_device() != ops[10]:
             _misplaced(x, one, xs)
         kind, inv, ps = L.NORM_FP8_GIVEN_TILED if tiled else L.NORM_FP8_GIVEN, one.data_ptr(), None
-    h = x.new_empty((M, K)) if with_h else None
+    h = x.new_empty(M, K) if with_h else None
     _launch(ops, eps, kind, inv, h.data_ptr() if with_h else None, x8.data_ptr(), ps)
     return (ops[7], x8, xs, h) if with_h else (ops[7], x8, xs)
 
@@ -184,8 +184,8 @@ def add_rmsnorm_mx(x, delta, ln, eps=1e-6, elem="e4m3", with_h=False, res_out=No
         raise ValueError(f"MX blocks need K={K} a multiple of {_mx.BLOCK}")
     e = _mx._elem(elem)
     at, nbytes = _mx._rows_bytes(M, K, e)
-    data = x.new_empty((nbytes,), dtype=torch.uint8)
-    h = x.new_empty((M, K)) if with_h else None
+    data = x.new_empty(nbytes, dtype=torch.uint8)
+    h = x.new_empty(M, K) if with_h else None
     p = data.data_ptr()
     _launch(ops, eps, L.NORM_MX_E4M3 if e == L.MX_E4M3 else L.NORM_MX_E2M1, None, h.data_ptr() if with_h else None, p, p + at)
     rows = _mx.MXRows(data, at, (M, K), elem)
