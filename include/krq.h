@@ -526,6 +526,9 @@ int krq_add_rmsnorm(const void* x, int64_t ldx, const void* delta, int split, in
  * 16 ranks, the same in 32 entries (zeros past ranks[i] and past the part); ranks int32 [slots], at most rank, 0 for an empty slot;
  * scales fp32 [slots] (all on the device). rank a multiple of 16 up to 256, parts up to 8, K a multiple of 16; K and ldx under
  * 2^22, slots under 2^23, M and every part's columns up to 2^24.
+ * krq_lora_add_parts takes the parts' own ranks beside: part_ranks int32 [slots][parts], at most ranks[i] (the layout goes by
+ * ranks[i]), 0 for a part that the adapter leaves alone. Ranks that a part does not have stay out of its sum, where the zeros that
+ * stand for them would turn an infinity or a NaN of x into a NaN; krq_lora_add sums ranks[i] in every part.
  * y, out: bf16, or fp32 with fp32 != 0, rows ldy and ldo apart; out may be y.
  * Sums in fp32, rounded once. ws: krq_lora_ws_bytes(M, K, parts, rank) bytes on 16 (overwritten; calls that overlap must
  * not share it).
@@ -533,6 +536,10 @@ int krq_add_rmsnorm(const void* x, int64_t ldx, const void* delta, int split, in
 int krq_lora_add(const void* x, int64_t ldx, const void* ids, int ids_64, const void* a, const void* b, const int32_t* ranks,
                  const float* scales, int64_t slots, int64_t M, int64_t K, const int64_t* parts_n, int parts, int rank,
                  const void* y, int64_t ldy, void* out, int64_t ldo, int fp32, void* ws, int64_t ws_bytes, void* stream);
+int krq_lora_add_parts(const void* x, int64_t ldx, const void* ids, int ids_64, const void* a, const void* b, const int32_t* ranks,
+                       const int32_t* part_ranks, const float* scales, int64_t slots, int64_t M, int64_t K, const int64_t* parts_n,
+                       int parts, int rank, const void* y, int64_t ldy, void* out, int64_t ldo, int fp32, void* ws,
+                       int64_t ws_bytes, void* stream);
 int64_t krq_lora_ws_bytes(int64_t M, int64_t K, int parts, int rank);
 
 /*

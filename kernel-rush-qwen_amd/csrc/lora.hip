@@ -32,16 +32,26 @@ namespace {
 constexpr int kMaxParts = 8, kMaxRank = 256, kWindow = 256;
 constexpr int kSplitFew = 4, kSplitMany = 2;  // parts of K at most, for up to kFewRows rows and for more
 
+// What k_lora_down found at a place, in the 16 bytes that k_lora_up waits for: the row (24 bits) and id + 1 (24), under each the ranks
+// of four parts (9 bits each), and above the row the 16 ranks past the first by which the slot's factors lie.
+typedef ulonglong2 Place;
+static_assert(kMaxParts <= 8 && kMaxRank <= 256);
+KRQ_DEV int place_row(Place p) { return static_cast<int>(p.x & 0xffffff); }
+KRQ_DEV int place_id(Place p) { return static_cast<int>(p.y & 0xffffff) - 1; }
+KRQ_DEV int place_r16(Place p) { return 16 * static_cast<int>(p.x >> 60) + 16; }
+KRQ_DEV int place_rank(Place p, int part) { return static_cast<int>((part < 4 ? p.x : p.y) >> (24 + 9 * (part & 3))) & 511; }
+
 struct LoraArgs {
   const uint16_t* x;
   const void* ids;
   const uint16_t* a;     // [slots][P][R / 16][steps][2][64][8]: lane order, zeros past K
   const uint16_t* b;     // [slots][tiles 16 R]: for each tile of 16 columns and the slot's rank, rounded up to 16, lane order
   const int32_t* ranks;  // [slots], up to R; 0: none
+  const int32_t* part_ranks;  // [slots][P], up to the slot's rank; null: the slot's for every part
   const float* scales;   // [slots]
   const void* y;
   void* out;
-  int4* place;           // [M] what k_lora_down found at each place: row, id, rank
+  Place* place;          // [M]
   float* h;              // [split][M][P R] by place, times the scale
   int64_t M, K, ldx, ldy, ldo;
   int slots, P, R, split, ids64, ways, window;
@@ -163,8 +173,24 @@ __global__ __launch_bounds__(64 * NW, TC <= 2 ? 4 : 2) void k_lora_down(LoraArgs
   uint64_t left = __ballot(real);
   const int rank = real ? rank_of(a, id) : 0;
   const float scale = real && id >= 0 && id < a.slots ? a.scales[id] : 0.0f;
-  if (real && w == 0 && way == 0 && blockIdx.y == 0 && blockIdx.z == 0)
-    a.place[m0 + slot] = make_int4(static_cast<int>(w0) + row_of(slot), id, rank, 0);
+  auto write_place = [&]() {
+    if (!real || w != 0 || way != 0 || blockIdx.y != 0 || blockIdx.z != 0) return;
+    int own_rank[kMaxParts];  // (a last part again for those past it: loads without branches, all in flight)
+    const bool own = a.part_ranks && id >= 0 && id < a.slots;
+    const int32_t* from = own ? a.part_ranks + id * (int64_t)a.P : a.ranks;
+#pragma unroll
+    for (int p = 0; p < kMaxParts; ++p) own_rank[p] = from[own ? min(p, a.P - 1) : 0];
+    auto four = [&](int p) {
+      uint64_t v = 0;
+#pragma unroll
+      for (int i = 3; i >= 0; --i) v = v << 9 | static_cast<uint32_t>(own ? min(max(own_rank[p + i], 0), rank) : rank);
+      return v << 24;
+    };
+    Place place;
+    place.x = static_cast<uint32_t>(static_cast<int>(w0) + row_of(slot)) | four(0) | static_cast<uint64_t>(max(rank - 1, 0) >> 4) << 60;
+    place.y = static_cast<uint32_t>(id + 1) | four(4);
+    a.place[m0 + slot] = place;
+  };
   // this workgroup's adapters of the tile: every `ways`-th, from the way-th
   int turn = -1, first, cur;
   uint64_t same;
@@ -184,9 +210,10 @@ __global__ __launch_bounds__(64 * NW, TC <= 2 ? 4 : 2) void k_lora_down(LoraArgs
     }
     return false;
   };
-  if (!next()) return;
+  if (!next()) return write_place();
 #pragma unroll
   for (int u = 0; u < NB; ++u) load_x(s0 + u, u);
+  write_place();
   bool fresh = true;
   do {
     const int R16 = a.R >> 4;
@@ -354,12 +381,12 @@ __global__ __launch_bounds__(256, 4) void k_lora_up(LoraArgs a) {
   };
   v4f f[SP][2];
   load_h(0, a.R == 16, f);
-  const int4 place = a.place[pc];
-  const int id = place.y;
+  const Place place = a.place[pc];
+  const int id = place_id(place), slot_r16 = place_r16(place), own_rank = place_rank(place, p);
   uint64_t left = __ballot(m0 + j < a.M) & 0xffff;
   uint4* st = stage + w * ((a.R + 31) / 32) * NT * 64 + lane;
-  const T* yr = static_cast<const T*>(a.y) + (int64_t)place.x * a.ldy;
-  T* orow = static_cast<T*>(a.out) + (int64_t)place.x * a.ldo;
+  const T* yr = static_cast<const T*>(a.y) + (int64_t)place_row(place) * a.ldy;
+  T* orow = static_cast<T*>(a.out) + (int64_t)place_row(place) * a.ldo;
   bool fresh = true;  // f holds the first step
   for (int turn = 0; left; ++turn) {
     uint64_t same;
@@ -375,8 +402,9 @@ __global__ __launch_bounds__(256, 4) void k_lora_up(LoraArgs a) {
       if (!ROWS && turn % a.ways != way) continue;
     }
     const bool me = same >> j & 1;
-    const int rank = __builtin_amdgcn_readlane(place.z, first), r16 = (rank + 15) & ~15;
-    if (r16 == 0 && cur < a.slots && a.out == a.y) continue;
+    // the factors lie by the slot's rank; the sum is over the part's own, past which they hold zeros for which an h may not be finite
+    const int r16 = __builtin_amdgcn_readlane(slot_r16, first), rank = __builtin_amdgcn_readlane(own_rank, first);
+    if (rank == 0 && cur < a.slots && a.out == a.y) continue;
     // whole blocks of the wave, all their y in flight before anything else; a last block that the part ends in by itself
     const int whole = min(NI, (n1 - n0) >> 6);
     Piece<T> v[NI][NP];
@@ -388,7 +416,7 @@ __global__ __launch_bounds__(256, 4) void k_lora_up(LoraArgs a) {
           for (int q = 0; q < NP; ++q) v[blk][q].load(yr + n0 + VEC * g + 64 * blk + 4 * VEC * q);
     }
     // this place's h, summed over the parts of K in order, in NT terms
-    for (int s = 0; 32 * s < r16; ++s) {
+    for (int s = 0; 32 * s < rank; ++s) {
       const bool odd = 32 * s + 16 == r16;
       if (!(fresh && s == 0 && odd == (a.R == 16))) load_h(s, odd, f);
       v4f v2[2] = {f[0][0], f[0][1]};
@@ -408,7 +436,7 @@ __global__ __launch_bounds__(256, 4) void k_lora_up(LoraArgs a) {
       }
       fresh = false;
     }
-    const uint8_t* bs = reinterpret_cast<const uint8_t*>(a.b) + (int64_t)(r16 ? cur : 0) * a.tile[a.P] * (32 * a.R);
+    const uint8_t* bs = reinterpret_cast<const uint8_t*>(a.b) + (int64_t)(rank ? cur : 0) * a.tile[a.P] * (32 * a.R);
     // the products of the 64 columns of block nb of the part. Column j of the operand of tile t: see above; of fp32 it is the
     // column j of the factor's tile t, of bf16 it lies in tile 2 (t / 2) + j / 8, there 8 (j / 4 % 2) + 4 (t % 2) + j % 4
     const int first_tile = a.tile[p] + ((n0 - a.part[p]) >> 4), last_tile = a.tile[p + 1] - 1;
@@ -419,7 +447,7 @@ __global__ __launch_bounds__(256, 4) void k_lora_up(LoraArgs a) {
       const int64_t size = 32 * r16;  // bytes of a tile
       const uint8_t* base = bs + (first_tile + 4 * blk) * size;
       const int most = last_tile - (first_tile + 4 * blk);
-      for (int s = 0; 32 * s < r16; ++s) {
+      for (int s = 0; 32 * s < rank; ++s) {
         const bool odd = 32 * s + 16 == r16;
         const uint32_t lane_at = 16u * (16 * (odd ? g & 1 : g) + row);
         uint4 bv[4];
@@ -439,7 +467,7 @@ __global__ __launch_bounds__(256, 4) void k_lora_up(LoraArgs a) {
       }
     };
     auto finish = [&](Piece<T>& u, const v4f* acc) {
-      if (r16) u.add(acc);
+      if (rank) u.add(acc);
       if (cur >= a.slots) {
         constexpr uint32_t nan = sizeof(T) == 2 ? 0x7fc07fc0u : 0x7fc00000u;
         u.u = v4u{nan, nan, nan, nan};
@@ -449,7 +477,7 @@ __global__ __launch_bounds__(256, 4) void k_lora_up(LoraArgs a) {
 #pragma unroll
     for (int blk = 0; blk < NI; ++blk) {
       if (blk < whole) {
-        if (r16) product(blk, false, acc);
+        if (rank) product(blk, false, acc);
 #pragma unroll
         for (int q = 0; q < NP; ++q) {
           finish(v[blk][q], acc + TP * q);
@@ -459,7 +487,7 @@ __global__ __launch_bounds__(256, 4) void k_lora_up(LoraArgs a) {
     }
     const int ne = n0 + 64 * whole;
     if (whole < NI && ne < n1) {
-      if (r16) product(whole, true, acc);
+      if (rank) product(whole, true, acc);
 #pragma unroll
       for (int q = 0; q < NP; ++q) {
         const int n = ne + VEC * g + 4 * VEC * q;
@@ -543,7 +571,7 @@ void launch_up_any(const LoraArgs& a, hipStream_t s) {
 }
 
 // places, then h
-int64_t place_bytes(int64_t M) { return (M * (int64_t)sizeof(int4) + 255) / 256 * 256; }
+int64_t place_bytes(int64_t M) { return (M * (int64_t)sizeof(Place) + 255) / 256 * 256; }
 
 }  // namespace
 
@@ -552,9 +580,12 @@ extern "C" int64_t krq_lora_ws_bytes(int64_t M, int64_t K, int parts, int rank) 
   return place_bytes(M) + most_parts(M, K) * M * parts * rank * (int64_t)sizeof(float);
 }
 
-extern "C" int krq_lora_add(const void* x, int64_t ldx, const void* ids, int ids_64, const void* a, const void* b, const int32_t* ranks,
-                            const float* scales, int64_t slots, int64_t M, int64_t K, const int64_t* parts_n, int parts, int rank,
-                            const void* y, int64_t ldy, void* out, int64_t ldo, int fp32, void* ws, int64_t ws_bytes, void* stream) {
+namespace {
+
+int lora_add(const void* x, int64_t ldx, const void* ids, int ids_64, const void* a, const void* b, const int32_t* ranks,
+                    const int32_t* part_ranks, const float* scales, int64_t slots, int64_t M, int64_t K, const int64_t* parts_n,
+                    int parts, int rank, const void* y, int64_t ldy, void* out, int64_t ldo, int fp32, void* ws, int64_t ws_bytes,
+                    void* stream) {
   KRQ_REQUIRE(x && ids && a && b && ranks && scales && parts_n && y && out && ws, "lora_add: null pointer");
   KRQ_REQUIRE(M >= 1 && M <= (1 << 24) && K >= 16 && K % 16 == 0 && K < (1 << 22), "lora_add: bad shape M=%lld K=%lld (K a multiple of 16)",
               (long long)M, (long long)K);
@@ -586,10 +617,11 @@ extern "C" int krq_lora_add(const void* x, int64_t ldx, const void* ids, int ids
   l.a = (const uint16_t*)a;
   l.b = (const uint16_t*)b;
   l.ranks = ranks;
+  l.part_ranks = part_ranks;
   l.scales = scales;
   l.y = y;
   l.out = out;
-  l.place = (int4*)ws;
+  l.place = (Place*)ws;
   l.h = (float*)((uint8_t*)ws + place_bytes(M));
   l.M = M;
   l.K = K;
@@ -619,4 +651,22 @@ extern "C" int krq_lora_add(const void* x, int64_t ldx, const void* ids, int ids
   if (fp32) launch_up_any<float>(l, s);
   else launch_up_any<uint16_t>(l, s);
   return krq_check_launch("lora_add");
+}
+
+}  // namespace
+
+extern "C" int krq_lora_add(const void* x, int64_t ldx, const void* ids, int ids_64, const void* a, const void* b, const int32_t* ranks,
+                            const float* scales, int64_t slots, int64_t M, int64_t K, const int64_t* parts_n, int parts, int rank,
+                            const void* y, int64_t ldy, void* out, int64_t ldo, int fp32, void* ws, int64_t ws_bytes, void* stream) {
+  return lora_add(x, ldx, ids, ids_64, a, b, ranks, nullptr, scales, slots, M, K, parts_n, parts, rank, y, ldy, out, ldo, fp32, ws,
+                  ws_bytes, stream);
+}
+
+extern "C" int krq_lora_add_parts(const void* x, int64_t ldx, const void* ids, int ids_64, const void* a, const void* b,
+                                  const int32_t* ranks, const int32_t* part_ranks, const float* scales, int64_t slots, int64_t M,
+                                  int64_t K, const int64_t* parts_n, int parts, int rank, const void* y, int64_t ldy, void* out,
+                                  int64_t ldo, int fp32, void* ws, int64_t ws_bytes, void* stream) {
+  KRQ_REQUIRE(part_ranks, "lora_add: null pointer");
+  return lora_add(x, ldx, ids, ids_64, a, b, ranks, part_ranks, scales, slots, M, K, parts_n, parts, rank, y, ldy, out, ldo, fp32, ws,
+                  ws_bytes, stream);
 }

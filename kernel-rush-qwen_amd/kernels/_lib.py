@@ -93,6 +93,8 @@ EXPORTS = {
     "krq_lora_ws_bytes": (_i64, [_i64, _i64, _i32, _i32]),
     "krq_lora_add": (_i32, [_vp, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i32, _i32, _vp, _i64, _vp, _i64,
                             _i32, _vp, _i64, _vp]),
+    "krq_lora_add_parts": (_i32, [_vp, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i32, _i32, _vp, _i64, _vp,
+                                  _i64, _i32, _vp, _i64, _vp]),
     "krq_beam_select_ws_bytes": (_i64, [_i64, _i64, _i64, _i64, _i32]),
     "krq_beam_select": (_i32, [_vp, _i32, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp]),
     "krq_beam_reorder": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i32, _vp, _i32, _vp]),

@@ -46,7 +46,8 @@ class Adapters:
                              dtype=torch.bfloat16)
         self._tiles = [-(-p // 16) for p in self.parts]
         self.b = torch.zeros((self.slots, sum(self._tiles) * 16 * self.rank), device=device, dtype=torch.bfloat16)
-        self.ranks = torch.zeros((self.slots,), device=device, dtype=torch.int32)
+        self.ranks = torch.zeros((self.slots,), device=device, dtype=torch.int32)  # the parts' largest, by which a slot's factors lie
+        self.part_ranks = torch.zeros((self.slots, len(self.parts)), device=device, dtype=torch.int32)
         self.scales = torch.zeros((self.slots,), device=device, dtype=torch.float32)
         self._set_n()
 
@@ -58,6 +59,8 @@ class Adapters:
 
     def __setstate__(self, state):
         self.__dict__.update(state)
+        if "part_ranks" not in state:  # (saved with one rank for all parts of a slot)
+            self.part_ranks = self.ranks[:, None].repeat(1, len(self.parts))
         self._set_n()
 
     def _slot(self, slot):
@@ -69,13 +72,13 @@ class Adapters:
     def load(self, slot, pairs, scale=1.0):
         """Put an adapter into a slot: pairs, for each part its (A [r, K], B [part's columns, r]), rounded to bf16, or None where the
         adapter leaves the part alone; a single (A, B) for a projection of one part. Parts may differ in r, which is at most
-        the rank the Adapters were made for (each then takes the largest's memory). scale: the adapter's alpha / r."""
+        the rank the Adapters were made for (each then takes the largest's memory; its sum is over its own ranks). scale: the adapter's alpha / r."""
         slot = self._slot(slot)
         if len(self.parts) == 1 and len(pairs) == 2 and all(isinstance(t, torch.Tensor) for t in pairs):
             pairs = [pairs]
         if len(pairs) != len(self.parts):
             raise ValueError(f"{len(pairs)} pairs for {len(self.parts)} parts")
-        rank = 0
+        own = []
         for p, n in zip(pairs, self.parts):
             if p is not None:
                 a, b = p
@@ -83,9 +86,10 @@ class Adapters:
                     raise ValueError(f"A {tuple(a.shape)} and B {tuple(b.shape)} do not match [r, {self.K}] and [{n}, r]")
                 if not 1 <= a.shape[0] <= self.rank:
                     raise ValueError(f"rank {a.shape[0]} (1 to {self.rank})")
-                rank = max(rank, a.shape[0])
+            own.append(0 if p is None else p[0].shape[0])
+        rank = max(own)
         if rank == 0:  # (no part has a pair)
-            self.ranks[slot] = 0
+            self.clear(slot)
             return
         r16 = (rank + 15) // 16 * 16
         packed = self.b[slot, :sum(self._tiles) * 16 * r16].view(-1, 16 * r16)
@@ -107,6 +111,8 @@ class Adapters:
                 cols[:, 16 * full:].view(-1, 2, 16, 8).copy_(b[:, :, full:].view(-1, 16, 2, 8).permute(0, 2, 1, 3))
         self.scales[slot] = float(scale)
         self.ranks[slot] = rank
+        for i, r in enumerate(own):
+            self.part_ranks[slot, i] = r
 
     def _whole(self, t, rows, cols):
         """t in bf16 on the slots' device, with zeros up to [rows, cols]."""
@@ -120,6 +126,7 @@ class Adapters:
     def clear(self, slot):
         """Empty a slot."""
         self.ranks[self._slot(slot)] = 0
+        self.part_ranks[slot] = 0
 
 
 def _ld(t, cols):
@@ -188,6 +195,6 @@ def add(y, x, adapters, ids, out=None):
     parts = len(ad.parts)
     nbytes = _ws_bytes(M, K, parts, ad.rank)
     ws = x.new_empty((nbytes + 1) // 2)
-    _mx._call(dev, "krq_lora_add", px, ldx, ids.data_ptr(), wide, ad.a.data_ptr(), ad.b.data_ptr(), ad.ranks.data_ptr(),
-              ad.scales.data_ptr(), ad.slots, M, K, ad._n, parts, ad.rank, y.data_ptr(), ldy, out.data_ptr(), ldo, fp32, ws.data_ptr(), nbytes)
+    _mx._call(dev, "krq_lora_add_parts", px, ldx, ids.data_ptr(), wide, ad.a.data_ptr(), ad.b.data_ptr(), ad.ranks.data_ptr(),
+              ad.part_ranks.data_ptr(), ad.scales.data_ptr(), ad.slots, M, K, ad._n, parts, ad.rank, y.data_ptr(), ldy, out.data_ptr(), ldo, fp32, ws.data_ptr(), nbytes)
     return out

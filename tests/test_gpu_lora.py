@@ -10,11 +10,12 @@ whose mean square is a small part of 2^-16, and sqrt(K) 2^-24 stay under 2^-16."
 import pytest
 import torch
 
+from kernels import _lib as L
 from kernels import gemv as G
 from kernels import lora
 
 pytestmark = pytest.mark.gpu
-BF = torch.bfloat16
+BF, INF, NAN = torch.bfloat16, float("inf"), float("nan")
 
 
 def factors(g, K, parts, ranks, dev):
@@ -280,3 +281,45 @@ def test_a_bank_past_32_bit_offsets(dev):
     ad.load(slots - 1, pairs[0], scales[0])
     ids = torch.tensor([slots - 1, -1, slots - 1], device=dev)
     check(lora.add(y, x, ad, ids), y, x, [pairs[0]], scales, torch.where(ids < 0, -1, 0), [N])
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("M", [7, 40, 390, 2100])
+def test_parts_of_their_own_ranks(dev, M, dtype):
+    """A part that an adapter leaves alone, or in which it has fewer ranks than in another, takes part with its own: what is not
+    finite in x meets no rank that the part does not have. Positive factors, so that an infinity stays one."""
+    K, parts = 160, [96, 40, 33]
+    pairs, scales, x, y, ids = make(dev, M, K, parts, [40, 17, 33, 16], dtype, seed=11)
+    for i, own in enumerate(([None, 20, 5], [3, None, 17], [16, 33, None], [None, None, 7])):
+        pairs[i] = [None if r is None else (a[:r].abs().contiguous(), b[:, :r].abs().contiguous()) for r, (a, b) in zip(own, pairs[i])]
+    ad = bank(dev, K, parts, 40, pairs, scales)
+    check(lora.add(y, x, ad, ids), y, x, pairs, scales, ids, parts)
+    bad = torch.arange(M, device=dev) % 3 == 0
+    x[bad, 5] = torch.where(torch.arange(M, device=dev) % 2 == 0, INF, NAN).to(BF)[bad]
+    got = lora.add(y, x, ad, ids)
+    want, at = y.clone(), 0
+    for p, n in enumerate(parts):
+        for i, pair in enumerate(pairs):
+            if pair[p] is not None:
+                rows = torch.nonzero((ids == i) & bad)[:, 0]
+                want[rows, at:at + n] = x[rows, 5:6].to(dtype)
+        at += n
+    assert torch.equal(got[bad].isnan(), want[bad].isnan())
+    fine = bad[:, None] & ~want.isnan()
+    assert torch.equal(got[fine], want[fine])
+    check(got[~bad], y[~bad], x[~bad], pairs, scales, ids[~bad], parts)
+    assert lora.add(y, x, ad, ids, out=y) is y and torch.equal(y[fine], want[fine]) and torch.equal(y[~bad], got[~bad])
+
+
+@pytest.mark.parametrize("M", [9, 400])
+def test_entry_point_with_one_rank_for_a_slot(dev, M):
+    """krq_lora_add: every part has the slot's rank, as where a bank's parts have the same."""
+    K, parts = 160, [96, 40]
+    pairs, scales, x, y, ids = make(dev, M, K, parts, [40, 17], BF, seed=12)
+    ad = bank(dev, K, parts, 40, pairs, scales)
+    want, got, lib = lora.add(y, x, ad, ids), torch.empty_like(y), L.lib()
+    nbytes = lib.krq_lora_ws_bytes(M, K, 2, ad.rank)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    L.call("krq_lora_add", L.ptr(x), K, L.ptr(ids), True, L.ptr(ad.a), L.ptr(ad.b), L.ptr(ad.ranks), L.ptr(ad.scales), ad.slots, M, K, ad._n, 2,
+           ad.rank, L.ptr(y), sum(parts), L.ptr(got), sum(parts), False, L.ptr(ws), nbytes, L.stream(x))
+    assert torch.equal(got, want)

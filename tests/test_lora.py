@@ -210,3 +210,32 @@ def test_more_threads_than_a_launch_has():
         n = (ctypes.c_int64 * 8)(*[N // 8] * 8)
         assert lib.krq_lora_add(p, 64, p, 0, p, p, p, p, 4, M, 64, n, 8, 16, p, N, p, N, fp32, p, 1 << 50, None) == L.KRQ_EINVAL
         assert b"too large" in lib.krq_last_error()
+
+
+def test_ranks_of_parts():
+    ad = lora.Adapters(32, (3, 2), 40, 2, "cpu")
+    ad.load(1, [(torch.randn(17, 32), torch.randn(3, 17)), None])
+    assert ad.ranks.tolist() == [0, 17] and ad.part_ranks.tolist() == [[0, 0], [17, 0]]
+    ad.load(1, [(torch.randn(4, 32), torch.randn(3, 4)), (torch.randn(40, 32), torch.randn(2, 40))])
+    assert ad.ranks.tolist() == [0, 40] and ad.part_ranks.tolist() == [[0, 0], [4, 40]]
+    ad.load(1, [None, None])
+    assert ad.ranks.tolist() == [0, 0] and ad.part_ranks.tolist() == [[0, 0], [0, 0]]
+    ad.load(0, [None, (torch.randn(5, 32), torch.randn(2, 5))])
+    ad.clear(0)
+    assert not ad.ranks.any() and not ad.part_ranks.any()
+    state = {k: v for k, v in ad.__getstate__().items() if k != "part_ranks"}  # a bank saved with a rank for each slot only
+    old = lora.Adapters.__new__(lora.Adapters)
+    old.__setstate__({**state, "ranks": torch.tensor([0, 17], dtype=torch.int32)})
+    assert old.part_ranks.tolist() == [[0, 0], [17, 17]] and old.part_ranks.dtype is torch.int32
+
+
+def test_entry_point_of_parts_refuses():
+    lib, p = L.lib(), ctypes.c_void_p(4096)
+    n = (ctypes.c_int64 * 2)(48, 16)
+
+    def call(ranks=p, part_ranks=p, M=3):
+        return lib.krq_lora_add_parts(p, 64, p, 0, p, p, ranks, part_ranks, p, 4, M, 64, n, 2, 16, p, 64, p, 64, 0, p, 1 << 20, None)
+
+    for kw in (dict(ranks=None), dict(part_ranks=None), dict(M=0)):
+        assert call(**kw) == L.KRQ_EINVAL, kw
+        assert b"lora_add" in lib.krq_last_error(), kw
