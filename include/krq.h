@@ -546,10 +546,12 @@ int64_t krq_lora_ws_bytes(int64_t M, int64_t K, int parts, int rank);
  * Beam search's selection behind the lm head (reference engine/engine.py:1021-1022 takes the argmax): for every batch entry b
  * the n largest of
  *   v[w, t] = scores[b, w] + (logits[b W + w, t] - lse[b W + w]),  lse = log sum_t exp(logits)
- * over its W beams and V tokens, in order, with v in fp64; ties to the lower beam, then (equal logits of a beam) to the lower token.
+ * over its W beams and V tokens, in order; ties to the lower beam, then (equal logits of a beam) to the lower token. lse comes of
+ * exponentials and sums in fp32 and is off by less than 2^-18, the rest is fp64: candidates of one beam are in the order of their
+ * logits, candidates of two beams whose v are within 2^-17 may come in either order. Beams of the same logits have the same lse.
  * A beam whose logits are all -inf, or whose score is -inf, has v = -inf; one with a NaN or +inf among its logits, or as
  * its score, NaN, which counts as largest. logits bf16, or fp32 with fp32 != 0, [B W, V], rows ld apart; scores fp32 [B, W].
- * out_scores fp32 [B, n] (v rounded), out_beams and out_tokens int64 [B, n]. W and n up to 64, n <= W V, V up to 2^20,
+ * out_scores fp32 [B, n] (v with that lse, rounded), out_beams and out_tokens int64 [B, n]. W and n up to 64, n <= W V, V up to 2^20,
  * B W up to 65535. ws: krq_beam_select_ws_bytes bytes on 16 (overwritten; calls that overlap must not share it).
  */
 int krq_beam_select(const void* logits, int fp32, int64_t ld, const float* scores, int64_t B, int64_t W, int64_t V, int64_t n,

@@ -5,8 +5,13 @@
 // entry's W beams, ties to the lower beam, then to the lower token. Within a beam v goes as the logit, so the logits are
 // read once, by k_beam_rows: a workgroup takes a chunk of a row, keeps it in registers, and leaves the chunk's largest
 // value, its sum of exponentials and its n largest logits (with tokens, in order). k_beam_pick then takes a batch
-// entry: lse and the merged n of every row, and the merge of the rows by v in fp64 (candidates of two beams can lie
-// closer than fp32 tells apart).
+// entry: lse and the merged n of every row, and the merge of the rows by v, added and compared in fp64.
+//
+// lse is as good as the fp32 exponentials and sums behind it, off by less than 64 u = 2^-18 (u = 2^-24, vocabularies up to 2^20): a term's
+// distance t to the chunk's largest and on to the row's takes three roundings, 2.3 u |t|, whose mean over the terms is at most
+// 24 u (the weighed mean of |t| is W(V / e) at most); two exponentials and a product 5 u; 17 additions 17 u. Candidates of
+// one beam are in the order of their logits; those of two beams within 2^-17 may come in either order. (Exponentials in fp64 settle that: 8 x 8
+// beams 16.1 -> 21.1 us, 1 x 4 9.2 -> 9.9; the fp32 argument's rest carried to first order halves the bound: 17.9.)
 //
 // The n largest of a chunk. The n-th largest of 64 groups' largest values, found by its upper 16 bits with ballots, has n
 // values at or above it, and few more: those go to LDS, and each finds its place by counting the larger ones. Logit and
@@ -197,10 +202,10 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_rows(const T* __restrict_
     }
   }
   if (lane == 0 && (mine & 1) && mine < kSegKeys) seg[mine] = 0;  // (read in pairs)
-  float s = 0.0f;
+  float s4[4] = {};  // (four sums: fewer roundings behind each other)
 #pragma unroll
-  for (int i = 0; i < P; ++i) s += __builtin_amdgcn_exp2f((f[i] - m) * 1.44269504f);
-  s = wave_sum(s);
+  for (int i = 0; i < P; ++i) s4[i & 3] += __builtin_amdgcn_exp2f((f[i] - m) * 1.44269504f);
+  const float s = wave_sum((s4[0] + s4[1]) + (s4[2] + s4[3]));
   if (lane == 0) sums[w] = s, counts[w] = mine;
   __syncthreads();
   const int most = max(max(counts[0], counts[1]), max(counts[2], counts[3]));

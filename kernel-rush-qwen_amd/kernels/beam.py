@@ -38,10 +38,13 @@ def select(logits, scores, n=None):
     """logits [B W, V] (or [B, W, V]) bf16 or fp32, scores [B, W] fp32 (sums of log probabilities so far) -> (scores [B, n]
     fp32, beams [B, n] int64, tokens [B, n] int64): the n (default 2 W) largest of
       scores[b, w] + log_softmax(logits[b, w])[t]
-    over beams and tokens, best first, compared in fp64; ties to the lower beam, then to the lower token. -inf logits are
-    never preferred to others; a beam with nothing else, or with the score -inf (a first step's copies), has candidates of -inf. A beam with
-    a NaN or +inf among its logits, or as its score, has candidates of NaN, which count as the largest, as in lm_head_argmax. W and n up to
-    64, n <= W V, V up to 2^20, B W up to 65,535."""
+    over beams and tokens, best first; ties to the lower beam, then to the lower token. The log of the sum of exponentials is
+    off by less than 2^-18 (fp32 terms; all behind them is fp64): a beam's candidates are in the order of its logits, those of
+    two beams within 2^-17 of each other may come in either order, and beams of the same logits have the same sum. -inf logits
+    are never preferred to others; a beam with nothing else, or with the score -inf (a first step's copies), has candidates of
+    -inf. Mask with -inf: beside logits past 2^34, a type's lowest value among them, the log of the sum is below fp64's last place, so that
+    a beam of nothing else counts its tokens as certain. A beam with a NaN or +inf among its logits, or as its score, has candidates
+    of NaN, which count as the largest, as in lm_head_argmax. W and n up to 64, n <= W V, V up to 2^20, B W up to 65,535."""
     fp32 = logits.dtype is torch.float32
     shape = logits.shape
     if not (fp32 or logits.dtype is torch.bfloat16) or not 2 <= len(shape) <= 3:

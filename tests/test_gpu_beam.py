@@ -312,3 +312,69 @@ def test_reorder_past_32_bit_offsets(dev):
     lengths = torch.tensor([2000], device=dev)
     beam.reorder(state, beams, 1, lengths, 3)
     assert same_bits(state[-1], expected(last, beams, 0, lengths, 2)) and not state[:-1].any()
+
+
+# ---------------------------------------------------------------------------------------------
+# how far lse may be off, and the order between beams with it
+# ---------------------------------------------------------------------------------------------
+LSE_OFF = 2.0 ** -18
+"""With u = 2^-24 and V up to 2^20. A term exp(t), t the distance to its chunk's largest and that chunk's to the row's: t, its product with log2 e and that
+constant are rounded, 2.23 u |t|, and the mean of |t| weighed by the terms is at most the w with w e^(w + 1) = V, 10.6: 23.7 u. Two exponentials of 1 ulp, 2 u
+each, and their product: 5 u. Sums of 8 in a lane and of four such, then of 64 lanes and 4 waves: 9 + 8 u. 46 u in all, below 64 u = 2^-18."""
+
+
+def check_bounds(logits, scores, n):
+    """Candidates of two beams within 2 LSE_OFF may come in either order, all others and those of one beam may not."""
+    got, beams, tokens = beam.select(logits, scores, n)
+    v, W = values(logits, scores), scores.shape[1]
+    best, at = torch.sort(v, dim=-1, descending=True, stable=True)
+    best, at = best[:, :n], at[:, :n]
+    flat = (beams * (v.shape[1] // W) + tokens).cpu()
+    mine, other = torch.gather(v, 1, flat), flat != at
+    assert ((mine - best).abs()[other] <= 2 * LSE_OFF).all()
+    assert all(len(set(r)) == n for r in flat.tolist())
+    for row, b in zip(mine, beams.cpu()):
+        for w in range(W):
+            assert (row[b == w].diff() <= 0).all()
+    g, fine = got.double().cpu(), mine.isfinite()
+    assert ((g - mine).abs()[fine] <= LSE_OFF + 2.0 ** -24 * mine.abs()[fine]).all()
+    assert (got[:, :-1] >= got[:, 1:]).all()
+    return got, beams, tokens
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("V", [700, 20001, 151936, 1 << 20])
+@pytest.mark.parametrize("B,W,n", [(6, 2, 4), (5, 6, 3), (3, 6, 12), (2, 17, 20)])
+def test_one_peak_over_a_floor(dev, B, W, n, V, dtype):
+    """Equal logits 11 to 12 below the largest, another floor for every beam: the errors of their exponentials are the same and add up.
+    Scores that put all beams' peaks next to each other."""
+    g = torch.Generator(device=dev).manual_seed(V + W)
+    for i in range(3):
+        logits = (torch.randint(0, 17, (B * W, 1), generator=g, device=dev) / 16).expand(B * W, V).contiguous()
+        if i == 2:  # a beam's own noise over its floor
+            logits += torch.randn(B * W, V, generator=g, device=dev) * 0.25
+        logits[torch.arange(B * W, device=dev), torch.randint(V, (B * W,), generator=g, device=dev)] = 12.0
+        logits = logits.to(dtype)
+        lse = torch.logsumexp(logits.double().cpu(), -1).view(B, W)
+        check_bounds(logits, (lse - 12.5 - torch.rand(B, 1, dtype=torch.float64)).float().to(dev), n)
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("B,W,V,n", [(1, 4, 151936, 8), (8, 8, 151936, 16), (3, 5, 8191, 10), (16, 32, 2048, 64), (1, 64, 40000, 64), (64, 4, 999, 8)])
+def test_drawn_logits_within_the_bound(dev, B, W, V, n, dtype):
+    for seed in range(4):
+        check_bounds(*make(dev, B, W, V, dtype, seed=100 + seed), n)
+
+
+def test_equal_beams_beside_others(dev):
+    """Copies of a beam with its score: equal sums, so each token's candidates in the order of the beams."""
+    logits, scores = make(dev, 3, 6, 9000, torch.float32, seed=70)
+    logits = logits.view(3, 6, -1)
+    logits[:, 3], logits[:, 5] = logits[:, 1], logits[:, 1]
+    scores[:, 3], scores[:, 5] = scores[:, 1], scores[:, 1]
+    _, beams, tokens = check_bounds(logits, scores, 18)
+    for b, t in zip(beams.tolist(), tokens.tolist()):
+        first = [t[i] for i in range(18) if b[i] == 1]
+        copies = [(t[i], b[i]) for i in range(18) if b[i] in (1, 3, 5)]
+        want = [(x, w) for x in first for w in (1, 3, 5)]
+        assert copies == want[:len(copies)]
