@@ -191,3 +191,68 @@ def test_graph_and_streams(dev):
         eager = norm.add_rmsnorm_fp8(x, delta, ln, with_h=True)
         for a, b in zip(out, eager):
             assert same(a, b)
+
+
+# Both sides of every border between the thread layouts: rows 600 and 1,536, K 2,560, 4,096, 5,120 and 8,192, and what is left of 16 rows and of
+# a wave's chunks. (M, K): <4 waves a workgroup, 1 a row, 5 chunks a lane>, <4, 1, 8>, <2, 2, 5>, <8, 8, 1>, <8, 8, 2>, <16, 16, 2>
+BORDERS = [(600, 2560), (599, 2560), (613, 16), (600, 2576), (1537, 4096), (1541, 2624), (1536, 2592), (1535, 2592), (1535, 4096),
+           (601, 5120), (613, 4112), (600, 4608), (1600, 4160), (599, 5120), (600, 5136), (1550, 8192), (603, 8208)]
+
+
+@pytest.mark.parametrize("src", [None, "bf16", 2])
+@pytest.mark.parametrize("M,K", BORDERS)
+def test_layouts(dev, M, K, src):
+    """Against the formula and the quantizers, and the same bytes as a few rows that go alone, eight or sixteen waves to a row."""
+    x, delta, ln = make(dev, M, K, src, seed=8)
+    r, want = reference(x, delta, ln)
+    res, h = check_outputs(x, delta, ln)
+    assert same(res, r) and same(h, want)
+    for rows in (slice(0, 3), slice(M // 2, M // 2 + 17), slice(M - 5, M)):
+        d = delta if delta is None else delta[..., rows, :].contiguous()
+        for few, many in zip(norm.add_rmsnorm_fp8(x[rows].contiguous(), d, ln, with_h=True), norm.add_rmsnorm_fp8(x, delta, ln, with_h=True)):
+            assert same(few, many[rows])
+
+
+@pytest.mark.parametrize("M,K", [(1541, 4096), (1539, 2656), (605, 5120), (613, 4160)])
+def test_layouts_with_nan_inf_and_zero_rows(dev, M, K):
+    test_nan_inf_and_zero_rows(dev, M, K)
+
+
+@pytest.mark.parametrize("M,K", [(1541, 4096), (605, 5120), (700, 2560)])
+def test_layouts_in_place_and_strided(dev, M, K):
+    x, delta, ln = make(dev, M, K, "bf16", seed=9)
+    r, want = reference(x, delta, ln)
+    wide = torch.full((M, K + 40), 7.0, device=dev, dtype=BF)
+    wide[:, 16:16 + K] = x
+    res, h = norm.add_rmsnorm(wide[:, 16:16 + K], delta, ln)
+    assert same(res, r) and same(h, want) and (wide[:, :16] == 7).all() and (wide[:, 16 + K:] == 7).all()
+    for own in (x, delta):
+        xx, dd = x.clone(), delta.clone()
+        out = xx if own is x else dd
+        res, x8, xs = norm.add_rmsnorm_fp8(xx, dd, ln, res_out=out)
+        q8, qs = fp8.quant_rows(h)
+        assert res is out and same(out, r) and torch.equal(x8.view(torch.uint8), q8.view(torch.uint8)) and same(xs, qs)
+
+
+def test_more_than_2_31_elements(dev):
+    """Rows behind 2^31 elements, and 2^32 bytes of 8-bit rows in tiles: the last ones against the same rows alone."""
+    M, K = (1 << 31) // 16384 + 21, 16384
+    g = torch.Generator(device=dev).manual_seed(10)
+    x, delta = (torch.empty(M, K, device=dev, dtype=BF).normal_(generator=g) for _ in range(2))
+    ln = (1 + 0.3 * torch.randn(K, generator=g, device=dev)).to(BF)
+    at = M // 16 * 16 - 16
+    for call in (lambda a, b: norm.add_rmsnorm_fp8(a, b, ln, with_h=True), lambda a, b: norm.add_rmsnorm_fp8(a, b, ln, tiled=True),
+                 lambda a, b: norm.add_rmsnorm_mx(a, b, ln)):
+        out, tail = call(x, delta), call(x[at:].contiguous(), delta[at:].contiguous())
+        assert same(out[0][at:], tail[0])
+        if isinstance(out[1], mxfp4.MXRows):  # (data, then scales, each in blocks of sixteen rows)
+            a, b = out[1], tail[1]
+            size = b.scale_at
+            assert torch.equal(a.data[a.scale_at - size:a.scale_at], b.data[:size])
+            rest = b.data.numel() - size
+            assert torch.equal(a.data[-rest:], b.data[-rest:])
+        elif out[1].dtype is torch.uint8:
+            assert torch.equal(out[1][at * K:], tail[1]) and same(out[2][at:], tail[2])
+        else:
+            assert all(same(a[at:], b) for a, b in zip(out[1:], tail[1:]))
+        del out, tail
