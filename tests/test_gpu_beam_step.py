@@ -172,3 +172,19 @@ def test_captured_step(dev, kind):
         want = m.step(*new)
         for a, b in zip((*out, *caches), (*want, *new[3])):
             assert same(a, b)
+
+
+@pytest.mark.parametrize("kind", ["fp8", "mxfp4"])
+def test_first_residual_and_gate_up(dev, kind):
+    """The links between the attention's output and the activation: the residual by its formula, gate_up's adapters in 64 bits beside the
+    product of the same rows."""
+    m, t = Model(dev, kind), {}
+    tokens, ids, scores, caches, lengths = state(dev, 3)
+    m.step(tokens, ids, scores, caches, lengths, t)
+    assert same(t["res"], (t["x"].float() + t["p"][0].to(BF).float()).to(BF))
+    y = m.product(m.rows(t["h2"]), m.gu)
+    want, got = low_rank(m, "gu", t["h2"], ids, y), t["gu"]
+    assert not torch.equal(got, y) and same(got[ids < 0], y[ids < 0])
+    assert ((got.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -14 * (want - y.double()).abs().amax(1, keepdim=True)).all()
+    act = (torch.nn.functional.silu(got[:, :I].float()).to(BF).float() * got[:, I:].float()).to(BF)
+    assert same(t["act"], act)
