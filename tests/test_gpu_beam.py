@@ -378,3 +378,14 @@ def test_equal_beams_beside_others(dev):
         copies = [(t[i], b[i]) for i in range(18) if b[i] in (1, 3, 5)]
         want = [(x, w) for x in first for w in (1, 3, 5)]
         assert copies == want[:len(copies)]
+
+
+def test_reorder_of_short_lengths_in_a_large_room(dev):
+    """A static cache of 32,768 positions of which a few hundred are in use: only those move."""
+    for W in (4, 8, 16, 20):
+        state = random_state((2 * W, 2, 32768, 64), BF, dev, seed=W)
+        beams = torch.randint(W, (2, W), device=dev, generator=torch.Generator(device=dev).manual_seed(W))
+        lengths = torch.tensor([512, 3], device=dev)
+        want = expected(state, beams, 0, lengths, 2)
+        beam.reorder(state, beams, 0, lengths, 2)
+        assert same_bits(state, want)
