@@ -512,13 +512,17 @@ int64_t most_parts(int64_t M, int64_t K) {
   return std::max<int64_t>(1, std::min<int64_t>(K / (64 * 2 * kDownWaves), M <= kFewRows ? kSplitFew : kSplitMany));
 }
 
-// The first launch's tiles. Rows: 16 at a time, from kShortTiles products of 16 ranks on 32, so that the factors are read half as
+// The first launch's tiles. Rows: 16 at a time; 32 from kShortTiles products of a row and 16 ranks on, so that the factors are read half as
 // often (both launches, us, 16 / 32 rows: 1,715 x 4,976, rank 32, 23.5 / 27.9; 3,744 x 464, two parts of rank 24, 21.0 / 18.1).
 // Ranks: up to two tiles of 16 together, or four from kFewRows rows on, so that the rows are read fewer times; one where
-// that would leave the chip empty (186 x 7,056, two parts of rank 32, one / two / four: 18.4 / 17.0 / 18.9). The adapters that a tile
-// meets go to `ways` workgroups, the mean of a bank whose slots are all in use and two more (75 rows of 14 adapters, 1,984 x three
-// parts of rank 32: 14.2, with one way less 16.9). K in as many parts as leave a workgroup for each CU and no second round of
-// them (85 x 8,592, 13 adapters, three parts of rank 24, one / two / four: 22.1 / 18.1 / 19.9).
+// there would be less than 64 workgroups with work, a quarter of the CUs (186 x 7,056, two parts of rank 32, one / two / four:
+// 18.4 / 17.0 / 18.9). The adapters that a tile meets go to `ways` workgroups: the mean, slots 16 mt / window, of a bank whose slots
+// are all in use, and two more (75 rows of 14 adapters, 1,984 x three parts of rank 32: 14.2, with one way less 16.9). K in as many
+// parts as keep the workgroups with work to 192 at few rows, three quarters of the CUs, so that there is no second round of them
+// (85 x 8,592, 13 adapters, three parts of rank 24, one / two / four: 22.1 / 18.1 / 19.9), and to 5 K / 64 at many: the more
+// steps of 64 a wave has, the more of a second round its halving is worth.
+// kShortTiles, the 64, the 192 and the 5 are fits to this card, over 140 drawn calls of 17 to 4,096 rows: at the mean 2 % behind
+// the best of 16 plans each. Another count of CUs or another kernel needs them again.
 LoraPlan lora_plan(int64_t M, int64_t K, int P, int R, int64_t slots) {
   LoraPlan p;
   const int T = P * R / 16;

@@ -6,9 +6,11 @@
 //   h    = bf16(bf16(r * rstd) * ln)
 //   out  = h, and/or e4m3 rows with a per-token or a given scale (the arithmetic of krq_quant_rows and krq_cast_fp8,
 //          their bytes), or MX blocks of 32 (krq_quant_mx_rows' bytes)
-// The sum of squares is held in fp64: a square of a bf16 is exact in fp32, and with the sum exact to 2^-50 rstd does
-// not depend on the order of the sum, so that the roundings to bf16 and e4m3 behind it, which have borders, come out the
-// same for every thread layout below. It costs two fp64 operations per value, hidden under the loads.
+// The sum of squares is held in fp64: a square of a bf16 is exact in fp32, and its 70 additions of a lane and across lanes at the
+// most leave the sum off by less than 2^-46 and rstd, before its rounding to fp32, by less than 2^-47: it is the rounding of
+// the exact value, whatever the order of the sum, but for at most one row in some 2^22 that lies so near a border; the
+// roundings to bf16 and e4m3 behind it, which have borders of their own, come out the same for every thread layout
+// below. It costs two fp64 operations per value, hidden under the loads.
 //
 // A row is held in registers between the passes over it: W waves, C chunks of 8 values per lane, so that every value
 // is read once and written once. W = 1 needs no barrier.
@@ -248,10 +250,12 @@ int launch(const NormArgs& a, hipStream_t s) {
   return krq_check_launch("add_rmsnorm");
 }
 
-// Rows by one or two waves each where there are enough rows to fill the chip that way and K leaves those waves no idle
-// chunks, else by eight or sixteen waves, whose loads are all in flight at once. Calls of a graph, per-token scales, a bf16 addend, us, few
-// waves / many: 2,560 x 512 rows 5.0 / 4.9, 1,001 rows 6.5 / 7.5, 2,048 rows 9.1 / -; 4,096 x 1,001 8.7 / 8.5; 5,120 x 1,001 9.6 / 10.6,
-// 4,096 rows 27.4 / 31.2; 8,192 x 1,001 13.1 / 12.6 and 16,384 x 1,001 (four waves) 22.9 / 22.7.
+// Rows by one or two waves each where there are enough rows to fill the chip that way, else by eight or sixteen waves, whose loads
+// are all in flight at once. Calls of a graph, per-token scales, a bf16 addend, us, few waves / many: 2,560 x 512 rows 5.0 / 4.9, 601 rows
+// 5.1 / 5.7, 1,001 6.4 / 7.4, 2,048 9.2 / 11.3, 4,096 14.0 / 18.1; 4,096 x 1,001 8.7 / 8.5; 5,120 x 1,001 9.6 / 10.6, 4,096 rows 27.4 / 31.2; 8,192 x 1,001
+// 13.1 / 12.6 and 16,384 x 1,001 (four waves) 22.9 / 22.7. One wave has five chunks a lane for every K up to 2,560, of which a smaller K leaves
+// some idle (loaded again at the row's end, squared as zeros): 256 x 601 rows 3.9 / 4.9, 4,096 rows 7.8 / 14.9; 1,024 x 601 4.0 / 4.9, 4,096
+// rows 9.8 / 16.4.
 constexpr int64_t kManyRows = 600, kMoreRows = 1536;
 
 template <int SRC, int OUT>

@@ -87,8 +87,8 @@ def reorder(states, beams, dim=0, lengths=None, length_dim=None):
     b W + beams[b, w] was. states: a contiguous tensor of any type, or a list of them that do not overlap, with the same B W rows along dim; beams
     int64 or int32 [B, W] (the first W columns of what select gave, or the W that stayed; repeats are the rule). lengths int32 or int64
     [B] with length_dim (after dim): of each entry only the positions before its length move, those behind stay as they are.
-    A beam outside [0, W) leaves its row as it is. Rows whose beam is their own are neither read nor written. One launch for all states
-    of a shape (of up to 64). Returns states."""
+    A beam outside [0, W) leaves its row as it is. Rows whose beam is their own are neither read nor written. One launch for every 64 states
+    of a shape, behind a copy of beams where they are columns of a wider tensor. Returns states."""
     many = [states] if isinstance(states, torch.Tensor) else list(states)
     shape, dev = beams.shape, beams.get_device()
     if not (beams.dtype is torch.int64 or beams.dtype is torch.int32) or len(shape) != 2:
