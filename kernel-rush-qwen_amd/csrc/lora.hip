@@ -176,14 +176,14 @@ __global__ __launch_bounds__(64 * NW, TC <= 2 ? 4 : 2) void k_lora_down(LoraArgs
   auto write_place = [&]() {
     if (!real || w != 0 || way != 0 || blockIdx.y != 0 || blockIdx.z != 0) return;
     int own_rank[kMaxParts];  // (a last part again for those past it: loads without branches, all in flight)
-    const bool own = a.part_ranks && id >= 0 && id < a.slots;
-    const int32_t* from = own ? a.part_ranks + id * (int64_t)a.P : a.ranks;
+    const bool known = a.part_ranks && id >= 0 && id < a.slots;
+    const int32_t* from = known ? a.part_ranks + id * (int64_t)a.P : a.ranks;
 #pragma unroll
-    for (int p = 0; p < kMaxParts; ++p) own_rank[p] = from[own ? min(p, a.P - 1) : 0];
+    for (int p = 0; p < kMaxParts; ++p) own_rank[p] = from[known ? min(p, a.P - 1) : 0];
     auto four = [&](int p) {
       uint64_t v = 0;
 #pragma unroll
-      for (int i = 3; i >= 0; --i) v = v << 9 | static_cast<uint32_t>(own ? min(max(own_rank[p + i], 0), rank) : rank);
+      for (int i = 3; i >= 0; --i) v = v << 9 | static_cast<uint32_t>(known ? min(max(own_rank[p + i], 0), rank) : rank);
       return v << 24;
     };
     Place place;

@@ -323,3 +323,24 @@ def test_entry_point_with_one_rank_for_a_slot(dev, M):
     L.call("krq_lora_add", L.ptr(x), K, L.ptr(ids), True, L.ptr(ad.a), L.ptr(ad.b), L.ptr(ad.ranks), L.ptr(ad.scales), ad.slots, M, K, ad._n, 2,
            ad.rank, L.ptr(y), sum(parts), L.ptr(got), sum(parts), False, L.ptr(ws), nbytes, L.stream(x))
     assert torch.equal(got, want)
+
+
+def test_the_most_rows_and_slots(dev):
+    """2^24 rows, and a bank of 2^23 - 1 slots: places and ids as long as the kernels keep them."""
+    M, K, N = 1 << 24, 16, 3
+    pairs, scales, x, y, ids = make(dev, 64, K, [N], [16, 5], BF, seed=13)
+    ad = bank(dev, K, [N], 16, pairs, scales)
+    want = lora.add(y, x, ad, ids)
+    got = lora.add(y.repeat(M // 64, 1), x.repeat(M // 64, 1), ad, ids.repeat(M // 64))
+    assert torch.equal(got.view(M // 64, 64, N), want.expand(M // 64, 64, N))
+    del ad, got
+    slots = (1 << 23) - 1
+    ad = lora.Adapters(K, N, 5, slots, dev)
+    for i, s in enumerate((slots - 1, 0)):
+        ad.load(s, pairs[1], scales[i])
+    ids = torch.tensor([slots - 1, 0, -1, slots, 1 << 40] * 80, device=dev)
+    x, y = x[:40].repeat(10, 1), y[:40].repeat(10, 1)
+    got = lora.add(y, x, ad, ids)
+    fine = ids < slots
+    check(got[fine], y[fine], x[fine], [pairs[1], pairs[1]], scales, torch.where(ids < 0, -1, torch.where(ids == 0, 1, 0))[fine], [N])
+    assert got[~fine].isnan().all()
